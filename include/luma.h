@@ -42,6 +42,10 @@
  *   luma_hyper_rows    -- the step-dependent scalars of functional.py:209-213,
  *                         262-264, 278 as the device derives them (for
  *                         checking against the host's double arithmetic).
+ *   luma_grad_norm, luma_grad_clip, luma_grad_scale
+ *                      -- torch.nn.utils.get_total_norm, clip_grad_norm_ and
+ *                         clip_grads_with_norm_ as the reference's benchmark
+ *                         uses them around its step (no kernel of its own).
  *   luma_philox4x32    -- host-side Philox4x32-10 block function used by the
  *                         stochastic rounding (Salmon et al., SC'11); the
  *                         reference's Triton path draws from tl.rand
@@ -57,7 +61,7 @@
 extern "C" {
 #endif
 
-#define LUMA_ABI_VERSION 10
+#define LUMA_ABI_VERSION 11
 
 /*
  * Elements per chunk-table entry (one workgroup's share of a tensor): the
@@ -359,6 +363,73 @@ int luma_quantize(const float *m, const float *v, int64_t numel, int16_t *q_m, i
  * 1-beta2, decay, -eta, bc2, eps.
  */
 int luma_hyper_rows(const LumaGroup *group, int64_t t0, int32_t n, float *out, void *stream);
+
+/*
+ * The global norm of many gradients, and clipping by it.
+ *
+ * ||g||_p over all elements of all rows together; the reference's benchmark
+ * clips with torch.nn.utils.clip_grad_norm_ between backward() and step()
+ * (benchmarks/bench_nanogpt.py).  Sums are formed in float64 (a float32
+ * gradient's square is exact there and cannot overflow or vanish) in an order
+ * that only the rows' sizes determine, so that a result is reproduced bit for
+ * bit.  A NaN anywhere makes the norm NaN.
+ */
+#define LUMA_NORM_L2 0
+#define LUMA_NORM_L1 1
+#define LUMA_NORM_INF 2
+
+/* Elements per tile: the unit in which the rows are shared out to wavefronts. */
+#define LUMA_GRAD_TILE 2048
+/* Rows that one launch carries among its arguments (no device table). */
+#define LUMA_GRADS_INLINE 144
+/* Rows that may go without a device table. */
+#define LUMA_GRADS_NO_TABLE (LUMA_GRADS_INLINE * 256)
+/* Doubles of workspace (LumaNormArgs.partials). */
+#define LUMA_NORM_PARTIALS 1024
+
+/* One gradient; dense, elements in any order, aligned to its element type. */
+typedef struct LumaGrad {
+  void *data;          /* device f32 / bf16 / f16 [numel]                       */
+  int64_t numel;       /* >= 1                                                   */
+  int32_t dtype;       /* LUMA_GRAD_*                                            */
+  int32_t first_tile;  /* sum of ceil(numel / LUMA_GRAD_TILE) of the rows before */
+} LumaGrad;
+
+typedef struct LumaNormArgs {
+  const LumaGrad *grads; /* HOST: the rows, read during the call                 */
+  const LumaGrad *table; /* device copy of them; NULL (n <= LUMA_GRADS_NO_TABLE):
+                            the rows travel as launch arguments, a launch per
+                            LUMA_GRADS_INLINE of them (may then be captured into
+                            a HIP graph)                                         */
+  int32_t n;             /* rows                                                 */
+  int32_t norm;          /* LUMA_NORM_*                                          */
+  double max_norm;       /* clipping: the largest norm, >= 0                     */
+  double *partials;      /* device workspace, LUMA_NORM_PARTIALS doubles         */
+  float *total;          /* device scalar: the norm (luma_grad_scale reads it)   */
+  double *power;         /* device scalar or NULL: the norm before its root (the
+                            sum of |g|^p; the largest |g|), to be joined with
+                            other GPUs'                                          */
+  const float *grad_scale; /* device scalar or NULL: the gradients hold scale * g,
+                            and *total and *step_scale are for g
+                            (luma_grad_norm only)                                */
+  float *step_scale;     /* device scalar or NULL: what LumaScaling.grad_scale has
+                            to be for a step that clips by max_norm as it reads
+                            the gradients: grad_scale (or 1) over the clip factor
+                            (luma_grad_norm only)                                */
+} LumaNormArgs;
+
+/* *total (and *power) of the rows; the gradients are only read. */
+int luma_grad_norm(const LumaNormArgs *args, void *stream);
+
+/*
+ * luma_grad_norm, then every gradient times min(1, max_norm / (*total + 1e-6))
+ * in place, rounded to nearest in its own type (nothing is written where the
+ * factor is 1).  No two rows may share memory.
+ */
+int luma_grad_clip(const LumaNormArgs *args, void *stream);
+
+/* The second half of luma_grad_clip, with the norm that *total holds. */
+int luma_grad_scale(const LumaNormArgs *args, void *stream);
 
 /* Host: one Philox4x32-10 block. */
 void luma_philox4x32(const uint32_t ctr[4], const uint32_t key[2], uint32_t out[4]);

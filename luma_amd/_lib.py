@@ -24,9 +24,13 @@ STEP_TENSOR_CHUNK_MIN = 16384  # LUMA_STEP_TENSOR_CHUNK_MIN
 SLOT_BYTES = 512             # LUMA_SLOT_BYTES
 NOALLOC_MAX_CHUNKS = 262144  # LUMA_NOALLOC_MAX_CHUNKS
 SUMMARY_WORDS = 256          # LUMA_SUMMARY_WORDS (per chunk)
-ABI_VERSION = 10             # LUMA_ABI_VERSION
+ABI_VERSION = 11             # LUMA_ABI_VERSION
+GRAD_TILE = 2048             # LUMA_GRAD_TILE
+GRADS_INLINE = 144           # LUMA_GRADS_INLINE
+NORM_PARTIALS = 1024         # LUMA_NORM_PARTIALS
 
 GRAD_F32, GRAD_BF16, GRAD_F16 = 0, 1, 2
+NORM_L2, NORM_L1, NORM_INF = 0, 1, 2
 NOISE_PHILOX, NOISE_INJECTED = 0, 1
 FLAG_EXACT_ONLY = 1
 FLAG_SPLIT = 2               # LUMA_FLAG_SPLIT
@@ -46,6 +50,9 @@ GROUP_DTYPE = np.dtype([
 ])
 SCALE_INIT_DTYPE = np.dtype([
     ("slot", "<u8"), ("step", "<i8"), ("s_m", "<f8"), ("s_v", "<f8"), ("eps", "<f8"),
+])
+GRAD_DTYPE = np.dtype([                    # LumaGrad
+    ("data", "<u8"), ("numel", "<i8"), ("dtype", "<i4"), ("first_tile", "<i4"),
 ])
 # luma_hyper_rows output columns
 HYPER_ROW_FIELDS = ("beta1", "omb1", "beta2", "omb2", "decay", "neg_eta", "bc2", "eps")
@@ -72,6 +79,22 @@ class StepArgs(ctypes.Structure):
         ("medium_chunks", ctypes.c_int32),
         ("reserved", ctypes.c_int32),
         ("scaling", Scaling),
+    ]
+
+
+class NormArgs(ctypes.Structure):
+    """LumaNormArgs."""
+    _fields_ = [
+        ("grads", ctypes.c_void_p),
+        ("table", ctypes.c_void_p),
+        ("n", ctypes.c_int32),
+        ("norm", ctypes.c_int32),
+        ("max_norm", ctypes.c_double),
+        ("partials", ctypes.c_void_p),
+        ("total", ctypes.c_void_p),
+        ("power", ctypes.c_void_p),
+        ("grad_scale", ctypes.c_void_p),
+        ("step_scale", ctypes.c_void_p),
     ]
 
 
@@ -104,6 +127,9 @@ _SIGNATURES = {
                                      ctypes.c_double, ctypes.c_uint64, ctypes.c_int32, _VP, _VP,
                                      _VP, _VP]),
     "luma_hyper_rows": (ctypes.c_int, [_VP, ctypes.c_int64, ctypes.c_int32, _VP, _VP]),
+    "luma_grad_norm": (ctypes.c_int, [ctypes.POINTER(NormArgs), _VP]),
+    "luma_grad_clip": (ctypes.c_int, [ctypes.POINTER(NormArgs), _VP]),
+    "luma_grad_scale": (ctypes.c_int, [ctypes.POINTER(NormArgs), _VP]),
     "luma_philox4x32": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32),
                                ctypes.POINTER(ctypes.c_uint32)]),
 }

@@ -1,0 +1,306 @@
+"""The global norm of many gradients, and clipping by it.
+
+``get_total_norm``, ``clip_grad_norm_`` and ``clip_grads_with_norm_`` take the
+arguments of ``torch.nn.utils``' functions of these names, which the
+reference's benchmark calls between ``backward()`` and ``step()``
+(benchmarks/bench_nanogpt.py)::
+
+    loss.backward()
+    norm = luma_amd.clip_grad_norm_(model.parameters(), 1.0)
+    opt.step()
+
+All gradients are read by one launch and, where they have to be clipped,
+scaled in place by a second (luma_grad_clip in include/luma.h), with no host
+synchronisation.  The norm is a float32 scalar on the gradients' device,
+summed in float64, whatever the gradients' types.  Differences from torch:
+float32, bfloat16 and float16 gradients on one ROCm GPU; p = 1, 2 or inf; a
+parameter listed twice counts, and is clipped, once; the norm of bfloat16
+gradients is not rounded to bfloat16.
+
+DTensor gradients (FSDP2) are normed by their local shards, the sums joined by
+an all-reduce over the mesh dimensions that they are sharded over.
+"""
+
+from __future__ import annotations
+
+import ctypes
+import functools
+import math
+from typing import Iterable, List, Optional, Union
+
+import numpy as np
+import torch
+
+from . import _lib as L
+
+_GRAD_CODES = {torch.float32: L.GRAD_F32, torch.bfloat16: L.GRAD_BF16, torch.float16: L.GRAD_F16}
+_NORMS = {2.0: L.NORM_L2, 1.0: L.NORM_L1, math.inf: L.NORM_INF}
+_Tensors = Union[torch.Tensor, Iterable[torch.Tensor]]
+
+
+def _norm_code(norm_type) -> int:
+    code = _NORMS.get(float(norm_type))
+    if code is None:
+        raise ValueError(f"Invalid norm_type: {norm_type}. Expected 1, 2 or inf")
+    return code
+
+
+def _max_norm(max_norm) -> float:
+    max_norm = float(max_norm)
+    if not max_norm >= 0.0:
+        raise ValueError(f"Invalid max_norm: {max_norm}")
+    return max_norm
+
+
+class _Batch:
+    """Dense gradients on one device as the rows of one call."""
+
+    def __init__(self, rows: np.ndarray, device: torch.device, hold=None):
+        self.rows = rows
+        self.device = device
+        self.hold = hold      # keeps tensors alive that only the rows point to
+
+    def args(self, norm: int, max_norm: float, total: Optional[torch.Tensor],
+             power: Optional[torch.Tensor] = None) -> L.NormArgs:
+        """The call's arguments, with a workspace (and, for a long list, a
+        device copy of the rows) of their own."""
+        partials = torch.empty(L.NORM_PARTIALS, dtype=torch.float64, device=self.device)
+        table, n = None, len(self.rows)
+        if n > L.GRADS_INLINE and not torch.cuda.is_current_stream_capturing():
+            host = torch.empty(self.rows.nbytes, dtype=torch.uint8, pin_memory=True)
+            ctypes.memmove(host.data_ptr(), self.rows.ctypes.data, self.rows.nbytes)
+            table = host.to(self.device, non_blocking=True)
+        self.keep = (partials, table)
+        return L.NormArgs(
+            grads=self.rows.ctypes.data, table=None if table is None else table.data_ptr(), n=n,
+            norm=norm, max_norm=max_norm, partials=partials.data_ptr(),
+            total=None if total is None else total.data_ptr(),
+            power=None if power is None else power.data_ptr())
+
+    def call(self, name: str, args: L.NormArgs) -> None:
+        lib = L.load()
+        with torch.cuda.device(self.device):
+            stream = torch.cuda.current_stream(self.device).cuda_stream
+            L.check(getattr(lib, name)(ctypes.byref(args), stream), name)
+
+
+@functools.lru_cache(maxsize=1)
+def _host():
+    return L.load_host()
+
+
+def _as_list(tensors: _Tensors) -> List[torch.Tensor]:
+    if isinstance(tensors, torch.Tensor):
+        return [tensors]
+    return tensors if type(tensors) is list else list(tensors)
+
+
+def _quick(tensors, of_grad: bool, apart: bool) -> Optional[_Batch]:
+    """The rows by the host module, where every gradient can be taken as it is."""
+    host = _host()
+    got = None if host is None else host.grad_rows(tensors, of_grad, apart)
+    if got is None:
+        return None
+    data, device = got
+    return _Batch(np.frombuffer(data, dtype=L.GRAD_DTYPE), torch.device("cuda", max(device, 0)))
+
+
+def _rows(grads, device) -> np.ndarray:
+    rows = np.zeros(len(grads), dtype=L.GRAD_DTYPE)
+    rows["data"] = [g.data_ptr() for g in grads]
+    rows["numel"] = [g.numel() for g in grads]
+    rows["dtype"] = [_GRAD_CODES[g.dtype] for g in grads]
+    tiles = (rows["numel"] + L.GRAD_TILE - 1) // L.GRAD_TILE
+    if tiles.sum() >= 2**31:
+        raise ValueError("luma_amd: too many gradient elements for one call")
+    rows["first_tile"] = np.cumsum(tiles) - tiles
+    return rows
+
+
+def _shard_dims(t) -> tuple:
+    """The mesh dimensions over which a DTensor's elements are spread."""
+    dims = []
+    for d, place in enumerate(t.placements):
+        if place.is_partial():
+            raise ValueError("luma_amd: the norm of a DTensor with a Partial placement needs its "
+                             "sum: redistribute it first")
+        if place.is_shard():
+            dims.append(d)
+    return tuple(dims)
+
+
+class _Slow:
+    """Any gradients that torch knows: DTensors by their local shards, those
+    that are not dense by a copy."""
+
+    def __init__(self, grads, apart: bool):
+        if apart:     # a gradient listed twice is one gradient
+            grads = list({id(g): g for g in grads}.values())
+        self.copies = []        # (a gradient that is not dense, its dense copy)
+        self.sharded = {}       # (mesh, its dimensions) or None -> local gradients
+        device = None
+        for g in grads:
+            key = None
+            if hasattr(g, "_local_tensor") and hasattr(g, "device_mesh"):
+                dims = _shard_dims(g)
+                key = (g.device_mesh, dims) if dims else None
+                g = g._local_tensor
+            if g.is_sparse or g.layout != torch.strided:
+                raise RuntimeError("luma_amd: sparse gradients are not supported")
+            if not g.is_cuda:
+                raise RuntimeError("luma_amd: gradients must be on a ROCm GPU; got device "
+                                   f"{g.device}")
+            if g.dtype not in _GRAD_CODES:
+                raise ValueError(f"luma_amd: gradient dtype {g.dtype} is not "
+                                 "float32/bfloat16/float16")
+            device = device or g.device
+            if g.device != device:
+                raise RuntimeError("luma_amd: all gradients must be on one device "
+                                   f"({device} vs {g.device})")
+            if not _is_dense(g):
+                dense = g.contiguous()
+                self.copies.append((g, dense))
+                g = dense
+            self.sharded.setdefault(key, []).append(g)
+        self.device = device
+        self.batches = [(key, _Batch(_rows([g for g in gs if g.numel()], device), device, gs))
+                        for key, gs in self.sharded.items()]
+        if apart:
+            _check_apart([g for gs in self.sharded.values() for g in gs if g.numel()])
+
+    def norm(self, code: int) -> torch.Tensor:
+        powers = []
+        for key, batch in self.batches:
+            power = torch.zeros((), dtype=torch.float64, device=self.device)
+            if len(batch.rows):
+                batch.call("luma_grad_norm", batch.args(code, 0.0, None, power))
+            if key is not None:
+                _join_shards(power, code, *key)
+            powers.append(power)
+        if code == L.NORM_INF:
+            return torch.stack(powers).amax().float()
+        power = torch.stack(powers).sum()
+        return (power.sqrt() if code == L.NORM_L2 else power).float()
+
+    def scale(self, max_norm: float, total: torch.Tensor) -> None:
+        for _, batch in self.batches:
+            if len(batch.rows):
+                batch.call("luma_grad_scale", batch.args(L.NORM_L2, max_norm, total))
+        for g, dense in self.copies:
+            g.copy_(dense)
+
+
+def _is_dense(t: torch.Tensor) -> bool:
+    """Whether the elements fill one run of memory, each once, in any order."""
+    if t.is_neg() or t._is_zerotensor():
+        return False
+    span = 1
+    for size, stride in sorted(((n, s) for n, s in zip(t.shape, t.stride()) if n != 1),
+                               key=lambda d: d[1]):
+        if stride != span:
+            return t.numel() == 0
+        span *= size
+    return True
+
+
+def _check_apart(grads) -> None:
+    spans = sorted((g.data_ptr(), g.data_ptr() + g.numel() * g.element_size()) for g in grads)
+    if any(a[1] > b[0] for a, b in zip(spans, spans[1:])):
+        raise ValueError("luma_amd: gradients that share memory cannot be clipped in place")
+
+
+def _join_shards(power: torch.Tensor, code: int, mesh, dims) -> None:
+    """The power over all shards: summed (the largest one for inf) along each
+    of the mesh's dimensions."""
+    import torch.distributed as dist
+
+    op = dist.ReduceOp.MAX if code == L.NORM_INF else dist.ReduceOp.SUM
+    for d in dims:
+        dist.all_reduce(power, op=op, group=mesh.get_group(d))
+
+
+def _grads(params) -> List[torch.Tensor]:
+    return [p.grad for p in params if p.grad is not None]
+
+
+def _check_finite(total: torch.Tensor, norm_type) -> None:
+    if not torch.isfinite(total):
+        raise RuntimeError(
+            f"The total norm of order {float(norm_type)} for gradients from `parameters` is "
+            "non-finite, so it cannot be clipped. To disable this error and scale the gradients "
+            "by the non-finite norm anyway, set `error_if_nonfinite=False`")
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def get_total_norm(tensors: _Tensors, norm_type: float = 2.0, error_if_nonfinite: bool = False,
+                   foreach: Optional[bool] = None) -> torch.Tensor:
+    """The norm of all elements of all tensors together (``norm_type`` 1, 2 or
+    inf), as a float32 scalar on their device.  ``foreach`` is accepted for
+    torch's signature and selects nothing."""
+    code = _norm_code(norm_type)
+    tensors = _as_list(tensors)
+    batch = _quick(tensors, False, False)
+    if batch is not None:
+        if not len(batch.rows):
+            return torch.tensor(0.0)
+        total = torch.empty((), dtype=torch.float32, device=batch.device)
+        batch.call("luma_grad_norm", batch.args(code, 0.0, total))
+    else:
+        total = _Slow(tensors, False).norm(code)
+    if error_if_nonfinite:
+        _check_finite(total, norm_type)
+    return total
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def clip_grad_norm_(parameters: _Tensors, max_norm: float, norm_type: float = 2.0,
+                    error_if_nonfinite: bool = False,
+                    foreach: Optional[bool] = None) -> torch.Tensor:
+    """Scales the parameters' gradients in place by
+    ``min(1, max_norm / (norm + 1e-6))``, ``norm`` being the norm of all of
+    them together, which is returned (a float32 scalar on their device).  A norm
+    that is not finite scales by 0 or NaN, as in torch, unless
+    ``error_if_nonfinite``, which waits for the norm and raises."""
+    code = _norm_code(norm_type)
+    max_norm = _max_norm(max_norm)
+    parameters = _as_list(parameters)
+    batch = _quick(parameters, True, True)
+    if batch is not None and not error_if_nonfinite:
+        if not len(batch.rows):
+            return torch.tensor(0.0)
+        total = torch.empty((), dtype=torch.float32, device=batch.device)
+        batch.call("luma_grad_clip", batch.args(code, max_norm, total))
+        return total
+    grads = _grads(parameters)
+    if not grads:
+        return torch.tensor(0.0)
+    slow = _Slow(grads, True)
+    total = slow.norm(code)
+    if error_if_nonfinite:
+        _check_finite(total, norm_type)
+    slow.scale(max_norm, total)
+    return total
+
+
+@torch.compiler.disable
+@torch.no_grad()
+def clip_grads_with_norm_(parameters: _Tensors, max_norm: float, total_norm: torch.Tensor,
+                          foreach: Optional[bool] = None) -> None:
+    """The scaling of ``clip_grad_norm_`` by a norm that is known already (a
+    one-element tensor, e.g. ``get_total_norm``'s)."""
+    max_norm = _max_norm(max_norm)
+    parameters = _as_list(parameters)
+    if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1:
+        raise ValueError("clip_grads_with_norm_: total_norm must be a one-element tensor")
+    batch = _quick(parameters, True, True)
+    if batch is not None:
+        if len(batch.rows):
+            total = total_norm.to(device=batch.device, dtype=torch.float32)
+            batch.call("luma_grad_scale", batch.args(L.NORM_L2, max_norm, total))
+        return
+    grads = _grads(parameters)
+    if grads:
+        slow = _Slow(grads, True)
+        slow.scale(max_norm, total_norm.to(device=slow.device, dtype=torch.float32))

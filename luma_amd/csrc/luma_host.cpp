@@ -394,8 +394,127 @@ void bump_steps(py::list states) {
   }
 }
 
+// The gradients of a list of tensors, or the tensors themselves, as rows of the
+// C ABI's LumaGrad table (the walk of check_range: in stages, with prefetch).
+struct GradRow {
+  uint64_t data;
+  int64_t numel;
+  int32_t dtype, first_tile;
+};
+static_assert(sizeof(GradRow) == 24, "LumaGrad");
+constexpr int64_t kGradTile = 2048;   // LUMA_GRAD_TILE
+
+// One part's rows; false for a tensor that the kernels cannot take as it is.
+// *device: the CUDA device of all of them (-1 before the first).
+bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<GradRow> &rows,
+                int64_t *device) noexcept {
+  try {
+    std::vector<const c10::TensorImpl *> impl(n);
+    for (int64_t i = 0; i < n; ++i) {
+      if (i + kAhead < n) prefetch(objs[i + kAhead]);
+      if (Py_TYPE(objs[i]) != g_tensor_type && Py_TYPE(objs[i]) != g_param_type) return false;
+      impl[i] = THPVariable_Unpack(objs[i]).unsafeGetTensorImpl();
+    }
+    if (of_grad) {
+      std::vector<const c10::AutogradMetaInterface *> meta(n);
+      for (int64_t i = 0; i < n; ++i) {
+        if (i + kAhead < n) prefetch_impl(impl[i + kAhead]);
+        meta[i] = impl[i]->autograd_meta();
+      }
+      for (int64_t i = 0; i < n; ++i) {
+        if (i + kAhead < n && meta[i + kAhead]) {
+          prefetch(meta[i + kAhead]);
+          prefetch(reinterpret_cast<const char *>(meta[i + kAhead]) + 64);
+        }
+        impl[i] = nullptr;
+        if (meta[i]) {
+          const at::Tensor &grad = meta[i]->grad();
+          if (grad.defined()) impl[i] = grad.unsafeGetTensorImpl();
+        }
+      }
+    }
+    rows.reserve(n);
+    for (int64_t i = 0; i < n; ++i) {
+      if (i + kAhead < n && impl[i + kAhead]) prefetch_impl(impl[i + kAhead]);
+      const c10::TensorImpl *g = impl[i];
+      if (!g) continue;
+      if (g->key_set().has(c10::DispatchKey::Python) ||
+          g->key_set().has(c10::DispatchKey::PythonTLSSnapshot) || !g->is_cuda() ||
+          g->layout() != at::kStrided || g->is_neg() || !g->has_storage())
+        return false;
+      const int code = grad_code(g->dtype().toScalarType());
+      if (code < 0 || !g->is_non_overlapping_and_dense()) return false;
+      if (*device >= 0 && g->device().index() != *device) return false;
+      *device = g->device().index();
+      if (g->numel() == 0) continue;
+      const uint64_t p = (uint64_t)(uintptr_t)g->data();
+      if (!p) return false;
+      rows.push_back({p, g->numel(), code, 0});
+    }
+    return true;
+  } catch (...) {
+    return false;   // an unusual tensor: the caller looks at it
+  }
+}
+
+// Whether no two rows share memory.
+bool disjoint(const std::vector<GradRow> &rows) {
+  auto bytes = [](const GradRow &r) { return (uint64_t)r.numel * (r.dtype == 0 ? 4 : 2); };
+  bool up = true, down = true;
+  for (size_t i = 1; i < rows.size() && (up || down); ++i) {
+    up &= rows[i - 1].data + bytes(rows[i - 1]) <= rows[i].data;
+    down &= rows[i].data + bytes(rows[i]) <= rows[i - 1].data;
+  }
+  if (up || down) return true;
+  std::vector<std::pair<uint64_t, uint64_t>> spans(rows.size());
+  for (size_t i = 0; i < rows.size(); ++i)
+    spans[i] = {rows[i].data, rows[i].data + bytes(rows[i])};
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    if (spans[i].first < spans[i - 1].second) return false;
+  return true;
+}
+
+// (rows as bytes, device index) of the tensors in objs (of_grad: of their
+// gradients, those without one left out), or None when one of them is a
+// subclass, sparse, not dense, of another type or device, or (apart) shares
+// memory with another: the caller then looks at each.  device is -1 for none.
+py::object grad_rows(py::list objs, bool of_grad, bool apart) {
+  const int64_t n = (int64_t)objs.size();
+  PyObject *const *o = n ? &PyList_GET_ITEM(objs.ptr(), 0) : nullptr;
+  const int T = (int)std::min<int64_t>(kMaxThreads, std::max<int64_t>(1, n / kPerThread));
+  std::vector<std::vector<GradRow>> part(T);
+  std::vector<int64_t> device(T, -1);
+  std::vector<char> ok(T, 0);
+  const std::function<void(int)> job = [&](int t) {
+    const int64_t a = n * t / T, b = n * (t + 1) / T;
+    ok[t] = grad_range(o + a, b - a, of_grad, part[t], &device[t]);
+  };
+  if (T == 1)
+    job(0);
+  else
+    Pool::get().run(T, job);
+  int64_t dev = -1;
+  std::vector<GradRow> &rows = part[0];
+  for (int t = 0; t < T; ++t) {
+    if (!ok[t] || (device[t] >= 0 && dev >= 0 && device[t] != dev)) return py::none();
+    if (device[t] >= 0) dev = device[t];
+    if (t) rows.insert(rows.end(), part[t].begin(), part[t].end());
+  }
+  int64_t tiles = 0;
+  for (GradRow &r : rows) {
+    if (tiles > INT32_MAX) return py::none();
+    r.first_tile = (int32_t)tiles;
+    tiles += (r.numel - 1) / kGradTile + 1;
+  }
+  if (apart && !disjoint(rows)) return py::none();
+  return py::make_tuple(
+      py::bytes(reinterpret_cast<const char *>(rows.data()), rows.size() * sizeof(GradRow)), dev);
+}
+
 PYBIND11_MODULE(_luma_host, m) {
-  m.doc() = "Host-side bookkeeping of LUMA.step (pointer refresh of a planned step).";
+  m.doc() = "Host-side bookkeeping of LUMA.step (pointer refresh of a planned step) and of the "
+            "gradient norm (its table).";
   py::object torch = py::module_::import("torch");
   g_tensor_type = reinterpret_cast<PyTypeObject *>(torch.attr("Tensor").ptr());
   g_param_type = reinterpret_cast<PyTypeObject *>(torch.attr("nn").attr("Parameter").ptr());
@@ -408,6 +527,7 @@ PYBIND11_MODULE(_luma_host, m) {
         py::arg("device"), py::arg("cands") = py::none());
   m.def("same_pointers", &same_pointers);
   m.def("bump_steps", &bump_steps);
+  m.def("grad_rows", &grad_rows);
   // the torch whose headers this module was compiled against: it reads
   // TensorImpl fields in that version's inline layout
   m.attr("torch_version") = LUMA_TORCH_VERSION;

@@ -45,6 +45,7 @@
 #include <string.h>
 
 #include "../../include/luma.h"
+#include "luma_error.h"
 #include "luma_exact.h"
 #include "luma_fast.h"
 #include "luma_philox.h"
@@ -3011,7 +3012,9 @@ static float *g_scratch_ptr[kMaxDevices] = {};
 
 static thread_local char g_err[512] = "";
 
-static int fail(const char *msg, hipError_t e = hipSuccess) {
+namespace luma {
+
+int fail(const char *msg, hipError_t e) {
   if (e != hipSuccess)
     snprintf(g_err, sizeof(g_err), "%s: %s", msg, hipGetErrorString(e));
   else
@@ -3019,10 +3022,12 @@ static int fail(const char *msg, hipError_t e = hipSuccess) {
   return e != hipSuccess ? (int)e : -1;
 }
 
-static int check_launch(const char *what) {
+int check_launch(const char *what) {
   const hipError_t e = hipGetLastError();
   return e == hipSuccess ? 0 : fail(what, e);
 }
+
+}  // namespace luma
 
 extern "C" {
 
