@@ -46,6 +46,10 @@
  *                      -- torch.nn.utils.get_total_norm, clip_grad_norm_ and
  *                         clip_grads_with_norm_ as the reference's benchmark
  *                         uses them around its step (no kernel of its own).
+ *   luma_xent_forward, luma_xent_backward
+ *                      -- torch.nn.functional.cross_entropy of a linear
+ *                         layer's outputs, as the reference's benchmark
+ *                         trains on (no kernel of its own).
  *   luma_philox4x32    -- host-side Philox4x32-10 block function used by the
  *                         stochastic rounding (Salmon et al., SC'11); the
  *                         reference's Triton path draws from tl.rand
@@ -430,6 +434,51 @@ int luma_grad_clip(const LumaNormArgs *args, void *stream);
 
 /* The second half of luma_grad_clip, with the norm that *total holds. */
 int luma_grad_scale(const LumaNormArgs *args, void *stream);
+
+/*
+ * The cross entropy of a vocabulary's logits, without the logits.
+ *
+ * For token i with hidden state x_i, target t_i and the weight's rows w_j:
+ *   l_ij = x_i . w_j,  lse_i = log sum_j exp(l_ij),  loss_i = lse_i - l_i,t_i
+ * and for the gradient g_i of loss_i
+ *   D_ij = g_i (exp(l_ij - lse_i) - [j = t_i]),  d_hidden = D W,  d_weight = D^T X.
+ * The logits are formed tile by tile on the matrix cores and never written; the
+ * backward forms them again and keeps D for one piece of the vocabulary at a
+ * time, in the operands' type.  The reference's benchmark takes torch's cross
+ * entropy of whole logits (benchmarks/bench_nanogpt.py).
+ *
+ * A target equal to ignore_index has loss 0 and gradient 0, and does not count
+ * in the mean; any other target outside [0, v) has loss (and gradients) NaN.
+ */
+#define LUMA_XENT_NONE 0   /* loss[n]                                              */
+#define LUMA_XENT_SUM 1    /* loss[1]                                              */
+#define LUMA_XENT_MEAN 2   /* loss[1], over the targets that are not ignored       */
+
+typedef struct LumaXentArgs {
+  const void *hidden;    /* device [n][h], rows ld_hidden elements apart         */
+  const void *weight;    /* device [v][h], rows ld_weight elements apart         */
+  const int64_t *target; /* device [n]                                           */
+  int64_t n, h, v;       /* each >= 1                                            */
+  int64_t ld_hidden, ld_weight;
+  int64_t ignore_index;
+  int32_t dtype;         /* LUMA_GRAD_*: both operands and both gradients        */
+  int32_t reduction;     /* LUMA_XENT_*                                          */
+  float *loss;           /* forward: device [n] or [1]                           */
+  float *stats;          /* device [n + 1]: each token's lse, then the number of
+                            targets that count; the forward writes it, the
+                            backward reads it                                    */
+  const float *grad_loss;/* backward: device [n] or [1]                          */
+  void *d_hidden;        /* backward: device [n][h] dense, or NULL               */
+  void *d_weight;        /* backward: device [v][h] dense, or NULL               */
+  void *workspace;       /* device, 256-byte aligned                             */
+  int64_t workspace_bytes;
+} LumaXentArgs;
+
+/* Bytes of workspace that the call needs (from the sizes, the type and the
+ * operands' addresses and strides); < 0: the arguments are refused. */
+int64_t luma_xent_workspace_bytes(const LumaXentArgs *args, int32_t backward);
+int luma_xent_forward(const LumaXentArgs *args, void *stream);
+int luma_xent_backward(const LumaXentArgs *args, void *stream);
 
 /* Host: one Philox4x32-10 block. */
 void luma_philox4x32(const uint32_t ctr[4], const uint32_t key[2], uint32_t out[4]);

@@ -31,6 +31,7 @@ NORM_PARTIALS = 1024         # LUMA_NORM_PARTIALS
 
 GRAD_F32, GRAD_BF16, GRAD_F16 = 0, 1, 2
 NORM_L2, NORM_L1, NORM_INF = 0, 1, 2
+XENT_NONE, XENT_SUM, XENT_MEAN = 0, 1, 2
 NOISE_PHILOX, NOISE_INJECTED = 0, 1
 FLAG_EXACT_ONLY = 1
 FLAG_SPLIT = 2               # LUMA_FLAG_SPLIT
@@ -98,6 +99,30 @@ class NormArgs(ctypes.Structure):
     ]
 
 
+class XentArgs(ctypes.Structure):
+    """LumaXentArgs."""
+    _fields_ = [
+        ("hidden", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("target", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("h", ctypes.c_int64),
+        ("v", ctypes.c_int64),
+        ("ld_hidden", ctypes.c_int64),
+        ("ld_weight", ctypes.c_int64),
+        ("ignore_index", ctypes.c_int64),
+        ("dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("loss", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("grad_loss", ctypes.c_void_p),
+        ("d_hidden", ctypes.c_void_p),
+        ("d_weight", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 class LumaLibraryError(RuntimeError):
     pass
 
@@ -130,6 +155,9 @@ _SIGNATURES = {
     "luma_grad_norm": (ctypes.c_int, [ctypes.POINTER(NormArgs), _VP]),
     "luma_grad_clip": (ctypes.c_int, [ctypes.POINTER(NormArgs), _VP]),
     "luma_grad_scale": (ctypes.c_int, [ctypes.POINTER(NormArgs), _VP]),
+    "luma_xent_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(XentArgs), ctypes.c_int32]),
+    "luma_xent_forward": (ctypes.c_int, [ctypes.POINTER(XentArgs), _VP]),
+    "luma_xent_backward": (ctypes.c_int, [ctypes.POINTER(XentArgs), _VP]),
     "luma_philox4x32": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32),
                                ctypes.POINTER(ctypes.c_uint32)]),
 }

@@ -24,7 +24,8 @@ ROOT = os.path.dirname(HERE)
 # (source, units): luma_step.hip is compiled once per LUMA_UNIT, side by side
 # (its fast kernels take 1 to 4 minutes each)
 SOURCES = [(os.path.join(HERE, "csrc", "luma_step.hip"), (3, 2, 1, 0)),
-           (os.path.join(HERE, "csrc", "luma_norm.hip"), (0,))]
+           (os.path.join(HERE, "csrc", "luma_norm.hip"), (0,)),
+           (os.path.join(HERE, "csrc", "luma_xent.hip"), (0,))]
 
 OUT = os.path.join(HERE, "libluma_hip.so")
 HOST_SOURCE = os.path.join(HERE, "csrc", "luma_host.cpp")

@@ -1,0 +1,657 @@
+// Cross entropy over a vocabulary without the logits (include/luma.h,
+// luma_xent_forward / luma_xent_backward).
+//
+// Forward:   logits tile by tile (W X^T, vocabulary along the accumulators'
+//            rows, so that a lane holds many words of one token), and from each
+//            tile, in registers, every token's largest logit, its sum of
+//            exp(l - largest), and the target's logit; then a join over the
+//            vocabulary's tiles.
+// Backward:  for each piece of the vocabulary: the logits again, from them
+//            D = r_i (exp(l - lse_i) - [target]) in the operands' type; then
+//            d_weight's rows of the piece = D^T X and d_hidden += D W.
+//            r_i is the token's gradient times a power of two that brings the
+//            largest to about 2^kTop (float16's range is short); the products
+//            are scaled back in float32, which is exact.
+#include <hip/hip_fp16.h>
+#include <hip/hip_runtime.h>
+
+#include "../../include/luma.h"
+#include "luma_error.h"
+#include "luma_gemm.h"
+
+namespace luma {
+namespace {
+
+using namespace gemm;
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr float kLn2 = 0.69314718055994530942f;
+
+template <int DT>
+struct Elem;
+template <>
+struct Elem<LUMA_GRAD_F32> {
+  typedef float type;
+  static __device__ __forceinline__ float round(float f) { return f; }
+};
+template <>
+struct Elem<LUMA_GRAD_BF16> {
+  typedef __bf16 type;
+  static __device__ __forceinline__ __bf16 round(float f) { return (__bf16)f; }
+};
+template <>
+struct Elem<LUMA_GRAD_F16> {
+  typedef _Float16 type;
+  static __device__ __forceinline__ _Float16 round(float f) { return (_Float16)f; }
+};
+
+template <int DT>
+using Four = typename Elem<DT>::type __attribute__((ext_vector_type(4), aligned(2)));
+
+// Stores four consecutive elements of a row, those before `end`.
+template <int DT>
+__device__ __forceinline__ void store4(typename Elem<DT>::type *p, int64_t at, int64_t end, v4f f) {
+  if (at + 4 <= end) {
+    Four<DT> o;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) o[r] = Elem<DT>::round(f[r]);
+    if constexpr (DT == LUMA_GRAD_F32) {
+      typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
+      *(v4fu *)(p + at) = v4fu{o[0], o[1], o[2], o[3]};
+    } else {
+      *(Four<DT> *)(p + at) = o;
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+      if (at + r < end) p[at + r] = Elem<DT>::round(f[r]);
+  }
+}
+
+struct Grid {
+  int tiles_m, tiles_n, splits;
+};
+
+// This lane's place in the accumulators of its wavefront: acc[i][j][r] is row
+// m + 16 i + r and column n + 16 j.
+template <typename S>
+struct Place {
+  int64_t m, n;
+  __device__ __forceinline__ Place(int tm, int tn) {
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    m = (int64_t)tm * S::BM + (wave / S::WN) * S::TM * 16 + (lane >> 4) * 4;
+    n = (int64_t)tn * S::BN + (wave % S::WN) * S::TN * 16 + (lane & 15);
+  }
+};
+
+template <typename S>
+__device__ __forceinline__ void clear(v4f (&acc)[S::TM][S::TN]) {
+#pragma unroll
+  for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+    for (int j = 0; j < S::TN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
+}
+
+// -- forward --------------------------------------------------------------------
+
+// Every token's (largest logit, sum of exp(l - largest)) over each wavefront's
+// words: part[tile of words][token]; picked[token] = the target's logit.
+template <int DT, typename S>
+__global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand x, int64_t v,
+                                                             int64_t n, int64_t h,
+                                                             const int64_t *target, Grid g,
+                                                             float2 *part, float *picked) {
+  int tm, tn, split;
+  tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
+  v4f acc[S::TM][S::TN];
+  clear<S>(acc);
+  product<DT, kAlongK, kAlongK, S>(w, x, (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0, h, acc);
+  const Place<S> at(tm, tn);
+  const bool whole = (int64_t)(tm + 1) * S::BM <= v;
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int j = 0; j < S::TN; ++j) {
+    const int64_t token = at.n + 16 * j;
+    const int64_t t = token < n ? target[token] : -1;
+    const int64_t d = t - at.m;                  // the target's word from this lane's first
+    if (t >= 0 && t < v && d >= 0 && d < 16 * S::TM && (d & 15) < 4) {
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (d == 16 * i + r) picked[token] = acc[i][j][r];
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        if (!whole && at.m + 16 * i + r >= v) acc[i][j][r] = -__builtin_inff();
+        top = fmaxf(top, acc[i][j][r]);
+      }
+    top = fmaxf(top, __shfl_xor(top, 16));
+    top = fmaxf(top, __shfl_xor(top, 32));
+    // (all -inf: their exponentials are 0 and not NaN)
+    const float base = (top == -__builtin_inff() ? 0.0f : top) * kLog2e;
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -base));
+    sum += __shfl_xor(sum, 16);
+    sum += __shfl_xor(sum, 32);
+    if (lane < 16 && token < n) {
+      const int wm = (threadIdx.x >> 6) / S::WN;
+      part[((int64_t)tm * S::WM + wm) * n + token] = make_float2(top, sum);
+    }
+  }
+}
+
+constexpr int kJoinTokens = 32, kJoinSlices = 32, kJoinThreads = kJoinTokens * kJoinSlices;
+
+// (largest, sum) of two sets of words together.
+__device__ __forceinline__ float2 join(float2 a, float2 b) {
+  const float top = fmaxf(a.x, b.x);
+  if (top == -__builtin_inff()) return make_float2(top, a.y + b.y);
+  return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - top) * kLog2e) +
+                              b.y * __builtin_amdgcn_exp2f((b.x - top) * kLog2e));
+}
+
+// Each token's lse and loss from its `parts` records; with a reduction, each
+// workgroup's sums (in float64) of the losses and of the targets that count.
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2 *part, int parts,
+                                                            const float *picked,
+                                                            const int64_t *target, int64_t n,
+                                                            int64_t v, int64_t ignore,
+                                                            float *stats, float *loss,
+                                                            double2 *sums) {
+  __shared__ float2 lds[kJoinSlices][kJoinTokens + 1];
+  const int tok = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
+  const int64_t token = (int64_t)blockIdx.x * kJoinTokens + tok;
+  float2 a = make_float2(-__builtin_inff(), 0.0f);
+  if (token < n)
+    for (int p = slice; p < parts; p += kJoinSlices) a = join(a, part[(int64_t)p * n + token]);
+  lds[slice][tok] = a;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;      // (the rest is the first wavefront's)
+  double value = 0.0, count = 0.0;
+  if (slice == 0) {
+    for (int s = 1; s < kJoinSlices; ++s) a = join(a, lds[s][tok]);
+    if (token < n) {
+      const float lse = a.x == -__builtin_inff() ? __builtin_nanf("")
+                                                 : a.x + __builtin_amdgcn_logf(a.y) * kLn2;
+      const int64_t t = target[token];
+      float l = 0.0f;
+      if (t != ignore) {
+        l = t >= 0 && t < v ? lse - picked[token] : __builtin_nanf("");
+        count = 1.0;
+      }
+      stats[token] = lse;
+      if (!sums) loss[token] = l;
+      value = (double)l;
+    }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    value += __shfl_xor(value, o);
+    count += __shfl_xor(count, o);
+  }
+  if (sums && threadIdx.x == 0) sums[blockIdx.x] = make_double2(value, count);
+}
+
+// The loss from the workgroups' sums.
+__global__ __launch_bounds__(256) void reduce_kernel(const double2 *sums, int64_t count,
+                                                     int reduction, float *stats_n, float *loss) {
+  __shared__ double2 lds[4];
+  double a = 0.0, b = 0.0;
+  for (int64_t i = threadIdx.x; i < count; i += 256) {
+    a += sums[i].x;
+    b += sums[i].y;
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    a += __shfl_xor(a, o);
+    b += __shfl_xor(b, o);
+  }
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = make_double2(a, b);
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  a = lds[0].x + lds[1].x + lds[2].x + lds[3].x;
+  b = lds[0].y + lds[1].y + lds[2].y + lds[3].y;
+  *stats_n = (float)b;
+  *loss = (float)(reduction == LUMA_XENT_MEAN ? a / b : a);
+}
+
+// -- backward -------------------------------------------------------------------
+
+// The header of the backward's row factors: what the products are scaled back by.
+struct Rows {
+  float back;
+  float pad[63];
+};
+
+// r_i, the gradient of each token's loss times a power of two; 0 for an ignored
+// target, NaN for one outside the vocabulary.
+template <int TOP>
+__global__ __launch_bounds__(1024) void rows_kernel(const float *grad, const int64_t *target,
+                                                    const float *stats, int64_t n, int64_t v,
+                                                    int64_t ignore, int reduction, Rows *head,
+                                                    float *rows) {
+  __shared__ float lds[16];
+  const float scale = reduction == LUMA_XENT_MEAN ? 1.0f / stats[n] : 1.0f;
+  auto value = [&](int64_t i) -> float {
+    const int64_t t = target[i];
+    if (t == ignore) return 0.0f;
+    if (t < 0 || t >= v) return __builtin_nanf("");
+    return reduction == LUMA_XENT_NONE ? grad[i] : grad[0] * scale;
+  };
+  float top = 0.0f;      // the largest finite |g|
+  for (int64_t i = threadIdx.x; i < n; i += 1024) {
+    const float a = __builtin_fabsf(value(i));
+    if (a < __builtin_inff()) top = fmaxf(top, a);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor(top, o));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = top;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < 16; ++w) top = fmaxf(top, lds[w]);
+  int e = 0;
+  if (top > 0.0f) {
+    __builtin_frexpf(top, &e);           // top = f 2^e, f in [0.5, 1)
+    e = TOP - e;
+    e = e > 100 ? 100 : e < -100 ? -100 : e;
+  }
+  const float up = __builtin_ldexpf(1.0f, e);
+  for (int64_t i = threadIdx.x; i < n; i += 1024) rows[i] = value(i) * up;
+  if (threadIdx.x == 0) head->back = __builtin_ldexpf(1.0f, -e);
+}
+
+// D of words [v0, v0 + tiles_m BM), 0 past the vocabulary: d[token][word - v0].
+template <int DT, typename S>
+__global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x, int64_t v0,
+                                                            int64_t v, int64_t n, int64_t h,
+                                                            const int64_t *target,
+                                                            const float *stats, const float *rows,
+                                                            Grid g, typename Elem<DT>::type *d,
+                                                            int64_t ld) {
+  int tm, tn, split;
+  tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
+  v4f acc[S::TM][S::TN];
+  clear<S>(acc);
+  product<DT, kAlongK, kAlongK, S>(w, x, v0 + (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0, h, acc);
+  const Place<S> at(tm, tn);
+#pragma unroll
+  for (int j = 0; j < S::TN; ++j) {
+    const int64_t token = at.n + 16 * j;
+    if (token >= n) continue;
+    const float base = stats[token] * kLog2e, row = rows[token];
+    const int64_t t = target[token] - v0 - at.m;
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i) {
+      v4f f;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -base));
+        if (t == 16 * i + r) p -= 1.0f;
+        // (an ignored token's logits may be anything)
+        f[r] = row == 0.0f || v0 + at.m + 16 * i + r >= v ? 0.0f : p * row;
+      }
+      store4<DT>(d + token * ld, at.m + 16 * i, ld, f);
+    }
+  }
+}
+
+// A product into float32 (out[split][n][m], added to what is there with `add`)
+// or, with out16, times *back into the operands' type.
+template <int DT, int AB, typename S>
+__global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand b, int64_t m,
+                                                              int64_t n, int64_t k,
+                                                              int64_t k_split, Grid g, int add,
+                                                              float *out, const float *back,
+                                                              typename Elem<DT>::type *out16) {
+  int tm, tn, split;
+  tile_of(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
+  const int64_t k0 = split * k_split, k1 = min(k, k0 + k_split);
+  v4f acc[S::TM][S::TN];
+  clear<S>(acc);
+  product<DT, kAlongM, AB, S>(a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
+  const Place<S> at(tm, tn);
+  const float f = out16 ? *back : 1.0f;
+#pragma unroll
+  for (int j = 0; j < S::TN; ++j) {
+    const int64_t row = at.n + 16 * j;
+    if (row >= n) continue;
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i) {
+      const int64_t col = at.m + 16 * i;
+      if (out16) {
+        store4<DT>(out16 + row * m, col, m, acc[i][j] * f);
+      } else {
+        float *o = out + (int64_t)split * n * m + row * m;
+        v4f c = acc[i][j];
+        if (add)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (col + r < m) c[r] += o[col + r];
+        store4<LUMA_GRAD_F32>(o, col, m, c);
+      }
+    }
+  }
+}
+
+// The sum of `splits` float32 products, times *back, in the operands' type.
+template <int DT>
+__global__ __launch_bounds__(256) void sum_kernel(const float *part, int splits, int64_t count,
+                                                  const float *back,
+                                                  typename Elem<DT>::type *out) {
+  const float f = *back;
+  for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < count; i += gridDim.x * 1024ll) {
+    v4f s = {0.f, 0.f, 0.f, 0.f};
+    for (int k = 0; k < splits; ++k) {
+      const float *p = part + k * count + i;
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (i + r < count) s[r] += p[r];
+    }
+    store4<DT>(out, i, count, s * f);
+  }
+}
+
+// A copy of a strided matrix with rows of `ld` elements, zeros past its columns.
+template <typename T>
+__global__ __launch_bounds__(256) void pack_kernel(const T *in, int64_t rows, int64_t cols,
+                                                   int64_t ld_in, T *out, int64_t ld) {
+  for (int64_t i = blockIdx.x * 256ll + threadIdx.x; i < rows * ld; i += gridDim.x * 256ll) {
+    const int64_t r = i / ld, c = i % ld;
+    out[i] = c < cols ? in[r * ld_in + c] : (T)0;
+  }
+}
+
+// -- host -----------------------------------------------------------------------
+
+typedef Shape<8, 4, 2, 4> Big;       // 256 x 256
+typedef Shape<4, 4, 2, 2> Mid;       // 128 x 128
+typedef Shape<2, 2, 2, 2> Small;     // 64 x 64
+typedef Shape<2, 4, 4, 1> Thin64;    // 128 x 64: few tokens
+typedef Shape<2, 1, 4, 1> Thin16;    // 128 x 16
+enum ShapeId { kBig, kMid, kSmall, kThin64, kThin16 };
+constexpr int kBM[] = {256, 128, 64, 128, 128}, kBN[] = {256, 128, 64, 64, 16};
+
+constexpr int64_t kPieceBytes = 256 << 20;     // of D: what the last-level cache holds
+
+int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
+int64_t tiles(int64_t x, int64_t size) { return (x + size - 1) / size; }
+
+// The tile for a product of m x n: the largest whose tiles fill the chip.
+int shape_for(int64_t m, int64_t n) {
+  if (n <= 16) return kThin16;
+  if (n <= 64) return kThin64;
+  if (tiles(m, 256) * tiles(n, 256) >= 192) return kBig;
+  if (tiles(m, 128) * tiles(n, 128) >= 128) return kMid;
+  return kSmall;
+}
+
+struct Plan {
+  int64_t size;                 // bytes of an element
+  bool pack_x, pack_w;
+  int64_t ld_x, ld_w;           // elements, of what the products read
+  int64_t at_x, at_w;           // of the packed copies
+  int logits;                   // tile shapes
+  // forward
+  int64_t parts, at_part, at_picked, at_sums, blocks;
+  // backward
+  int64_t piece, ld_d;          // words per piece; elements per row of D
+  int hidden, weight;           // tile shapes
+  int64_t hidden_splits, hidden_k, weight_splits, weight_k;
+  int64_t at_head, at_rows, at_d, at_hidden, at_weight;
+  int64_t bytes;
+};
+
+// Splits of a product over k so that its tiles fill the chip, and each one's k.
+void split_k(int shape, int64_t m, int64_t n, int64_t k, int64_t round, int64_t &splits,
+             int64_t &each) {
+  const int64_t t = tiles(m, kBM[shape]) * tiles(n, kBN[shape]);
+  const int64_t want = shape == kBig ? 256 : 1024;
+  int64_t s = t >= want / 2 ? 1 : want / t;
+  const int64_t most = tiles(k, 4 * round);
+  s = s < most ? s : most;
+  s = s < 64 ? s : 64;
+  each = up(tiles(k, s), round);
+  splits = tiles(k, each);
+}
+
+bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
+  p = Plan{};
+  p.size = a->dtype == LUMA_GRAD_F32 ? 4 : 2;
+  const int64_t group = 16 / p.size, round = (kStages * kRow) / p.size;
+  auto direct = [&](const void *q, int64_t ld, int64_t rows) {
+    return (uintptr_t)q % 16 == 0 && a->h % group == 0 && (ld % group == 0 || rows == 1);
+  };
+  p.pack_x = !direct(a->hidden, a->ld_hidden, a->n);
+  p.pack_w = !direct(a->weight, a->ld_weight, a->v);
+  p.ld_x = p.pack_x ? up(a->h, group) : a->ld_hidden;
+  p.ld_w = p.pack_w ? up(a->h, group) : a->ld_weight;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t here = at;
+    at += up(bytes, 256);
+    return here;
+  };
+  if (p.pack_x) p.at_x = take(a->n * p.ld_x * p.size);
+  if (p.pack_w) p.at_w = take(a->v * p.ld_w * p.size);
+  if (!backward) {
+    p.logits = shape_for(a->v, a->n);
+    const int wm[] = {2, 2, 2, 4, 4};
+    p.parts = tiles(a->v, kBM[p.logits]) * wm[p.logits];
+    p.blocks = tiles(a->n, kJoinTokens);
+    p.at_part = take(p.parts * a->n * sizeof(float2));
+    p.at_picked = take(a->n * sizeof(float));
+    p.at_sums = take(p.blocks * sizeof(double2));
+  } else {
+    p.piece = kPieceBytes / (a->n * p.size) / 256 * 256;
+    if (p.piece < 256) p.piece = 256;
+    if (p.piece > up(a->v, 256)) p.piece = up(a->v, 256);
+    p.logits = shape_for(p.piece < a->v ? p.piece : a->v, a->n);
+    p.ld_d = p.piece;
+    p.at_head = take(sizeof(Rows));
+    p.at_rows = take(a->n * sizeof(float));
+    p.at_d = take(a->n * p.ld_d * p.size);
+    if (a->d_hidden) {
+      p.hidden = shape_for(a->h, a->n);
+      split_k(p.hidden, a->h, a->n, p.ld_d, round, p.hidden_splits, p.hidden_k);
+      if (p.hidden_splits > 1 || p.piece < a->v)
+        p.at_hidden = take(p.hidden_splits * a->n * a->h * sizeof(float));
+    }
+    if (a->d_weight) {
+      const int64_t v = p.piece < a->v ? p.piece : a->v;
+      p.weight = shape_for(a->h, v < 65 ? 65 : v);
+      split_k(p.weight, a->h, v, a->n, round, p.weight_splits, p.weight_k);
+      if (p.weight_splits > 1) p.at_weight = take(p.weight_splits * v * a->h * sizeof(float));
+    }
+  }
+  p.bytes = at;
+  return true;
+}
+
+bool check_args(const LumaXentArgs *a, bool backward) {
+  if (!a) return fail("luma_xent: null arguments"), false;
+  if (a->n < 1 || a->h < 1 || a->v < 1) return fail("luma_xent: empty operands"), false;
+  if (a->n > INT32_MAX || a->h > 1 << 20 || a->v > INT32_MAX)
+    return fail("luma_xent: operands too large"), false;
+  if (a->dtype < LUMA_GRAD_F32 || a->dtype > LUMA_GRAD_F16)
+    return fail("luma_xent: unknown type"), false;
+  if (a->reduction < LUMA_XENT_NONE || a->reduction > LUMA_XENT_MEAN)
+    return fail("luma_xent: unknown reduction"), false;
+  if (!a->hidden || !a->weight || !a->target || !a->stats || (!backward && !a->loss) ||
+      (backward && !a->grad_loss))
+    return fail("luma_xent: null operand"), false;
+  if ((a->ld_hidden < a->h && a->n > 1) || (a->ld_weight < a->h && a->v > 1))
+    return fail("luma_xent: rows overlap"), false;
+  if (a->ld_hidden > 1 << 21 || a->ld_weight > 1 << 21)
+    return fail("luma_xent: rows too far apart"), false;
+  return true;
+}
+
+template <typename F>
+void with_shape(int shape, F f) {
+  switch (shape) {
+    case kBig: return f(Big{});
+    case kMid: return f(Mid{});
+    case kSmall: return f(Small{});
+    case kThin64: return f(Thin64{});
+    default: return f(Thin16{});
+  }
+}
+
+Grid grid_of(int shape, int64_t m, int64_t n, int64_t splits) {
+  return Grid{(int)tiles(m, kBM[shape]), (int)tiles(n, kBN[shape]), (int)splits};
+}
+
+template <int DT>
+void pack(const void *in, int64_t rows, int64_t cols, int64_t ld_in, char *out, int64_t ld,
+          hipStream_t s) {
+  typedef typename Elem<DT>::type T;
+  const int64_t blocks = tiles(rows * ld, 256 * 8);
+  pack_kernel<T><<<(int)(blocks < 8192 ? blocks : 8192), 256, 0, s>>>((const T *)in, rows, cols,
+                                                                      ld_in, (T *)out, ld);
+}
+
+// The operands as the products read them.
+template <int DT>
+void operands(const LumaXentArgs *a, const Plan &p, Operand &x, Operand &w, hipStream_t s) {
+  char *ws = (char *)a->workspace;
+  if (p.pack_x) pack<DT>(a->hidden, a->n, a->h, a->ld_hidden, ws + p.at_x, p.ld_x, s);
+  if (p.pack_w) pack<DT>(a->weight, a->v, a->h, a->ld_weight, ws + p.at_w, p.ld_w, s);
+  const int64_t bytes = up(a->h, 16 / p.size) * p.size;
+  x = Operand{p.pack_x ? ws + p.at_x : (const char *)a->hidden, p.ld_x * p.size, a->n, bytes};
+  w = Operand{p.pack_w ? ws + p.at_w : (const char *)a->weight, p.ld_w * p.size, a->v, bytes};
+}
+
+template <int DT>
+void forward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
+  Operand x, w;
+  operands<DT>(a, p, x, w, s);
+  char *ws = (char *)a->workspace;
+  float2 *part = (float2 *)(ws + p.at_part);
+  float *picked = (float *)(ws + p.at_picked);
+  double2 *sums = a->reduction == LUMA_XENT_NONE ? nullptr : (double2 *)(ws + p.at_sums);
+  with_shape(p.logits, [&](auto shape) {
+    typedef decltype(shape) S;
+    const Grid g = grid_of(p.logits, a->v, a->n, 1);
+    logits_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(w, x, a->v, a->n, a->h,
+                                                                       a->target, g, part, picked);
+  });
+  join_kernel<<<(int)p.blocks, kJoinThreads, 0, s>>>(part, (int)p.parts, picked, a->target, a->n,
+                                                     a->v, a->ignore_index, a->stats, a->loss,
+                                                     sums);
+  if (sums)
+    reduce_kernel<<<1, 256, 0, s>>>(sums, p.blocks, a->reduction, a->stats + a->n, a->loss);
+}
+
+template <int DT>
+void sum_splits(const float *part, int64_t splits, int64_t count, const float *back, void *out,
+                hipStream_t s) {
+  const int64_t blocks = tiles(count, 1024);
+  sum_kernel<DT><<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(
+      part, (int)splits, count, back, (typename Elem<DT>::type *)out);
+}
+
+template <int DT>
+void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
+  typedef typename Elem<DT>::type T;
+  Operand x, w;
+  operands<DT>(a, p, x, w, s);
+  char *ws = (char *)a->workspace;
+  Rows *head = (Rows *)(ws + p.at_head);
+  float *rows = (float *)(ws + p.at_rows);
+  T *d = (T *)(ws + p.at_d);
+  float *hidden = (float *)(ws + p.at_hidden), *weight = (float *)(ws + p.at_weight);
+  rows_kernel<(DT == LUMA_GRAD_F16 ? 15 : 0)><<<1, 1024, 0, s>>>(
+      a->grad_loss, a->target, a->stats, a->n, a->v, a->ignore_index, a->reduction, head, rows);
+  const bool whole = p.piece >= a->v;        // one piece
+  const bool direct = p.hidden_splits == 1 && whole;
+  for (int64_t v0 = 0; v0 < a->v; v0 += p.piece) {
+    const int64_t words = a->v - v0 < p.piece ? a->v - v0 : p.piece;
+    // (the products take k up to the padding: D is 0 there)
+    const int64_t padded = up(words, 256);
+    with_shape(p.logits, [&](auto shape) {
+      typedef decltype(shape) S;
+      const Grid g = grid_of(p.logits, padded, a->n, 1);
+      slope_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(
+          w, x, v0, a->v, a->n, a->h, a->target, a->stats, rows, g, d, p.ld_d);
+    });
+    const Operand wp = {w.p + v0 * w.ld, w.ld, words, w.row_bytes};
+    if (a->d_hidden) {
+      const Operand dk = {(const char *)d, p.ld_d * p.size, a->n, padded * p.size};
+      with_shape(p.hidden, [&](auto shape) {
+        typedef decltype(shape) S;
+        const Grid g = grid_of(p.hidden, a->h, a->n, p.hidden_splits);
+        product_kernel<DT, kAlongK, S><<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
+            wp, dk, a->h, a->n, padded, p.hidden_k, g, v0 > 0, hidden, &head->back,
+            direct ? (T *)a->d_hidden : nullptr);
+      });
+    }
+    if (a->d_weight) {
+      const Operand dm = {(const char *)d, p.ld_d * p.size, a->n, padded * p.size};
+      T *out = (T *)a->d_weight + v0 * a->h;
+      with_shape(p.weight, [&](auto shape) {
+        typedef decltype(shape) S;
+        if constexpr (S::BN >= 64) {
+          const Grid g = grid_of(p.weight, a->h, words, p.weight_splits);
+          product_kernel<DT, kAlongM, S><<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
+              x, dm, a->h, words, a->n, p.weight_k, g, 0, weight, &head->back,
+              p.weight_splits == 1 ? out : nullptr);
+        }
+      });
+      if (p.weight_splits > 1)
+        sum_splits<DT>(weight, p.weight_splits, words * a->h, &head->back, out, s);
+    }
+  }
+  if (a->d_hidden && !direct)
+    sum_splits<DT>(hidden, p.hidden_splits, a->n * a->h, &head->back, a->d_hidden, s);
+}
+
+template <typename F>
+void with_type(int dtype, F f) {
+  switch (dtype) {
+    case LUMA_GRAD_F32: return f(std::integral_constant<int, LUMA_GRAD_F32>{});
+    case LUMA_GRAD_BF16: return f(std::integral_constant<int, LUMA_GRAD_BF16>{});
+    default: return f(std::integral_constant<int, LUMA_GRAD_F16>{});
+  }
+}
+
+}  // namespace
+}  // namespace luma
+
+using namespace luma;
+
+extern "C" {
+
+int64_t luma_xent_workspace_bytes(const LumaXentArgs *a, int32_t backward) {
+  Plan p;
+  if (!check_args(a, backward != 0) || !plan(a, backward != 0, p)) return -1;
+  return p.bytes;
+}
+
+int luma_xent_forward(const LumaXentArgs *a, void *stream) {
+  Plan p;
+  if (!check_args(a, false) || !plan(a, false, p)) return -1;
+  if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < p.bytes)
+    return fail("luma_xent_forward: workspace too small or not aligned");
+  with_type(a->dtype, [&](auto dt) { forward<decltype(dt)::value>(a, p, (hipStream_t)stream); });
+  return check_launch("luma_xent_forward");
+}
+
+int luma_xent_backward(const LumaXentArgs *a, void *stream) {
+  Plan p;
+  if (!check_args(a, true) || !plan(a, true, p)) return -1;
+  if (!a->workspace || (uintptr_t)a->workspace % 256 || a->workspace_bytes < p.bytes)
+    return fail("luma_xent_backward: workspace too small or not aligned");
+  if (!a->d_hidden && !a->d_weight) return 0;
+  with_type(a->dtype, [&](auto dt) { backward<decltype(dt)::value>(a, p, (hipStream_t)stream); });
+  return check_launch("luma_xent_backward");
+}
+
+}  // extern "C"
