@@ -15,7 +15,7 @@
 //
 // The rows of a stage lie in LDS without padding (what the direct loads need),
 // their 16-byte chunks permuted so that the lanes of one read meet different
-// banks: k-contiguous rows of 64 bytes by chunk ^ (row / 2 % 4), m-contiguous
+// banks: k-contiguous rows of 64 bytes by chunk ^ (a function of the row), m-contiguous
 // ones by whole 16-element blocks, block ^ (a function of k).
 //
 // Loads go through buffer descriptors that end where the operand ends: rows
@@ -56,22 +56,42 @@ struct Operand {
   int64_t ld, rows, row_bytes;
 };
 
-template <int DT>
-__device__ __forceinline__ v4f mma(const v4u &a, const v4u &b, v4f c) {
-  if constexpr (DT == LUMA_GRAD_BF16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a),
-                                                   __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
-  } else if constexpr (DT == LUMA_GRAD_F16) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8h, a),
-                                                  __builtin_bit_cast(v8h, b), c, 0, 0, 0);
-  } else {
+// A tile's shape: WM x WN wavefronts of TM x TN blocks of 16 x 16.
+template <int TM_, int TN_, int WM_, int WN_>
+struct Shape {
+  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
+  static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN;
+  static constexpr int kThreads = 64 * WM * WN;
+};
+
+// A wavefront's accumulators: TM x TN blocks of 16 x 16 (instructions of 32 x 32
+// took 7% longer here).  A block is a quad per lane: four consecutive rows of
+// one column.
+template <int DT, typename S>
+struct Acc {
+  v4f t[S::TM][S::TN];
+
+  __device__ __forceinline__ Acc() {
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-      c = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[j]), __uint_as_float(b[j]), c, 0,
-                                               0, 0);
-    return c;
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) t[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
-}
+  __device__ __forceinline__ void mma(int i, int j, const v4u &a, const v4u &b) {
+    if constexpr (DT == LUMA_GRAD_BF16) {
+      t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+          __builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), t[i][j], 0, 0, 0);
+    } else if constexpr (DT == LUMA_GRAD_F16) {
+      t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+          __builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), t[i][j], 0, 0, 0);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        t[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(a[k]),
+                                                       __uint_as_float(b[k]), t[i][j], 0, 0, 0);
+    }
+  }
+};
 
 // The block of a kAlongM row in whose place a block's elements lie: block ^ this.
 template <int DT>
@@ -80,8 +100,16 @@ __device__ __forceinline__ int turn(int k) {
   return (k & 3) | ((k >> 1) & 4);                 // k = 8 g .. 8 g + 3
 }
 
+// The row of a pair of blocks of 16 that row `r` of block `i` of them takes, so
+// that a lane's two quads are eight consecutive rows (kPaired), or 16 i + r.
+constexpr int kPlain = 0, kPaired = 1;
+template <int ORDER>
+__device__ __forceinline__ constexpr int row_of(int i, int r) {
+  return ORDER == kPaired ? 8 * (r >> 2) + 4 * i + (r & 3) : 16 * i + r;
+}
+
 // One operand's stages: ROWS of m (or n) by 64 bytes of k.
-template <int DT, int ALONG, int ROWS, int THREADS>
+template <int DT, int ALONG, int ORDER, int ROWS, int THREADS>
 struct Tile {
   static constexpr int kBytes = ROWS * kRow;
   static constexpr int kWaves = THREADS / 64;
@@ -93,63 +121,77 @@ struct Tile {
   static constexpr int kBlock = 16 * kSize<DT>;                 // bytes of 16 elements
   static constexpr int kTurn = kLine / kBlock - 1;              // mask of block numbers
 
-  const char *base;      // of the next stage to be loaded
+  // The chunk in whose place a kAlongK row's chunk lies: chunk ^ this (of the
+  // eight rows that eight lanes read, two share it, one in each half of 128 bytes).
+  static __device__ __forceinline__ int swap(int row) {
+    return ORDER == kPaired ? ((row >> 1) & 1) | ((row >> 2) & 2) : (row >> 1) & 3;
+  }
+
+  const char *base;      // of the next pair of stages to be loaded
   int64_t left;          // bytes from base to the operand's end
-  int64_t step;          // bytes from stage to stage
-  int k_left;            // kAlongK: bytes of k from base to the row's end
+  int64_t step;          // bytes from pair to pair
+  int past;              // kAlongK: this lane's first byte of k past the row's end is at < 0
+  int at_lds[kLoads];
   uint32_t voff[kLoads];
-  uint32_t chunk[kLoads];
 
   __device__ __forceinline__ void init(const Operand &o, int64_t m0, int64_t k0) {
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63;
     const int64_t end = (o.rows - 1) * o.ld + o.row_bytes;
     const int64_t at = ALONG == kAlongK ? m0 * o.ld + k0 * kSize<DT> : k0 * o.ld + m0 * kSize<DT>;
     base = o.p + at;
     left = end - at;
-    step = ALONG == kAlongK ? kRow : kStep<DT> * o.ld;
-    const int64_t kl = o.row_bytes - k0 * kSize<DT>;
-    k_left = ALONG == kAlongK ? (int)(kl < 0x40000000 ? kl : 0x40000000) : 0;
+    step = 2 * (ALONG == kAlongK ? kRow : kStep<DT> * o.ld);
 #pragma unroll
     for (int q = 0; q < kLoads; ++q) {
-      const int at_lds = ((wave * kLoads + q) % kTotal) * 1024 + lane * 16;
+      at_lds[q] = ((wave * kLoads + q) % kTotal) * 1024;
+      const int at = at_lds[q] + lane * 16;
       if (ALONG == kAlongK) {
-        const int row = at_lds / kRow, pos = (at_lds % kRow) / 16;
-        chunk[q] = (pos ^ ((row >> 1) & 3)) * 16;
-        voff[q] = (uint32_t)(row * o.ld) + chunk[q];
+        const int row = at / kRow, pos = (at % kRow) / 16;
+        // (every row of this lane has the same chunk)
+        const int chunk = (pos ^ swap(row)) * 16;
+        voff[q] = (uint32_t)(row * o.ld) + chunk;
+        const int64_t kl = o.row_bytes - k0 * kSize<DT>;
+        past = (int)(kl < 0x40000000 ? kl : 0x40000000) - 1 - chunk;
       } else {
-        const int k = at_lds / kLine, in = at_lds % kLine;
+        const int k = at / kLine, in = at % kLine;
         const int block = (in / kBlock) ^ (turn<DT>(k) & kTurn);
-        chunk[q] = 0;
         voff[q] = (uint32_t)(k * o.ld) + block * kBlock + in % kBlock;
       }
     }
   }
 
-  // Sends the next stage on its way into s.
-  __device__ __forceinline__ void load(char *s) {
-    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-    const int records = left <= 0 ? 0 : left < 0x7FFFFFFF ? (int)left : 0x7FFFFFFF;
+  // Sends the next pair of stages on its way into s0 and s1.
+  __device__ __forceinline__ void load(char *s0, char *s1) {
+    typedef __attribute__((address_space(3))) void lds_void;
+    const int high = (int)(left >> 31);
+    const int records = high == 0 ? (int)left : high < 0 ? 0 : 0x7FFFFFFF;
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
+    // (an offset past any end where k is)
+    const uint32_t none0 = ALONG == kAlongK ? past & 0x80000000u : 0u;
+    const uint32_t none1 = ALONG == kAlongK ? (past - kRow) & 0x80000000u : 0u;
+    // (not as the instruction's offset, which moves the place in LDS too)
+    const uint32_t next = ALONG == kAlongK ? kRow : (uint32_t)(step >> 1);
 #pragma unroll
-    for (int q = 0; q < kLoads; ++q) {
-      uint32_t v = voff[q];
-      if (ALONG == kAlongK && k_left < kRow && (int)chunk[q] >= k_left) v = 0xFFFFFFF0u;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(
-          rsrc, (__attribute__((address_space(3))) void *)(s + ((wave * kLoads + q) % kTotal) * 1024),
-          16, v, 0, 0, 0);
-    }
+    for (int q = 0; q < kLoads; ++q)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(s0 + at_lds[q]), 16,
+                                               voff[q] | none0, 0, 0, 0);
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(s1 + at_lds[q]), 16,
+                                               (voff[q] + next) | none1, 0, 0, 0);
     base += step;
     left -= step;
-    if (ALONG == kAlongK) k_left -= kRow;
+    if (ALONG == kAlongK) past -= 2 * kRow;
   }
 
-  // Where this lane's part of the fragments of COUNT blocks from block `first`
-  // (a multiple of COUNT) lies.
+  // Where this lane's part of the fragments of a run of blocks lies, the run
+  // starting at block `first` and its length a power of two that divides it.
   static __device__ __forceinline__ int where(int first) {
     const int lane = threadIdx.x & 63;
     if (ALONG == kAlongK) {
-      const int row = first * 16 + (lane & 15);
-      return row * kRow + (((lane >> 4) ^ ((row >> 1) & 3)) * 16);
+      const int row = first * 16 + row_of<ORDER>(0, lane & 15);
+      return row * kRow + (((lane >> 4) ^ swap(row)) * 16);
     }
     if (DT == LUMA_GRAD_F32)
       return (lane >> 4) * 4 * kLine + ((first ^ ((lane >> 4) & kTurn)) * kBlock) + (lane & 15) * 4;
@@ -159,7 +201,10 @@ struct Tile {
 
   // Fragment of block first + i.
   static __device__ __forceinline__ v4u read(const char *s, int where, int i) {
-    if constexpr (ALONG == kAlongK) {
+    if constexpr (ALONG == kAlongK && ORDER == kPaired) {
+      // (row_of(1, r) = row_of(0, r) + 4: the same swap)
+      return *(const v4u *)(s + where + (i >> 1) * 32 * kRow + (i & 1) * 4 * kRow);
+    } else if constexpr (ALONG == kAlongK) {
       return *(const v4u *)(s + where + i * 16 * kRow);
     } else if constexpr (DT == LUMA_GRAD_F32) {
       const char *p = s + (where ^ (i * kBlock));
@@ -178,14 +223,6 @@ struct Tile {
   }
 };
 
-// A tile's shape: WM x WN wavefronts of TM x TN 16x16 blocks.
-template <int TM_, int TN_, int WM_, int WN_>
-struct Shape {
-  static constexpr int TM = TM_, TN = TN_, WM = WM_, WN = WN_;
-  static constexpr int BM = 16 * TM * WM, BN = 16 * TN * WN;
-  static constexpr int kThreads = 64 * WM * WN;
-};
-
 // Outstanding direct loads at most N, this wavefront's LDS reads done, then all
 // wavefronts here.
 template <int N>
@@ -194,16 +231,37 @@ __device__ __forceinline__ void wait_and_meet() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
-// acc[i][j] (+)= the product over k0 <= k < k1 of this wavefront's blocks.
+// The order of one half of a pair of stages: a fragment's read after every few
+// matrix instructions, and LOADS loads into LDS after the first ones.
+template <int MMAS, int READS, int LOADS>
+__device__ __forceinline__ void spread() {
+#pragma unroll
+  for (int q = 0; q < LOADS; ++q) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
+  }
+  constexpr int kEach = (MMAS - LOADS) / READS > 0 ? (MMAS - LOADS) / READS : 1;
+#pragma unroll
+  for (int q = 0; q < READS; ++q) {
+    __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x8, kEach, 0);
+  }
+  __builtin_amdgcn_sched_group_barrier(0x8, MMAS, 0);
+  __builtin_amdgcn_sched_barrier(0);
+}
+
+// acc (+)= the product over k0 <= k < k1 of this wavefront's blocks.
 // k1 - k0 is rounded up to whole rounds of the ring: past k1 operands must
 // read as zeros (past the operands' end), unless k1 - k0 is a multiple of
 // kStages * kStep.
-template <int DT, int AA, int AB, typename S>
+template <int DT, int AA, int AB, int ORDER, typename S>
 __device__ __forceinline__ void product(const Operand &a, const Operand &b, int64_t m0, int64_t n0,
-                                        int64_t k0, int64_t k1, v4f (&acc)[S::TM][S::TN]) {
-  typedef Tile<DT, AA, S::BM, S::kThreads> A;
-  typedef Tile<DT, AB, S::BN, S::kThreads> B;
+                                        int64_t k0, int64_t k1, Acc<DT, S> &acc) {
+#ifdef __HIP_DEVICE_COMPILE__   // (the host's compiler has no use for it)
+  typedef Tile<DT, AA, ORDER, S::BM, S::kThreads> A;
+  typedef Tile<DT, AB, kPlain, S::BN, S::kThreads> B;
   constexpr int kLoads = A::kLoads + B::kLoads;
+  constexpr int kMmas = S::TM * S::TN * (DT == LUMA_GRAD_F32 ? 4 : 1), kReads = S::TM + S::TN;
   // (a variable for each stage: the compiler then knows that a stage's reads
   // do not wait for another's loads)
   __shared__ __align__(1024) char a0[A::kBytes], a1[A::kBytes], a2[A::kBytes], a3[A::kBytes];
@@ -213,12 +271,13 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
   ta.init(a, m0, k0);
   tb.init(b, n0, k0);
   const int wave = threadIdx.x >> 6;
-  const int wa = A::where((wave / S::WN) * S::TM), wb = B::where((wave % S::WN) * S::TN);
+  const int wa = A::where((wave / S::WN) * S::TM);
+  const int wb = B::where((wave % S::WN) * S::TN);
   v4u fa[2][S::TM], fb[2][S::TN];
 
-  auto fill = [&](char *sa, char *sb) {
-    ta.load(sa);
-    tb.load(sb);
+  auto fill = [&](char *sa0, char *sb0, char *sa1, char *sb1) {
+    ta.load(sa0, sa1);
+    tb.load(sb0, sb1);
   };
   auto fetch = [&](const char *sa, const char *sb, v4u (&xa)[S::TM], v4u (&xb)[S::TN]) {
 #pragma unroll
@@ -230,35 +289,34 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
 #pragma unroll
     for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j) acc[i][j] = mma<DT>(xa[i], xb[j], acc[i][j]);
+      for (int j = 0; j < S::TN; ++j) acc.mma(i, j, xa[i], xb[j]);
   };
 
-  fill(a0, b0);
-  fill(a1, b1);
-  fill(a2, b2);
+  // One pair of stages: x0, x1 hold it, y0, y1 the next one, which the loads
+  // under way fill.
+  auto pair = [&](char *xa0, char *xb0, char *xa1, char *xb1, char *ya0, char *yb0) {
+    fetch(xa1, xb1, fa[1], fb[1]);
+    multiply(fa[0], fb[0]);
+    spread<kMmas, kReads, 0>();
+    wait_and_meet<0>();
+    fill(xa0, xb0, xa1, xb1);
+    fetch(ya0, yb0, fa[0], fb[0]);
+    multiply(fa[1], fb[1]);
+    spread<kMmas, kReads, 2 * kLoads>();
+  };
+
+  fill(a0, b0, a1, b1);
+  fill(a2, b2, a3, b3);
   wait_and_meet<2 * kLoads>();
   fetch(a0, b0, fa[0], fb[0]);
   const int rounds = (int)((k1 - k0 + kStages * kStep<DT> - 1) / (kStages * kStep<DT>));
   for (int r = 0; r < rounds; ++r) {
-    wait_and_meet<kLoads>();
-    fill(a3, b3);
-    fetch(a1, b1, fa[1], fb[1]);
-    multiply(fa[0], fb[0]);
-    wait_and_meet<kLoads>();
-    fill(a0, b0);
-    fetch(a2, b2, fa[0], fb[0]);
-    multiply(fa[1], fb[1]);
-    wait_and_meet<kLoads>();
-    fill(a1, b1);
-    fetch(a3, b3, fa[1], fb[1]);
-    multiply(fa[0], fb[0]);
-    wait_and_meet<kLoads>();
-    fill(a2, b2);
-    fetch(a0, b0, fa[0], fb[0]);
-    multiply(fa[1], fb[1]);
+    pair(a0, b0, a1, b1, a2, b2);
+    pair(a2, b2, a3, b3, a0, b0);
   }
   // (nothing of the ring is in flight when the workgroup goes on or ends)
   wait_and_meet<0>();
+#endif
 }
 
 // The tile of this workgroup: consecutive workgroups go to the eight XCDs in

@@ -48,6 +48,10 @@ struct Elem<LUMA_GRAD_F16> {
 template <int DT>
 using Four = typename Elem<DT>::type __attribute__((ext_vector_type(4), aligned(2)));
 
+// (D is the workspace's: its rows are whole tiles of words, 512 bytes aligned)
+template <int DT>
+using Eight = typename Elem<DT>::type __attribute__((ext_vector_type(8), aligned(16)));
+
 // Stores four consecutive elements of a row, those before `end`.
 template <int DT>
 __device__ __forceinline__ void store4(typename Elem<DT>::type *p, int64_t at, int64_t end, v4f f) {
@@ -72,83 +76,22 @@ struct Grid {
   int tiles_m, tiles_n, splits;
 };
 
-// This lane's place in the accumulators of its wavefront: acc[i][j][r] is row
-// m + 16 i + r and column n + 16 j.
-template <typename S>
+// This lane's first row and column of its wavefront's accumulators; its quad i
+// of column j is rows m + row(i) .. + 3 and column n + 16 j.
+template <typename S, int ORDER>
 struct Place {
   int64_t m, n;
   __device__ __forceinline__ Place(int tm, int tn) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    m = (int64_t)tm * S::BM + (wave / S::WN) * S::TM * 16 + (lane >> 4) * 4;
+    m = (int64_t)tm * S::BM + (wave / S::WN) * S::TM * 16 + row_of<ORDER>(0, lane >> 4 << 2);
     n = (int64_t)tn * S::BN + (wave % S::WN) * S::TN * 16 + (lane & 15);
+  }
+  static __device__ __forceinline__ constexpr int row(int i) {
+    return i / 2 * 32 + row_of<ORDER>(i & 1, 0);
   }
 };
 
-template <typename S>
-__device__ __forceinline__ void clear(v4f (&acc)[S::TM][S::TN]) {
-#pragma unroll
-  for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-    for (int j = 0; j < S::TN; ++j) acc[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
-}
-
 // -- forward --------------------------------------------------------------------
-
-// Every token's (largest logit, sum of exp(l - largest)) over each wavefront's
-// words: part[tile of words][token]; picked[token] = the target's logit.
-template <int DT, typename S>
-__global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand x, int64_t v,
-                                                             int64_t n, int64_t h,
-                                                             const int64_t *target, Grid g,
-                                                             float2 *part, float *picked) {
-  int tm, tn, split;
-  tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
-  v4f acc[S::TM][S::TN];
-  clear<S>(acc);
-  product<DT, kAlongK, kAlongK, S>(w, x, (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0, h, acc);
-  const Place<S> at(tm, tn);
-  const bool whole = (int64_t)(tm + 1) * S::BM <= v;
-  const int lane = threadIdx.x & 63;
-#pragma unroll
-  for (int j = 0; j < S::TN; ++j) {
-    const int64_t token = at.n + 16 * j;
-    const int64_t t = token < n ? target[token] : -1;
-    const int64_t d = t - at.m;                  // the target's word from this lane's first
-    if (t >= 0 && t < v && d >= 0 && d < 16 * S::TM && (d & 15) < 4) {
-#pragma unroll
-      for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-          if (d == 16 * i + r) picked[token] = acc[i][j][r];
-    }
-    float top = -__builtin_inff();
-#pragma unroll
-    for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        if (!whole && at.m + 16 * i + r >= v) acc[i][j][r] = -__builtin_inff();
-        top = fmaxf(top, acc[i][j][r]);
-      }
-    top = fmaxf(top, __shfl_xor(top, 16));
-    top = fmaxf(top, __shfl_xor(top, 32));
-    // (all -inf: their exponentials are 0 and not NaN)
-    const float base = (top == -__builtin_inff() ? 0.0f : top) * kLog2e;
-    float sum = 0.0f;
-#pragma unroll
-    for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-      for (int r = 0; r < 4; ++r)
-        sum += __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -base));
-    sum += __shfl_xor(sum, 16);
-    sum += __shfl_xor(sum, 32);
-    if (lane < 16 && token < n) {
-      const int wm = (threadIdx.x >> 6) / S::WN;
-      part[((int64_t)tm * S::WM + wm) * n + token] = make_float2(top, sum);
-    }
-  }
-}
-
-constexpr int kJoinTokens = 32, kJoinSlices = 32, kJoinThreads = kJoinTokens * kJoinSlices;
 
 // (largest, sum) of two sets of words together.
 __device__ __forceinline__ float2 join(float2 a, float2 b) {
@@ -157,6 +100,78 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
   return make_float2(top, a.y * __builtin_amdgcn_exp2f((a.x - top) * kLog2e) +
                               b.y * __builtin_amdgcn_exp2f((b.x - top) * kLog2e));
 }
+
+// Every token's (largest logit, sum of exp(l - largest)) over each tile's words:
+// part[tile of words][token]; picked[token] = the target's logit.
+template <int DT, typename S>
+__global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand x, int64_t v,
+                                                             int64_t n, int64_t h,
+                                                             const int64_t *target, Grid g,
+                                                             float2 *part, float *picked) {
+  int tm, tn, split;
+  tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
+  Acc<DT, S> acc;
+  product<DT, kAlongK, kAlongK, kPlain, S>(w, x, (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0, h, acc);
+  typedef Place<S, kPlain> P;
+  const P at(tm, tn);
+  const bool whole = (int64_t)(tm + 1) * S::BM <= v;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = wave / S::WN, wn = wave % S::WN;
+  __shared__ float2 records[S::WM][S::BN];
+#pragma unroll
+  for (int j = 0; j < S::TN; ++j) {
+    const int64_t token = at.n + 16 * j;
+    const int64_t t = token < n ? target[token] : -1;
+    // the target's word from this lane's first; < 0 for none here
+    const int64_t far = t < v ? t - at.m : -1;
+    const int d = far >= 0 && far < 16 * S::TM ? (int)far : -1;
+    if (__ballot(d >= 0)) {
+      float mine = 0.0f;
+      bool found = false;
+#pragma unroll
+      for (int q = 0; q < S::TM; ++q)
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+          if (d == P::row(q) + r) {
+            mine = acc.t[q][j][r];
+            found = true;
+          }
+      if (found) picked[token] = mine;
+    }
+    float top = -__builtin_inff();
+#pragma unroll
+    for (int q = 0; q < S::TM; ++q)
+#pragma unroll
+      for (int r = 0; r < 4; ++r)
+        if (whole || at.m + P::row(q) + r < v) top = fmaxf(top, acc.t[q][j][r]);
+#pragma unroll
+    for (int o = 16; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
+    // (all -inf: their exponentials are 0 and not NaN)
+    const float base = (top == -__builtin_inff() ? 0.0f : top) * kLog2e;
+    float sum = 0.0f;
+#pragma unroll
+    for (int q = 0; q < S::TM; ++q)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.t[q][j][r], kLog2e, -base));
+        if (whole || at.m + P::row(q) + r < v) sum += e;
+      }
+#pragma unroll
+    for (int o = 16; o < 64; o *= 2) sum += __shfl_xor(sum, o);
+    if (lane < 16)
+      records[wm][wn * S::TN * 16 + 16 * j + lane] = make_float2(top, sum);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < S::BN; i += S::kThreads) {
+    const int64_t token = (int64_t)tn * S::BN + i;
+    float2 a = records[0][i];
+#pragma unroll
+    for (int k = 1; k < S::WM; ++k) a = join(a, records[k][i]);
+    if (token < n) part[(int64_t)tm * n + token] = a;
+  }
+}
+
+constexpr int kJoinTokens = 32, kJoinSlices = 32, kJoinThreads = kJoinTokens * kJoinSlices;
 
 // Each token's lse and loss from its `parts` records; with a reduction, each
 // workgroup's sums (in float64) of the losses and of the targets that count.
@@ -170,8 +185,20 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2 *part, 
   const int tok = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
   const int64_t token = (int64_t)blockIdx.x * kJoinTokens + tok;
   float2 a = make_float2(-__builtin_inff(), 0.0f);
-  if (token < n)
-    for (int p = slice; p < parts; p += kJoinSlices) a = join(a, part[(int64_t)p * n + token]);
+  if (token < n) {
+    // (kAhead records in flight: a token has hundreds, and the loads' latency
+    // is what they take)
+    constexpr int kAhead = 8;
+    int p = slice;
+    for (; p + (kAhead - 1) * kJoinSlices < parts; p += kAhead * kJoinSlices) {
+      float2 b[kAhead];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) b[k] = part[(int64_t)(p + k * kJoinSlices) * n + token];
+#pragma unroll
+      for (int k = 0; k < kAhead; ++k) a = join(a, b[k]);
+    }
+    for (; p < parts; p += kJoinSlices) a = join(a, part[(int64_t)p * n + token]);
+  }
   lds[slice][tok] = a;
   __syncthreads();
   if (threadIdx.x >= 64) return;      // (the rest is the first wavefront's)
@@ -268,6 +295,7 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float *grad, const int
   if (threadIdx.x == 0) head->back = __builtin_ldexpf(1.0f, -e);
 }
 
+// (Eight words of a token are a lane's: 16-byte stores.)
 // D of words [v0, v0 + tiles_m BM), 0 past the vocabulary: d[token][word - v0].
 template <int DT, typename S>
 __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x, int64_t v0,
@@ -278,27 +306,31 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
                                                             int64_t ld) {
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
-  v4f acc[S::TM][S::TN];
-  clear<S>(acc);
-  product<DT, kAlongK, kAlongK, S>(w, x, v0 + (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0, h, acc);
-  const Place<S> at(tm, tn);
+  Acc<DT, S> acc;
+  product<DT, kAlongK, kAlongK, kPaired, S>(w, x, v0 + (int64_t)tm * S::BM, (int64_t)tn * S::BN,
+                                            0, h, acc);
+  typedef Place<S, kPaired> P;
+  const P at(tm, tn);
 #pragma unroll
   for (int j = 0; j < S::TN; ++j) {
     const int64_t token = at.n + 16 * j;
     if (token >= n) continue;
     const float base = stats[token] * kLog2e, row = rows[token];
     const int64_t t = target[token] - v0 - at.m;
+    typename Elem<DT>::type *out = d + token * ld + at.m;
 #pragma unroll
-    for (int i = 0; i < S::TM; ++i) {
-      v4f f;
+    for (int q = 0; q < S::TM; q += 2) {
+      Eight<DT> f;
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        float p = __builtin_amdgcn_exp2f(__builtin_fmaf(acc[i][j][r], kLog2e, -base));
-        if (t == 16 * i + r) p -= 1.0f;
+      for (int e = 0; e < 8; ++e) {
+        float p = __builtin_amdgcn_exp2f(
+            __builtin_fmaf(acc.t[q + e / 4][j][e % 4], kLog2e, -base));
+        if (t == P::row(q) + e) p -= 1.0f;
         // (an ignored token's logits may be anything)
-        f[r] = row == 0.0f || v0 + at.m + 16 * i + r >= v ? 0.0f : p * row;
+        f[e] = Elem<DT>::round(
+            row == 0.0f || v0 + at.m + P::row(q) + e >= v ? 0.0f : p * row);
       }
-      store4<DT>(d + token * ld, at.m + 16 * i, ld, f);
+      *(Eight<DT> *)(out + P::row(q)) = f;
     }
   }
 }
@@ -314,23 +346,23 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
   const int64_t k0 = split * k_split, k1 = min(k, k0 + k_split);
-  v4f acc[S::TM][S::TN];
-  clear<S>(acc);
-  product<DT, kAlongM, AB, S>(a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
-  const Place<S> at(tm, tn);
+  Acc<DT, S> acc;
+  product<DT, kAlongM, AB, kPlain, S>(a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
+  typedef Place<S, kPlain> P;
+  const P at(tm, tn);
   const float f = out16 ? *back : 1.0f;
 #pragma unroll
   for (int j = 0; j < S::TN; ++j) {
     const int64_t row = at.n + 16 * j;
     if (row >= n) continue;
 #pragma unroll
-    for (int i = 0; i < S::TM; ++i) {
-      const int64_t col = at.m + 16 * i;
+    for (int q = 0; q < S::TM; ++q) {
+      const int64_t col = at.m + P::row(q);
+      v4f c = acc.t[q][j];
       if (out16) {
-        store4<DT>(out16 + row * m, col, m, acc[i][j] * f);
+        store4<DT>(out16 + row * m, col, m, c * f);
       } else {
         float *o = out + (int64_t)split * n * m + row * m;
-        v4f c = acc[i][j];
         if (add)
 #pragma unroll
           for (int r = 0; r < 4; ++r)
@@ -378,19 +410,60 @@ typedef Shape<2, 4, 4, 1> Thin64;    // 128 x 64: few tokens
 typedef Shape<2, 1, 4, 1> Thin16;    // 128 x 16
 enum ShapeId { kBig, kMid, kSmall, kThin64, kThin16 };
 constexpr int kBM[] = {256, 128, 64, 128, 128}, kBN[] = {256, 128, 64, 64, 16};
-
-constexpr int64_t kPieceBytes = 256 << 20;     // of D: what the last-level cache holds
+constexpr int64_t kChip = 256;                 // CUs
 
 int64_t up(int64_t x, int64_t to) { return (x + to - 1) / to * to; }
 int64_t tiles(int64_t x, int64_t size) { return (x + size - 1) / size; }
 
-// The tile for a product of m x n: the largest whose tiles fill the chip.
-int shape_for(int64_t m, int64_t n) {
+// The tile for a product of m x n whose k can be split in up to `splits`: the
+// largest whose workgroups fill the chip.
+int shape_for(int64_t m, int64_t n, int64_t splits) {
   if (n <= 16) return kThin16;
   if (n <= 64) return kThin64;
-  if (tiles(m, 256) * tiles(n, 256) >= 192) return kBig;
-  if (tiles(m, 128) * tiles(n, 128) >= 128) return kMid;
+  if (tiles(m, 256) * tiles(n, 256) * splits >= 192) return kBig;
+  if (tiles(m, 128) * tiles(n, 128) * splits >= 128) return kMid;
   return kSmall;
+}
+
+// Into how many parts k is split, and each part's length (a multiple of
+// `round`).  A part is a workgroup per tile: they should come in whole rounds of
+// the chip, but each part's float32 sums are written and read again.  The cost
+// of s parts, in bytes of that traffic's time: a round takes `deep` bytes' time
+// for an element of k (a 256 x 256 tile at about 5 TFLOP/s per CU of 16-bit
+// products takes 26 ns, in which the chip moves 100 KB), and the sums 8 s m n.
+int64_t split_k(int shape, int64_t m, int64_t n, int64_t k, int64_t round, int64_t &each) {
+  const int64_t t = tiles(m, kBM[shape]) * tiles(n, kBN[shape]);
+  const int64_t at_once = shape == kBig ? kChip : shape == kMid ? 2 * kChip : 4 * kChip;
+  const double deep = 100e3 * kBM[shape] * kBN[shape] / (256.0 * 256.0) * at_once / kChip;
+  const int64_t most = tiles(k, 4 * round) < 64 ? tiles(k, 4 * round) : 64;
+  int64_t best = 1;
+  double least = 0.0;
+  for (int64_t s = 1; s <= most; ++s) {
+    const int64_t part = up(tiles(k, s), round);
+    const double cost = (double)tiles(t * s, at_once) * part * deep +
+                        (s > 1 ? 8.0 * s * m * n + 16e6 : 0.0);
+    if (s == 1 || cost < least) best = s, least = cost;
+  }
+  each = up(tiles(k, best), round);
+  return tiles(k, each);
+}
+
+// Of `words` words, those whose 256 x 256 tiles of d_weight make whole rounds of
+// the chip (0: fewer than one).
+int64_t whole_rounds(int64_t h, int64_t words) {
+  const int64_t rows = tiles(h, 256), rounds = tiles(words, 256) * rows / kChip;
+  const int64_t main = kChip * rounds / rows * 256;
+  return main < words ? main : words;
+}
+
+// Words per piece of the vocabulary: pieces of about equal length, each at most
+// kPieceBytes of D.
+constexpr int64_t kPieceBytes = 1 << 30;
+int64_t piece_for(int64_t n, int64_t v, int64_t size) {
+  const int64_t all = tiles(v, 256);
+  int64_t most = kPieceBytes / (n * size * 256);
+  if (most < 1) most = 1;
+  return tiles(all, tiles(all, most)) * 256;
 }
 
 struct Plan {
@@ -403,23 +476,14 @@ struct Plan {
   int64_t parts, at_part, at_picked, at_sums, blocks;
   // backward
   int64_t piece, ld_d;          // words per piece; elements per row of D
-  int hidden, weight;           // tile shapes
-  int64_t hidden_splits, hidden_k, weight_splits, weight_k;
+  int hidden;                   // tile shape
+  int64_t hidden_splits, hidden_k;
   int64_t at_head, at_rows, at_d, at_hidden, at_weight;
   int64_t bytes;
 };
 
-// Splits of a product over k so that its tiles fill the chip, and each one's k.
-void split_k(int shape, int64_t m, int64_t n, int64_t k, int64_t round, int64_t &splits,
-             int64_t &each) {
-  const int64_t t = tiles(m, kBM[shape]) * tiles(n, kBN[shape]);
-  const int64_t want = shape == kBig ? 256 : 1024;
-  int64_t s = t >= want / 2 ? 1 : want / t;
-  const int64_t most = tiles(k, 4 * round);
-  s = s < most ? s : most;
-  s = s < 64 ? s : 64;
-  each = up(tiles(k, s), round);
-  splits = tiles(k, each);
+int weight_shape(const LumaXentArgs *a, int64_t words) {
+  return shape_for(a->h, words < 65 ? 65 : words, tiles(a->n, 1024));
 }
 
 bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
@@ -442,33 +506,37 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
   if (p.pack_x) p.at_x = take(a->n * p.ld_x * p.size);
   if (p.pack_w) p.at_w = take(a->v * p.ld_w * p.size);
   if (!backward) {
-    p.logits = shape_for(a->v, a->n);
-    const int wm[] = {2, 2, 2, 4, 4};
-    p.parts = tiles(a->v, kBM[p.logits]) * wm[p.logits];
+    p.logits = shape_for(a->v, a->n, 1);
+    p.parts = tiles(a->v, kBM[p.logits]);
     p.blocks = tiles(a->n, kJoinTokens);
     p.at_part = take(p.parts * a->n * sizeof(float2));
     p.at_picked = take(a->n * sizeof(float));
     p.at_sums = take(p.blocks * sizeof(double2));
   } else {
-    p.piece = kPieceBytes / (a->n * p.size) / 256 * 256;
-    if (p.piece < 256) p.piece = 256;
-    if (p.piece > up(a->v, 256)) p.piece = up(a->v, 256);
-    p.logits = shape_for(p.piece < a->v ? p.piece : a->v, a->n);
+    p.piece = piece_for(a->n, a->v, p.size);
+    p.logits = shape_for(p.piece < a->v ? p.piece : a->v, a->n, 1);
     p.ld_d = p.piece;
     p.at_head = take(sizeof(Rows));
     p.at_rows = take(a->n * sizeof(float));
     p.at_d = take(a->n * p.ld_d * p.size);
+    int64_t each, sums = 0;
     if (a->d_hidden) {
-      p.hidden = shape_for(a->h, a->n);
-      split_k(p.hidden, a->h, a->n, p.ld_d, round, p.hidden_splits, p.hidden_k);
+      p.hidden = shape_for(a->h, a->n, tiles(p.ld_d, 1024));
+      p.hidden_splits = split_k(p.hidden, a->h, a->n, p.ld_d, round, p.hidden_k);
       if (p.hidden_splits > 1 || p.piece < a->v)
         p.at_hidden = take(p.hidden_splits * a->n * a->h * sizeof(float));
     }
     if (a->d_weight) {
-      const int64_t v = p.piece < a->v ? p.piece : a->v;
-      p.weight = shape_for(a->h, v < 65 ? 65 : v);
-      split_k(p.weight, a->h, v, a->n, round, p.weight_splits, p.weight_k);
-      if (p.weight_splits > 1) p.at_weight = take(p.weight_splits * v * a->h * sizeof(float));
+      const int64_t last = a->v - (a->v - 1) / p.piece * p.piece;
+      const int64_t first = p.piece < a->v ? p.piece : a->v;
+      for (const int64_t words : {whole_rounds(a->h, first), first - whole_rounds(a->h, first),
+                                  whole_rounds(a->h, last), last - whole_rounds(a->h, last)}) {
+        if (words == 0) continue;
+        const int shape = weight_shape(a, words);
+        const int64_t splits = split_k(shape, a->h, words, a->n, round, each);
+        if (splits > 1 && splits * words > sums) sums = splits * words;
+      }
+      if (sums) p.at_weight = take(sums * a->h * sizeof(float));
     }
   }
   p.bytes = at;
@@ -594,19 +662,31 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
       });
     }
     if (a->d_weight) {
-      const Operand dm = {(const char *)d, p.ld_d * p.size, a->n, padded * p.size};
-      T *out = (T *)a->d_weight + v0 * a->h;
-      with_shape(p.weight, [&](auto shape) {
-        typedef decltype(shape) S;
-        if constexpr (S::BN >= 64) {
-          const Grid g = grid_of(p.weight, a->h, words, p.weight_splits);
-          product_kernel<DT, kAlongM, S><<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
-              x, dm, a->h, words, a->n, p.weight_k, g, 0, weight, &head->back,
-              p.weight_splits == 1 ? out : nullptr);
-        }
-      });
-      if (p.weight_splits > 1)
-        sum_splits<DT>(weight, p.weight_splits, words * a->h, &head->back, out, s);
+      // (the tiles that make whole rounds of the chip, then the rest)
+      const int64_t main = whole_rounds(a->h, words);
+      const int64_t cut[] = {0, main, words};
+      for (int c = 0; c < 2; ++c) {
+        const int64_t w0 = cut[c], count = cut[c + 1] - w0;
+        if (count == 0) continue;
+        const Operand dm = {(const char *)(d + w0), p.ld_d * p.size, a->n,
+                            (padded - w0) * p.size};
+        T *out = (T *)a->d_weight + (v0 + w0) * a->h;
+        const int shape_id = weight_shape(a, count);
+        int64_t each;
+        const int64_t splits =
+            split_k(shape_id, a->h, count, a->n, kStages * kRow / p.size, each);
+        with_shape(shape_id, [&](auto shape) {
+          typedef decltype(shape) S;
+          if constexpr (S::BN >= 64) {
+            const Grid g = grid_of(shape_id, a->h, count, splits);
+            product_kernel<DT, kAlongM, S>
+                <<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
+                    x, dm, a->h, count, a->n, each, g, 0, weight, &head->back,
+                    splits == 1 ? out : nullptr);
+          }
+        });
+        if (splits > 1) sum_splits<DT>(weight, splits, count * a->h, &head->back, out, s);
+      }
     }
   }
   if (a->d_hidden && !direct)
