@@ -29,10 +29,12 @@
 namespace luma {
 namespace gemm {
 
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef uint32_t v4u __attribute__((ext_vector_type(4)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 typedef short v4s __attribute__((ext_vector_type(4)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) char lds_char;
@@ -71,16 +73,31 @@ template <int DT, typename S>
 struct Acc {
   v4f t[S::TM][S::TN];
 
-  __device__ __forceinline__ Acc() {
+  __device__ __forceinline__ Acc() { clear(); }
+  // Whether any of this lane's sums is a NaN.
+  __device__ __forceinline__ bool nan() const {
+    bool any = false;
+#pragma unroll
+    for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) any |= t[i][j][r] != t[i][j][r];
+    return any;
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < S::TM; ++i)
 #pragma unroll
       for (int j = 0; j < S::TN; ++j) t[i][j] = v4f{0.f, 0.f, 0.f, 0.f};
   }
+  __device__ __forceinline__ void mma_bf16(int i, int j, const v4u &a, const v4u &b) {
+    t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+        __builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), t[i][j], 0, 0, 0);
+  }
   __device__ __forceinline__ void mma(int i, int j, const v4u &a, const v4u &b) {
     if constexpr (DT == LUMA_GRAD_BF16) {
-      t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-          __builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), t[i][j], 0, 0, 0);
+      mma_bf16(i, j, a, b);
     } else if constexpr (DT == LUMA_GRAD_F16) {
       t[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(
           __builtin_bit_cast(v8h, a), __builtin_bit_cast(v8h, b), t[i][j], 0, 0, 0);
@@ -250,6 +267,29 @@ __device__ __forceinline__ void spread() {
   __builtin_amdgcn_sched_barrier(0);
 }
 
+// Float32 as a sum of three bfloat16, x = hi + mid + lo with nothing left over
+// (each takes the next 8 of its 24 bits; a lo below 2^-126 may be lost).
+struct Split {
+  v4u hi, mid, lo;
+  // of the eight values of two fragments
+  __device__ __forceinline__ Split(const v4u &a, const v4u &b) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const v4u &x = e < 2 ? a : b;
+      v2f f = {__uint_as_float(x[2 * (e & 1)]), __uint_as_float(x[2 * (e & 1) + 1])};
+      hi[e] = take(f);
+      mid[e] = take(f);
+      lo[e] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2bf));
+    }
+  }
+  static __device__ __forceinline__ uint32_t take(v2f &f) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, v2bf));
+    f[0] -= __uint_as_float(b << 16);
+    f[1] -= __uint_as_float(b & 0xFFFF0000u);
+    return b;
+  }
+};
+
 // acc (+)= the product over k0 <= k < k1 of this wavefront's blocks.
 // k1 - k0 is rounded up to whole rounds of the ring: past k1 operands must
 // read as zeros (past the operands' end), unless k1 - k0 is a multiple of
@@ -268,51 +308,130 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
   __shared__ __align__(1024) char b0[B::kBytes], b1[B::kBytes], b2[B::kBytes], b3[B::kBytes];
   A ta;
   B tb;
-  ta.init(a, m0, k0);
-  tb.init(b, n0, k0);
   const int wave = threadIdx.x >> 6;
   const int wa = A::where((wave / S::WN) * S::TM);
   const int wb = B::where((wave % S::WN) * S::TN);
-  v4u fa[2][S::TM], fb[2][S::TN];
-
   auto fill = [&](char *sa0, char *sb0, char *sa1, char *sb1) {
     ta.load(sa0, sa1);
     tb.load(sb0, sb1);
   };
-  auto fetch = [&](const char *sa, const char *sb, v4u (&xa)[S::TM], v4u (&xb)[S::TN]) {
-#pragma unroll
-    for (int j = 0; j < S::TN; ++j) xb[j] = B::read(sb, wb, j);
-#pragma unroll
-    for (int i = 0; i < S::TM; ++i) xa[i] = A::read(sa, wa, i);
-  };
-  auto multiply = [&](const v4u (&xa)[S::TM], const v4u (&xb)[S::TN]) {
-#pragma unroll
-    for (int i = 0; i < S::TM; ++i)
-#pragma unroll
-      for (int j = 0; j < S::TN; ++j) acc.mma(i, j, xa[i], xb[j]);
-  };
-
-  // One pair of stages: x0, x1 hold it, y0, y1 the next one, which the loads
-  // under way fill.
-  auto pair = [&](char *xa0, char *xb0, char *xa1, char *xb1, char *ya0, char *yb0) {
-    fetch(xa1, xb1, fa[1], fb[1]);
-    multiply(fa[0], fb[0]);
-    spread<kMmas, kReads, 0>();
-    wait_and_meet<0>();
-    fill(xa0, xb0, xa1, xb1);
-    fetch(ya0, yb0, fa[0], fb[0]);
-    multiply(fa[1], fb[1]);
-    spread<kMmas, kReads, 2 * kLoads>();
-  };
-
-  fill(a0, b0, a1, b1);
-  fill(a2, b2, a3, b3);
-  wait_and_meet<2 * kLoads>();
-  fetch(a0, b0, fa[0], fb[0]);
   const int rounds = (int)((k1 - k0 + kStages * kStep<DT> - 1) / (kStages * kStep<DT>));
-  for (int r = 0; r < rounds; ++r) {
-    pair(a0, b0, a1, b1, a2, b2);
-    pair(a2, b2, a3, b3, a0, b0);
+
+  if constexpr (DT == LUMA_GRAD_F32 && S::TM * S::TN >= 16) {
+    // Six products of bfloat16 parts for one of float32 (all but mid lo, lo mid
+    // and lo lo, together about 2^-24 of the product): the matrix unit takes
+    // bfloat16 16 times as fast as float32.  A pair of stages (32 of k) makes
+    // one bfloat16 fragment.  (Smaller tiles take the float32 instruction: their
+    // time is latency, which taking the parts adds to.)
+    auto parts = [&](const char *xa0, const char *xb0, const char *xa1, const char *xb1) {
+      v4u hi[S::TN], mid[S::TN], lo[S::TN];
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) {
+        const Split y(B::read(xb0, wb, j), B::read(xb1, wb, j));
+        hi[j] = y.hi, mid[j] = y.mid, lo[j] = y.lo;
+      }
+      // (while block i is multiplied, the parts of the next are taken and the one
+      // behind is read; the fences keep the compiler from doing all at once,
+      // for which there are no registers)
+      Split x(A::read(xa0, wa, 0), A::read(xa1, wa, 0));
+      v4u f0 = A::read(xa0, wa, 1), f1 = A::read(xa1, wa, 1);
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        const Split now = x;
+        if (i + 1 < S::TM) x = Split(f0, f1);
+        if (i + 2 < S::TM) f0 = A::read(xa0, wa, i + 2), f1 = A::read(xa1, wa, i + 2);
+        // (the small ones first)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.lo, hi[j]);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.hi, lo[j]);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.mid, mid[j]);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.mid, hi[j]);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.hi, mid[j]);
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.hi, hi[j]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto run = [&](auto pair) {
+      ta.init(a, m0, k0);
+      tb.init(b, n0, k0);
+      fill(a0, b0, a1, b1);
+      for (int r = 0; r < rounds; ++r) {
+        wait_and_meet<0>();
+        fill(a2, b2, a3, b3);
+        pair(a0, b0, a1, b1);
+        wait_and_meet<0>();
+        fill(a0, b0, a1, b1);
+        pair(a2, b2, a3, b3);
+      }
+      wait_and_meet<0>();
+    };
+    run(parts);
+    // Of an infinity (or a value that rounds to one) the parts leave NaN: a sum
+    // that is NaN is formed again by the float32 instruction, a row of blocks
+    // at a time.
+    if (__syncthreads_or(acc.nan())) {
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) {
+        Acc<DT, Shape<1, S::TN, S::WM, S::WN>> again;
+        run([&](const char *xa0, const char *xb0, const char *xa1, const char *xb1) {
+#pragma unroll
+          for (int j = 0; j < S::TN; ++j) {
+            again.mma(0, j, A::read(xa0, wa, i), B::read(xb0, wb, j));
+            again.mma(0, j, A::read(xa1, wa, i), B::read(xb1, wb, j));
+          }
+        });
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r)
+            if (acc.t[i][j][r] != acc.t[i][j][r]) acc.t[i][j][r] = again.t[0][j][r];
+      }
+    }
+  } else {
+    ta.init(a, m0, k0);
+    tb.init(b, n0, k0);
+    v4u fa[2][S::TM], fb[2][S::TN];
+
+    auto fetch = [&](const char *sa, const char *sb, v4u (&xa)[S::TM], v4u (&xb)[S::TN]) {
+#pragma unroll
+      for (int j = 0; j < S::TN; ++j) xb[j] = B::read(sb, wb, j);
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i) xa[i] = A::read(sa, wa, i);
+    };
+    auto multiply = [&](const v4u (&xa)[S::TM], const v4u (&xb)[S::TN]) {
+#pragma unroll
+      for (int i = 0; i < S::TM; ++i)
+#pragma unroll
+        for (int j = 0; j < S::TN; ++j) acc.mma(i, j, xa[i], xb[j]);
+    };
+
+    // One pair of stages: x0, x1 hold it, y0, y1 the next one, which the loads
+    // under way fill.
+    auto pair = [&](char *xa0, char *xb0, char *xa1, char *xb1, char *ya0, char *yb0) {
+      fetch(xa1, xb1, fa[1], fb[1]);
+      multiply(fa[0], fb[0]);
+      spread<kMmas, kReads, 0>();
+      wait_and_meet<0>();
+      fill(xa0, xb0, xa1, xb1);
+      fetch(ya0, yb0, fa[0], fb[0]);
+      multiply(fa[1], fb[1]);
+      spread<kMmas, kReads, 2 * kLoads>();
+    };
+
+    fill(a0, b0, a1, b1);
+    fill(a2, b2, a3, b3);
+    wait_and_meet<2 * kLoads>();
+    fetch(a0, b0, fa[0], fb[0]);
+    for (int r = 0; r < rounds; ++r) {
+      pair(a0, b0, a1, b1, a2, b2);
+      pair(a2, b2, a3, b3, a0, b0);
+    }
   }
   // (nothing of the ring is in flight when the workgroup goes on or ends)
   wait_and_meet<0>();
