@@ -15,14 +15,18 @@
 // threads only read C++ objects while the calling thread holds the GIL, so
 // nothing they read can change under them.  The module computes nothing of
 // the step itself: the step runs in libluma_hip.so.
-#include <ATen/core/Tensor.h>
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/utils/pybind.h>
 
 #include <unistd.h>
 
 #include <algorithm>
+#include <cmath>
 #include <condition_variable>
 #include <cstdint>
 #include <cstring>
@@ -30,6 +34,8 @@
 #include <mutex>
 #include <thread>
 #include <vector>
+
+#include "../../include/luma.h"
 
 namespace py = pybind11;
 
@@ -408,6 +414,7 @@ constexpr int64_t kGradTile = 2048;   // LUMA_GRAD_TILE
 // *device: the CUDA device of all of them (-1 before the first).
 bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<GradRow> &rows,
                 int64_t *device) noexcept {
+  int64_t dev = -1;     // (not *device: its neighbours are other threads')
   try {
     std::vector<const c10::TensorImpl *> impl(n);
     for (int64_t i = 0; i < n; ++i) {
@@ -444,13 +451,14 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<Grad
         return false;
       const int code = grad_code(g->dtype().toScalarType());
       if (code < 0 || !g->is_non_overlapping_and_dense()) return false;
-      if (*device >= 0 && g->device().index() != *device) return false;
-      *device = g->device().index();
+      if (dev >= 0 && g->device().index() != dev) return false;
+      dev = g->device().index();
       if (g->numel() == 0) continue;
       const uint64_t p = (uint64_t)(uintptr_t)g->data();
       if (!p) return false;
       rows.push_back({p, g->numel(), code, 0});
     }
+    *device = dev;
     return true;
   } catch (...) {
     return false;   // an unusual tensor: the caller looks at it
@@ -512,9 +520,135 @@ py::object grad_rows(py::list objs, bool of_grad, bool apart) {
       py::bytes(reinterpret_cast<const char *>(rows.data()), rows.size() * sizeof(GradRow)), dev);
 }
 
+// -- linear_cross_entropy's calls ---------------------------------------------
+// The eager path of luma_amd.linear_cross_entropy: allocations, the library's
+// calls and the autograd node (from Python they take 120 us of a call whose
+// kernels take 45).  The library's entry points come from the caller (bind),
+// which checked its ABI.
+struct XentLibrary {
+  int64_t (*workspace)(const LumaXentArgs *, int32_t) = nullptr;
+  int (*forward)(const LumaXentArgs *, void *) = nullptr;
+  int (*backward)(const LumaXentArgs *, void *) = nullptr;
+  const char *(*error)() = nullptr;
+  PyObject *stream = nullptr;    // torch's current stream of a device, as an address
+} g_xent;
+
+// t, or a copy, with elements of a row next to each other and rows apart.
+at::Tensor rows_of(const at::Tensor &t) {
+  const bool plain = !t.is_neg() && !t._is_zerotensor() && (t.size(1) <= 1 || t.stride(1) == 1) &&
+                     (t.size(0) <= 1 || (t.stride(0) >= t.size(1) && t.stride(0) <= 1 << 21));
+  return plain ? t : t.contiguous();
+}
+
+LumaXentArgs xent_args(const at::Tensor &hidden, const at::Tensor &weight,
+                       const at::Tensor &target, const at::Tensor &stats, int64_t ignore,
+                       int64_t reduction) {
+  LumaXentArgs a{};
+  a.hidden = hidden.const_data_ptr();
+  a.weight = weight.const_data_ptr();
+  a.target = target.const_data_ptr<int64_t>();
+  a.n = hidden.size(0);
+  a.h = hidden.size(1);
+  a.v = weight.size(0);
+  a.ld_hidden = a.n > 1 ? hidden.stride(0) : a.h;
+  a.ld_weight = a.v > 1 ? weight.stride(0) : a.h;
+  a.ignore_index = ignore;
+  a.dtype = grad_code(hidden.scalar_type());
+  a.reduction = (int32_t)reduction;
+  a.stats = stats.mutable_data_ptr<float>();
+  return a;
+}
+
+void xent_call(LumaXentArgs &a, bool backward, const at::Tensor &like) {
+  const c10::DeviceGuard guard(like.device());
+  const int64_t bytes = g_xent.workspace(&a, backward);
+  TORCH_CHECK(bytes >= 0, g_xent.error());
+  const at::Tensor workspace =
+      at::empty({std::max<int64_t>(bytes, 1)}, like.options().dtype(at::kByte));
+  a.workspace = workspace.mutable_data_ptr();
+  a.workspace_bytes = bytes;
+  void *stream;
+  {
+    py::gil_scoped_acquire gil;    // (the backward runs on autograd's thread)
+    stream = reinterpret_cast<void *>(
+        py::handle(g_xent.stream)((int)like.device().index()).cast<uintptr_t>());
+  }
+  const int rc = (backward ? g_xent.backward : g_xent.forward)(&a, stream);
+  TORCH_CHECK(rc == 0, g_xent.error());
+}
+
+struct Xent : torch::autograd::Function<Xent> {
+  static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &hidden,
+                            const at::Tensor &weight, const at::Tensor &target, int64_t ignore,
+                            int64_t reduction) {
+    const int64_t n = hidden.size(0);
+    const auto f32 = hidden.options().dtype(at::kFloat);
+    at::Tensor loss, stats;
+    const std::vector<int64_t> shape =
+        reduction == LUMA_XENT_NONE ? std::vector<int64_t>{n} : std::vector<int64_t>{};
+    if (n == 0) {
+      loss = at::full(shape, reduction == LUMA_XENT_MEAN ? NAN : 0.0, f32);
+      stats = at::zeros({1}, f32);
+    } else {
+      loss = at::empty(shape, f32);
+      stats = at::empty({n + 1}, f32);
+      const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
+      LumaXentArgs a = xent_args(x, w, t, stats, ignore, reduction);
+      a.loss = loss.mutable_data_ptr<float>();
+      xent_call(a, false, hidden);
+    }
+    ctx->save_for_backward({hidden, weight, target, stats});
+    ctx->saved_data["ignore"] = ignore;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->set_materialize_grads(false);
+    return loss;
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *ctx,
+                                                 torch::autograd::variable_list grads) {
+    const bool want_hidden = ctx->needs_input_grad(0), want_weight = ctx->needs_input_grad(1);
+    at::Tensor d_hidden, d_weight;
+    if (grads[0].defined() && (want_hidden || want_weight)) {
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor &hidden = saved[0], &weight = saved[1], &target = saved[2];
+      at::AutoDispatchBelowADInplaceOrView below;
+      if (want_hidden) d_hidden = at::empty(hidden.sizes(), hidden.options());
+      if (want_weight) d_weight = at::empty(weight.sizes(), weight.options());
+      if (hidden.size(0) == 0) {
+        if (want_weight) d_weight.zero_();
+      } else {
+        const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
+        const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+        LumaXentArgs a = xent_args(x, w, t, saved[3], ctx->saved_data["ignore"].toInt(),
+                                   ctx->saved_data["reduction"].toInt());
+        a.grad_loss = g.const_data_ptr<float>();
+        a.d_hidden = want_hidden ? d_hidden.mutable_data_ptr() : nullptr;
+        a.d_weight = want_weight ? d_weight.mutable_data_ptr() : nullptr;
+        xent_call(a, true, hidden);
+      }
+    }
+    return {d_hidden, d_weight, at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// hidden [n][h], weight [v][h] and target [n] as linear_cross_entropy checked them.
+at::Tensor xent(const at::Tensor &hidden, const at::Tensor &weight, const at::Tensor &target,
+                int64_t ignore, int64_t reduction) {
+  if (!g_xent.forward) throw py::value_error("xent: the library is not bound");
+  return Xent::apply(hidden, weight, target, ignore, reduction);
+}
+
+void xent_bind(uintptr_t workspace, uintptr_t forward, uintptr_t backward, uintptr_t error,
+               py::object stream) {
+  g_xent = {reinterpret_cast<int64_t (*)(const LumaXentArgs *, int32_t)>(workspace),
+            reinterpret_cast<int (*)(const LumaXentArgs *, void *)>(forward),
+            reinterpret_cast<int (*)(const LumaXentArgs *, void *)>(backward),
+            reinterpret_cast<const char *(*)()>(error), stream.release().ptr()};
+}
+
 PYBIND11_MODULE(_luma_host, m) {
   m.doc() = "Host-side bookkeeping of LUMA.step (pointer refresh of a planned step) and of the "
-            "gradient norm (its table).";
+            "gradient norm (its table); linear_cross_entropy's eager calls.";
   py::object torch = py::module_::import("torch");
   g_tensor_type = reinterpret_cast<PyTypeObject *>(torch.attr("Tensor").ptr());
   g_param_type = reinterpret_cast<PyTypeObject *>(torch.attr("nn").attr("Parameter").ptr());
@@ -528,6 +662,8 @@ PYBIND11_MODULE(_luma_host, m) {
   m.def("same_pointers", &same_pointers);
   m.def("bump_steps", &bump_steps);
   m.def("grad_rows", &grad_rows);
+  m.def("xent", &xent);
+  m.def("xent_bind", &xent_bind);
   // the torch whose headers this module was compiled against: it reads
   // TensorImpl fields in that version's inline layout
   m.attr("torch_version") = LUMA_TORCH_VERSION;

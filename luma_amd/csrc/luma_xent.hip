@@ -102,19 +102,21 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
 }
 
 // Every token's (largest logit, sum of exp(l - largest)) over each tile's words:
-// part[tile of words][token]; picked[token] = the target's logit.
+// part[tile of words from v0][token]; picked[token] = the target's logit.
 template <int DT, typename S>
-__global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand x, int64_t v,
-                                                             int64_t n, int64_t h,
+__global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand x, int64_t v0,
+                                                             int64_t v, int64_t n, int64_t h,
                                                              const int64_t *target, Grid g,
                                                              float2 *part, float *picked) {
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
   Acc<DT, S> acc;
-  product<DT, kAlongK, kAlongK, kPlain, S>(w, x, (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0, h, acc);
+  product<DT, kAlongK, kAlongK, kPlain, S>(w, x, v0 + (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0,
+                                           h, acc);
   typedef Place<S, kPlain> P;
-  const P at(tm, tn);
-  const bool whole = (int64_t)(tm + 1) * S::BM <= v;
+  P at(tm, tn);
+  at.m += v0;
+  const bool whole = v0 + (int64_t)(tm + 1) * S::BM <= v;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const int wm = wave / S::WN, wn = wave % S::WN;
   __shared__ float2 records[S::WM][S::BN];
@@ -204,7 +206,7 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2 *part, 
   if (threadIdx.x >= 64) return;      // (the rest is the first wavefront's)
   double value = 0.0, count = 0.0;
   if (slice == 0) {
-    for (int s = 1; s < kJoinSlices; ++s) a = join(a, lds[s][tok]);
+    for (int s = 1; s < min(kJoinSlices, parts); ++s) a = join(a, lds[s][tok]);
     if (token < n) {
       const float lse = a.x == -__builtin_inff() ? __builtin_nanf("")
                                                  : a.x + __builtin_amdgcn_logf(a.y) * kLn2;
@@ -381,11 +383,15 @@ __global__ __launch_bounds__(256) void sum_kernel(const float *part, int splits,
   const float f = *back;
   for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < count; i += gridDim.x * 1024ll) {
     v4f s = {0.f, 0.f, 0.f, 0.f};
-    for (int k = 0; k < splits; ++k) {
-      const float *p = part + k * count + i;
+    if (i + 4 <= count) {
+      typedef float v4fu __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll 4
+      for (int k = 0; k < splits; ++k) s += *(const v4fu *)(part + k * count + i);
+    } else {
+      for (int k = 0; k < splits; ++k)
 #pragma unroll
-      for (int r = 0; r < 4; ++r)
-        if (i + r < count) s[r] += p[r];
+        for (int r = 0; r < 4; ++r)
+          if (i + r < count) s[r] += part[k * count + i + r];
     }
     store4<DT>(out, i, count, s * f);
   }
@@ -448,12 +454,24 @@ int64_t split_k(int shape, int64_t m, int64_t n, int64_t k, int64_t round, int64
   return tiles(k, each);
 }
 
-// Of `words` words, those whose 256 x 256 tiles of d_weight make whole rounds of
-// the chip (0: fewer than one).
-int64_t whole_rounds(int64_t h, int64_t words) {
-  const int64_t rows = tiles(h, 256), rounds = tiles(words, 256) * rows / kChip;
+// Of `words` words, those whose 256 x 256 tiles with `others` along the other
+// side make whole rounds of the chip (0: fewer than one round).
+int64_t whole_rounds(int64_t others, int64_t words) {
+  const int64_t rows = tiles(others, 256), rounds = tiles(words, 256) * rows / kChip;
   const int64_t main = kChip * rounds / rows * 256;
   return main < words ? main : words;
+}
+
+// Of `words` words of logits, those that take 256 x 256 tiles; the others take
+// 128 x 128, where that is shorter than a last round that few tiles fill (two of
+// them are on a CU at a time and take about 0.55 of a round; their launch
+// starts after the rounds').
+int64_t big_words(int64_t n, int64_t words) {
+  if (shape_for(words, n, 1) != kBig) return 0;
+  const int64_t main = whole_rounds(n, words);
+  if (main == 0 || main == words) return words;
+  const int64_t rest = tiles(words - main, 128) * tiles(n, 128);
+  return 0.55 * tiles(rest, 2 * kChip) + 0.1 < 1.0 ? main : words;
 }
 
 // Words per piece of the vocabulary: pieces of about equal length, each at most
@@ -471,7 +489,8 @@ struct Plan {
   bool pack_x, pack_w;
   int64_t ld_x, ld_w;           // elements, of what the products read
   int64_t at_x, at_w;           // of the packed copies
-  int logits;                   // tile shapes
+  int64_t big;                  // words of logits (of a piece) in 256 x 256 tiles
+  int rest;                     // tile shape of the others
   // forward
   int64_t parts, at_part, at_picked, at_sums, blocks;
   // backward
@@ -503,18 +522,22 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
     at += up(bytes, 256);
     return here;
   };
+  auto logits_plan = [&](int64_t words) {
+    p.big = big_words(a->n, words);
+    p.rest = p.big ? kMid : shape_for(words, a->n, 1);
+  };
   if (p.pack_x) p.at_x = take(a->n * p.ld_x * p.size);
   if (p.pack_w) p.at_w = take(a->v * p.ld_w * p.size);
   if (!backward) {
-    p.logits = shape_for(a->v, a->n, 1);
-    p.parts = tiles(a->v, kBM[p.logits]);
+    logits_plan(a->v);
+    p.parts = tiles(p.big, 256) + tiles(a->v - p.big, kBM[p.rest]);
     p.blocks = tiles(a->n, kJoinTokens);
     p.at_part = take(p.parts * a->n * sizeof(float2));
     p.at_picked = take(a->n * sizeof(float));
     p.at_sums = take(p.blocks * sizeof(double2));
   } else {
     p.piece = piece_for(a->n, a->v, p.size);
-    p.logits = shape_for(p.piece < a->v ? p.piece : a->v, a->n, 1);
+    logits_plan(p.piece);
     p.ld_d = p.piece;
     p.at_head = take(sizeof(Rows));
     p.at_rows = take(a->n * sizeof(float));
@@ -605,12 +628,17 @@ void forward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
   float2 *part = (float2 *)(ws + p.at_part);
   float *picked = (float *)(ws + p.at_picked);
   double2 *sums = a->reduction == LUMA_XENT_NONE ? nullptr : (double2 *)(ws + p.at_sums);
-  with_shape(p.logits, [&](auto shape) {
-    typedef decltype(shape) S;
-    const Grid g = grid_of(p.logits, a->v, a->n, 1);
-    logits_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(w, x, a->v, a->n, a->h,
-                                                                       a->target, g, part, picked);
-  });
+  auto logits = [&](int shape_id, int64_t v0, int64_t words, float2 *out) {
+    if (words == 0) return;
+    with_shape(shape_id, [&](auto shape) {
+      typedef decltype(shape) S;
+      const Grid g = grid_of(shape_id, words, a->n, 1);
+      logits_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(
+          w, x, v0, a->v, a->n, a->h, a->target, g, out, picked);
+    });
+  };
+  logits(kBig, 0, p.big, part);
+  logits(p.rest, p.big, a->v - p.big, part + tiles(p.big, 256) * a->n);
   join_kernel<<<(int)p.blocks, kJoinThreads, 0, s>>>(part, (int)p.parts, picked, a->target, a->n,
                                                      a->v, a->ignore_index, a->stats, a->loss,
                                                      sums);
@@ -644,12 +672,17 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
     const int64_t words = a->v - v0 < p.piece ? a->v - v0 : p.piece;
     // (the products take k up to the padding: D is 0 there)
     const int64_t padded = up(words, 256);
-    with_shape(p.logits, [&](auto shape) {
-      typedef decltype(shape) S;
-      const Grid g = grid_of(p.logits, padded, a->n, 1);
-      slope_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(
-          w, x, v0, a->v, a->n, a->h, a->target, a->stats, rows, g, d, p.ld_d);
-    });
+    auto slope = [&](int shape_id, int64_t w0, int64_t count) {
+      if (count <= 0) return;
+      with_shape(shape_id, [&](auto shape) {
+        typedef decltype(shape) S;
+        const Grid g = grid_of(shape_id, count, a->n, 1);
+        slope_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(
+            w, x, v0 + w0, a->v, a->n, a->h, a->target, a->stats, rows, g, d + w0, p.ld_d);
+      });
+    };
+    slope(kBig, 0, p.big < padded ? p.big : padded);
+    slope(p.rest, p.big, padded - p.big);
     const Operand wp = {w.p + v0 * w.ld, w.ld, words, w.row_bytes};
     if (a->d_hidden) {
       const Operand dk = {(const char *)d, p.ld_d * p.size, a->n, padded * p.size};

@@ -16,6 +16,7 @@ them, and they do no host synchronisation::
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import Tuple
 
 import torch
@@ -162,6 +163,23 @@ def _backward(ctx, grad, _):
 _forward_op.register_autograd(_backward, setup_context=_setup)
 
 
+@functools.lru_cache(maxsize=1)
+def _eager():
+    """The host module's form of both ops and their autograd node; None without it."""
+    host = L.load_host()
+    if host is not None:
+        lib = L.load()
+        host.xent_bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "luma_xent_workspace_bytes", "luma_xent_forward", "luma_xent_backward",
+            "luma_last_error")), torch._C._cuda_getCurrentRawStream)
+    return None if host is None else host.xent
+
+
+def _plain(*tensors) -> bool:
+    """Whether no tensor is of a subclass with a dispatch of its own."""
+    return all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
+
+
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
                          ignore_index: int = -100, reduction: str = "mean") -> torch.Tensor:
     """``F.cross_entropy`` of ``hidden @ weight.T`` against ``target``, float32.
@@ -184,8 +202,18 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
         dtype = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dtype), weight.to(dtype)
     _check_types(hidden, weight, target)
-    if not hidden.is_cuda:
+    shape = target.shape
+    if len(shape) != 1:
+        hidden, target = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
+    if torch.compiler.is_compiling():
+        loss, _ = torch.ops.luma_amd.linear_cross_entropy(hidden, weight, target, ignore_index,
+                                                          code)
+    else:
         _check(hidden, weight, target)
-    loss, _ = torch.ops.luma_amd.linear_cross_entropy(
-        hidden.reshape(-1, hidden.shape[-1]), weight, target.reshape(-1), ignore_index, code)
-    return loss.view(target.shape) if reduction == "none" else loss
+        eager = _eager() if _plain(hidden, weight, target) else None
+        if eager is not None:
+            loss = eager(hidden, weight, target, ignore_index, code)
+        else:
+            loss, _ = torch.ops.luma_amd.linear_cross_entropy(hidden, weight, target,
+                                                              ignore_index, code)
+    return loss.view(shape) if code == L.XENT_NONE and len(shape) != 1 else loss
