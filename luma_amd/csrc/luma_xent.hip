@@ -11,7 +11,8 @@
 //            d_weight's rows of the piece = D^T X and d_hidden += D W.
 //            r_i is the token's gradient times a power of two that brings the
 //            largest to about 2^kTop (float16's range is short); the products
-//            are scaled back in float32, which is exact.
+//            are scaled back in float32, which is exact.  For one gradient for
+//            all tokens (a mean, a sum) it is formed where it is used.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -254,30 +255,63 @@ __global__ __launch_bounds__(256) void reduce_kernel(const double2 *sums, int64_
 
 // -- backward -------------------------------------------------------------------
 
-// The header of the backward's row factors: what the products are scaled back by.
+// The header of the tokens' factors: what the products are scaled back by.
 struct Rows {
   float back;
   float pad[63];
 };
 
-// r_i, the gradient of each token's loss times a power of two; 0 for an ignored
-// target, NaN for one outside the vocabulary.
+// Each token's factor r_i: the gradient of its loss times a power of two that
+// brings the largest to 2^(TOP - 1) .. 2^TOP; 0 for an ignored target, NaN for
+// one outside the vocabulary.  One gradient for all tokens needs no pass over
+// them; with one per token, rows_kernel has looked for the largest.
+struct Factors {
+  const float *grad;
+  const int64_t *target;
+  const float *stats;
+  int64_t n, v, ignore;
+  int reduction;
+  Rows *head;       // rows_kernel's (LUMA_XENT_NONE)
+  float *rows;
+
+  __device__ __forceinline__ float grad_of(int64_t i) const {
+    if (reduction == LUMA_XENT_NONE) return grad[i];
+    return reduction == LUMA_XENT_MEAN ? grad[0] / stats[n] : grad[0];
+  }
+  __device__ __forceinline__ float factor(int64_t t, float g) const {
+    return t == ignore ? 0.0f : t >= 0 && t < v ? g : __builtin_nanf("");
+  }
+  // the exponent of the power of two, of the largest finite |g|
+  template <int TOP>
+  static __device__ __forceinline__ int power(float top) {
+    if (!(top > 0.0f && top < __builtin_inff())) return 0;
+    int e;
+    __builtin_frexpf(top, &e);           // top = f 2^e, f in [0.5, 1)
+    e = TOP - e;
+    return e > 100 ? 100 : e < -100 ? -100 : e;
+  }
+  template <int TOP>
+  __device__ __forceinline__ float row(int64_t i, int64_t t) const {
+    if (reduction == LUMA_XENT_NONE) return rows[i];
+    const float g = grad_of(0);
+    return factor(t, g * __builtin_ldexpf(1.0f, power<TOP>(__builtin_fabsf(g))));
+  }
+  template <int TOP>
+  __device__ __forceinline__ float back() const {
+    if (reduction == LUMA_XENT_NONE) return head->back;
+    return __builtin_ldexpf(1.0f, -power<TOP>(__builtin_fabsf(grad_of(0))));
+  }
+};
+
+template <int DT>
+constexpr int kTop = DT == LUMA_GRAD_F16 ? 15 : 0;
+
 template <int TOP>
-__global__ __launch_bounds__(1024) void rows_kernel(const float *grad, const int64_t *target,
-                                                    const float *stats, int64_t n, int64_t v,
-                                                    int64_t ignore, int reduction, Rows *head,
-                                                    float *rows) {
+__global__ __launch_bounds__(1024) void rows_kernel(Factors f) {
   __shared__ float lds[16];
-  const float scale = reduction == LUMA_XENT_MEAN ? 1.0f / stats[n] : 1.0f;
-  auto value = [&](int64_t i) -> float {
-    const int64_t t = target[i];
-    if (t == ignore) return 0.0f;
-    if (t < 0 || t >= v) return __builtin_nanf("");
-    return reduction == LUMA_XENT_NONE ? grad[i] : grad[0] * scale;
-  };
   float top = 0.0f;      // the largest finite |g|
-  for (int64_t i = threadIdx.x; i < n; i += 1024) {
-    const float a = __builtin_fabsf(value(i));
+  for (int64_t i = threadIdx.x; i < f.n; i += 1024) {
+    const float a = __builtin_fabsf(f.factor(f.target[i], f.grad[i]));
     if (a < __builtin_inff()) top = fmaxf(top, a);
   }
 #pragma unroll
@@ -286,15 +320,11 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float *grad, const int
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 16; ++w) top = fmaxf(top, lds[w]);
-  int e = 0;
-  if (top > 0.0f) {
-    __builtin_frexpf(top, &e);           // top = f 2^e, f in [0.5, 1)
-    e = TOP - e;
-    e = e > 100 ? 100 : e < -100 ? -100 : e;
-  }
+  const int e = Factors::power<TOP>(top);
   const float up = __builtin_ldexpf(1.0f, e);
-  for (int64_t i = threadIdx.x; i < n; i += 1024) rows[i] = value(i) * up;
-  if (threadIdx.x == 0) head->back = __builtin_ldexpf(1.0f, -e);
+  for (int64_t i = threadIdx.x; i < f.n; i += 1024)
+    f.rows[i] = f.factor(f.target[i], f.grad[i] * up);
+  if (threadIdx.x == 0) f.head->back = __builtin_ldexpf(1.0f, -e);
 }
 
 // (Eight words of a token are a lane's: 16-byte stores.)
@@ -302,9 +332,8 @@ __global__ __launch_bounds__(1024) void rows_kernel(const float *grad, const int
 template <int DT, typename S>
 __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x, int64_t v0,
                                                             int64_t v, int64_t n, int64_t h,
-                                                            const int64_t *target,
-                                                            const float *stats, const float *rows,
-                                                            Grid g, typename Elem<DT>::type *d,
+                                                            Factors factors, Grid g,
+                                                            typename Elem<DT>::type *d,
                                                             int64_t ld) {
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
@@ -317,8 +346,9 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
   for (int j = 0; j < S::TN; ++j) {
     const int64_t token = at.n + 16 * j;
     if (token >= n) continue;
-    const float base = stats[token] * kLog2e, row = rows[token];
-    const int64_t t = target[token] - v0 - at.m;
+    const int64_t word = factors.target[token];
+    const float base = factors.stats[token] * kLog2e, row = factors.row<kTop<DT>>(token, word);
+    const int64_t t = word - v0 - at.m;
     typename Elem<DT>::type *out = d + token * ld + at.m;
 #pragma unroll
     for (int q = 0; q < S::TM; q += 2) {
@@ -338,12 +368,12 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
 }
 
 // A product into float32 (out[split][n][m], added to what is there with `add`)
-// or, with out16, times *back into the operands' type.
+// or, with out16, scaled back into the operands' type.
 template <int DT, int AB, typename S>
 __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand b, int64_t m,
                                                               int64_t n, int64_t k,
                                                               int64_t k_split, Grid g, int add,
-                                                              float *out, const float *back,
+                                                              float *out, Factors factors,
                                                               typename Elem<DT>::type *out16) {
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
@@ -352,7 +382,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand
   product<DT, kAlongM, AB, kPlain, S>(a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
   typedef Place<S, kPlain> P;
   const P at(tm, tn);
-  const float f = out16 ? *back : 1.0f;
+  const float f = out16 ? factors.back<kTop<DT>>() : 1.0f;
 #pragma unroll
   for (int j = 0; j < S::TN; ++j) {
     const int64_t row = at.n + 16 * j;
@@ -375,12 +405,12 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand
   }
 }
 
-// The sum of `splits` float32 products, times *back, in the operands' type.
+// The sum of `splits` float32 products, scaled back, in the operands' type.
 template <int DT>
 __global__ __launch_bounds__(256) void sum_kernel(const float *part, int splits, int64_t count,
-                                                  const float *back,
+                                                  Factors factors,
                                                   typename Elem<DT>::type *out) {
-  const float f = *back;
+  const float f = factors.back<kTop<DT>>();
   for (int64_t i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < count; i += gridDim.x * 1024ll) {
     v4f s = {0.f, 0.f, 0.f, 0.f};
     if (i + 4 <= count) {
@@ -647,11 +677,11 @@ void forward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
 }
 
 template <int DT>
-void sum_splits(const float *part, int64_t splits, int64_t count, const float *back, void *out,
-                hipStream_t s) {
+void sum_splits(const float *part, int64_t splits, int64_t count, const Factors &factors,
+                void *out, hipStream_t s) {
   const int64_t blocks = tiles(count, 1024);
   sum_kernel<DT><<<(int)(blocks < 4096 ? blocks : 4096), 256, 0, s>>>(
-      part, (int)splits, count, back, (typename Elem<DT>::type *)out);
+      part, (int)splits, count, factors, (typename Elem<DT>::type *)out);
 }
 
 template <int DT>
@@ -664,8 +694,9 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
   float *rows = (float *)(ws + p.at_rows);
   T *d = (T *)(ws + p.at_d);
   float *hidden = (float *)(ws + p.at_hidden), *weight = (float *)(ws + p.at_weight);
-  rows_kernel<(DT == LUMA_GRAD_F16 ? 15 : 0)><<<1, 1024, 0, s>>>(
-      a->grad_loss, a->target, a->stats, a->n, a->v, a->ignore_index, a->reduction, head, rows);
+  const Factors factors = {a->grad_loss, a->target,    a->stats, a->n, a->v,
+                           a->ignore_index, a->reduction, head,     rows};
+  if (a->reduction == LUMA_XENT_NONE) rows_kernel<kTop<DT>><<<1, 1024, 0, s>>>(factors);
   const bool whole = p.piece >= a->v;        // one piece
   const bool direct = p.hidden_splits == 1 && whole;
   for (int64_t v0 = 0; v0 < a->v; v0 += p.piece) {
@@ -678,7 +709,7 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
         typedef decltype(shape) S;
         const Grid g = grid_of(shape_id, count, a->n, 1);
         slope_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(
-            w, x, v0 + w0, a->v, a->n, a->h, a->target, a->stats, rows, g, d + w0, p.ld_d);
+            w, x, v0 + w0, a->v, a->n, a->h, factors, g, d + w0, p.ld_d);
       });
     };
     slope(kBig, 0, p.big < padded ? p.big : padded);
@@ -690,7 +721,7 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
         typedef decltype(shape) S;
         const Grid g = grid_of(p.hidden, a->h, a->n, p.hidden_splits);
         product_kernel<DT, kAlongK, S><<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
-            wp, dk, a->h, a->n, padded, p.hidden_k, g, v0 > 0, hidden, &head->back,
+            wp, dk, a->h, a->n, padded, p.hidden_k, g, v0 > 0, hidden, factors,
             direct ? (T *)a->d_hidden : nullptr);
       });
     }
@@ -714,16 +745,16 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
             const Grid g = grid_of(shape_id, a->h, count, splits);
             product_kernel<DT, kAlongM, S>
                 <<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
-                    x, dm, a->h, count, a->n, each, g, 0, weight, &head->back,
+                    x, dm, a->h, count, a->n, each, g, 0, weight, factors,
                     splits == 1 ? out : nullptr);
           }
         });
-        if (splits > 1) sum_splits<DT>(weight, splits, count * a->h, &head->back, out, s);
+        if (splits > 1) sum_splits<DT>(weight, splits, count * a->h, factors, out, s);
       }
     }
   }
   if (a->d_hidden && !direct)
-    sum_splits<DT>(hidden, p.hidden_splits, a->n * a->h, &head->back, a->d_hidden, s);
+    sum_splits<DT>(hidden, p.hidden_splits, a->n * a->h, factors, a->d_hidden, s);
 }
 
 template <typename F>
