@@ -52,12 +52,20 @@ def _max_norm(max_norm) -> float:
     return max_norm
 
 
-class _Batch:
-    """Dense gradients on one device as the rows of one call."""
+# Up to this many rows travel as launch arguments, a launch for each 144; more
+# take a device table (a copy of 24 bytes per row, which a launch or two less
+# does not pay for).
+_NO_TABLE = 2 * L.GRADS_INLINE
 
-    def __init__(self, rows: np.ndarray, device: torch.device, hold=None):
+
+class _Batch:
+    """Dense gradients on one device as the rows of one call: a numpy array, or
+    (host) a pinned tensor that holds them."""
+
+    def __init__(self, rows: np.ndarray, device: torch.device, host=None, hold=None):
         self.rows = rows
         self.device = device
+        self.host = host
         self.hold = hold      # keeps tensors alive that only the rows point to
 
     def args(self, norm: int, max_norm: float, total: Optional[torch.Tensor],
@@ -66,10 +74,11 @@ class _Batch:
         device copy of the rows) of their own."""
         partials = torch.empty(L.NORM_PARTIALS, dtype=torch.float64, device=self.device)
         table, n = None, len(self.rows)
-        if n > L.GRADS_INLINE and not torch.cuda.is_current_stream_capturing():
-            host = torch.empty(self.rows.nbytes, dtype=torch.uint8, pin_memory=True)
-            ctypes.memmove(host.data_ptr(), self.rows.ctypes.data, self.rows.nbytes)
-            table = host.to(self.device, non_blocking=True)
+        if n > _NO_TABLE and not torch.cuda.is_current_stream_capturing():
+            host = self.host
+            if host is None:
+                host = torch.from_numpy(self.rows.view(np.uint8)).pin_memory()
+            table = host[:n * L.GRAD_DTYPE.itemsize].to(self.device, non_blocking=True)
         self.keep = (partials, table)
         return L.NormArgs(
             grads=self.rows.ctypes.data, table=None if table is None else table.data_ptr(), n=n,
@@ -97,12 +106,19 @@ def _as_list(tensors: _Tensors) -> List[torch.Tensor]:
 
 def _quick(tensors, of_grad: bool, apart: bool) -> Optional[_Batch]:
     """The rows by the host module, where every gradient can be taken as it is."""
-    host = _host()
-    got = None if host is None else host.grad_rows(tensors, of_grad, apart)
+    module = _host()
+    if module is None:
+        return None
+    host, n = None, len(tensors)
+    if n > _NO_TABLE and torch.cuda.is_available():
+        host = torch.empty(n * L.GRAD_DTYPE.itemsize, dtype=torch.uint8, pin_memory=True)
+        rows = host.numpy().view(L.GRAD_DTYPE)
+    else:
+        rows = np.empty(n, dtype=L.GRAD_DTYPE)
+    got = module.grad_rows(tensors, of_grad, apart, rows.ctypes.data)
     if got is None:
         return None
-    data, device = got
-    return _Batch(np.frombuffer(data, dtype=L.GRAD_DTYPE), torch.device("cuda", max(device, 0)))
+    return _Batch(rows[:got[0]], torch.device("cuda", max(got[1], 0)), host)
 
 
 def _rows(grads, device) -> np.ndarray:
@@ -163,7 +179,7 @@ class _Slow:
                 g = dense
             self.sharded.setdefault(key, []).append(g)
         self.device = device
-        self.batches = [(key, _Batch(_rows([g for g in gs if g.numel()], device), device, gs))
+        self.batches = [(key, _Batch(_rows([g for g in gs if g.numel()], device), device, hold=gs))
                         for key, gs in self.sharded.items()]
         if apart:
             _check_apart([g for gs in self.sharded.values() for g in gs if g.numel()])

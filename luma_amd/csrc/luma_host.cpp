@@ -410,11 +410,13 @@ struct GradRow {
 static_assert(sizeof(GradRow) == 24, "LumaGrad");
 constexpr int64_t kGradTile = 2048;   // LUMA_GRAD_TILE
 
-// One part's rows; false for a tensor that the kernels cannot take as it is.
-// *device: the CUDA device of all of them (-1 before the first).
-bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<GradRow> &rows,
+// One part's *count rows, their first_tile within the part; false for a tensor
+// that the kernels cannot take as it is.  *device: the CUDA device of all of them
+// (-1 for none).
+bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, GradRow *rows, int64_t *count,
                 int64_t *device) noexcept {
-  int64_t dev = -1;     // (not *device: its neighbours are other threads')
+  int64_t dev = -1, tiles = 0;     // (not *device: its neighbours are other threads')
+  GradRow *row = rows;
   try {
     std::vector<const c10::TensorImpl *> impl(n);
     for (int64_t i = 0; i < n; ++i) {
@@ -440,7 +442,6 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<Grad
         }
       }
     }
-    rows.reserve(n);
     for (int64_t i = 0; i < n; ++i) {
       if (i + kAhead < n && impl[i + kAhead]) prefetch_impl(impl[i + kAhead]);
       const c10::TensorImpl *g = impl[i];
@@ -456,9 +457,13 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<Grad
       if (g->numel() == 0) continue;
       const uint64_t p = (uint64_t)(uintptr_t)g->data();
       if (!p) return false;
-      rows.push_back({p, g->numel(), code, 0});
+      if (tiles > INT32_MAX) return false;
+      *row++ = {p, g->numel(), code, (int32_t)tiles};
+      tiles += (g->numel() - 1) / kGradTile + 1;
     }
+    if (tiles > INT32_MAX) return false;
     *device = dev;
+    *count = row - rows;
     return true;
   } catch (...) {
     return false;   // an unusual tensor: the caller looks at it
@@ -466,58 +471,61 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, std::vector<Grad
 }
 
 // Whether no two rows share memory.
-bool disjoint(const std::vector<GradRow> &rows) {
-  auto bytes = [](const GradRow &r) { return (uint64_t)r.numel * (r.dtype == 0 ? 4 : 2); };
+bool disjoint(const GradRow *rows, int64_t n) {
+  auto end = [](const GradRow &r) { return r.data + (uint64_t)r.numel * (r.dtype == 0 ? 4 : 2); };
   bool up = true, down = true;
-  for (size_t i = 1; i < rows.size() && (up || down); ++i) {
-    up &= rows[i - 1].data + bytes(rows[i - 1]) <= rows[i].data;
-    down &= rows[i].data + bytes(rows[i]) <= rows[i - 1].data;
+  for (int64_t i = 1; i < n && (up || down); ++i) {
+    up &= end(rows[i - 1]) <= rows[i].data;
+    down &= end(rows[i]) <= rows[i - 1].data;
   }
   if (up || down) return true;
-  std::vector<std::pair<uint64_t, uint64_t>> spans(rows.size());
-  for (size_t i = 0; i < rows.size(); ++i)
-    spans[i] = {rows[i].data, rows[i].data + bytes(rows[i])};
+  std::vector<std::pair<uint64_t, uint64_t>> spans(n);
+  for (int64_t i = 0; i < n; ++i) spans[i] = {rows[i].data, end(rows[i])};
   std::sort(spans.begin(), spans.end());
-  for (size_t i = 1; i < spans.size(); ++i)
+  for (int64_t i = 1; i < n; ++i)
     if (spans[i].first < spans[i - 1].second) return false;
   return true;
 }
 
-// (rows as bytes, device index) of the tensors in objs (of_grad: of their
-// gradients, those without one left out), or None when one of them is a
+// Writes the rows of the tensors in objs (of_grad: of their gradients, those
+// without one left out) to `table`, which has room for one per object.  Returns
+// (rows, device index or -1 for no rows), or None when one of them is a
 // subclass, sparse, not dense, of another type or device, or (apart) shares
-// memory with another: the caller then looks at each.  device is -1 for none.
-py::object grad_rows(py::list objs, bool of_grad, bool apart) {
+// memory with another: the caller then looks at each.
+py::object grad_rows(py::list objs, bool of_grad, bool apart, uintptr_t table) {
   const int64_t n = (int64_t)objs.size();
   PyObject *const *o = n ? &PyList_GET_ITEM(objs.ptr(), 0) : nullptr;
+  GradRow *rows = reinterpret_cast<GradRow *>(table);
   const int T = (int)std::min<int64_t>(kMaxThreads, std::max<int64_t>(1, n / kPerThread));
-  std::vector<std::vector<GradRow>> part(T);
-  std::vector<int64_t> device(T, -1);
-  std::vector<char> ok(T, 0);
+  int64_t device[kMaxThreads], count[kMaxThreads];
+  bool ok[kMaxThreads];
   const std::function<void(int)> job = [&](int t) {
     const int64_t a = n * t / T, b = n * (t + 1) / T;
-    ok[t] = grad_range(o + a, b - a, of_grad, part[t], &device[t]);
+    ok[t] = grad_range(o + a, b - a, of_grad, rows + a, &count[t], &device[t]);
   };
   if (T == 1)
     job(0);
   else
     Pool::get().run(T, job);
-  int64_t dev = -1;
-  std::vector<GradRow> &rows = part[0];
+  int64_t dev = -1, at = 0, tiles = 0;
   for (int t = 0; t < T; ++t) {
     if (!ok[t] || (device[t] >= 0 && dev >= 0 && device[t] != dev)) return py::none();
     if (device[t] >= 0) dev = device[t];
-    if (t) rows.insert(rows.end(), part[t].begin(), part[t].end());
+    // the part's rows behind those of the parts before it
+    const GradRow *from = rows + n * t / T;
+    int64_t last = tiles;
+    for (int64_t i = 0; i < count[t]; ++i) {
+      GradRow r = from[i];
+      const int64_t first = tiles + r.first_tile;
+      last = first + (r.numel - 1) / kGradTile + 1;
+      if (last > INT32_MAX) return py::none();
+      r.first_tile = (int32_t)first;
+      rows[at++] = r;
+    }
+    tiles = last;
   }
-  int64_t tiles = 0;
-  for (GradRow &r : rows) {
-    if (tiles > INT32_MAX) return py::none();
-    r.first_tile = (int32_t)tiles;
-    tiles += (r.numel - 1) / kGradTile + 1;
-  }
-  if (apart && !disjoint(rows)) return py::none();
-  return py::make_tuple(
-      py::bytes(reinterpret_cast<const char *>(rows.data()), rows.size() * sizeof(GradRow)), dev);
+  if (apart && !disjoint(rows, at)) return py::none();
+  return py::make_tuple(at, dev);
 }
 
 // -- linear_cross_entropy's calls ---------------------------------------------

@@ -10,6 +10,9 @@
 // a 64-way search (a 20,000-row table takes three loads) and walks on from
 // there, so a row of one element costs one iteration and not a workgroup, and
 // a long row is read in 16-byte loads, kInFlight of them in flight per lane.
+// The norm's loads are non-temporal (2.8e9 bfloat16: 914 us, so 815, 6.9 TB/s;
+// in the scaling, which finds part of the rows in the last-level cache, they
+// cost a tenth).  Loading rows and tiles a step ahead gained nothing.
 // Partial sums go to one double per workgroup; the kernel behind (the join, or
 // every workgroup of the scaling) sums those in a fixed order: no atomics, so
 // no order that changes from run to run, and no counter to reset.
@@ -26,7 +29,9 @@ namespace {
 
 constexpr int kWaves = 8;                 // wavefronts per workgroup
 constexpr int kThreads = 64 * kWaves;
-constexpr int kBlocks = LUMA_NORM_PARTIALS;   // four workgroups to a CU: every wavefront slot
+// Two workgroups to a CU (1,024 in two rounds: 141 us for the norm of 20,000
+// tensors of 118M float32 together, 512: 112).
+constexpr int kBlocks = 512;
 constexpr int kInFlight = 8;
 constexpr float kTiny = 1e-6f;            // torch's guard against a norm of zero
 
@@ -159,21 +164,24 @@ __device__ __forceinline__ int find_row(const LumaGrad *rows, int n, int t) {
   return __builtin_amdgcn_readfirstlane(lo);
 }
 
-// Runs f(type, data, first element, end element) over this wavefront's share
-// of the tiles [base, base + tiles).
-template <typename F>
+// Runs f(row, first element, end element) over this wavefront's share of the
+// tiles [base, base + tiles), upwards or (DOWN) from its end.
+template <bool DOWN, typename F>
 __device__ __forceinline__ void walk(const LumaGrad *rows, int n, int base, int tiles, F f) {
   const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
   const int64_t w = (int64_t)blockIdx.x * kWaves + wave, W = (int64_t)gridDim.x * kWaves;
   int t = base + (int)(tiles * w / W);
-  const int end = base + (int)(tiles * (w + 1) / W);
+  int end = base + (int)(tiles * (w + 1) / W);
   if (t >= end) return;
-  for (int r = find_row(rows, n, t); t < end; ++r) {
+  for (int r = find_row(rows, n, DOWN ? end - 1 : t); t < end; r += DOWN ? -1 : 1) {
     const LumaGrad g = rows[r];
-    const int64_t a = (int64_t)(t - g.first_tile) * LUMA_GRAD_TILE;
+    const int64_t a = (int64_t)max(t - g.first_tile, 0) * LUMA_GRAD_TILE;
     const int64_t b = min(g.numel, (int64_t)(end - g.first_tile) * LUMA_GRAD_TILE);
     f(g, a, b);
-    t = g.first_tile + (int)((g.numel + LUMA_GRAD_TILE - 1) / LUMA_GRAD_TILE);
+    if (DOWN)
+      end = g.first_tile;
+    else
+      t = g.first_tile + (int)((g.numel + LUMA_GRAD_TILE - 1) / LUMA_GRAD_TILE);
   }
 }
 
@@ -188,14 +196,14 @@ __device__ __forceinline__ void sum_span(const void *data, int64_t a, int64_t b,
   for (; i + (int64_t)(kInFlight - 1) * kStep + T::kVec <= b; i += kInFlight * kStep) {
     vec v[kInFlight];
 #pragma unroll
-    for (int k = 0; k < kInFlight; ++k) v[k] = *(const vec *)(p + i + k * kStep);
+    for (int k = 0; k < kInFlight; ++k) v[k] = __builtin_nontemporal_load((const vec *)(p + i + k * kStep));
 #pragma unroll
     for (int k = 0; k < kInFlight; ++k)
 #pragma unroll
       for (int j = 0; j < T::kVec; ++j) sum.take(T::get(v[k], j));
   }
   for (; i + T::kVec <= b; i += kStep) {
-    const vec v = *(const vec *)(p + i);
+    const vec v = __builtin_nontemporal_load((const vec *)(p + i));
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) sum.take(T::get(v, j));
   }
@@ -208,7 +216,7 @@ __device__ __forceinline__ void norm_body(const LumaGrad *rows, int n, int base,
                                           double *partials) {
   __shared__ double lds[kWaves];
   Sum<NORM> sum;
-  walk(rows, n, base, tiles, [&](const LumaGrad &g, int64_t a, int64_t b) {
+  walk<false>(rows, n, base, tiles, [&](const LumaGrad &g, int64_t a, int64_t b) {
     if (g.dtype == LUMA_GRAD_F32)
       sum_span<LUMA_GRAD_F32>(g.data, a, b, sum);
     else if (g.dtype == LUMA_GRAD_BF16)
@@ -267,6 +275,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const double *partials, 
   if (step_scale) *step_scale = scale / clip_factor(norm, max_norm);
 }
 
+// From the end down: what the norm read last is read first, while the last-level
+// cache (256 MB) still holds it.
 template <int DT>
 __device__ __forceinline__ void scale_span(void *data, int64_t a, int64_t b, float c) {
   typedef Type<DT> T;
@@ -274,23 +284,26 @@ __device__ __forceinline__ void scale_span(void *data, int64_t a, int64_t b, flo
   constexpr int kStep = 64 * T::kVec;
   typename T::elem *p = (typename T::elem *)data;
   const int lane = threadIdx.x & 63;
-  int64_t i = a + lane * T::kVec;
+  const int64_t last = a + ((b - a) & ~(int64_t)(T::kVec - 1)) + lane;   // the row's partial group
+  if (last < b) p[last] = T::round(times(T::one(p[last]), c));
   auto scaled = [&](const vec &v) {
     vec o;
 #pragma unroll
     for (int j = 0; j < T::kVec; ++j) T::put(o, j, times(T::get(v, j), c));
     return o;
   };
-  for (; i + (int64_t)(kInFlight - 1) * kStep + T::kVec <= b; i += kInFlight * kStep) {
+  // whole steps of the wavefront and one that some lanes have
+  int64_t i = a + ((b - a) / kStep * kStep) + lane * T::kVec;
+  if (i + T::kVec <= b) *(vec *)(p + i) = scaled(*(const vec *)(p + i));
+  i -= kStep;
+  for (; i - (int64_t)(kInFlight - 1) * kStep >= a; i -= kInFlight * kStep) {
     vec v[kInFlight];
 #pragma unroll
-    for (int k = 0; k < kInFlight; ++k) v[k] = *(const vec *)(p + i + k * kStep);
+    for (int k = 0; k < kInFlight; ++k) v[k] = *(const vec *)(p + i - k * kStep);
 #pragma unroll
-    for (int k = 0; k < kInFlight; ++k) *(vec *)(p + i + k * kStep) = scaled(v[k]);
+    for (int k = 0; k < kInFlight; ++k) *(vec *)(p + i - k * kStep) = scaled(v[k]);
   }
-  for (; i + T::kVec <= b; i += kStep) *(vec *)(p + i) = scaled(*(const vec *)(p + i));
-  const int64_t last = a + ((b - a) & ~(int64_t)(T::kVec - 1)) + lane;
-  if (last < b) p[last] = T::round(times(T::one(p[last]), c));
+  for (; i >= a; i -= kStep) *(vec *)(p + i) = scaled(*(const vec *)(p + i));
 }
 
 // NORM < 0: the norm is *total's; else from the partial sums (workgroup 0
@@ -312,7 +325,7 @@ __device__ __forceinline__ void scale_body(const LumaGrad *rows, int n, int base
   }
   const float c = clip_factor(norm, max_norm);
   if (c == 1.0f) return;
-  walk(rows, n, base, tiles, [&](const LumaGrad &g, int64_t a, int64_t b) {
+  walk<true>(rows, n, base, tiles, [&](const LumaGrad &g, int64_t a, int64_t b) {
     if (g.dtype == LUMA_GRAD_F32)
       scale_span<LUMA_GRAD_F32>(g.data, a, b, c);
     else if (g.dtype == LUMA_GRAD_BF16)

@@ -93,12 +93,14 @@ def test_host_module_leaves_what_it_cannot_take():
     host = L.load_host()
     if host is None:
         pytest.skip("the host module is not built")
-    assert host.grad_rows([], True, True) == (b"", -1)
+    rows = np.zeros(1, dtype=L.GRAD_DTYPE)
+    at = rows.ctypes.data
+    assert host.grad_rows([], True, True, at) == (0, -1)
     p = torch.nn.Parameter(torch.ones(3))
-    assert host.grad_rows([p], True, True) == (b"", -1)      # no gradient
+    assert host.grad_rows([p], True, True, at) == (0, -1)      # no gradient
     p.grad = torch.ones(3)
-    assert host.grad_rows([p], True, True) is None           # not on a GPU
-    assert host.grad_rows([3], True, True) is None
+    assert host.grad_rows([p], True, True, at) is None           # not on a GPU
+    assert host.grad_rows([3], True, True, at) is None
 
 
 def _join(rank, world, path, out):
