@@ -3,20 +3,21 @@
 // with either operand stored k-contiguous or m- (n-) contiguous.
 //
 // A workgroup's K loop runs in stages of 64 bytes of k per row (32 elements of
-// 16 bits, 16 of float32).  Stages go from memory into LDS without passing
-// registers (16 bytes a lane), kStages of them in a ring, two in flight while
-// one is multiplied; each wavefront reads the fragments of the stage behind
-// into a second set of registers while the matrix unit works on the first.
+// 16 bits, 16 of float32), two to a pair.  Pairs go from memory into LDS without
+// passing registers (16 bytes a lane), one under way while the other is
+// multiplied, with one barrier a pair; each wavefront reads the fragments of the
+// next stage into a second set of registers while the matrix unit works on the
+// first.
 // Fragments are 16 bytes a lane: lane l of a 16x16 tile holds row l % 16 and
 // the 16 bytes of k at 16 * (l / 16), which is what v_mfma_f32_16x16x32 takes;
 // four v_mfma_f32_16x16x4_f32 take its four floats (any order of k serves, as
 // long as both operands have it).  An m-contiguous operand of 16 bits is read
 // with ds_read_b64_tr_b16, which turns a 4 x 16 block on the way.
 //
-// The rows of a stage lie in LDS without padding (what the direct loads need),
-// their 16-byte chunks permuted so that the lanes of one read meet different
-// banks: k-contiguous rows of 64 bytes by chunk ^ (a function of the row), m-contiguous
-// ones by whole 16-element blocks, block ^ (a function of k).
+// The rows lie in LDS without padding (what the direct loads need), their
+// 16-byte chunks permuted so that the lanes of one read meet different banks:
+// k-contiguous rows by chunk ^ (row % 8), m-contiguous ones by whole 16-element
+// blocks, block ^ (a function of k).
 //
 // Loads go through buffer descriptors that end where the operand ends: rows
 // past the end read as zeros, and so does k past the end of a k-contiguous row
@@ -40,7 +41,7 @@ typedef _Float16 v8h __attribute__((ext_vector_type(8)));
 typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int kRow = 64;       // bytes of k per stage and row
-constexpr int kStages = 4;
+constexpr int kStages = 4;     // in LDS: two pairs
 
 // Which direction of an operand is contiguous.
 constexpr int kAlongK = 0, kAlongM = 1;
@@ -125,29 +126,25 @@ __device__ __forceinline__ constexpr int row_of(int i, int r) {
   return ORDER == kPaired ? 8 * (r >> 2) + 4 * i + (r & 3) : 16 * i + r;
 }
 
-// One operand's stages: ROWS of m (or n) by 64 bytes of k.
+// One operand's pairs of stages: ROWS of m (or n) by 128 bytes of k.  In LDS, a
+// kAlongK pair is ROWS lines of 128 bytes (a whole cache line of the operand: its
+// two stages are its halves), a kAlongM pair a line of ROWS elements for each k.
 template <int DT, int ALONG, int ORDER, int ROWS, int THREADS>
 struct Tile {
-  static constexpr int kBytes = ROWS * kRow;
+  static constexpr int kBytes = 2 * ROWS * kRow;                // of a pair
   static constexpr int kWaves = THREADS / 64;
   // 1 KB loads of a wavefront; with more wavefronts than loads some load the same bytes twice
   static constexpr int kTotal = kBytes / 1024;
   static constexpr int kLoads = (kTotal + kWaves - 1) / kWaves;
   static_assert(kBytes % 1024 == 0 && (kTotal % kWaves == 0 || kTotal < kWaves), "tile size");
-  static constexpr int kLine = ROWS * kSize<DT>;                // bytes of a kAlongM row
+  static constexpr int kLine = ROWS * kSize<DT>;                // bytes of a kAlongM line
   static constexpr int kBlock = 16 * kSize<DT>;                 // bytes of 16 elements
   static constexpr int kTurn = kLine / kBlock - 1;              // mask of block numbers
-
-  // The chunk in whose place a kAlongK row's chunk lies: chunk ^ this (of the
-  // eight rows that eight lanes read, two share it, one in each half of 128 bytes).
-  static __device__ __forceinline__ int swap(int row) {
-    return ORDER == kPaired ? ((row >> 1) & 1) | ((row >> 2) & 2) : (row >> 1) & 3;
-  }
 
   const char *base;      // of the next pair of stages to be loaded
   int64_t left;          // bytes from base to the operand's end
   int64_t step;          // bytes from pair to pair
-  int past;              // kAlongK: this lane's first byte of k past the row's end is at < 0
+  int past;              // kAlongK: < 0 where this lane's chunk is past the row's end
   int at_lds[kLoads];
   uint32_t voff[kLoads];
 
@@ -164,9 +161,9 @@ struct Tile {
       at_lds[q] = ((wave * kLoads + q) % kTotal) * 1024;
       const int at = at_lds[q] + lane * 16;
       if (ALONG == kAlongK) {
-        const int row = at / kRow, pos = (at % kRow) / 16;
-        // (every row of this lane has the same chunk)
-        const int chunk = (pos ^ swap(row)) * 16;
+        // (line r % 8 is the same for all of a lane's loads, and so is the chunk)
+        const int line = at / (2 * kRow), chunk = (at % (2 * kRow) / 16 ^ (line & 7)) * 16;
+        const int row = line / 32 * 32 + row_of<ORDER>(line / 16 % 2, line % 16);
         voff[q] = (uint32_t)(row * o.ld) + chunk;
         const int64_t kl = o.row_bytes - k0 * kSize<DT>;
         past = (int)(kl < 0x40000000 ? kl : 0x40000000) - 1 - chunk;
@@ -178,25 +175,20 @@ struct Tile {
     }
   }
 
-  // Sends the next pair of stages on its way into s0 and s1.
-  __device__ __forceinline__ void load(char *s0, char *s1) {
+  // Sends the next pair of stages on its way into s.  ONCE: nothing else reads
+  // these bytes (non-temporal).
+  template <bool ONCE>
+  __device__ __forceinline__ void load(char *s) {
     typedef __attribute__((address_space(3))) void lds_void;
     const int high = (int)(left >> 31);
     const int records = high == 0 ? (int)left : high < 0 ? 0 : 0x7FFFFFFF;
     const auto rsrc = __builtin_amdgcn_make_buffer_rsrc((void *)base, 0, records, 0x00020000);
     // (an offset past any end where k is)
-    const uint32_t none0 = ALONG == kAlongK ? past & 0x80000000u : 0u;
-    const uint32_t none1 = ALONG == kAlongK ? (past - kRow) & 0x80000000u : 0u;
-    // (not as the instruction's offset, which moves the place in LDS too)
-    const uint32_t next = ALONG == kAlongK ? kRow : (uint32_t)(step >> 1);
+    const uint32_t none = ALONG == kAlongK ? past & 0x80000000u : 0u;
 #pragma unroll
     for (int q = 0; q < kLoads; ++q)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(s0 + at_lds[q]), 16,
-                                               voff[q] | none0, 0, 0, 0);
-#pragma unroll
-    for (int q = 0; q < kLoads; ++q)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(s1 + at_lds[q]), 16,
-                                               (voff[q] + next) | none1, 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void *)(s + at_lds[q]), 16,
+                                               voff[q] | none, 0, 0, ONCE ? 2 : 0);
     base += step;
     left -= step;
     if (ALONG == kAlongK) past -= 2 * kRow;
@@ -207,8 +199,8 @@ struct Tile {
   static __device__ __forceinline__ int where(int first) {
     const int lane = threadIdx.x & 63;
     if (ALONG == kAlongK) {
-      const int row = first * 16 + row_of<ORDER>(0, lane & 15);
-      return row * kRow + (((lane >> 4) ^ swap(row)) * 16);
+      const int line = first * 16 + (lane & 15);
+      return line * 2 * kRow + (((lane >> 4) ^ (line & 7)) * 16);
     }
     if (DT == LUMA_GRAD_F32)
       return (lane >> 4) * 4 * kLine + ((first ^ ((lane >> 4) & kTurn)) * kBlock) + (lane & 15) * 4;
@@ -216,21 +208,18 @@ struct Tile {
     return k * kLine + ((first ^ (turn<DT>(k) & kTurn)) * kBlock) + (lane & 3) * 8;
   }
 
-  // Fragment of block first + i.
-  static __device__ __forceinline__ v4u read(const char *s, int where, int i) {
-    if constexpr (ALONG == kAlongK && ORDER == kPaired) {
-      // (row_of(1, r) = row_of(0, r) + 4: the same swap)
-      return *(const v4u *)(s + where + (i >> 1) * 32 * kRow + (i & 1) * 4 * kRow);
-    } else if constexpr (ALONG == kAlongK) {
-      return *(const v4u *)(s + where + i * 16 * kRow);
+  // Fragment of block first + i in the pair's stage h.
+  static __device__ __forceinline__ v4u read(const char *s, int h, int where, int i) {
+    if constexpr (ALONG == kAlongK) {
+      return *(const v4u *)(s + (where ^ (h * kRow)) + i * 16 * 2 * kRow);
     } else if constexpr (DT == LUMA_GRAD_F32) {
-      const char *p = s + (where ^ (i * kBlock));
+      const char *p = s + h * kStep<DT> * kLine + (where ^ (i * kBlock));
       v4u f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[j] = *(const uint32_t *)(p + j * kLine);
       return f;
     } else {
-      const char *p = s + (where ^ (i * kBlock));
+      const char *p = s + h * kStep<DT> * kLine + (where ^ (i * kBlock));
       typedef __attribute__((address_space(3))) v4s lds_v4s;
       const v2u lo = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p));
       const v2u hi = __builtin_bit_cast(
@@ -294,7 +283,7 @@ struct Split {
 // k1 - k0 is rounded up to whole rounds of the ring: past k1 operands must
 // read as zeros (past the operands' end), unless k1 - k0 is a multiple of
 // kStages * kStep.
-template <int DT, int AA, int AB, int ORDER, typename S>
+template <int DT, int AA, int AB, int ORDER, typename S, bool ONCE>
 __device__ __forceinline__ void product(const Operand &a, const Operand &b, int64_t m0, int64_t n0,
                                         int64_t k0, int64_t k1, Acc<DT, S> &acc) {
 #ifdef __HIP_DEVICE_COMPILE__   // (the host's compiler has no use for it)
@@ -302,18 +291,18 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
   typedef Tile<DT, AB, kPlain, S::BN, S::kThreads> B;
   constexpr int kLoads = A::kLoads + B::kLoads;
   constexpr int kMmas = S::TM * S::TN * (DT == LUMA_GRAD_F32 ? 4 : 1), kReads = S::TM + S::TN;
-  // (a variable for each stage: the compiler then knows that a stage's reads
-  // do not wait for another's loads)
-  __shared__ __align__(1024) char a0[A::kBytes], a1[A::kBytes], a2[A::kBytes], a3[A::kBytes];
-  __shared__ __align__(1024) char b0[B::kBytes], b1[B::kBytes], b2[B::kBytes], b3[B::kBytes];
+  // (a variable for each pair: the compiler then knows that a pair's reads do not
+  // wait for another's loads)
+  __shared__ __align__(1024) char a0[A::kBytes], a1[A::kBytes];
+  __shared__ __align__(1024) char b0[B::kBytes], b1[B::kBytes];
   A ta;
   B tb;
   const int wave = threadIdx.x >> 6;
   const int wa = A::where((wave / S::WN) * S::TM);
   const int wb = B::where((wave % S::WN) * S::TN);
-  auto fill = [&](char *sa0, char *sb0, char *sa1, char *sb1) {
-    ta.load(sa0, sa1);
-    tb.load(sb0, sb1);
+  auto fill = [&](char *sa, char *sb) {
+    ta.template load<ONCE>(sa);
+    tb.template load<false>(sb);
   };
   const int rounds = (int)((k1 - k0 + kStages * kStep<DT> - 1) / (kStages * kStep<DT>));
 
@@ -323,24 +312,24 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
     // bfloat16 16 times as fast as float32.  A pair of stages (32 of k) makes
     // one bfloat16 fragment.  (Smaller tiles take the float32 instruction: their
     // time is latency, which taking the parts adds to.)
-    auto parts = [&](const char *xa0, const char *xb0, const char *xa1, const char *xb1) {
+    auto parts = [&](const char *xa, const char *xb) {
       v4u hi[S::TN], mid[S::TN], lo[S::TN];
 #pragma unroll
       for (int j = 0; j < S::TN; ++j) {
-        const Split y(B::read(xb0, wb, j), B::read(xb1, wb, j));
+        const Split y(B::read(xb, 0, wb, j), B::read(xb, 1, wb, j));
         hi[j] = y.hi, mid[j] = y.mid, lo[j] = y.lo;
       }
       // (while block i is multiplied, the parts of the next are taken and the one
       // behind is read; the fences keep the compiler from doing all at once,
       // for which there are no registers)
-      Split x(A::read(xa0, wa, 0), A::read(xa1, wa, 0));
-      v4u f0 = A::read(xa0, wa, 1), f1 = A::read(xa1, wa, 1);
+      Split x(A::read(xa, 0, wa, 0), A::read(xa, 1, wa, 0));
+      v4u f0 = A::read(xa, 0, wa, 1), f1 = A::read(xa, 1, wa, 1);
 #pragma unroll
       for (int i = 0; i < S::TM; ++i) {
         __builtin_amdgcn_sched_barrier(0);
         const Split now = x;
         if (i + 1 < S::TM) x = Split(f0, f1);
-        if (i + 2 < S::TM) f0 = A::read(xa0, wa, i + 2), f1 = A::read(xa1, wa, i + 2);
+        if (i + 2 < S::TM) f0 = A::read(xa, 0, wa, i + 2), f1 = A::read(xa, 1, wa, i + 2);
         // (the small ones first)
 #pragma unroll
         for (int j = 0; j < S::TN; ++j) acc.mma_bf16(i, j, now.lo, hi[j]);
@@ -360,14 +349,14 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
     auto run = [&](auto pair) {
       ta.init(a, m0, k0);
       tb.init(b, n0, k0);
-      fill(a0, b0, a1, b1);
+      fill(a0, b0);
       for (int r = 0; r < rounds; ++r) {
         wait_and_meet<0>();
-        fill(a2, b2, a3, b3);
-        pair(a0, b0, a1, b1);
+        fill(a1, b1);
+        pair(a0, b0);
         wait_and_meet<0>();
-        fill(a0, b0, a1, b1);
-        pair(a2, b2, a3, b3);
+        fill(a0, b0);
+        pair(a1, b1);
       }
       wait_and_meet<0>();
     };
@@ -379,12 +368,12 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
 #pragma unroll
       for (int i = 0; i < S::TM; ++i) {
         Acc<DT, Shape<1, S::TN, S::WM, S::WN>> again;
-        run([&](const char *xa0, const char *xb0, const char *xa1, const char *xb1) {
+        run([&](const char *xa, const char *xb) {
 #pragma unroll
-          for (int j = 0; j < S::TN; ++j) {
-            again.mma(0, j, A::read(xa0, wa, i), B::read(xb0, wb, j));
-            again.mma(0, j, A::read(xa1, wa, i), B::read(xb1, wb, j));
-          }
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int j = 0; j < S::TN; ++j)
+              again.mma(0, j, A::read(xa, h, wa, i), B::read(xb, h, wb, j));
         });
 #pragma unroll
         for (int j = 0; j < S::TN; ++j)
@@ -398,39 +387,38 @@ __device__ __forceinline__ void product(const Operand &a, const Operand &b, int6
     tb.init(b, n0, k0);
     v4u fa[2][S::TM], fb[2][S::TN];
 
-    auto fetch = [&](const char *sa, const char *sb, v4u (&xa)[S::TM], v4u (&xb)[S::TN]) {
+    auto fetch = [&](const char *sa, const char *sb, int h) {
 #pragma unroll
-      for (int j = 0; j < S::TN; ++j) xb[j] = B::read(sb, wb, j);
+      for (int j = 0; j < S::TN; ++j) fb[h][j] = B::read(sb, h, wb, j);
 #pragma unroll
-      for (int i = 0; i < S::TM; ++i) xa[i] = A::read(sa, wa, i);
+      for (int i = 0; i < S::TM; ++i) fa[h][i] = A::read(sa, h, wa, i);
     };
-    auto multiply = [&](const v4u (&xa)[S::TM], const v4u (&xb)[S::TN]) {
+    auto multiply = [&](int h) {
 #pragma unroll
       for (int i = 0; i < S::TM; ++i)
 #pragma unroll
-        for (int j = 0; j < S::TN; ++j) acc.mma(i, j, xa[i], xb[j]);
+        for (int j = 0; j < S::TN; ++j) acc.mma(i, j, fa[h][i], fb[h][j]);
     };
 
-    // One pair of stages: x0, x1 hold it, y0, y1 the next one, which the loads
-    // under way fill.
-    auto pair = [&](char *xa0, char *xb0, char *xa1, char *xb1, char *ya0, char *yb0) {
-      fetch(xa1, xb1, fa[1], fb[1]);
-      multiply(fa[0], fb[0]);
+    // One pair of stages, x; the loads under way fill the next one, y.
+    auto pair = [&](char *xa, char *xb, char *ya, char *yb) {
+      fetch(xa, xb, 1);
+      multiply(0);
       spread<kMmas, kReads, 0>();
       wait_and_meet<0>();
-      fill(xa0, xb0, xa1, xb1);
-      fetch(ya0, yb0, fa[0], fb[0]);
-      multiply(fa[1], fb[1]);
-      spread<kMmas, kReads, 2 * kLoads>();
+      fill(xa, xb);
+      fetch(ya, yb, 0);
+      multiply(1);
+      spread<kMmas, kReads, kLoads>();
     };
 
-    fill(a0, b0, a1, b1);
-    fill(a2, b2, a3, b3);
-    wait_and_meet<2 * kLoads>();
-    fetch(a0, b0, fa[0], fb[0]);
+    fill(a0, b0);
+    fill(a1, b1);
+    wait_and_meet<kLoads>();
+    fetch(a0, b0, 0);
     for (int r = 0; r < rounds; ++r) {
-      pair(a0, b0, a1, b1, a2, b2);
-      pair(a2, b2, a3, b3, a0, b0);
+      pair(a0, b0, a1, b1);
+      pair(a1, b1, a0, b0);
     }
   }
   // (nothing of the ring is in flight when the workgroup goes on or ends)

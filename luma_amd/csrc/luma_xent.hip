@@ -77,6 +77,10 @@ struct Grid {
   int tiles_m, tiles_n, splits;
 };
 
+// Few tokens: one tile holds them all, and the weight is read once.
+template <typename S>
+constexpr bool kFew = S::BM > S::BN;
+
 // This lane's first row and column of its wavefront's accumulators; its quad i
 // of column j is rows m + row(i) .. + 3 and column n + 16 j.
 template <typename S, int ORDER>
@@ -112,8 +116,8 @@ __global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand 
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
   Acc<DT, S> acc;
-  product<DT, kAlongK, kAlongK, kPlain, S>(w, x, v0 + (int64_t)tm * S::BM, (int64_t)tn * S::BN, 0,
-                                           h, acc);
+  product<DT, kAlongK, kAlongK, kPlain, S, kFew<S>>(w, x, v0 + (int64_t)tm * S::BM,
+                                                    (int64_t)tn * S::BN, 0, h, acc);
   typedef Place<S, kPlain> P;
   P at(tm, tn);
   at.m += v0;
@@ -338,8 +342,8 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, 1, tm, tn, split);
   Acc<DT, S> acc;
-  product<DT, kAlongK, kAlongK, kPaired, S>(w, x, v0 + (int64_t)tm * S::BM, (int64_t)tn * S::BN,
-                                            0, h, acc);
+  product<DT, kAlongK, kAlongK, kPaired, S, kFew<S>>(w, x, v0 + (int64_t)tm * S::BM,
+                                                     (int64_t)tn * S::BN, 0, h, acc);
   typedef Place<S, kPaired> P;
   const P at(tm, tn);
 #pragma unroll
@@ -379,7 +383,8 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand
   tile_of(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
   const int64_t k0 = split * k_split, k1 = min(k, k0 + k_split);
   Acc<DT, S> acc;
-  product<DT, kAlongM, AB, kPlain, S>(a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
+  product<DT, kAlongM, AB, kPlain, S, kFew<S> && AB == kAlongK>(
+      a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
   typedef Place<S, kPlain> P;
   const P at(tm, tn);
   const float f = out16 ? factors.back<kTop<DT>>() : 1.0f;
