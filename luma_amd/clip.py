@@ -45,7 +45,7 @@ def _norm_code(norm_type) -> int:
     return code
 
 
-def _max_norm(max_norm) -> float:
+def check_max_norm(max_norm) -> float:
     max_norm = float(max_norm)
     if not max_norm >= 0.0:
         raise ValueError(f"Invalid max_norm: {max_norm}")
@@ -55,7 +55,7 @@ def _max_norm(max_norm) -> float:
 # Up to this many rows travel as launch arguments, a launch for each 144; more
 # take a device table (a copy of 24 bytes per row, which a launch or two less
 # does not pay for).
-_NO_TABLE = 2 * L.GRADS_INLINE
+NO_TABLE = 2 * L.GRADS_INLINE
 
 
 class _Batch:
@@ -74,7 +74,7 @@ class _Batch:
         device copy of the rows) of their own."""
         partials = torch.empty(L.NORM_PARTIALS, dtype=torch.float64, device=self.device)
         table, n = None, len(self.rows)
-        if n > _NO_TABLE and not torch.cuda.is_current_stream_capturing():
+        if n > NO_TABLE and not torch.cuda.is_current_stream_capturing():
             host = self.host
             if host is None:
                 host = torch.from_numpy(self.rows.view(np.uint8)).pin_memory()
@@ -110,7 +110,7 @@ def _quick(tensors, of_grad: bool, apart: bool) -> Optional[_Batch]:
     if module is None:
         return None
     host, n = None, len(tensors)
-    if n > _NO_TABLE and torch.cuda.is_available():
+    if n > NO_TABLE and torch.cuda.is_available():
         host = torch.empty(n * L.GRAD_DTYPE.itemsize, dtype=torch.uint8, pin_memory=True)
         rows = host.numpy().view(L.GRAD_DTYPE)
     else:
@@ -121,16 +121,22 @@ def _quick(tensors, of_grad: bool, apart: bool) -> Optional[_Batch]:
     return _Batch(rows[:got[0]], torch.device("cuda", max(got[1], 0)), host)
 
 
-def _rows(grads, device) -> np.ndarray:
-    rows = np.zeros(len(grads), dtype=L.GRAD_DTYPE)
-    rows["data"] = [g.data_ptr() for g in grads]
-    rows["numel"] = [g.numel() for g in grads]
-    rows["dtype"] = [_GRAD_CODES[g.dtype] for g in grads]
+def grad_rows(data, numel, dtype) -> np.ndarray:
+    """The rows of gradients at these addresses, of these sizes (>= 1) and type codes."""
+    rows = np.empty(len(numel), dtype=L.GRAD_DTYPE)
+    rows["data"] = data
+    rows["numel"] = numel
+    rows["dtype"] = dtype
     tiles = (rows["numel"] + L.GRAD_TILE - 1) // L.GRAD_TILE
     if tiles.sum() >= 2**31:
         raise ValueError("luma_amd: too many gradient elements for one call")
     rows["first_tile"] = np.cumsum(tiles) - tiles
     return rows
+
+
+def _rows(grads) -> np.ndarray:
+    return grad_rows([g.data_ptr() for g in grads], [g.numel() for g in grads],
+                     [_GRAD_CODES[g.dtype] for g in grads])
 
 
 def _shard_dims(t) -> tuple:
@@ -179,7 +185,7 @@ class _Slow:
                 g = dense
             self.sharded.setdefault(key, []).append(g)
         self.device = device
-        self.batches = [(key, _Batch(_rows([g for g in gs if g.numel()], device), device, hold=gs))
+        self.batches = [(key, _Batch(_rows([g for g in gs if g.numel()]), device, hold=gs))
                         for key, gs in self.sharded.items()]
         if apart:
             _check_apart([g for gs in self.sharded.values() for g in gs if g.numel()])
@@ -247,6 +253,14 @@ def _check_finite(total: torch.Tensor, norm_type) -> None:
             "by the non-finite norm anyway, set `error_if_nonfinite=False`")
 
 
+def sharded_norm(grads) -> Optional[torch.Tensor]:
+    """The 2-norm of gradients some of which are spread over several GPUs; None
+    where none is."""
+    if not any(hasattr(g, "_local_tensor") and _shard_dims(g) for g in grads):
+        return None
+    return _Slow(grads, False).norm(L.NORM_L2)
+
+
 @torch.compiler.disable
 @torch.no_grad()
 def get_total_norm(tensors: _Tensors, norm_type: float = 2.0, error_if_nonfinite: bool = False,
@@ -280,7 +294,7 @@ def clip_grad_norm_(parameters: _Tensors, max_norm: float, norm_type: float = 2.
     that is not finite scales by 0 or NaN, as in torch, unless
     ``error_if_nonfinite``, which waits for the norm and raises."""
     code = _norm_code(norm_type)
-    max_norm = _max_norm(max_norm)
+    max_norm = check_max_norm(max_norm)
     parameters = _as_list(parameters)
     batch = _quick(parameters, True, True)
     if batch is not None and not error_if_nonfinite:
@@ -306,7 +320,7 @@ def clip_grads_with_norm_(parameters: _Tensors, max_norm: float, total_norm: tor
                           foreach: Optional[bool] = None) -> None:
     """The scaling of ``clip_grad_norm_`` by a norm that is known already (a
     one-element tensor, e.g. ``get_total_norm``'s)."""
-    max_norm = _max_norm(max_norm)
+    max_norm = check_max_norm(max_norm)
     parameters = _as_list(parameters)
     if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1:
         raise ValueError("clip_grads_with_norm_: total_norm must be a one-element tensor")

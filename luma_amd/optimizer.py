@@ -33,6 +33,7 @@ from torch.optim import Optimizer
 
 from . import _lib as L
 
+from .clip import NO_TABLE, check_max_norm, grad_rows, sharded_norm
 from .config import SCALE_FLOOR_M  # noqa: F401  (re-exported constant)
 from .config import STEP_CHUNK_MIN, STEP_TARGET_CHUNKS
 
@@ -176,6 +177,10 @@ class _Engine:
         self._captured = []          # tables that a captured graph may read
         # torch.cuda.Event x4 (already recorded once) -> per-kernel timing
         self.profile_events = None
+        self._norm = None            # gradient norm of a clipped step: (tensor table, rows,
+                                     # device copy of the rows or None)
+        self._norm_out = None        # its norm and the step's scale (two float32)
+        self._norm_ws = None
 
     # -- helpers ------------------------------------------------------------
     def _stream(self) -> int:
@@ -332,6 +337,38 @@ class _Engine:
             evs = (ctypes.c_void_p * 4)(*[e.cuda_event for e in self.profile_events])
             L.check(self.lib.luma_step_profiled(ctypes.byref(args), self._stream(), evs),
                     "luma_step_profiled")
+
+    def clip_scale(self, tt: np.ndarray, max_norm: float, grad_scale: int) -> torch.Tensor:
+        """The norm of the gradients of table tt (over grad_scale, a device
+        scalar's address or 0) and the scale that makes a step clip by
+        max_norm as it reads them: two float32, overwritten by the next call
+        (a captured step reads them at one address)."""
+        capturing = torch.cuda.is_current_stream_capturing()
+        if self._norm_out is None:
+            if capturing:
+                raise self._capture_error("max_grad_norm")
+            self._norm_out = torch.empty(2, dtype=torch.float32, device=self.device)
+            self._norm_ws = torch.empty(L.NORM_PARTIALS, dtype=torch.float64, device=self.device)
+        same = self._norm is not None and self._norm[0] is tt and np.array_equal(
+            self._norm[1]["data"], tt["grad"])
+        if same:
+            _, rows, table = self._norm
+        else:
+            rows = grad_rows(tt["grad"], tt["numel"], tt["grad_dtype"])
+            table = None
+        # (as launch arguments a list of any length is captured)
+        if table is None and len(rows) > NO_TABLE and not capturing:
+            table = self._upload(rows)
+        self._norm = (tt, rows, table)
+        args = L.NormArgs(
+            grads=rows.ctypes.data, table=None if table is None else table.data_ptr(),
+            n=len(rows), norm=L.NORM_L2, max_norm=max_norm, partials=self._norm_ws.data_ptr(),
+            total=self._norm_out.data_ptr(), grad_scale=grad_scale or None,
+            step_scale=self._norm_out.data_ptr() + 4)
+        if capturing:
+            self._captured.append((rows, table))
+        L.check(self.lib.luma_grad_norm(ctypes.byref(args), self._stream()), "luma_grad_norm")
+        return self._norm_out
 
     def _small_limit(self) -> int:
         """Largest tensor stepped a wavefront each by the exact kernels (0: none)."""
@@ -614,6 +651,15 @@ class LUMA(Optimizer):
     PyTorch backend.  Parameters must be float32 and live on a ROCm GPU;
     gradients may be float32, bfloat16 or float16 (others are promoted to
     float32 first).
+
+    ``max_grad_norm`` (an attribute too, which may be set at any time; None:
+    no clipping) clips the gradients by their global 2-norm inside ``step()``:
+    the kernels multiply each gradient by ``min(1, max_grad_norm / (norm +
+    1e-6))`` as they read it, rounded once to its type, so ``.grad`` keeps its
+    values and nothing is rewritten.  Under ``torch.amp.GradScaler`` both
+    factors are one.  ``grad_norm`` is the norm of the last such step (a
+    float32 scalar on the device, unscaled and before clipping, which the
+    next step overwrites).  Neither is part of ``state_dict()``.
     """
 
     _BACKENDS = ("auto", "triton", "pytorch", "hip")
@@ -626,7 +672,8 @@ class LUMA(Optimizer):
     _step_supports_amp_scaling = True
 
     def __init__(self, params, lr: float = 1e-3, betas: Tuple[float, float] = (0.9, 0.999),
-                 eps: float = 1e-8, weight_decay: float = 0.01, backend: str = "auto"):
+                 eps: float = 1e-8, weight_decay: float = 0.01, backend: str = "auto",
+                 max_grad_norm: Optional[float] = None):
         # optimizer.py:80-89
         if lr < 0.0:
             raise ValueError(f"Invalid learning rate: {lr}")
@@ -654,6 +701,16 @@ class LUMA(Optimizer):
         self._summaries = True   # pass per-parameter code summaries to the step
         self._plan: Optional[_Plan] = None
         self._scaling_keep = []
+        self.max_grad_norm = max_grad_norm
+        self.grad_norm: Optional[torch.Tensor] = None
+
+    @property
+    def max_grad_norm(self) -> Optional[float]:
+        return self._max_grad_norm
+
+    @max_grad_norm.setter
+    def max_grad_norm(self, value: Optional[float]) -> None:
+        self._max_grad_norm = None if value is None else check_max_norm(value)
 
     # ------------------------------------------------------------------
     #  Helpers
@@ -722,6 +779,24 @@ class LUMA(Optimizer):
             ptrs.append(t.data_ptr())
         self._scaling_keep = keep
         return ptrs[0], ptrs[1]
+
+    def _clip(self, tt: np.ndarray, scaling: Tuple[int, int]) -> Tuple[int, int]:
+        """The step's scaling with max_grad_norm's clipping in it."""
+        if self._max_grad_norm is None:
+            return scaling
+        total = sharded_norm([p.grad for g in self.param_groups for p in g["params"]
+                              if p.grad is not None])
+        if total is None:
+            out = self._engine.clip_scale(tt, self._max_grad_norm, scaling[0])
+        else:
+            # (shards of other GPUs count: their sums are joined first)
+            scale = (self._scaling_keep[0] if scaling[0] else torch.ones_like(total)).reshape(())
+            total = total / scale
+            factor = (self._max_grad_norm / (total + 1e-6)).clamp(max=1.0)
+            out = torch.stack([total, scale / factor])
+            self._scaling_keep.append(out)
+        self.grad_norm = out[0]
+        return out.data_ptr() + 4, scaling[1]
 
     def _group_table(self) -> np.ndarray:
         """Hyper-parameters of every param group as the Python doubles the
@@ -899,10 +974,10 @@ class LUMA(Optimizer):
             r, same = res & 3, res >> 2
             match = next((k for i, (k, _) in enumerate(cands) if (same >> i) & 1), None)
             if r:
+                scaling = self._clip(plan.tt, self._scaling(self._engine.device))
                 self._engine.launch(plan.tt, self._group_table(), self._base_seed,
-                                    L.NOISE_PHILOX, self._flags,
-                                    self._scaling(self._engine.device), same_table=(r == 1),
-                                    moved=(r == 2), ptr_match=match)
+                                    L.NOISE_PHILOX, self._flags, scaling,
+                                    same_table=(r == 1), moved=(r == 2), ptr_match=match)
                 plan.host.bump_steps(plan.states)
                 return loss
         self._plan = None
@@ -1000,7 +1075,7 @@ class LUMA(Optimizer):
                          state["param_id"], code, gi, shard_offset(p), summ))
         tt = engine.table(rows)
         engine.launch(tt, self._group_table(), self._base_seed, noise_mode, self._flags,
-                      self._scaling(engine.device))
+                      self._clip(tt, self._scaling(engine.device)))
         # host count of step() calls; the kernels use the slot's device count
         for state in states:
             state["step"] += 1

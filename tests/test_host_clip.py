@@ -39,7 +39,7 @@ def test_dense(shape, stride, dense):
 
 def test_rows_add_up_their_tiles():
     grads = [torch.empty(n) for n in (1, 2048, 2049, 5000)]
-    rows = clip._rows(grads, None)
+    rows = clip._rows(grads)
     assert rows["first_tile"].tolist() == [0, 1, 2, 4]
     assert rows["numel"].tolist() == [1, 2048, 2049, 5000]
     assert rows["data"].tolist() == [g.data_ptr() for g in grads]
