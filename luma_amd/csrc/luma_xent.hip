@@ -331,9 +331,10 @@ __global__ __launch_bounds__(1024) void rows_kernel(Factors f) {
   if (threadIdx.x == 0) f.head->back = __builtin_ldexpf(1.0f, -e);
 }
 
-// (Eight words of a token are a lane's: 16-byte stores.)
+// (Eight words of a token are a lane's: 16-byte stores.)  TWO: what the rounding
+// leaves too, n rows further down.
 // D of words [v0, v0 + tiles_m BM), 0 past the vocabulary: d[token][word - v0].
-template <int DT, typename S>
+template <int DT, typename S, bool TWO>
 __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x, int64_t v0,
                                                             int64_t v, int64_t n, int64_t h,
                                                             Factors factors, Grid g,
@@ -356,17 +357,171 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
     typename Elem<DT>::type *out = d + token * ld + at.m;
 #pragma unroll
     for (int q = 0; q < S::TM; q += 2) {
-      Eight<DT> f;
+      Eight<DT> f, rest;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         float p = __builtin_amdgcn_exp2f(
             __builtin_fmaf(acc.t[q + e / 4][j][e % 4], kLog2e, -base));
         if (t == P::row(q) + e) p -= 1.0f;
         // (an ignored token's logits may be anything)
-        f[e] = Elem<DT>::round(
-            row == 0.0f || v0 + at.m + P::row(q) + e >= v ? 0.0f : p * row);
+        const float g = row == 0.0f || v0 + at.m + P::row(q) + e >= v ? 0.0f : p * row;
+        f[e] = Elem<DT>::round(g);
+        if (TWO) rest[e] = Elem<DT>::round(g - (float)f[e]);
       }
       *(Eight<DT> *)(out + P::row(q)) = f;
+      if (TWO) *(Eight<DT> *)(out + n * ld + P::row(q)) = rest;
+    }
+  }
+}
+
+// -- logits of few tokens, or of few words ----------------------------------------
+//
+// A tile's workgroup walks along k a pair of stages at a time, each a memory's
+// latency long: with one tile to a CU or less that is the time.  Here a tile is
+// kFewRows words by 16 TN tokens, k is shared out to the workgroup's wavefronts,
+// which read their fragments straight from memory, a row's 512 (TN 4: 256) bytes
+// at a time, wait for nobody and join their sums in LDS.  For few tokens the
+// weight is read once, in longer runs than a tile's 128 bytes a row.
+
+constexpr int kFewRows = 32, kFewWaves = 8, kFewThreads = 64 * kFewWaves;
+
+template <int DT, int TN>
+struct FewSums {
+  static constexpr int kTokens = 16 * TN;
+  static constexpr int kAhead = TN == 1 ? 8 : 4;      // 64-byte chunks of k per step
+  static constexpr int kPer = kFewRows * kTokens / kFewThreads;    // sums per thread
+  static_assert(kPer == TN, "a thread's sums are consecutive words of one token");
+  // (padded: the four rows that a wavefront writes at a time lie in other banks)
+  typedef float Lds[kFewWaves][kFewRows][kTokens + 4];
+
+  // This thread's token and first word of a tile.
+  static __device__ __forceinline__ int token() { return threadIdx.x % kTokens; }
+  static __device__ __forceinline__ int word() { return threadIdx.x / kTokens * kPer; }
+
+  template <bool WHOLE>
+  static __device__ __forceinline__ void step(const char *const (&a)[2], const char *const (&b)[TN],
+                                              int chunk, int bytes,
+                                              Acc<DT, Shape<2, TN, 1, 1>> &acc) {
+    const int part = (threadIdx.x & 63) >> 4;
+    v4u fa[kAhead][2], fb[kAhead][TN];
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u) {
+      const int at = (chunk + u) * kRow;
+      const bool in = WHOLE || at + part * 16 < bytes;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        // (one tile holds all tokens: nothing else reads these words)
+        fa[u][i] = !in ? v4u{0, 0, 0, 0}
+                   : TN == 1 ? __builtin_nontemporal_load((const v4u *)(a[i] + at))
+                             : *(const v4u *)(a[i] + at);
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+        fb[u][j] = in ? *(const v4u *)(b[j] + at) : v4u{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int u = 0; u < kAhead; ++u)
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) acc.mma(i, j, fa[u][i], fb[u][j]);
+  }
+
+  // This thread's logits: words m0 + word() .. of token n0 + token().  Words and
+  // tokens past the operands' ends take the last one's.
+  static __device__ __forceinline__ void run(const Operand &w, const Operand &x, int64_t m0,
+                                             int64_t n0, Lds &lds, float (&out)[kPer]) {
+    const int wave = __builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const int lane = threadIdx.x & 63, r = lane & 15;
+    const char *a[2], *b[TN];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      a[i] = w.p + min(m0 + 16 * i + r, w.rows - 1) * w.ld + (lane >> 4) * 16;
+#pragma unroll
+    for (int j = 0; j < TN; ++j)
+      b[j] = x.p + min(n0 + 16 * j + r, x.rows - 1) * x.ld + (lane >> 4) * 16;
+    Acc<DT, Shape<2, TN, 1, 1>> acc;
+    const int bytes = (int)w.row_bytes, chunks = (bytes + kRow - 1) / kRow;
+    for (int c = wave * kAhead; c < chunks; c += kFewWaves * kAhead) {
+      if ((c + kAhead) * kRow <= bytes)
+        step<true>(a, b, c, bytes, acc);
+      else
+        step<false>(a, b, c, bytes, acc);
+    }
+    __syncthreads();               // (the tile before has been read)
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int j = 0; j < TN; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          lds[wave][16 * i + (lane >> 4) * 4 + e][16 * j + r] = acc.t[i][j][e];
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      out[e] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kFewWaves; ++k) out[e] += lds[k][word() + e][token()];
+    }
+  }
+};
+
+// logits_kernel's records, one for each of gridDim.x runs of tiles of words.
+template <int DT, int TN>
+__global__ __launch_bounds__(kFewThreads) void few_logits_kernel(Operand w, Operand x, int64_t v,
+                                                                 int64_t n, const int64_t *target,
+                                                                 float2 *part, float *picked) {
+  typedef FewSums<DT, TN> F;
+  __shared__ typename F::Lds lds;
+  __shared__ float2 records[kFewThreads / F::kTokens][F::kTokens];
+  const int64_t n0 = (int64_t)blockIdx.y * F::kTokens, token = n0 + F::token();
+  const int64_t t = token < n ? target[token] : -1;
+  float2 a = make_float2(-__builtin_inff(), 0.0f);
+  for (int64_t m0 = (int64_t)blockIdx.x * kFewRows; m0 < v; m0 += (int64_t)gridDim.x * kFewRows) {
+    float l[F::kPer];
+    F::run(w, x, m0, n0, lds, l);
+#pragma unroll
+    for (int e = 0; e < F::kPer; ++e) {
+      const int64_t word = m0 + F::word() + e;
+      if (word >= v) continue;
+      if (word == t) picked[token] = l[e];
+      // (exp(l - l): 0 for -inf, NaN for inf and NaN)
+      a = join(a, make_float2(l[e], l[e] == -__builtin_inff() ? 0.0f : 1.0f + (l[e] - l[e])));
+    }
+  }
+  records[threadIdx.x / F::kTokens][F::token()] = a;
+  __syncthreads();
+  if (threadIdx.x >= F::kTokens || token >= n) return;
+  for (int k = 1; k < kFewThreads / F::kTokens; ++k) a = join(a, records[k][F::token()]);
+  part[(int64_t)blockIdx.x * n + token] = a;
+}
+
+// slope_kernel's D.
+template <int DT, int TN, bool TWO>
+__global__ __launch_bounds__(kFewThreads) void few_slope_kernel(Operand w, Operand x, int64_t v0,
+                                                                int64_t v, int64_t padded,
+                                                                int64_t n, Factors factors,
+                                                                typename Elem<DT>::type *d,
+                                                                int64_t ld) {
+  typedef FewSums<DT, TN> F;
+  __shared__ typename F::Lds lds;
+  const int64_t n0 = (int64_t)blockIdx.y * F::kTokens, token = n0 + F::token();
+  const int64_t t = token < n ? factors.target[token] : 0;
+  const float base = token < n ? factors.stats[token] * kLog2e : 0.0f;
+  const float row = token < n ? factors.row<kTop<DT>>(token, t) : 0.0f;
+  for (int64_t m0 = (int64_t)blockIdx.x * kFewRows; m0 < padded;
+       m0 += (int64_t)gridDim.x * kFewRows) {
+    float l[F::kPer];
+    F::run(w, x, v0 + m0, n0, lds, l);
+    if (token >= n) continue;
+#pragma unroll
+    for (int e = 0; e < F::kPer; ++e) {
+      const int64_t at = m0 + F::word() + e, word = v0 + at;
+      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(l[e], kLog2e, -base));
+      if (word == t) p -= 1.0f;
+      const float f = row == 0.0f || word >= v ? 0.0f : p * row;
+      const typename Elem<DT>::type hi = Elem<DT>::round(f);
+      d[token * ld + at] = hi;
+      if (TWO) d[(n + token) * ld + at] = Elem<DT>::round(f - (float)hi);
     }
   }
 }
@@ -450,6 +605,7 @@ typedef Shape<2, 2, 2, 2> Small;     // 64 x 64
 typedef Shape<2, 4, 4, 1> Thin64;    // 128 x 64: few tokens
 typedef Shape<2, 1, 4, 1> Thin16;    // 128 x 16
 enum ShapeId { kBig, kMid, kSmall, kThin64, kThin16 };
+constexpr int64_t kTwoParts = 64;    // tokens: up to here D is kept in two parts (kFew's shapes)
 constexpr int kBM[] = {256, 128, 64, 128, 128}, kBN[] = {256, 128, 64, 64, 16};
 constexpr int64_t kChip = 256;                 // CUs
 
@@ -524,17 +680,38 @@ struct Plan {
   bool pack_x, pack_w;
   int64_t ld_x, ld_w;           // elements, of what the products read
   int64_t at_x, at_w;           // of the packed copies
-  int64_t big;                  // words of logits (of a piece) in 256 x 256 tiles
+  bool few;                     // logits by few_logits_kernel, few_slope_kernel
+  int64_t big;                  // else: words of logits (of a piece) in 256 x 256 tiles
   int rest;                     // tile shape of the others
   // forward
   int64_t parts, at_part, at_picked, at_sums, blocks;
   // backward
+  int64_t rows_d;               // rows of D: n, or 2 n where it is kept in two parts
   int64_t piece, ld_d;          // words per piece; elements per row of D
   int hidden;                   // tile shape
   int64_t hidden_splits, hidden_k;
   int64_t at_head, at_rows, at_d, at_hidden, at_weight;
   int64_t bytes;
 };
+
+// Whether the logits of n tokens and `words` words go without tiles: where less
+// than a quarter of the chip would have one, and k is long (us for the loss,
+// tiles / without; tokens x h x words): float32 10 x 4096 x 100 92 / 31, 300 x
+// 4096 x 28 76 / 64, bfloat16 1 x 4096 x 28 42 / 23; but 50 x 768 x 5000 24 / 25,
+// 128 x 2048 x 3000 23 / 27, 1 x 4096 x 128256 171 / 334.
+bool few_for(int64_t words, int64_t n, int64_t k_bytes) {
+  const int shape = shape_for(words, n, 1);
+  return tiles(words, kBM[shape]) * tiles(n, kBN[shape]) < kChip / 4 && k_bytes >= 32 * kRow;
+}
+int few_tn(int64_t words, int64_t n) {
+  return tiles(words, kFewRows) * tiles(n, 16) < kChip ? 1 : 4;
+}
+// Runs of tiles of words: about four workgroups to a CU in all.
+int64_t few_runs(int64_t words, int64_t n) {
+  const int64_t groups = tiles(n, 16 * few_tn(words, n)), most = groups < 1024 ? 1024 / groups : 1;
+  const int64_t all = tiles(words, kFewRows);
+  return all < most ? all : most;
+}
 
 int weight_shape(const LumaXentArgs *a, int64_t words) {
   return shape_for(a->h, words < 65 ? 65 : words, tiles(a->n, 1024));
@@ -558,31 +735,43 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
     return here;
   };
   auto logits_plan = [&](int64_t words) {
+    p.few = few_for(words, a->n, a->h * p.size);
     p.big = big_words(a->n, words);
     p.rest = p.big ? kMid : shape_for(words, a->n, 1);
   };
-  if (p.pack_x) p.at_x = take(a->n * p.ld_x * p.size);
+  // What 16 bits leave of D averages out over many tokens; of a few, the
+  // target's entry, nearly the whole of a gradient, is off by up to half a step.
+  // Their products wait for the weight (or write its gradient), so a second part
+  // costs nothing: it is n more rows of D, and X is there twice.
+  const bool two = backward && a->n <= kTwoParts && p.size == 2;
+  p.rows_d = two ? 2 * a->n : a->n;
+  if (two) {
+    p.pack_x = true;
+    p.ld_x = up(a->h, group);
+  }
+  if (p.pack_x) p.at_x = take(p.rows_d * p.ld_x * p.size);
   if (p.pack_w) p.at_w = take(a->v * p.ld_w * p.size);
   if (!backward) {
     logits_plan(a->v);
-    p.parts = tiles(p.big, 256) + tiles(a->v - p.big, kBM[p.rest]);
+    p.parts = p.few ? few_runs(a->v, a->n)
+                    : tiles(p.big, 256) + tiles(a->v - p.big, kBM[p.rest]);
     p.blocks = tiles(a->n, kJoinTokens);
     p.at_part = take(p.parts * a->n * sizeof(float2));
     p.at_picked = take(a->n * sizeof(float));
     p.at_sums = take(p.blocks * sizeof(double2));
   } else {
-    p.piece = piece_for(a->n, a->v, p.size);
+    p.piece = piece_for(p.rows_d, a->v, p.size);
     logits_plan(p.piece);
     p.ld_d = p.piece;
     p.at_head = take(sizeof(Rows));
     p.at_rows = take(a->n * sizeof(float));
-    p.at_d = take(a->n * p.ld_d * p.size);
+    p.at_d = take(p.rows_d * p.ld_d * p.size);
     int64_t each, sums = 0;
     if (a->d_hidden) {
-      p.hidden = shape_for(a->h, a->n, tiles(p.ld_d, 1024));
-      p.hidden_splits = split_k(p.hidden, a->h, a->n, p.ld_d, round, p.hidden_k);
-      if (p.hidden_splits > 1 || p.piece < a->v)
-        p.at_hidden = take(p.hidden_splits * a->n * a->h * sizeof(float));
+      p.hidden = shape_for(a->h, p.rows_d, tiles(p.ld_d, 1024));
+      p.hidden_splits = split_k(p.hidden, a->h, p.rows_d, p.ld_d, round, p.hidden_k);
+      if (p.hidden_splits > 1 || p.piece < a->v || p.rows_d > a->n)
+        p.at_hidden = take(p.hidden_splits * p.rows_d * a->h * sizeof(float));
     }
     if (a->d_weight) {
       const int64_t last = a->v - (a->v - 1) / p.piece * p.piece;
@@ -591,7 +780,7 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
                                   whole_rounds(a->h, last), last - whole_rounds(a->h, last)}) {
         if (words == 0) continue;
         const int shape = weight_shape(a, words);
-        const int64_t splits = split_k(shape, a->h, words, a->n, round, each);
+        const int64_t splits = split_k(shape, a->h, words, p.rows_d, round, each);
         if (splits > 1 && splits * words > sums) sums = splits * words;
       }
       if (sums) p.at_weight = take(sums * a->h * sizeof(float));
@@ -631,6 +820,14 @@ void with_shape(int shape, F f) {
   }
 }
 
+template <typename F>
+void with_few(int64_t words, int64_t n, F f) {
+  if (few_tn(words, n) == 1)
+    f(std::integral_constant<int, 1>{});
+  else
+    f(std::integral_constant<int, 4>{});
+}
+
 Grid grid_of(int shape, int64_t m, int64_t n, int64_t splits) {
   return Grid{(int)tiles(m, kBM[shape]), (int)tiles(n, kBN[shape]), (int)splits};
 }
@@ -648,7 +845,8 @@ void pack(const void *in, int64_t rows, int64_t cols, int64_t ld_in, char *out, 
 template <int DT>
 void operands(const LumaXentArgs *a, const Plan &p, Operand &x, Operand &w, hipStream_t s) {
   char *ws = (char *)a->workspace;
-  if (p.pack_x) pack<DT>(a->hidden, a->n, a->h, a->ld_hidden, ws + p.at_x, p.ld_x, s);
+  for (int64_t r = 0; p.pack_x && r < p.rows_d; r += a->n)
+    pack<DT>(a->hidden, a->n, a->h, a->ld_hidden, ws + p.at_x + r * p.ld_x * p.size, p.ld_x, s);
   if (p.pack_w) pack<DT>(a->weight, a->v, a->h, a->ld_weight, ws + p.at_w, p.ld_w, s);
   const int64_t bytes = up(a->h, 16 / p.size) * p.size;
   x = Operand{p.pack_x ? ws + p.at_x : (const char *)a->hidden, p.ld_x * p.size, a->n, bytes};
@@ -672,8 +870,17 @@ void forward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
           w, x, v0, a->v, a->n, a->h, a->target, g, out, picked);
     });
   };
-  logits(kBig, 0, p.big, part);
-  logits(p.rest, p.big, a->v - p.big, part + tiles(p.big, 256) * a->n);
+  if (p.few) {
+    with_few(a->v, a->n, [&](auto tn) {
+      constexpr int TN = decltype(tn)::value;
+      const dim3 grid((int)p.parts, (int)tiles(a->n, 16 * TN));
+      few_logits_kernel<DT, TN><<<grid, kFewThreads, 0, s>>>(w, x, a->v, a->n, a->target, part,
+                                                            picked);
+    });
+  } else {
+    logits(kBig, 0, p.big, part);
+    logits(p.rest, p.big, a->v - p.big, part + tiles(p.big, 256) * a->n);
+  }
   join_kernel<<<(int)p.blocks, kJoinThreads, 0, s>>>(part, (int)p.parts, picked, a->target, a->n,
                                                      a->v, a->ignore_index, a->stats, a->loss,
                                                      sums);
@@ -703,7 +910,8 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
                            a->ignore_index, a->reduction, head,     rows};
   if (a->reduction == LUMA_XENT_NONE) rows_kernel<kTop<DT>><<<1, 1024, 0, s>>>(factors);
   const bool whole = p.piece >= a->v;        // one piece
-  const bool direct = p.hidden_splits == 1 && whole;
+  const bool direct = p.hidden_splits == 1 && whole && p.rows_d == a->n;
+  const Operand twice = {x.p, x.ld, p.rows_d, x.row_bytes};
   for (int64_t v0 = 0; v0 < a->v; v0 += p.piece) {
     const int64_t words = a->v - v0 < p.piece ? a->v - v0 : p.piece;
     // (the products take k up to the padding: D is 0 there)
@@ -713,20 +921,42 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
       with_shape(shape_id, [&](auto shape) {
         typedef decltype(shape) S;
         const Grid g = grid_of(shape_id, count, a->n, 1);
-        slope_kernel<DT, S><<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(
-            w, x, v0 + w0, a->v, a->n, a->h, factors, g, d + w0, p.ld_d);
+        auto go = [&](auto two) {
+          slope_kernel<DT, S, decltype(two)::value>
+              <<<g.tiles_m * g.tiles_n, S::kThreads, 0, s>>>(w, x, v0 + w0, a->v, a->n, a->h,
+                                                             factors, g, d + w0, p.ld_d);
+        };
+        if constexpr (kFew<S> && DT != LUMA_GRAD_F32) {
+          if (p.rows_d > a->n) return go(std::true_type{});
+        }
+        go(std::false_type{});
       });
     };
-    slope(kBig, 0, p.big < padded ? p.big : padded);
-    slope(p.rest, p.big, padded - p.big);
+    if (p.few) {
+      with_few(padded, a->n, [&](auto tn) {
+        constexpr int TN = decltype(tn)::value;
+        const dim3 grid((int)few_runs(padded, a->n), (int)tiles(a->n, 16 * TN));
+        auto go = [&](auto two) {
+          few_slope_kernel<DT, TN, decltype(two)::value><<<grid, kFewThreads, 0, s>>>(
+              w, x, v0, a->v, padded, a->n, factors, d, p.ld_d);
+        };
+        if constexpr (DT != LUMA_GRAD_F32) {
+          if (p.rows_d > a->n) return go(std::true_type{});
+        }
+        go(std::false_type{});
+      });
+    } else {
+      slope(kBig, 0, p.big < padded ? p.big : padded);
+      slope(p.rest, p.big, padded - p.big);
+    }
     const Operand wp = {w.p + v0 * w.ld, w.ld, words, w.row_bytes};
     if (a->d_hidden) {
-      const Operand dk = {(const char *)d, p.ld_d * p.size, a->n, padded * p.size};
+      const Operand dk = {(const char *)d, p.ld_d * p.size, p.rows_d, padded * p.size};
       with_shape(p.hidden, [&](auto shape) {
         typedef decltype(shape) S;
-        const Grid g = grid_of(p.hidden, a->h, a->n, p.hidden_splits);
+        const Grid g = grid_of(p.hidden, a->h, p.rows_d, p.hidden_splits);
         product_kernel<DT, kAlongK, S><<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
-            wp, dk, a->h, a->n, padded, p.hidden_k, g, v0 > 0, hidden, factors,
+            wp, dk, a->h, p.rows_d, padded, p.hidden_k, g, v0 > 0, hidden, factors,
             direct ? (T *)a->d_hidden : nullptr);
       });
     }
@@ -737,20 +967,20 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
       for (int c = 0; c < 2; ++c) {
         const int64_t w0 = cut[c], count = cut[c + 1] - w0;
         if (count == 0) continue;
-        const Operand dm = {(const char *)(d + w0), p.ld_d * p.size, a->n,
+        const Operand dm = {(const char *)(d + w0), p.ld_d * p.size, p.rows_d,
                             (padded - w0) * p.size};
         T *out = (T *)a->d_weight + (v0 + w0) * a->h;
         const int shape_id = weight_shape(a, count);
         int64_t each;
         const int64_t splits =
-            split_k(shape_id, a->h, count, a->n, kStages * kRow / p.size, each);
+            split_k(shape_id, a->h, count, p.rows_d, kStages * kRow / p.size, each);
         with_shape(shape_id, [&](auto shape) {
           typedef decltype(shape) S;
           if constexpr (S::BN >= 64) {
             const Grid g = grid_of(shape_id, a->h, count, splits);
             product_kernel<DT, kAlongM, S>
                 <<<g.tiles_m * g.tiles_n * g.splits, S::kThreads, 0, s>>>(
-                    x, dm, a->h, count, a->n, each, g, 0, weight, factors,
+                    twice, dm, a->h, count, p.rows_d, each, g, 0, weight, factors,
                     splits == 1 ? out : nullptr);
           }
         });
@@ -759,7 +989,8 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
     }
   }
   if (a->d_hidden && !direct)
-    sum_splits<DT>(hidden, p.hidden_splits, a->n * a->h, factors, a->d_hidden, s);
+    sum_splits<DT>(hidden, p.hidden_splits * (p.rows_d / a->n), a->n * a->h, factors,
+                   a->d_hidden, s);
 }
 
 template <typename F>
