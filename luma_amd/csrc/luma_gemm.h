@@ -111,19 +111,21 @@ struct Acc {
   }
 };
 
-// The block of a kAlongM row in whose place a block's elements lie: block ^ this.
-template <int DT>
-__device__ __forceinline__ int turn(int k) {
-  if (DT == LUMA_GRAD_F32) return (k >> 2) & 3;    // lanes of one read: k = j, 4 + j, 8 + j, 12 + j
-  return (k & 3) | ((k >> 1) & 4);                 // k = 8 g .. 8 g + 3
-}
-
 // The row of a pair of blocks of 16 that row `r` of block `i` of them takes, so
 // that a lane's two quads are eight consecutive rows (kPaired), or 16 i + r.
 constexpr int kPlain = 0, kPaired = 1;
 template <int ORDER>
 __device__ __forceinline__ constexpr int row_of(int i, int r) {
   return ORDER == kPaired ? 8 * (r >> 2) + 4 * i + (r & 3) : 16 * i + r;
+}
+
+// The block of a kAlongM row in whose place a block's elements lie: block ^ this.
+// (The lanes of one read have k = j, 4 + j, 8 + j, 12 + j; of 16 bits 8 g .. 8 g + 3,
+// one block of each or, kPaired, half of two.)
+template <int DT, int ORDER>
+__device__ __forceinline__ int turn(int k) {
+  if (DT == LUMA_GRAD_F32) return (k >> 2) & 3;
+  return ((k & 3) | ((k >> 1) & 4)) << (ORDER == kPaired ? 1 : 0);
 }
 
 // One operand's pairs of stages: ROWS of m (or n) by 128 bytes of k.  In LDS, a
@@ -169,7 +171,7 @@ struct Tile {
         past = (int)(kl < 0x40000000 ? kl : 0x40000000) - 1 - chunk;
       } else {
         const int k = at / kLine, in = at % kLine;
-        const int block = (in / kBlock) ^ (turn<DT>(k) & kTurn);
+        const int block = (in / kBlock) ^ (turn<DT, ORDER>(k) & kTurn);
         voff[q] = (uint32_t)(k * o.ld) + block * kBlock + in % kBlock;
       }
     }
@@ -204,8 +206,10 @@ struct Tile {
     }
     if (DT == LUMA_GRAD_F32)
       return (lane >> 4) * 4 * kLine + ((first ^ ((lane >> 4) & kTurn)) * kBlock) + (lane & 15) * 4;
-    const int k = 8 * (lane >> 4) + ((lane & 15) >> 2);
-    return k * kLine + ((first ^ (turn<DT>(k) & kTurn)) * kBlock) + (lane & 3) * 8;
+    const int k = 8 * (lane >> 4) + ((lane & 15) >> 2), q = lane & 3;
+    const int block = ORDER == kPaired ? first + (q >> 1) : first;
+    return k * kLine + ((block ^ (turn<DT, ORDER>(k) & kTurn)) * kBlock) +
+           (ORDER == kPaired ? (q & 1) * 16 : q * 8);
   }
 
   // Fragment of block first + i in the pair's stage h.
@@ -219,7 +223,9 @@ struct Tile {
       for (int j = 0; j < 4; ++j) f[j] = *(const uint32_t *)(p + j * kLine);
       return f;
     } else {
-      const char *p = s + h * kStep<DT> * kLine + (where ^ (i * kBlock));
+      const char *p = s + h * kStep<DT> * kLine +
+                      (ORDER == kPaired ? (where ^ (i / 2 * 2 * kBlock)) + i % 2 * 8
+                                        : where ^ (i * kBlock));
       typedef __attribute__((address_space(3))) v4s lds_v4s;
       const v2u lo = __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_v4s *)p));
       const v2u hi = __builtin_bit_cast(

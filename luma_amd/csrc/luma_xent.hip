@@ -537,29 +537,45 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand
   int tm, tn, split;
   tile_of(g.tiles_m, g.tiles_n, g.splits, tm, tn, split);
   const int64_t k0 = split * k_split, k1 = min(k, k0 + k_split);
+  // (a lane's eight consecutive columns are one store; of float32 four are)
+  constexpr int kOrder = DT == LUMA_GRAD_F32 ? kPlain : kPaired;
   Acc<DT, S> acc;
-  product<DT, kAlongM, AB, kPlain, S, kFew<S> && AB == kAlongK>(
+  product<DT, kAlongM, AB, kOrder, S, kFew<S> && AB == kAlongK>(
       a, b, (int64_t)tm * S::BM, (int64_t)tn * S::BN, k0, k1, acc);
-  typedef Place<S, kPlain> P;
+  typedef Place<S, kOrder> P;
   const P at(tm, tn);
+  const bool aligned = m % 8 == 0 && (uintptr_t)out16 % 16 == 0;
   const float f = out16 ? factors.back<kTop<DT>>() : 1.0f;
 #pragma unroll
   for (int j = 0; j < S::TN; ++j) {
     const int64_t row = at.n + 16 * j;
     if (row >= n) continue;
 #pragma unroll
-    for (int q = 0; q < S::TM; ++q) {
-      const int64_t col = at.m + P::row(q);
-      v4f c = acc.t[q][j];
+    for (int q = 0; q < S::TM; q += 2) {
+      const int64_t col = at.m + P::row(q), next = at.m + P::row(q + 1);
       if (out16) {
-        store4<DT>(out16 + row * m, col, m, c * f);
+        const v4f c = acc.t[q][j] * f, d = acc.t[q + 1][j] * f;
+        if (kOrder == kPaired && aligned && col + 8 <= m) {
+          Eight<DT> o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] = Elem<DT>::round(e < 4 ? c[e & 3] : d[e & 3]);
+          *(Eight<DT> *)(out16 + row * m + col) = o;
+        } else {
+          store4<DT>(out16 + row * m, col, m, c);
+          store4<DT>(out16 + row * m, next, m, d);
+        }
       } else {
         float *o = out + (int64_t)split * n * m + row * m;
-        if (add)
 #pragma unroll
-          for (int r = 0; r < 4; ++r)
-            if (col + r < m) c[r] += o[col + r];
-        store4<LUMA_GRAD_F32>(o, col, m, c);
+        for (int k = 0; k < 2; ++k) {
+          const int64_t at = k ? next : col;
+          v4f c = acc.t[q + k][j];
+          if (add)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+              if (at + r < m) c[r] += o[at + r];
+          store4<LUMA_GRAD_F32>(o, at, m, c);
+        }
       }
     }
   }
