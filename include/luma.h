@@ -385,7 +385,7 @@ int luma_hyper_rows(const LumaGroup *group, int64_t t0, int32_t n, float *out, v
 /* Elements per tile: the unit in which the rows are shared out to wavefronts. */
 #define LUMA_GRAD_TILE 2048
 /* Rows that one launch carries among its arguments (no device table). */
-#define LUMA_GRADS_INLINE 144
+#define LUMA_GRADS_INLINE 160
 /* Rows that may go without a device table. */
 #define LUMA_GRADS_NO_TABLE (LUMA_GRADS_INLINE * 256)
 /* Doubles of workspace (LumaNormArgs.partials). */

@@ -8,6 +8,7 @@ is no fallback implementation of the step.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import numpy as np
@@ -26,7 +27,7 @@ NOALLOC_MAX_CHUNKS = 262144  # LUMA_NOALLOC_MAX_CHUNKS
 SUMMARY_WORDS = 256          # LUMA_SUMMARY_WORDS (per chunk)
 ABI_VERSION = 11             # LUMA_ABI_VERSION
 GRAD_TILE = 2048             # LUMA_GRAD_TILE
-GRADS_INLINE = 144           # LUMA_GRADS_INLINE
+GRADS_INLINE = 160           # LUMA_GRADS_INLINE
 NORM_PARTIALS = 1024         # LUMA_NORM_PARTIALS
 
 GRAD_F32, GRAD_BF16, GRAD_F16 = 0, 1, 2
@@ -210,6 +211,22 @@ def load_host():
                       "step).  Rebuild it with `python -m luma_amd.build`.")
         return None
     return _luma_host
+
+
+@functools.lru_cache(maxsize=1)
+def host_calls():
+    """The host module with the library's entry points bound (the eager paths
+    of the norm, clipping and linear_cross_entropy); None without it."""
+    import torch
+
+    host = load_host()
+    if host is not None:
+        lib = load()
+        host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
+            "luma_xent_workspace_bytes", "luma_xent_forward", "luma_xent_backward",
+            "luma_grad_norm", "luma_grad_clip", "luma_last_error")),
+            torch._C._cuda_getCurrentRawStream)
+    return host
 
 
 def check_layout(lib) -> None:

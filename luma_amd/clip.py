@@ -24,7 +24,6 @@ an all-reduce over the mesh dimensions that they are sharded over.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import Iterable, List, Optional, Union
 
@@ -52,7 +51,7 @@ def check_max_norm(max_norm) -> float:
     return max_norm
 
 
-# Up to this many rows travel as launch arguments, a launch for each 144; more
+# Up to this many rows travel as launch arguments, a launch for each 160; more
 # take a device table (a copy of 24 bytes per row, which a launch or two less
 # does not pay for).
 NO_TABLE = 2 * L.GRADS_INLINE
@@ -93,9 +92,8 @@ class _Batch:
             L.check(getattr(lib, name)(ctypes.byref(args), stream), name)
 
 
-@functools.lru_cache(maxsize=1)
 def _host():
-    return L.load_host()
+    return L.host_calls()
 
 
 def _as_list(tensors: _Tensors) -> List[torch.Tensor]:
@@ -261,8 +259,13 @@ def sharded_norm(grads) -> Optional[torch.Tensor]:
     return _Slow(grads, False).norm(L.NORM_L2)
 
 
+def _quick_norm(tensors, clip: bool, code: int, max_norm: float) -> Optional[torch.Tensor]:
+    """The whole call by the host module, for a list without a device table."""
+    host = _host()
+    return None if host is None else host.grad_norm(tensors, clip, code, max_norm, NO_TABLE)
+
+
 @torch.compiler.disable
-@torch.no_grad()
 def get_total_norm(tensors: _Tensors, norm_type: float = 2.0, error_if_nonfinite: bool = False,
                    foreach: Optional[bool] = None) -> torch.Tensor:
     """The norm of all elements of all tensors together (``norm_type`` 1, 2 or
@@ -270,21 +273,27 @@ def get_total_norm(tensors: _Tensors, norm_type: float = 2.0, error_if_nonfinite
     torch's signature and selects nothing."""
     code = _norm_code(norm_type)
     tensors = _as_list(tensors)
-    batch = _quick(tensors, False, False)
-    if batch is not None:
-        if not len(batch.rows):
-            return torch.tensor(0.0)
-        total = torch.empty((), dtype=torch.float32, device=batch.device)
-        batch.call("luma_grad_norm", batch.args(code, 0.0, total))
-    else:
-        total = _Slow(tensors, False).norm(code)
+    total = _quick_norm(tensors, False, code, 0.0)
+    if total is None:
+        total = _total_norm(tensors, code)
     if error_if_nonfinite:
         _check_finite(total, norm_type)
     return total
 
 
-@torch.compiler.disable
 @torch.no_grad()
+def _total_norm(tensors, code: int) -> torch.Tensor:
+    batch = _quick(tensors, False, False)
+    if batch is None:
+        return _Slow(tensors, False).norm(code)
+    if not len(batch.rows):
+        return torch.tensor(0.0)
+    total = torch.empty((), dtype=torch.float32, device=batch.device)
+    batch.call("luma_grad_norm", batch.args(code, 0.0, total))
+    return total
+
+
+@torch.compiler.disable
 def clip_grad_norm_(parameters: _Tensors, max_norm: float, norm_type: float = 2.0,
                     error_if_nonfinite: bool = False,
                     foreach: Optional[bool] = None) -> torch.Tensor:
@@ -296,8 +305,18 @@ def clip_grad_norm_(parameters: _Tensors, max_norm: float, norm_type: float = 2.
     code = _norm_code(norm_type)
     max_norm = check_max_norm(max_norm)
     parameters = _as_list(parameters)
-    batch = _quick(parameters, True, True)
-    if batch is not None and not error_if_nonfinite:
+    if not error_if_nonfinite:
+        total = _quick_norm(parameters, True, code, max_norm)
+        if total is not None:
+            return total
+    return _clip(parameters, max_norm, norm_type, code, error_if_nonfinite)
+
+
+@torch.no_grad()
+def _clip(parameters, max_norm: float, norm_type, code: int,
+          error_if_nonfinite: bool) -> torch.Tensor:
+    batch = None if error_if_nonfinite else _quick(parameters, True, True)
+    if batch is not None:
         if not len(batch.rows):
             return torch.tensor(0.0)
         total = torch.empty((), dtype=torch.float32, device=batch.device)

@@ -407,8 +407,8 @@ struct GradRow {
   int64_t numel;
   int32_t dtype, first_tile;
 };
-static_assert(sizeof(GradRow) == 24, "LumaGrad");
-constexpr int64_t kGradTile = 2048;   // LUMA_GRAD_TILE
+static_assert(sizeof(GradRow) == sizeof(LumaGrad), "LumaGrad");
+constexpr int64_t kGradTile = LUMA_GRAD_TILE;
 
 // One part's *count rows, their first_tile within the part; false for a tensor
 // that the kernels cannot take as it is.  *device: the CUDA device of all of them
@@ -528,18 +528,64 @@ py::object grad_rows(py::list objs, bool of_grad, bool apart, uintptr_t table) {
   return py::make_tuple(at, dev);
 }
 
-// -- linear_cross_entropy's calls ---------------------------------------------
-// The eager path of luma_amd.linear_cross_entropy: allocations, the library's
-// calls and the autograd node (from Python they take 120 us of a call whose
-// kernels take 45).  The library's entry points come from the caller (bind),
-// which checked its ABI.
-struct XentLibrary {
+// -- calls of the library -------------------------------------------------------
+// The eager paths of the operators beside the step: their allocations, the
+// library's calls and linear_cross_entropy's autograd node (from Python they take
+// 120 us of a call of the latter whose kernels take 45, and 20 of a clipping of
+// 50 tensors whose kernels take 10).  The entry points come from the caller
+// (bind), which checked the library's ABI.
+struct Library {
   int64_t (*workspace)(const LumaXentArgs *, int32_t) = nullptr;
   int (*forward)(const LumaXentArgs *, void *) = nullptr;
   int (*backward)(const LumaXentArgs *, void *) = nullptr;
+  int (*norm)(const LumaNormArgs *, void *) = nullptr;
+  int (*clip)(const LumaNormArgs *, void *) = nullptr;
   const char *(*error)() = nullptr;
   PyObject *stream = nullptr;    // torch's current stream of a device, as an address
-} g_xent;
+} g_lib;
+
+void bind(uintptr_t workspace, uintptr_t forward, uintptr_t backward, uintptr_t norm,
+          uintptr_t clip, uintptr_t error, py::object stream) {
+  g_lib = {reinterpret_cast<int64_t (*)(const LumaXentArgs *, int32_t)>(workspace),
+           reinterpret_cast<int (*)(const LumaXentArgs *, void *)>(forward),
+           reinterpret_cast<int (*)(const LumaXentArgs *, void *)>(backward),
+           reinterpret_cast<int (*)(const LumaNormArgs *, void *)>(norm),
+           reinterpret_cast<int (*)(const LumaNormArgs *, void *)>(clip),
+           reinterpret_cast<const char *(*)()>(error), stream.release().ptr()};
+}
+
+void *current_stream(int64_t device) {
+  py::gil_scoped_acquire gil;    // (the backward runs on autograd's thread)
+  return reinterpret_cast<void *>(py::handle(g_lib.stream)(device).cast<uintptr_t>());
+}
+
+// The norm of the tensors in objs or (clip) of their gradients, which are then
+// clipped by max_norm: the norm as a float32 scalar, or None for what grad_rows
+// cannot take, no rows and lists that need a device table (more than `most`).
+py::object grad_norm(py::list objs, bool clip, int32_t norm, double max_norm, int64_t most) {
+  const int64_t n = (int64_t)objs.size();
+  if (n > most || n == 0 || !g_lib.norm) return py::none();
+  std::vector<GradRow> rows(n);
+  int64_t count = 0, device = -1;
+  if (!grad_range(&PyList_GET_ITEM(objs.ptr(), 0), n, clip, rows.data(), &count, &device) ||
+      count == 0 || (clip && !disjoint(rows.data(), count)))
+    return py::none();
+  const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)device);
+  const c10::DeviceGuard guard(dev);
+  const at::Tensor partials =
+      at::empty({LUMA_NORM_PARTIALS}, at::TensorOptions().dtype(at::kDouble).device(dev));
+  at::Tensor total = at::empty({}, at::TensorOptions().dtype(at::kFloat).device(dev));
+  LumaNormArgs a{};
+  a.grads = reinterpret_cast<const LumaGrad *>(rows.data());
+  a.n = (int32_t)count;
+  a.norm = norm;
+  a.max_norm = max_norm;
+  a.partials = partials.mutable_data_ptr<double>();
+  a.total = total.mutable_data_ptr<float>();
+  const int rc = (clip ? g_lib.clip : g_lib.norm)(&a, current_stream(device));
+  TORCH_CHECK(rc == 0, g_lib.error());
+  return py::cast(total);
+}
 
 // t, or a copy, with elements of a row next to each other and rows apart.
 at::Tensor rows_of(const at::Tensor &t) {
@@ -569,20 +615,15 @@ LumaXentArgs xent_args(const at::Tensor &hidden, const at::Tensor &weight,
 
 void xent_call(LumaXentArgs &a, bool backward, const at::Tensor &like) {
   const c10::DeviceGuard guard(like.device());
-  const int64_t bytes = g_xent.workspace(&a, backward);
-  TORCH_CHECK(bytes >= 0, g_xent.error());
+  const int64_t bytes = g_lib.workspace(&a, backward);
+  TORCH_CHECK(bytes >= 0, g_lib.error());
   const at::Tensor workspace =
       at::empty({std::max<int64_t>(bytes, 1)}, like.options().dtype(at::kByte));
   a.workspace = workspace.mutable_data_ptr();
   a.workspace_bytes = bytes;
-  void *stream;
-  {
-    py::gil_scoped_acquire gil;    // (the backward runs on autograd's thread)
-    stream = reinterpret_cast<void *>(
-        py::handle(g_xent.stream)((int)like.device().index()).cast<uintptr_t>());
-  }
-  const int rc = (backward ? g_xent.backward : g_xent.forward)(&a, stream);
-  TORCH_CHECK(rc == 0, g_xent.error());
+  const int rc = (backward ? g_lib.backward : g_lib.forward)(
+      &a, current_stream(like.device().index()));
+  TORCH_CHECK(rc == 0, g_lib.error());
 }
 
 struct Xent : torch::autograd::Function<Xent> {
@@ -642,16 +683,8 @@ struct Xent : torch::autograd::Function<Xent> {
 // hidden [n][h], weight [v][h] and target [n] as linear_cross_entropy checked them.
 at::Tensor xent(const at::Tensor &hidden, const at::Tensor &weight, const at::Tensor &target,
                 int64_t ignore, int64_t reduction) {
-  if (!g_xent.forward) throw py::value_error("xent: the library is not bound");
+  if (!g_lib.forward) throw py::value_error("xent: the library is not bound");
   return Xent::apply(hidden, weight, target, ignore, reduction);
-}
-
-void xent_bind(uintptr_t workspace, uintptr_t forward, uintptr_t backward, uintptr_t error,
-               py::object stream) {
-  g_xent = {reinterpret_cast<int64_t (*)(const LumaXentArgs *, int32_t)>(workspace),
-            reinterpret_cast<int (*)(const LumaXentArgs *, void *)>(forward),
-            reinterpret_cast<int (*)(const LumaXentArgs *, void *)>(backward),
-            reinterpret_cast<const char *(*)()>(error), stream.release().ptr()};
 }
 
 PYBIND11_MODULE(_luma_host, m) {
@@ -671,7 +704,8 @@ PYBIND11_MODULE(_luma_host, m) {
   m.def("bump_steps", &bump_steps);
   m.def("grad_rows", &grad_rows);
   m.def("xent", &xent);
-  m.def("xent_bind", &xent_bind);
+  m.def("grad_norm", &grad_norm);
+  m.def("bind", &bind);
   // the torch whose headers this module was compiled against: it reads
   // TensorImpl fields in that version's inline layout
   m.attr("torch_version") = LUMA_TORCH_VERSION;

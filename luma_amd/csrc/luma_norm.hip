@@ -391,6 +391,7 @@ void launches(const LumaNormArgs *a, int64_t tiles, FT with_table, FI with_rows)
     return;
   }
   const int calls = (a->n + LUMA_GRADS_INLINE - 1) / LUMA_GRADS_INLINE;
+  const int most = LUMA_NORM_PARTIALS / calls < kBlocks ? LUMA_NORM_PARTIALS / calls : kBlocks;
   Rows rows;
   for (int c = 0; c < calls; ++c) {
     const int first = c * LUMA_GRADS_INLINE;
@@ -398,10 +399,12 @@ void launches(const LumaNormArgs *a, int64_t tiles, FT with_table, FI with_rows)
     memcpy(rows.row, a->grads + first, n * sizeof(LumaGrad));
     const int base = a->grads[first].first_tile;
     const int64_t end = first + n < a->n ? a->grads[first + n].first_tile : tiles;
-    with_rows(rows, n, base, (int)(end - base), blocks(end - base, kBlocks / calls));
+    with_rows(rows, n, base, (int)(end - base), blocks(end - base, most));
   }
 }
-static_assert(LUMA_GRADS_NO_TABLE / LUMA_GRADS_INLINE <= kBlocks, "a partial sum per launch");
+static_assert(LUMA_GRADS_NO_TABLE / LUMA_GRADS_INLINE <= LUMA_NORM_PARTIALS,
+              "a partial sum per launch");
+static_assert(sizeof(Rows) <= 4096 - 128, "the launch's arguments");
 
 template <int NORM>
 int partial_sums(const LumaNormArgs *a, int64_t tiles, hipStream_t s) {

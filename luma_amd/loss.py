@@ -16,7 +16,6 @@ them, and they do no host synchronisation::
 from __future__ import annotations
 
 import ctypes
-import functools
 from typing import Tuple
 
 import torch
@@ -163,18 +162,6 @@ def _backward(ctx, grad, _):
 _forward_op.register_autograd(_backward, setup_context=_setup)
 
 
-@functools.lru_cache(maxsize=1)
-def _eager():
-    """The host module's form of both ops and their autograd node; None without it."""
-    host = L.load_host()
-    if host is not None:
-        lib = L.load()
-        host.xent_bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "luma_xent_workspace_bytes", "luma_xent_forward", "luma_xent_backward",
-            "luma_last_error")), torch._C._cuda_getCurrentRawStream)
-    return None if host is None else host.xent
-
-
 def _plain(*tensors) -> bool:
     """Whether no tensor is of a subclass with a dispatch of its own."""
     return all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
@@ -210,9 +197,9 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
                                                           code)
     else:
         _check(hidden, weight, target)
-        eager = _eager() if _plain(hidden, weight, target) else None
-        if eager is not None:
-            loss = eager(hidden, weight, target, ignore_index, code)
+        host = L.host_calls() if _plain(hidden, weight, target) else None
+        if host is not None:
+            loss = host.xent(hidden, weight, target, ignore_index, code)
         else:
             loss, _ = torch.ops.luma_amd.linear_cross_entropy(hidden, weight, target,
                                                               ignore_index, code)
