@@ -809,7 +809,7 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
 bool check_args(const LumaXentArgs *a, bool backward) {
   if (!a) return fail("luma_xent: null arguments"), false;
   if (a->n < 1 || a->h < 1 || a->v < 1) return fail("luma_xent: empty operands"), false;
-  if (a->n > INT32_MAX || a->h > 1 << 20 || a->v > INT32_MAX)
+  if (a->n > INT32_MAX / 2 || a->h > 1 << 20 || a->v > INT32_MAX / 2)
     return fail("luma_xent: operands too large"), false;
   if (a->dtype < LUMA_GRAD_F32 || a->dtype > LUMA_GRAD_F16)
     return fail("luma_xent: unknown type"), false;
@@ -822,6 +822,11 @@ bool check_args(const LumaXentArgs *a, bool backward) {
     return fail("luma_xent: rows overlap"), false;
   if (a->ld_hidden > 1 << 21 || a->ld_weight > 1 << 21)
     return fail("luma_xent: rows too far apart"), false;
+  // (a launch's workgroups are counted in 32 bits)
+  if (tiles(a->n, 16) * tiles(a->v, 64) > INT32_MAX ||
+      tiles(a->h, 64) * tiles(a->v, 64) > INT32_MAX / 64 ||
+      tiles(a->h, 64) * tiles(a->n, 16) > INT32_MAX / 64)
+    return fail("luma_xent: operands too large"), false;
   return true;
 }
 

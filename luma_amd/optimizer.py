@@ -780,12 +780,13 @@ class LUMA(Optimizer):
         self._scaling_keep = keep
         return ptrs[0], ptrs[1]
 
-    def _clip(self, tt: np.ndarray, scaling: Tuple[int, int]) -> Tuple[int, int]:
-        """The step's scaling with max_grad_norm's clipping in it."""
+    def _clip(self, tt: np.ndarray, scaling: Tuple[int, int],
+              work=()) -> Tuple[int, int]:
+        """The step's scaling with max_grad_norm's clipping in it.  ``work``: the
+        step's parameters, unless they are known to be plain tensors."""
         if self._max_grad_norm is None:
             return scaling
-        total = sharded_norm([p.grad for g in self.param_groups for p in g["params"]
-                              if p.grad is not None])
+        total = sharded_norm([w[1].grad for w in work])
         if total is None:
             out = self._engine.clip_scale(tt, self._max_grad_norm, scaling[0])
         else:
@@ -1075,7 +1076,7 @@ class LUMA(Optimizer):
                          state["param_id"], code, gi, shard_offset(p), summ))
         tt = engine.table(rows)
         engine.launch(tt, self._group_table(), self._base_seed, noise_mode, self._flags,
-                      self._clip(tt, self._scaling(engine.device)))
+                      self._clip(tt, self._scaling(engine.device), work))
         # host count of step() calls; the kernels use the slot's device count
         for state in states:
             state["step"] += 1
