@@ -178,53 +178,57 @@ __global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand 
   }
 }
 
-constexpr int kJoinTokens = 32, kJoinSlices = 32, kJoinThreads = kJoinTokens * kJoinSlices;
+constexpr int kJoinThreads = 1024;
 
-// Each token's lse and loss from its `parts` records; with a reduction, each
+// Each token's lse and loss from its `parts` records, TOKENS to a workgroup (the
+// records of one shared out to 1024 / TOKENS threads); with a reduction, each
 // workgroup's sums (in float64) of the losses and of the targets that count.
+template <int TOKENS>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2 *part, int parts,
                                                             const float *picked,
                                                             const int64_t *target, int64_t n,
                                                             int64_t v, int64_t ignore,
                                                             float *stats, float *loss,
                                                             double2 *sums) {
-  __shared__ float2 lds[kJoinSlices][kJoinTokens + 1];
-  const int tok = threadIdx.x % kJoinTokens, slice = threadIdx.x / kJoinTokens;
-  const int64_t token = (int64_t)blockIdx.x * kJoinTokens + tok;
+  constexpr int kSlices = kJoinThreads / TOKENS;
+  __shared__ float2 lds[kSlices][TOKENS + 1];
+  const int tok = threadIdx.x % TOKENS, slice = threadIdx.x / TOKENS;
+  const int64_t token = (int64_t)blockIdx.x * TOKENS + tok;
   float2 a = make_float2(-__builtin_inff(), 0.0f);
   if (token < n) {
     // (kAhead records in flight: a token has hundreds, and the loads' latency
     // is what they take)
     constexpr int kAhead = 8;
     int p = slice;
-    for (; p + (kAhead - 1) * kJoinSlices < parts; p += kAhead * kJoinSlices) {
+    for (; p + (kAhead - 1) * kSlices < parts; p += kAhead * kSlices) {
       float2 b[kAhead];
 #pragma unroll
-      for (int k = 0; k < kAhead; ++k) b[k] = part[(int64_t)(p + k * kJoinSlices) * n + token];
+      for (int k = 0; k < kAhead; ++k) b[k] = part[(int64_t)(p + k * kSlices) * n + token];
 #pragma unroll
       for (int k = 0; k < kAhead; ++k) a = join(a, b[k]);
     }
-    for (; p < parts; p += kJoinSlices) a = join(a, part[(int64_t)p * n + token]);
+    for (; p < parts; p += kSlices) a = join(a, part[(int64_t)p * n + token]);
   }
   lds[slice][tok] = a;
   __syncthreads();
+  for (int s = kSlices / 2; s > 0; s /= 2) {
+    if (slice < s && slice + s < parts) lds[slice][tok] = a = join(a, lds[slice + s][tok]);
+    __syncthreads();
+  }
   if (threadIdx.x >= 64) return;      // (the rest is the first wavefront's)
   double value = 0.0, count = 0.0;
-  if (slice == 0) {
-    for (int s = 1; s < min(kJoinSlices, parts); ++s) a = join(a, lds[s][tok]);
-    if (token < n) {
-      const float lse = a.x == -__builtin_inff() ? __builtin_nanf("")
-                                                 : a.x + __builtin_amdgcn_logf(a.y) * kLn2;
-      const int64_t t = target[token];
-      float l = 0.0f;
-      if (t != ignore) {
-        l = t >= 0 && t < v ? lse - picked[token] : __builtin_nanf("");
-        count = 1.0;
-      }
-      stats[token] = lse;
-      if (!sums) loss[token] = l;
-      value = (double)l;
+  if (slice == 0 && token < n) {
+    const float lse = a.x == -__builtin_inff() ? __builtin_nanf("")
+                                               : a.x + __builtin_amdgcn_logf(a.y) * kLn2;
+    const int64_t t = target[token];
+    float l = 0.0f;
+    if (t != ignore) {
+      l = t >= 0 && t < v ? lse - picked[token] : __builtin_nanf("");
+      count = 1.0;
     }
+    stats[token] = lse;
+    if (!sums) loss[token] = l;
+    value = (double)l;
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -710,6 +714,9 @@ struct Plan {
   int64_t bytes;
 };
 
+// Tokens per workgroup of the join: one, while they are too few to fill the chip.
+int64_t join_tokens(int64_t n) { return n <= kChip ? 1 : 32; }
+
 // Whether the logits of n tokens and `words` words go without tiles: where less
 // than a quarter of the chip would have one, and k is long (us for the loss,
 // tiles / without; tokens x h x words): float32 10 x 4096 x 100 92 / 31, 300 x
@@ -771,7 +778,7 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
     logits_plan(a->v);
     p.parts = p.few ? few_runs(a->v, a->n)
                     : tiles(p.big, 256) + tiles(a->v - p.big, kBM[p.rest]);
-    p.blocks = tiles(a->n, kJoinTokens);
+    p.blocks = tiles(a->n, join_tokens(a->n));
     p.at_part = take(p.parts * a->n * sizeof(float2));
     p.at_picked = take(a->n * sizeof(float));
     p.at_sums = take(p.blocks * sizeof(double2));
@@ -902,9 +909,9 @@ void forward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
     logits(kBig, 0, p.big, part);
     logits(p.rest, p.big, a->v - p.big, part + tiles(p.big, 256) * a->n);
   }
-  join_kernel<<<(int)p.blocks, kJoinThreads, 0, s>>>(part, (int)p.parts, picked, a->target, a->n,
-                                                     a->v, a->ignore_index, a->stats, a->loss,
-                                                     sums);
+  const auto join = join_tokens(a->n) == 1 ? join_kernel<1> : join_kernel<32>;
+  join<<<(int)p.blocks, kJoinThreads, 0, s>>>(part, (int)p.parts, picked, a->target, a->n, a->v,
+                                              a->ignore_index, a->stats, a->loss, sums);
   if (sums)
     reduce_kernel<<<1, 256, 0, s>>>(sums, p.blocks, a->reduction, a->stats + a->n, a->loss);
 }

@@ -63,7 +63,7 @@ def test_workspace_does_not_hold_the_logits():
 
 
 def test_layout():
-    assert ctypes.sizeof(L.XentArgs) == 144
+    assert ctypes.sizeof(L.XentArgs) == 136
 
 
 def test_arguments():
