@@ -10,9 +10,9 @@
 // a 64-way search (a 20,000-row table takes three loads) and walks on from
 // there, so a row of one element costs one iteration and not a workgroup, and
 // a long row is read in 16-byte loads, kInFlight of them in flight per lane.
-// The norm's loads are non-temporal (2.8e9 bfloat16: 914 us, so 815, 6.9 TB/s;
-// in the scaling, which finds part of the rows in the last-level cache, they
-// cost a tenth).  Loading rows and tiles a step ahead gained nothing.
+// The norm's loads are non-temporal (2.8e9 bfloat16 take 815 us, 6.9 TB/s; cached
+// 914; the scaling, which finds part of the rows in the last-level cache, is a
+// tenth slower so).  Loading rows and tiles a step ahead gained nothing.
 // Partial sums go to one double per workgroup; the kernel behind (the join, or
 // every workgroup of the scaling) sums those in a fixed order: no atomics, so
 // no order that changes from run to run, and no counter to reset.
@@ -276,7 +276,8 @@ __global__ __launch_bounds__(kThreads) void join_kernel(const double *partials, 
 }
 
 // From the end down: what the norm read last is read first, while the last-level
-// cache (256 MB) still holds it.
+// cache (256 MB) still holds it (118M float32 in 20,000 rows: 173 us upwards, 165
+// down, 5.7 TB/s).
 template <int DT>
 __device__ __forceinline__ void scale_span(void *data, int64_t a, int64_t b, float c) {
   typedef Type<DT> T;

@@ -106,6 +106,15 @@ __device__ __forceinline__ float2 join(float2 a, float2 b) {
                               b.y * __builtin_amdgcn_exp2f((b.x - top) * kLog2e));
 }
 
+// Bound by the matrix cores (2 n h v operations; few tokens: by reading the
+// weight once).  The vocabulary lies along the accumulators' rows, so that a
+// lane holds 32 words of a token and the largest and the sum are formed in
+// registers, with two steps across lanes and one across wavefronts.  8,192
+// tokens: h = 4096, v = 128256 6.5 ms (1.3 PFLOP/s); h = 768, v = 50257 0.63 to
+// 0.72 ms (a library product of that size, its result written, 0.58: a third of
+// a tile's time is its first loads and its exponentials).  One token of the
+// former: 175 us (6.0 TB/s).
+//
 // Every token's (largest logit, sum of exp(l - largest)) over each tile's words:
 // part[tile of words from v0][token]; picked[token] = the target's logit.
 template <int DT, typename S>
@@ -180,6 +189,9 @@ __global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand 
 
 constexpr int kJoinThreads = 1024;
 
+// Bound by latency for few tokens (one token, 1,002 records: 4.5 us, with 32
+// threads to a token 10.5 us), by memory for many.
+//
 // Each token's lse and loss from its `parts` records, TOKENS to a workgroup (the
 // records of one shared out to 1024 / TOKENS threads); with a reduction, each
 // workgroup's sums (in float64) of the losses and of the targets that count.
@@ -335,7 +347,9 @@ __global__ __launch_bounds__(1024) void rows_kernel(Factors f) {
   if (threadIdx.x == 0) f.head->back = __builtin_ldexpf(1.0f, -e);
 }
 
-// (Eight words of a token are a lane's: 16-byte stores.)  TWO: what the rounding
+// As logits_kernel, and D written: 8,192 tokens, h = 4096, v = 128256 6.7 ms, h =
+// 768, v = 50257 0.72 to 0.80 ms (8-byte stores 0.84).  Eight words of a token are
+// a lane's (kPaired).  TWO: what the rounding
 // leaves too, n rows further down.
 // D of words [v0, v0 + tiles_m BM), 0 past the vocabulary: d[token][word - v0].
 template <int DT, typename S, bool TWO>
@@ -530,6 +544,13 @@ __global__ __launch_bounds__(kFewThreads) void few_slope_kernel(Operand w, Opera
   }
 }
 
+// D W and D^T X.  Bound by the matrix cores; both operands of the second and one
+// of the first lie with k along their lines, which the LDS reads turn, so that
+// nothing is transposed in memory.  8,192 tokens, h = 4096, v = 128256: 6.1 and
+// 6.3 ms (1.4 PFLOP/s); h = 768, v = 50257: 0.57 and 0.52 ms.  A few tokens'
+// d_weight is bound by writing it (one token: 1.05 GB in 325 us, 128 x 128 tiles
+// 400 us, non-temporal stores no faster).
+//
 // A product into float32 (out[split][n][m], added to what is there with `add`)
 // or, with out16, scaled back into the operands' type.
 template <int DT, int AB, typename S>
@@ -585,7 +606,7 @@ __global__ __launch_bounds__(S::kThreads) void product_kernel(Operand a, Operand
   }
 }
 
-// The sum of `splits` float32 products, scaled back, in the operands' type.
+// Bound by memory.  The sum of `splits` float32 products, scaled back, in the operands' type.
 template <int DT>
 __global__ __launch_bounds__(256) void sum_kernel(const float *part, int splits, int64_t count,
                                                   Factors factors,
@@ -686,7 +707,8 @@ int64_t big_words(int64_t n, int64_t words) {
 }
 
 // Words per piece of the vocabulary: pieces of about equal length, each at most
-// kPieceBytes of D.
+// kPieceBytes of D (pieces of 256 MB, which the last-level cache holds: d_hidden
+// of 8,192 x 768 tokens takes 0.90 ms in four, 0.60 in one).
 constexpr int64_t kPieceBytes = 1 << 30;
 int64_t piece_for(int64_t n, int64_t v, int64_t size) {
   const int64_t all = tiles(v, 256);
