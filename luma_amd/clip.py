@@ -206,6 +206,8 @@ class _Slow:
         for _, batch in self.batches:
             if len(batch.rows):
                 batch.call("luma_grad_scale", batch.args(L.NORM_L2, max_norm, total))
+        torch.autograd.graph.increment_version(
+            [g for gs in self.sharded.values() for g in gs if not g.is_inference()])
         for g, dense in self.copies:
             g.copy_(dense)
 

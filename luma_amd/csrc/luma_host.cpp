@@ -412,9 +412,10 @@ constexpr int64_t kGradTile = LUMA_GRAD_TILE;
 
 // One part's *count rows, their first_tile within the part; false for a tensor
 // that the kernels cannot take as it is.  *device: the CUDA device of all of them
-// (-1 for none).
-bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, GradRow *rows, int64_t *count,
-                int64_t *device) noexcept {
+// (-1 for none).  written: the kernels will write to them, as torch's in-place
+// operations record it (what autograd has saved of them is then stale).
+bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, bool written, GradRow *rows,
+                int64_t *count, int64_t *device) noexcept {
   int64_t dev = -1, tiles = 0;     // (not *device: its neighbours are other threads')
   GradRow *row = rows;
   try {
@@ -458,6 +459,10 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, GradRow *rows, i
       const uint64_t p = (uint64_t)(uintptr_t)g->data();
       if (!p) return false;
       if (tiles > INT32_MAX) return false;
+      if (written) {
+        c10::TensorImpl *w = const_cast<c10::TensorImpl *>(g);
+        if (!w->is_inference()) w->bump_version();
+      }
       *row++ = {p, g->numel(), code, (int32_t)tiles};
       tiles += (g->numel() - 1) / kGradTile + 1;
     }
@@ -501,7 +506,7 @@ py::object grad_rows(py::list objs, bool of_grad, bool apart, uintptr_t table) {
   bool ok[kMaxThreads];
   const std::function<void(int)> job = [&](int t) {
     const int64_t a = n * t / T, b = n * (t + 1) / T;
-    ok[t] = grad_range(o + a, b - a, of_grad, rows + a, &count[t], &device[t]);
+    ok[t] = grad_range(o + a, b - a, of_grad, apart, rows + a, &count[t], &device[t]);
   };
   if (T == 1)
     job(0);
@@ -567,7 +572,7 @@ py::object grad_norm(py::list objs, bool clip, int32_t norm, double max_norm, in
   if (n > most || n == 0 || !g_lib.norm) return py::none();
   std::vector<GradRow> rows(n);
   int64_t count = 0, device = -1;
-  if (!grad_range(&PyList_GET_ITEM(objs.ptr(), 0), n, clip, rows.data(), &count, &device) ||
+  if (!grad_range(&PyList_GET_ITEM(objs.ptr(), 0), n, clip, clip, rows.data(), &count, &device) ||
       count == 0 || (clip && !disjoint(rows.data(), count)))
     return py::none();
   const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)device);

@@ -163,8 +163,10 @@ _forward_op.register_autograd(_backward, setup_context=_setup)
 
 
 def _plain(*tensors) -> bool:
-    """Whether no tensor is of a subclass with a dispatch of its own."""
-    return all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors)
+    """Whether no tensor is of a subclass with a dispatch of its own, or one of
+    torch.func's."""
+    return (not torch._C._are_functorch_transforms_active()
+            and all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors))
 
 
 def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,

@@ -256,6 +256,16 @@ def test_without_the_host_module(monkeypatch):
     assert torch.equal(t, u) and all(torch.equal(x, y) for x, y in zip(a, b))
 
 
+@pytest.mark.parametrize("tensors", [3, 700])
+def test_autograd_sees_the_write(tensors):
+    grads = _make([17] * tensors + [5], torch.float32)
+    before = [g._version for g in grads]
+    luma_amd.get_total_norm(grads)
+    assert [g._version for g in grads] == before
+    luma_amd.clip_grad_norm_(_params(grads), 0.1)
+    assert all(g._version > v for g, v in zip(grads, before))
+
+
 def test_other_stream():
     grads = _make([1 << 20] * 4, torch.float32)
     want = _exact_norm(grads, 2.0)

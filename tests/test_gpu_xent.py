@@ -406,6 +406,45 @@ def test_compile():
     assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+def test_without_grad_and_in_inference_mode():
+    x, w, t = _inputs(50, 64, 300, torch.bfloat16, seed=22)
+    want = linear_cross_entropy(x, w, t)
+    with torch.no_grad():
+        got = linear_cross_entropy(x.requires_grad_(), w, t)
+    assert torch.equal(got, want) and not got.requires_grad
+    with torch.inference_mode():
+        assert torch.equal(linear_cross_entropy(x.clone(), w.clone(), t.clone()), want)
+
+
+def test_torch_func_is_refused():
+    """torch.func's transforms do not trace the ops (torch.autograd does)."""
+    x, w, t = _inputs(50, 64, 300, torch.float32, seed=23)
+    with pytest.raises(RuntimeError, match="functorch"):
+        torch.func.grad(lambda w: linear_cross_entropy(x, w, t))(w)
+
+
+def test_without_the_host_module(monkeypatch):
+    """The custom ops give what the eager path gives."""
+    x, w, t = _inputs(100, 64, 300, torch.bfloat16, seed=24)
+    outs = []
+    for _ in range(2):
+        a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+        loss = linear_cross_entropy(a, b, t)
+        outs.append((loss.detach(), *torch.autograd.grad(loss, (a, b))))
+        monkeypatch.setattr(luma_amd._lib, "host_calls", lambda: None)
+    assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+def test_operand_changed_before_the_backward_is_noticed():
+    x, w, t = _inputs(50, 64, 300, torch.float32, seed=25)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    loss = linear_cross_entropy(a, b, t)
+    with torch.no_grad():
+        b.mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+
+
 def test_refusals():
     x, w, t = _inputs(10, 16, 30, torch.float32)
     cases = [((x, w, t), dict(reduction="max"), ValueError, "reduction"),
