@@ -77,6 +77,8 @@ class _Batch:
             host = self.host
             if host is None:
                 host = torch.from_numpy(self.rows.view(np.uint8)).pin_memory()
+            # (on a stream of its own, beside what runs still, 20,000 tensors took
+            # 644 us in place of 323: the wait between the streams costs more)
             table = host[:n * L.GRAD_DTYPE.itemsize].to(self.device, non_blocking=True)
         self.keep = (partials, table)
         return L.NormArgs(

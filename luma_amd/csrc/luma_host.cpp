@@ -685,11 +685,24 @@ struct Xent : torch::autograd::Function<Xent> {
   }
 };
 
-// hidden [n][h], weight [v][h] and target [n] as linear_cross_entropy checked them.
-at::Tensor xent(const at::Tensor &hidden, const at::Tensor &weight, const at::Tensor &target,
+// linear_cross_entropy of plain tensors; None where its arguments do not fit (the
+// caller then says which).
+py::object xent(const at::Tensor &hidden, const at::Tensor &weight, const at::Tensor &target,
                 int64_t ignore, int64_t reduction) {
-  if (!g_lib.forward) throw py::value_error("xent: the library is not bound");
-  return Xent::apply(hidden, weight, target, ignore, reduction);
+  if (!g_lib.forward || !hidden.is_cuda() || weight.device() != hidden.device() ||
+      target.device() != hidden.device() || hidden.layout() != at::kStrided ||
+      weight.layout() != at::kStrided || target.layout() != at::kStrided)
+    return py::none();
+  const int64_t d = hidden.dim();
+  if (d < 1 || weight.dim() != 2 || weight.size(0) == 0 || weight.size(1) == 0 ||
+      hidden.size(d - 1) != weight.size(1) || grad_code(hidden.scalar_type()) < 0 ||
+      weight.scalar_type() != hidden.scalar_type() || target.scalar_type() != at::kLong ||
+      target.sizes() != hidden.sizes().slice(0, d - 1))
+    return py::none();
+  if (d == 2) return py::cast(Xent::apply(hidden, weight, target, ignore, reduction));
+  const at::Tensor loss = Xent::apply(hidden.reshape({-1, weight.size(1)}), weight,
+                                      target.reshape({-1}), ignore, reduction);
+  return py::cast(reduction == LUMA_XENT_NONE ? loss.view(target.sizes()) : loss);
 }
 
 PYBIND11_MODULE(_luma_host, m) {

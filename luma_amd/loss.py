@@ -190,19 +190,17 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     if hidden.is_cuda and torch.is_autocast_enabled("cuda"):
         dtype = torch.get_autocast_dtype("cuda")
         hidden, weight = hidden.to(dtype), weight.to(dtype)
+    compiling = torch.compiler.is_compiling()
+    if not compiling and _plain(hidden, weight, target):
+        host = L.host_calls()
+        loss = None if host is None else host.xent(hidden, weight, target, ignore_index, code)
+        if loss is not None:
+            return loss
     _check_types(hidden, weight, target)
+    if not compiling:
+        _check(hidden, weight, target)
     shape = target.shape
     if len(shape) != 1:
         hidden, target = hidden.reshape(-1, hidden.shape[-1]), target.reshape(-1)
-    if torch.compiler.is_compiling():
-        loss, _ = torch.ops.luma_amd.linear_cross_entropy(hidden, weight, target, ignore_index,
-                                                          code)
-    else:
-        _check(hidden, weight, target)
-        host = L.host_calls() if _plain(hidden, weight, target) else None
-        if host is not None:
-            loss = host.xent(hidden, weight, target, ignore_index, code)
-        else:
-            loss, _ = torch.ops.luma_amd.linear_cross_entropy(hidden, weight, target,
-                                                              ignore_index, code)
+    loss, _ = torch.ops.luma_amd.linear_cross_entropy(hidden, weight, target, ignore_index, code)
     return loss.view(shape) if code == L.XENT_NONE and len(shape) != 1 else loss
