@@ -464,9 +464,10 @@ typedef struct LumaXentArgs {
   int32_t dtype;         /* LUMA_GRAD_*: both operands and both gradients        */
   int32_t reduction;     /* LUMA_XENT_*                                          */
   float *loss;           /* forward: device [n] or [1]                           */
-  float *stats;          /* device [n + 1]: each token's lse, then the number of
-                            targets that count; the forward writes it, the
-                            backward reads it                                    */
+  float *stats;          /* device [2 n + 1]: each token's largest logit, then each
+                            one's sum of exp(l - largest), then the number of
+                            targets that count (a sum or a mean); the forward
+                            writes it, the backward reads it                     */
   const float *grad_loss;/* backward: device [n] or [1]                          */
   void *d_hidden;        /* backward: device [n][h] dense, or NULL               */
   void *d_weight;        /* backward: device [v][h] dense, or NULL               */

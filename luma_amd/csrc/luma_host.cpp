@@ -645,7 +645,7 @@ struct Xent : torch::autograd::Function<Xent> {
       stats = at::zeros({1}, f32);
     } else {
       loss = at::empty(shape, f32);
-      stats = at::empty({n + 1}, f32);
+      stats = at::empty({2 * n + 1}, f32);
       const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
       LumaXentArgs a = xent_args(x, w, t, stats, ignore, reduction);
       a.loss = loss.mutable_data_ptr<float>();

@@ -7,12 +7,12 @@
 //            exp(l - largest), and the target's logit; then a join over the
 //            vocabulary's tiles.
 // Backward:  for each piece of the vocabulary: the logits again, from them
-//            D = r_i (exp(l - lse_i) - [target]) in the operands' type; then
+//            D = r_i (exp(l - top_i) / sum_i - [target]) in the operands' type; then
 //            d_weight's rows of the piece = D^T X and d_hidden += D W.
 //            r_i is the token's gradient times a power of two that brings the
 //            largest to about 2^kTop (float16's range is short); the products
-//            are scaled back in float32, which is exact.  For one gradient for
-//            all tokens (a mean, a sum) it is formed where it is used.
+//            are scaled back in float32, which is exact.  One gradient for all
+//            tokens (a mean, a sum) stays out of D altogether.
 #include <hip/hip_fp16.h>
 #include <hip/hip_runtime.h>
 
@@ -26,7 +26,6 @@ namespace {
 using namespace gemm;
 
 constexpr float kLog2e = 1.44269504088896340736f;
-constexpr float kLn2 = 0.69314718055994530942f;
 
 template <int DT>
 struct Elem;
@@ -163,13 +162,13 @@ __global__ __launch_bounds__(S::kThreads) void logits_kernel(Operand w, Operand 
 #pragma unroll
     for (int o = 16; o < 64; o *= 2) top = fmaxf(top, __shfl_xor(top, o));
     // (all -inf: their exponentials are 0 and not NaN)
-    const float base = (top == -__builtin_inff() ? 0.0f : top) * kLog2e;
+    const float base = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f;
 #pragma unroll
     for (int q = 0; q < S::TM; ++q)
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const float e = __builtin_amdgcn_exp2f(__builtin_fmaf(acc.t[q][j][r], kLog2e, -base));
+        const float e = __builtin_amdgcn_exp2f((acc.t[q][j][r] - base) * kLog2e);
         if (whole || at.m + P::row(q) + r < v) sum += e;
       }
 #pragma unroll
@@ -192,7 +191,7 @@ constexpr int kJoinThreads = 1024;
 // Bound by latency for few tokens (one token, 1,002 records: 4.5 us, with 32
 // threads to a token 10.5 us), by memory for many.
 //
-// Each token's lse and loss from its `parts` records, TOKENS to a workgroup (the
+// Each token's largest logit, sum and loss from its `parts` records, TOKENS to a workgroup (the
 // records of one shared out to 1024 / TOKENS threads); with a reduction, each
 // workgroup's sums (in float64) of the losses and of the targets that count.
 template <int TOKENS>
@@ -230,15 +229,15 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(const float2 *part, 
   if (threadIdx.x >= 64) return;      // (the rest is the first wavefront's)
   double value = 0.0, count = 0.0;
   if (slice == 0 && token < n) {
-    const float lse = a.x == -__builtin_inff() ? __builtin_nanf("")
-                                               : a.x + __builtin_amdgcn_logf(a.y) * kLn2;
     const int64_t t = target[token];
     float l = 0.0f;
     if (t != ignore) {
-      l = t >= 0 && t < v ? lse - picked[token] : __builtin_nanf("");
+      // (not lse - l: a small loss is the difference of nearly equal numbers)
+      l = t >= 0 && t < v ? (a.x - picked[token]) + logf(a.y) : __builtin_nanf("");
       count = 1.0;
     }
-    stats[token] = lse;
+    stats[token] = a.x;
+    stats[n + token] = a.y;
     if (!sums) loss[token] = l;
     value = (double)l;
   }
@@ -283,8 +282,10 @@ struct Rows {
 
 // Each token's factor r_i: the gradient of its loss times a power of two that
 // brings the largest to 2^(TOP - 1) .. 2^TOP; 0 for an ignored target, NaN for
-// one outside the vocabulary.  One gradient for all tokens needs no pass over
-// them; with one per token, rows_kernel has looked for the largest.
+// one outside the vocabulary.  With one gradient g for all tokens r_i is the
+// power of two 2^(TOP - 1) alone and the products are scaled back by g over it: D is then
+// p - [target] itself, whose target's entry is nearly -1 and rounds to little; of
+// g (p - [target]) every token's would be off by the same up to 2^-9.
 struct Factors {
   const float *grad;
   const int64_t *target;
@@ -294,32 +295,25 @@ struct Factors {
   Rows *head;       // rows_kernel's (LUMA_XENT_NONE)
   float *rows;
 
-  __device__ __forceinline__ float grad_of(int64_t i) const {
-    if (reduction == LUMA_XENT_NONE) return grad[i];
-    return reduction == LUMA_XENT_MEAN ? grad[0] / stats[n] : grad[0];
+  // One gradient for all tokens.
+  __device__ __forceinline__ float one() const {
+    return reduction == LUMA_XENT_MEAN ? grad[0] / stats[2 * n] : grad[0];
   }
   __device__ __forceinline__ float factor(int64_t t, float g) const {
     return t == ignore ? 0.0f : t >= 0 && t < v ? g : __builtin_nanf("");
   }
-  // the exponent of the power of two, of the largest finite |g|
-  template <int TOP>
-  static __device__ __forceinline__ int power(float top) {
-    if (!(top > 0.0f && top < __builtin_inff())) return 0;
-    int e;
-    __builtin_frexpf(top, &e);           // top = f 2^e, f in [0.5, 1)
-    e = TOP - e;
-    return e > 100 ? 100 : e < -100 ? -100 : e;
-  }
   template <int TOP>
   __device__ __forceinline__ float row(int64_t i, int64_t t) const {
     if (reduction == LUMA_XENT_NONE) return rows[i];
-    const float g = grad_of(0);
-    return factor(t, g * __builtin_ldexpf(1.0f, power<TOP>(__builtin_fabsf(g))));
+    const float g = one();
+    // (an infinity's or a NaN's tokens get it, the ignored ones 0)
+    return factor(t, __builtin_isfinite(g) ? __builtin_ldexpf(0.5f, TOP) : g);
   }
   template <int TOP>
   __device__ __forceinline__ float back() const {
     if (reduction == LUMA_XENT_NONE) return head->back;
-    return __builtin_ldexpf(1.0f, -power<TOP>(__builtin_fabsf(grad_of(0))));
+    const float g = one();
+    return __builtin_isfinite(g) ? g * __builtin_ldexpf(2.0f, -TOP) : 1.0f;
   }
 };
 
@@ -340,7 +334,12 @@ __global__ __launch_bounds__(1024) void rows_kernel(Factors f) {
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < 16; ++w) top = fmaxf(top, lds[w]);
-  const int e = Factors::power<TOP>(top);
+  int e = 0;
+  if (top > 0.0f) {
+    __builtin_frexpf(top, &e);           // top = f 2^e, f in [0.5, 1)
+    e = TOP - e;
+    e = e > 100 ? 100 : e < -100 ? -100 : e;
+  }
   const float up = __builtin_ldexpf(1.0f, e);
   for (int64_t i = threadIdx.x; i < f.n; i += 1024)
     f.rows[i] = f.factor(f.target[i], f.grad[i] * up);
@@ -370,7 +369,8 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
     const int64_t token = at.n + 16 * j;
     if (token >= n) continue;
     const int64_t word = factors.target[token];
-    const float base = factors.stats[token] * kLog2e, row = factors.row<kTop<DT>>(token, word);
+    const float top = factors.stats[token], part = 1.0f / factors.stats[n + token];
+    const float row = factors.row<kTop<DT>>(token, word);
     const int64_t t = word - v0 - at.m;
     typename Elem<DT>::type *out = d + token * ld + at.m;
 #pragma unroll
@@ -378,8 +378,7 @@ __global__ __launch_bounds__(S::kThreads) void slope_kernel(Operand w, Operand x
       Eight<DT> f, rest;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        float p = __builtin_amdgcn_exp2f(
-            __builtin_fmaf(acc.t[q + e / 4][j][e % 4], kLog2e, -base));
+        float p = __builtin_amdgcn_exp2f((acc.t[q + e / 4][j][e % 4] - top) * kLog2e) * part;
         if (t == P::row(q) + e) p -= 1.0f;
         // (an ignored token's logits may be anything)
         const float g = row == 0.0f || v0 + at.m + P::row(q) + e >= v ? 0.0f : p * row;
@@ -524,7 +523,8 @@ __global__ __launch_bounds__(kFewThreads) void few_slope_kernel(Operand w, Opera
   __shared__ typename F::Lds lds;
   const int64_t n0 = (int64_t)blockIdx.y * F::kTokens, token = n0 + F::token();
   const int64_t t = token < n ? factors.target[token] : 0;
-  const float base = token < n ? factors.stats[token] * kLog2e : 0.0f;
+  const float top = token < n ? factors.stats[token] : 0.0f;
+  const float part = token < n ? 1.0f / factors.stats[n + token] : 0.0f;
   const float row = token < n ? factors.row<kTop<DT>>(token, t) : 0.0f;
   for (int64_t m0 = (int64_t)blockIdx.x * kFewRows; m0 < padded;
        m0 += (int64_t)gridDim.x * kFewRows) {
@@ -534,7 +534,7 @@ __global__ __launch_bounds__(kFewThreads) void few_slope_kernel(Operand w, Opera
 #pragma unroll
     for (int e = 0; e < F::kPer; ++e) {
       const int64_t at = m0 + F::word() + e, word = v0 + at;
-      float p = __builtin_amdgcn_exp2f(__builtin_fmaf(l[e], kLog2e, -base));
+      float p = __builtin_amdgcn_exp2f((l[e] - top) * kLog2e) * part;
       if (word == t) p -= 1.0f;
       const float f = row == 0.0f || word >= v ? 0.0f : p * row;
       const typename Elem<DT>::type hi = Elem<DT>::round(f);
@@ -806,7 +806,9 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
     p.at_sums = take(p.blocks * sizeof(double2));
   } else {
     p.piece = piece_for(p.rows_d, a->v, p.size);
-    logits_plan(p.piece);
+    // (the same tiles as the forward's: the largest logit is then the same
+    // number, and its probability 1 / sum exactly)
+    logits_plan(p.piece < a->v ? p.piece : a->v);
     p.ld_d = p.piece;
     p.at_head = take(sizeof(Rows));
     p.at_rows = take(a->n * sizeof(float));
@@ -935,7 +937,7 @@ void forward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
   join<<<(int)p.blocks, kJoinThreads, 0, s>>>(part, (int)p.parts, picked, a->target, a->n, a->v,
                                               a->ignore_index, a->stats, a->loss, sums);
   if (sums)
-    reduce_kernel<<<1, 256, 0, s>>>(sums, p.blocks, a->reduction, a->stats + a->n, a->loss);
+    reduce_kernel<<<1, 256, 0, s>>>(sums, p.blocks, a->reduction, a->stats + 2 * a->n, a->loss);
 }
 
 template <int DT>
@@ -983,9 +985,9 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
       });
     };
     if (p.few) {
-      with_few(padded, a->n, [&](auto tn) {
+      with_few(a->v, a->n, [&](auto tn) {
         constexpr int TN = decltype(tn)::value;
-        const dim3 grid((int)few_runs(padded, a->n), (int)tiles(a->n, 16 * TN));
+        const dim3 grid((int)few_runs(a->v, a->n), (int)tiles(a->n, 16 * TN));
         auto go = [&](auto two) {
           few_slope_kernel<DT, TN, decltype(two)::value><<<grid, kFewThreads, 0, s>>>(
               w, x, v0, a->v, padded, a->n, factors, d, p.ld_d);
@@ -996,8 +998,10 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
         go(std::false_type{});
       });
     } else {
-      slope(kBig, 0, p.big < padded ? p.big : padded);
-      slope(p.rest, p.big, padded - p.big);
+      // (whole tiles: all of the padding, or whole_rounds')
+      const int64_t big = p.big < words ? p.big : padded;
+      slope(kBig, 0, big);
+      slope(p.rest, big, padded - big);
     }
     const Operand wp = {w.p + v0 * w.ld, w.ld, words, w.row_bytes};
     if (a->d_hidden) {

@@ -98,7 +98,7 @@ def _forward_op(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor
     if n == 0:
         loss.fill_(float("nan") if reduction == L.XENT_MEAN else 0.0)
         return loss, torch.zeros(1, dtype=torch.float32, device=device)
-    stats = torch.empty(n + 1, dtype=torch.float32, device=device)
+    stats = torch.empty(2 * n + 1, dtype=torch.float32, device=device)
     hidden, weight, target = _rows(hidden), _rows(weight), target.contiguous()
     args = _args(hidden, weight, target, stats, ignore_index, reduction)
     args.loss = loss.data_ptr()
@@ -110,7 +110,7 @@ def _forward_op(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor
 def _(hidden, weight, target, ignore_index, reduction):
     n = hidden.shape[0]
     loss = hidden.new_empty((n,) if reduction == L.XENT_NONE else (), dtype=torch.float32)
-    return loss, hidden.new_empty((n + 1,), dtype=torch.float32)
+    return loss, hidden.new_empty((2 * n + 1,), dtype=torch.float32)
 
 
 @torch.library.custom_op("luma_amd::linear_cross_entropy_backward", mutates_args=(),
