@@ -528,8 +528,8 @@ __global__ __launch_bounds__(kFewThreads) void few_slope_kernel(Operand w, Opera
   const float row = token < n ? factors.row<kTop<DT>>(token, t) : 0.0f;
   for (int64_t m0 = (int64_t)blockIdx.x * kFewRows; m0 < padded;
        m0 += (int64_t)gridDim.x * kFewRows) {
-    float l[F::kPer];
-    F::run(w, x, v0 + m0, n0, lds, l);
+    float l[F::kPer] = {};
+    if (v0 + m0 < v) F::run(w, x, v0 + m0, n0, lds, l);     // (else padding)
     if (token >= n) continue;
 #pragma unroll
     for (int e = 0; e < F::kPer; ++e) {
@@ -752,8 +752,8 @@ int few_tn(int64_t words, int64_t n) {
   return tiles(words, kFewRows) * tiles(n, 16) < kChip ? 1 : 4;
 }
 // Runs of tiles of words: about four workgroups to a CU in all.
-int64_t few_runs(int64_t words, int64_t n) {
-  const int64_t groups = tiles(n, 16 * few_tn(words, n)), most = groups < 1024 ? 1024 / groups : 1;
+int64_t few_runs(int64_t words, int64_t n, int tn) {
+  const int64_t groups = tiles(n, 16 * tn), most = groups < 1024 ? 1024 / groups : 1;
   const int64_t all = tiles(words, kFewRows);
   return all < most ? all : most;
 }
@@ -798,7 +798,7 @@ bool plan(const LumaXentArgs *a, bool backward, Plan &p) {
   if (p.pack_w) p.at_w = take(a->v * p.ld_w * p.size);
   if (!backward) {
     logits_plan(a->v);
-    p.parts = p.few ? few_runs(a->v, a->n)
+    p.parts = p.few ? few_runs(a->v, a->n, few_tn(a->v, a->n))
                     : tiles(p.big, 256) + tiles(a->v - p.big, kBM[p.rest]);
     p.blocks = tiles(a->n, join_tokens(a->n));
     p.at_part = take(p.parts * a->n * sizeof(float2));
@@ -987,7 +987,7 @@ void backward(const LumaXentArgs *a, const Plan &p, hipStream_t s) {
     if (p.few) {
       with_few(a->v, a->n, [&](auto tn) {
         constexpr int TN = decltype(tn)::value;
-        const dim3 grid((int)few_runs(a->v, a->n), (int)tiles(a->n, 16 * TN));
+        const dim3 grid((int)few_runs(padded, a->n, TN), (int)tiles(a->n, 16 * TN));
         auto go = [&](auto two) {
           few_slope_kernel<DT, TN, decltype(two)::value><<<grid, kFewThreads, 0, s>>>(
               w, x, v0, a->v, padded, a->n, factors, d, p.ld_d);
