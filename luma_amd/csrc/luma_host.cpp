@@ -631,6 +631,19 @@ void xent_call(LumaXentArgs &a, bool backward, const at::Tensor &like) {
   TORCH_CHECK(rc == 0, g_lib.error());
 }
 
+// A gradient under create_graph=True: depends on the operands, and says so when it
+// is differentiated.
+struct XentOnce : torch::autograd::Function<XentOnce> {
+  static at::Tensor forward(torch::autograd::AutogradContext *, const at::Tensor &grad,
+                            const at::Tensor &, const at::Tensor &, const at::Tensor &) {
+    return grad.detach();
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext *,
+                                                 torch::autograd::variable_list) {
+    TORCH_CHECK(false, "linear_cross_entropy: its gradients cannot be differentiated again");
+  }
+};
+
 struct Xent : torch::autograd::Function<Xent> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &hidden,
                             const at::Tensor &weight, const at::Tensor &target, int64_t ignore,
@@ -665,21 +678,26 @@ struct Xent : torch::autograd::Function<Xent> {
     if (grads[0].defined() && (want_hidden || want_weight)) {
       const auto saved = ctx->get_saved_variables();
       const at::Tensor &hidden = saved[0], &weight = saved[1], &target = saved[2];
-      at::AutoDispatchBelowADInplaceOrView below;
-      if (want_hidden) d_hidden = at::empty(hidden.sizes(), hidden.options());
-      if (want_weight) d_weight = at::empty(weight.sizes(), weight.options());
-      if (hidden.size(0) == 0) {
-        if (want_weight) d_weight.zero_();
-      } else {
-        const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
-        const at::Tensor g = grads[0].to(at::kFloat).contiguous();
-        LumaXentArgs a = xent_args(x, w, t, saved[3], ctx->saved_data["ignore"].toInt(),
-                                   ctx->saved_data["reduction"].toInt());
-        a.grad_loss = g.const_data_ptr<float>();
-        a.d_hidden = want_hidden ? d_hidden.mutable_data_ptr() : nullptr;
-        a.d_weight = want_weight ? d_weight.mutable_data_ptr() : nullptr;
-        xent_call(a, true, hidden);
+      {
+        at::AutoDispatchBelowADInplaceOrView below;
+        if (want_hidden) d_hidden = at::empty(hidden.sizes(), hidden.options());
+        if (want_weight) d_weight = at::empty(weight.sizes(), weight.options());
+        if (hidden.size(0) == 0) {
+          if (want_weight) d_weight.zero_();
+        } else {
+          const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
+          const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+          LumaXentArgs a = xent_args(x, w, t, saved[3], ctx->saved_data["ignore"].toInt(),
+                                     ctx->saved_data["reduction"].toInt());
+          a.grad_loss = g.const_data_ptr<float>();
+          a.d_hidden = want_hidden ? d_hidden.mutable_data_ptr() : nullptr;
+          a.d_weight = want_weight ? d_weight.mutable_data_ptr() : nullptr;
+          xent_call(a, true, hidden);
+        }
       }
+      if (at::GradMode::is_enabled())
+        for (at::Tensor *d : {&d_hidden, &d_weight})
+          if (d->defined()) *d = XentOnce::apply(*d, hidden, weight, grads[0]);
     }
     return {d_hidden, d_weight, at::Tensor(), at::Tensor(), at::Tensor()};
   }

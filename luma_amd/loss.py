@@ -182,7 +182,7 @@ def linear_cross_entropy(hidden: torch.Tensor, weight: torch.Tensor, target: tor
     ``ignore_index``; NaN if there are none), "sum" or "none" (a loss per
     token, the target's shape).  A target that is neither a word nor
     ``ignore_index`` makes its loss NaN (nothing is read for it); torch stops
-    the program there.
+    the program there.  The gradients cannot be differentiated again (that raises).
     """
     code = _REDUCTIONS.get(reduction)
     if code is None:

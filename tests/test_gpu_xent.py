@@ -128,11 +128,44 @@ def test_large_tiles(n, h, v, dtype):
     _check(*_inputs(n, h, v, dtype, seed=3))
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("n,h,v", [(400, 1100, 500),      # 64 tokens to a workgroup
+                                   (200, 3000, 60),       # 16
+                                   (40, 2056, 90), (1, 1500, 33), (9, 8191, 31)])
+@pytest.mark.parametrize("ignored", [0.0, 0.4])
+def test_few_words_and_long_hidden_states(n, h, v, dtype, ignored):
+    x, w, t = _inputs(n, h, v, dtype, seed=n, ignored=ignored)
+    t[0] = v - 1
+    _check(x, w, t)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("n", [1, 8, 9, 32, 33, 64, 65])
+def test_two_parts_of_few_tokens(n, dtype):
+    """Up to 64 tokens a gradient is off by its own rounding alone: half a unit of
+    each entry, and the float32 terms' (D's second part holds what the first's
+    rounding left, so that u^2 of an entry of D, 2 at most, is lost)."""
+    x, w, t = _inputs(n, 72, 900, dtype, seed=n)
+    g = torch.rand(n, device="cuda") + 0.5
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    got = torch.autograd.grad(linear_cross_entropy(a, b, t, IGNORE, "none"), (a, b), g)
+    ref = Exact(x, w, t, g)
+    f32 = Exact(x.float(), w.float(), t, g)
+    u = UNIT[dtype]
+    for y, want, tol in ((got[0], ref.d_x, f32.tol_x), (got[1], ref.d_w, f32.tol_w)):
+        rel = float((y.double() - want).norm() / want.norm())
+        assert rel <= (u if n <= 64 else 2.0 * u)
+        if n <= 64:
+            dd = 2.0 ** -16 if dtype == torch.bfloat16 else 2.0 ** -22
+            slack = dd * (g.max().double() * 2.0) * (w if y is got[0] else x).double().abs().sum(0)
+            _within(y, want, 1.01 * u * want.abs() + tol + slack + 2.0 ** -25, "a gradient")
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 def test_pieces_of_the_vocabulary(dtype):
-    """More words than one piece holds (256 MB of D)."""
+    """More words than two pieces hold (1 GiB of D each)."""
     n = 8200
-    v = 2 * (256 << 20) // (n * (4 if dtype == torch.float32 else 2)) + 777
+    v = 2 * (1 << 30) // (n * (4 if dtype == torch.float32 else 2)) + 777
     _check(*_inputs(n, 40, v, dtype, seed=4))
 
 
@@ -433,6 +466,24 @@ def test_without_the_host_module(monkeypatch):
         outs.append((loss.detach(), *torch.autograd.grad(loss, (a, b))))
         monkeypatch.setattr(luma_amd._lib, "host_calls", lambda: None)
     assert all(torch.equal(p, q) for p, q in zip(*outs))
+
+
+@pytest.mark.parametrize("module", [True, False])
+def test_gradients_are_not_differentiated_again(module, monkeypatch):
+    """create_graph=True gives the same gradients; to differentiate them raises."""
+    if not module:
+        monkeypatch.setattr(luma_amd._lib, "host_calls", lambda: None)
+    x, w, t = _inputs(50, 64, 300, torch.float32, seed=26)
+    a, b = x.clone().requires_grad_(), w.clone().requires_grad_()
+    want = torch.autograd.grad(linear_cross_entropy(a, b, t), (a, b))
+    for operands in ((a, b), (a, w), (x, b)):
+        loss = linear_cross_entropy(*operands, t)
+        leaves = [p for p in operands if p.requires_grad]
+        got = torch.autograd.grad(loss, leaves, create_graph=True)
+        for p, leaf in zip(got, leaves):
+            assert torch.equal(p, want[0] if leaf is a else want[1])
+            with pytest.raises(RuntimeError):
+                torch.autograd.grad((p ** 2).sum(), leaves, retain_graph=True)
 
 
 def test_operand_changed_before_the_backward_is_noticed():
