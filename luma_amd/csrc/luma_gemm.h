@@ -25,8 +25,9 @@
 // that the power limit leaves.  Before: a barrier for each stage and the
 // compiler's order 7.2 ms (it sank the LDS reads below the matrix instructions,
 // to the barrier); stages of 64-byte lines 6.7.  Not kept: 32 x 32 x 16
-// instructions 7.2; wavefronts of 128 x 128 (accumulators moved and spilled) 25;
-// workgroups that run on from tile to tile 7.1 (no gain at h = 768 either).
+// instructions 7.2; wavefronts of 128 x 96 8.9; of 128 x 128 (accumulators moved
+// and spilled) 25; workgroups that run on from tile to tile 7.1 (no gain at
+// h = 768 either).
 //
 // Loads go through buffer descriptors that end where the operand ends: rows
 // past the end read as zeros, and so does k past the end of a k-contiguous row

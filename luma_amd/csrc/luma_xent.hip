@@ -710,10 +710,12 @@ int64_t big_words(int64_t n, int64_t words) {
 // kPieceBytes of D (pieces of 256 MB, which the last-level cache holds: d_hidden
 // of 8,192 x 768 tokens takes 0.90 ms in four, 0.60 in one).
 constexpr int64_t kPieceBytes = 1 << 30;
+constexpr int64_t kPieceTiles = 1 << 15;   // a tile's offsets into 64 rows of D stay below 2^31
 int64_t piece_for(int64_t n, int64_t v, int64_t size) {
   const int64_t all = tiles(v, 256);
   int64_t most = kPieceBytes / (n * size * 256);
   if (most < 1) most = 1;
+  if (most > kPieceTiles) most = kPieceTiles;
   return tiles(all, tiles(all, most)) * 256;
 }
 
@@ -853,8 +855,10 @@ bool check_args(const LumaXentArgs *a, bool backward) {
     return fail("luma_xent: rows overlap"), false;
   if (a->ld_hidden > 1 << 21 || a->ld_weight > 1 << 21)
     return fail("luma_xent: rows too far apart"), false;
-  // (a launch's workgroups are counted in 32 bits)
-  if (tiles(a->n, 16) * tiles(a->v, 64) > INT32_MAX ||
+  // (a launch's workgroups are counted in 32 bits, and so are its threads: 512 to
+  // a 256 x 256 tile)
+  if (tiles(a->n, 256) * tiles(a->v, 256) > UINT32_MAX / 512 ||
+      tiles(a->n, 16) * tiles(a->v, 64) > INT32_MAX ||
       tiles(a->h, 64) * tiles(a->v, 64) > INT32_MAX / 64 ||
       tiles(a->h, 64) * tiles(a->n, 16) > INT32_MAX / 64)
     return fail("luma_xent: operands too large"), false;

@@ -23,7 +23,7 @@ def _args(**change):
 @pytest.mark.parametrize("change,text", [
     (dict(n=0), "empty"), (dict(h=0), "empty"), (dict(v=-1), "empty"),
     (dict(n=1 << 31), "too large"), (dict(h=1 << 21, ld_hidden=1 << 21, ld_weight=1 << 21), "too large"),
-    (dict(n=1 << 24, v=1 << 24), "too large"),
+    (dict(n=1 << 24, v=1 << 24), "too large"), (dict(n=1 << 20, v=1 << 20), "too large"),
     (dict(dtype=3), "type"), (dict(dtype=-1), "type"), (dict(reduction=3), "reduction"),
     (dict(hidden=None), "null"), (dict(weight=None), "null"), (dict(target=None), "null"),
     (dict(stats=None), "null"), (dict(loss=None), "null"), (dict(ld_hidden=63), "overlap"),
