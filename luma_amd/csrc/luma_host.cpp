@@ -412,10 +412,9 @@ constexpr int64_t kGradTile = LUMA_GRAD_TILE;
 
 // One part's *count rows, their first_tile within the part; false for a tensor
 // that the kernels cannot take as it is.  *device: the CUDA device of all of them
-// (-1 for none).  written: the kernels will write to them, as torch's in-place
-// operations record it (what autograd has saved of them is then stale).
-bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, bool written, GradRow *rows,
-                int64_t *count, int64_t *device) noexcept {
+// (-1 for none).  impls: takes the rows' tensors, or null.
+bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, GradRow *rows,
+                const c10::TensorImpl **impls, int64_t *count, int64_t *device) noexcept {
   int64_t dev = -1, tiles = 0;     // (not *device: its neighbours are other threads')
   GradRow *row = rows;
   try {
@@ -459,10 +458,7 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, bool written, Gr
       const uint64_t p = (uint64_t)(uintptr_t)g->data();
       if (!p) return false;
       if (tiles > INT32_MAX) return false;
-      if (written) {
-        c10::TensorImpl *w = const_cast<c10::TensorImpl *>(g);
-        if (!w->is_inference()) w->bump_version();
-      }
+      if (impls) *impls++ = g;
       *row++ = {p, g->numel(), code, (int32_t)tiles};
       tiles += (g->numel() - 1) / kGradTile + 1;
     }
@@ -473,6 +469,25 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, bool written, Gr
   } catch (...) {
     return false;   // an unusual tensor: the caller looks at it
   }
+}
+
+// Records that the kernels will write to these tensors, as torch's in-place
+// operations do (what autograd has saved of them is then stale).  By the calling
+// thread: the counters are written, and eight threads that take the lines from
+// each other need 390 us for those of 20,000 tensors, one 200.
+void bump_versions(const c10::TensorImpl *const *impls, int64_t n) {
+  auto at = [&](int64_t i) { return const_cast<c10::TensorImpl *>(impls[i]); };
+  uint32_t seen = 0;
+  constexpr int64_t kRun = 64;
+  for (int64_t a = 0; a < n; a += kRun) {
+    const int64_t b = std::min(n, a + kRun);
+    // (an atomic increment waits for all loads before it: a run's lines first)
+    for (int64_t i = a; i < b; ++i)
+      if (!at(i)->is_inference()) seen += (uint32_t)at(i)->version_counter().current_version();
+    for (int64_t i = a; i < b; ++i)
+      if (!at(i)->is_inference()) at(i)->bump_version();
+  }
+  asm volatile("" ::"r"(seen));
 }
 
 // Whether no two rows share memory.
@@ -496,7 +511,7 @@ bool disjoint(const GradRow *rows, int64_t n) {
 // without one left out) to `table`, which has room for one per object.  Returns
 // (rows, device index or -1 for no rows), or None when one of them is a
 // subclass, sparse, not dense, of another type or device, or (apart) shares
-// memory with another: the caller then looks at each.
+// memory with another: the caller then looks at each.  apart: they will be written to.
 py::object grad_rows(py::list objs, bool of_grad, bool apart, uintptr_t table) {
   const int64_t n = (int64_t)objs.size();
   PyObject *const *o = n ? &PyList_GET_ITEM(objs.ptr(), 0) : nullptr;
@@ -504,9 +519,11 @@ py::object grad_rows(py::list objs, bool of_grad, bool apart, uintptr_t table) {
   const int T = (int)std::min<int64_t>(kMaxThreads, std::max<int64_t>(1, n / kPerThread));
   int64_t device[kMaxThreads], count[kMaxThreads];
   bool ok[kMaxThreads];
+  std::vector<const c10::TensorImpl *> impls(apart ? n : 0);
   const std::function<void(int)> job = [&](int t) {
     const int64_t a = n * t / T, b = n * (t + 1) / T;
-    ok[t] = grad_range(o + a, b - a, of_grad, apart, rows + a, &count[t], &device[t]);
+    ok[t] = grad_range(o + a, b - a, of_grad, rows + a, apart ? impls.data() + a : nullptr,
+                       &count[t], &device[t]);
   };
   if (T == 1)
     job(0);
@@ -525,11 +542,15 @@ py::object grad_rows(py::list objs, bool of_grad, bool apart, uintptr_t table) {
       last = first + (r.numel - 1) / kGradTile + 1;
       if (last > INT32_MAX) return py::none();
       r.first_tile = (int32_t)first;
+      if (apart) impls[at] = impls[n * t / T + i];
       rows[at++] = r;
     }
     tiles = last;
   }
-  if (apart && !disjoint(rows, at)) return py::none();
+  if (apart) {
+    if (!disjoint(rows, at)) return py::none();
+    bump_versions(impls.data(), at);
+  }
   return py::make_tuple(at, dev);
 }
 
@@ -571,10 +592,13 @@ py::object grad_norm(py::list objs, bool clip, int32_t norm, double max_norm, in
   const int64_t n = (int64_t)objs.size();
   if (n > most || n == 0 || !g_lib.norm) return py::none();
   std::vector<GradRow> rows(n);
+  std::vector<const c10::TensorImpl *> impls(clip ? n : 0);
   int64_t count = 0, device = -1;
-  if (!grad_range(&PyList_GET_ITEM(objs.ptr(), 0), n, clip, clip, rows.data(), &count, &device) ||
+  if (!grad_range(&PyList_GET_ITEM(objs.ptr(), 0), n, clip, rows.data(),
+                  clip ? impls.data() : nullptr, &count, &device) ||
       count == 0 || (clip && !disjoint(rows.data(), count)))
     return py::none();
+  if (clip) bump_versions(impls.data(), count);
   const c10::Device dev(c10::kCUDA, (c10::DeviceIndex)device);
   const c10::DeviceGuard guard(dev);
   const at::Tensor partials =
