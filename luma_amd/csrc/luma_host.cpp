@@ -16,7 +16,9 @@
 // nothing they read can change under them.  The module computes nothing of
 // the step itself: the step runs in libluma_hip.so.
 #include <ATen/ATen.h>
+#include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
 #include <torch/csrc/autograd/custom_function.h>
@@ -668,6 +670,17 @@ struct XentOnce : torch::autograd::Function<XentOnce> {
   }
 };
 
+// The custom op of the backward, which loss.py registers.
+const auto &backward_op() {
+  static const auto op =
+      c10::Dispatcher::singleton()
+          .findSchemaOrThrow("luma_amd::linear_cross_entropy_backward", "")
+          .typed<std::tuple<at::Tensor, at::Tensor>(
+              const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+              const at::Tensor &, int64_t, int64_t, bool, bool)>();
+  return op;
+}
+
 struct Xent : torch::autograd::Function<Xent> {
   static at::Tensor forward(torch::autograd::AutogradContext *ctx, const at::Tensor &hidden,
                             const at::Tensor &weight, const at::Tensor &target, int64_t ignore,
@@ -702,21 +715,32 @@ struct Xent : torch::autograd::Function<Xent> {
     if (grads[0].defined() && (want_hidden || want_weight)) {
       const auto saved = ctx->get_saved_variables();
       const at::Tensor &hidden = saved[0], &weight = saved[1], &target = saved[2];
+      const int64_t ignore = ctx->saved_data["ignore"].toInt();
+      const int64_t reduction = ctx->saved_data["reduction"].toInt();
       {
         at::AutoDispatchBelowADInplaceOrView below;
-        if (want_hidden) d_hidden = at::empty(hidden.sizes(), hidden.options());
-        if (want_weight) d_weight = at::empty(weight.sizes(), weight.options());
-        if (hidden.size(0) == 0) {
-          if (want_weight) d_weight.zero_();
+        if (c10::impl::dispatch_mode_enabled()) {
+          // (a tracer or another mode, begun since the forward, watches the operators
+          // called: it is given one, which holds the kernels)
+          std::tie(d_hidden, d_weight) =
+              backward_op().call(grads[0], hidden, weight, target, saved[3], ignore, reduction,
+                                 want_hidden, want_weight);
+          if (!want_hidden) d_hidden.reset();
+          if (!want_weight) d_weight.reset();
         } else {
-          const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
-          const at::Tensor g = grads[0].to(at::kFloat).contiguous();
-          LumaXentArgs a = xent_args(x, w, t, saved[3], ctx->saved_data["ignore"].toInt(),
-                                     ctx->saved_data["reduction"].toInt());
-          a.grad_loss = g.const_data_ptr<float>();
-          a.d_hidden = want_hidden ? d_hidden.mutable_data_ptr() : nullptr;
-          a.d_weight = want_weight ? d_weight.mutable_data_ptr() : nullptr;
-          xent_call(a, true, hidden);
+          if (want_hidden) d_hidden = at::empty(hidden.sizes(), hidden.options());
+          if (want_weight) d_weight = at::empty(weight.sizes(), weight.options());
+          if (hidden.size(0) == 0) {
+            if (want_weight) d_weight.zero_();
+          } else {
+            const at::Tensor x = rows_of(hidden), w = rows_of(weight), t = target.contiguous();
+            const at::Tensor g = grads[0].to(at::kFloat).contiguous();
+            LumaXentArgs a = xent_args(x, w, t, saved[3], ignore, reduction);
+            a.grad_loss = g.const_data_ptr<float>();
+            a.d_hidden = want_hidden ? d_hidden.mutable_data_ptr() : nullptr;
+            a.d_weight = want_weight ? d_weight.mutable_data_ptr() : nullptr;
+            xent_call(a, true, hidden);
+          }
         }
       }
       if (at::GradMode::is_enabled())

@@ -6,8 +6,10 @@ reference's benchmark trains on (benchmarks/bench_nanogpt.py), for a head of
 any size: the logits are formed tile by tile on the matrix cores and consumed
 there, and the backward forms them again, a piece of the vocabulary at a time
 (luma_xent_forward / luma_xent_backward in include/luma.h).  Both directions
-are ``torch.library`` custom ops, so ``torch.compile(fullgraph=True)`` traces
-them, and they do no host synchronisation::
+are ``torch.library`` custom ops, so ``torch.compile(fullgraph=True)``, ``make_fx``
+and ``torch.jit.trace`` record them, and they do no host synchronisation (an
+eager call that nothing records goes through the host module, to the same
+kernels)::
 
     loss = luma_amd.linear_cross_entropy(hidden, head.weight, target)
     loss.backward()
@@ -163,9 +165,13 @@ _forward_op.register_autograd(_backward, setup_context=_setup)
 
 
 def _plain(*tensors) -> bool:
-    """Whether no tensor is of a subclass with a dispatch of its own, or one of
-    torch.func's."""
-    return (not torch._C._are_functorch_transforms_active()
+    """Whether the host module may take the call: nothing records or watches the
+    operators called (a tracer or a dispatch mode would see the allocation of
+    the module's outputs, and not the kernels that fill them), and no tensor is
+    of a subclass with a dispatch of its own, or one of torch.func's."""
+    return (torch._C._len_torch_dispatch_stack() == 0
+            and torch._C._get_tracing_state() is None
+            and not torch._C._are_functorch_transforms_active()
             and all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors))
 
 
