@@ -15,7 +15,8 @@ synchronisation.  The norm is a float32 scalar on the gradients' device,
 summed in float64, whatever the gradients' types.  Differences from torch:
 float32, bfloat16 and float16 gradients on one ROCm GPU; p = 1, 2 or inf; a
 parameter listed twice counts, and is clipped, once; the norm of bfloat16
-gradients is not rounded to bfloat16.
+gradients is not rounded to bfloat16.  ``make_fx`` and ``torch.jit.trace``
+cannot record them (that raises); a HIP graph can capture them.
 
 DTensor gradients (FSDP2) are normed by their local shards, the sums joined by
 an all-reduce over the mesh dimensions that they are sharded over.
@@ -92,6 +93,17 @@ class _Batch:
         with torch.cuda.device(self.device):
             stream = torch.cuda.current_stream(self.device).cuda_stream
             L.check(getattr(lib, name)(ctypes.byref(args), stream), name)
+
+
+def _check_not_recorded() -> None:
+    """The calls below are no operators: a tracer would record the allocation of
+    their outputs and not the kernels that fill them."""
+    recorded = torch._C._get_tracing_state() is not None or (
+        torch._C._len_torch_dispatch_stack() > 0
+        and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None)
+    if recorded:
+        raise RuntimeError("luma_amd: the gradients' norm and clipping cannot be recorded by make_fx "
+                           "or torch.jit.trace (a HIP graph can capture them)")
 
 
 def _host():
@@ -275,6 +287,7 @@ def get_total_norm(tensors: _Tensors, norm_type: float = 2.0, error_if_nonfinite
     """The norm of all elements of all tensors together (``norm_type`` 1, 2 or
     inf), as a float32 scalar on their device.  ``foreach`` is accepted for
     torch's signature and selects nothing."""
+    _check_not_recorded()
     code = _norm_code(norm_type)
     tensors = _as_list(tensors)
     total = _quick_norm(tensors, False, code, 0.0)
@@ -306,6 +319,7 @@ def clip_grad_norm_(parameters: _Tensors, max_norm: float, norm_type: float = 2.
     them together, which is returned (a float32 scalar on their device).  A norm
     that is not finite scales by 0 or NaN, as in torch, unless
     ``error_if_nonfinite``, which waits for the norm and raises."""
+    _check_not_recorded()
     code = _norm_code(norm_type)
     max_norm = check_max_norm(max_norm)
     parameters = _as_list(parameters)
@@ -343,6 +357,7 @@ def clip_grads_with_norm_(parameters: _Tensors, max_norm: float, total_norm: tor
                           foreach: Optional[bool] = None) -> None:
     """The scaling of ``clip_grad_norm_`` by a norm that is known already (a
     one-element tensor, e.g. ``get_total_norm``'s)."""
+    _check_not_recorded()
     max_norm = check_max_norm(max_norm)
     parameters = _as_list(parameters)
     if not isinstance(total_norm, torch.Tensor) or total_norm.numel() != 1:

@@ -7,6 +7,7 @@ import torch
 from torch.fx.experimental.proxy_tensor import make_fx
 from torch.utils._python_dispatch import TorchDispatchMode
 
+import luma_amd
 from luma_amd import _lib as L
 from luma_amd import linear_cross_entropy
 
@@ -50,3 +51,25 @@ def test_loss_goes_to_the_operator(how, monkeypatch):
     with pytest.raises(RuntimeError, match="ROCm GPU"):
         WAYS[how](f, torch.ones(4, 8))
     assert calls == [1]
+
+
+def _clip(x):
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = x
+    return luma_amd.clip_grad_norm_([p], 1.0)
+
+
+def _scale(x):
+    p = torch.nn.Parameter(torch.ones(3))
+    p.grad = x
+    luma_amd.clip_grads_with_norm_([p], 1.0, torch.tensor(2.0))
+    return x
+
+
+@pytest.mark.parametrize("how", ["make_fx", "jit.trace"])
+@pytest.mark.parametrize("f", [lambda x: luma_amd.get_total_norm([x]), _clip, _scale],
+                         ids=["get_total_norm", "clip_grad_norm_", "clip_grads_with_norm_"])
+def test_norm_and_clipping_refuse_a_tracer(f, how):
+    """They are no operators: a graph of them would return memory that nothing fills."""
+    with pytest.raises(RuntimeError, match="cannot be recorded"):
+        WAYS[how](f, torch.ones(3))
