@@ -163,6 +163,11 @@ def _shard_dims(t) -> tuple:
     return tuple(dims)
 
 
+def _check_device(g) -> None:
+    if not g.is_cuda:
+        raise RuntimeError(f"luma_amd: gradients must be on a ROCm GPU; got device {g.device}")
+
+
 class _Slow:
     """Any gradients that torch knows: DTensors by their local shards, those
     that are not dense by a copy."""
@@ -181,9 +186,7 @@ class _Slow:
                 g = g._local_tensor
             if g.is_sparse or g.layout != torch.strided:
                 raise RuntimeError("luma_amd: sparse gradients are not supported")
-            if not g.is_cuda:
-                raise RuntimeError("luma_amd: gradients must be on a ROCm GPU; got device "
-                                   f"{g.device}")
+            _check_device(g)
             if g.dtype not in _GRAD_CODES:
                 raise ValueError(f"luma_amd: gradient dtype {g.dtype} is not "
                                  "float32/bfloat16/float16")

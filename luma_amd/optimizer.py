@@ -780,17 +780,25 @@ class LUMA(Optimizer):
         self._scaling_keep = keep
         return ptrs[0], ptrs[1]
 
-    def _clip(self, tt: np.ndarray, scaling: Tuple[int, int],
-              work=()) -> Tuple[int, int]:
-        """The step's scaling with max_grad_norm's clipping in it.  ``work``: the
-        step's parameters, unless they are known to be plain tensors."""
+    def _sharded_norm(self) -> Optional[torch.Tensor]:
+        """The norm of all gradients (as they are, not unscaled) where max_grad_norm
+        is set and some are shards of tensors that other GPUs hold parts of; else
+        None.  Empty shards count: the ranks that hold the rest wait for this
+        one in the same reductions, in the order of the parameters."""
+        if self._max_grad_norm is None:
+            return None
+        return sharded_norm([p.grad for group in self.param_groups for p in group["params"]
+                             if p.grad is not None])
+
+    def _clip(self, tt: Optional[np.ndarray], scaling: Tuple[int, int],
+              total: Optional[torch.Tensor] = None) -> Tuple[int, int]:
+        """The step's scaling with max_grad_norm's clipping in it.  ``total``:
+        _sharded_norm's; None: the norm is that of table tt's gradients."""
         if self._max_grad_norm is None:
             return scaling
-        total = sharded_norm([w[1].grad for w in work])
         if total is None:
             out = self._engine.clip_scale(tt, self._max_grad_norm, scaling[0])
         else:
-            # (shards of other GPUs count: their sums are joined first)
             scale = (self._scaling_keep[0] if scaling[0] else torch.ones_like(total)).reshape(())
             total = total / scale
             factor = (self._max_grad_norm / (total + 1e-6)).clamp(max=1.0)
@@ -983,7 +991,10 @@ class LUMA(Optimizer):
                 return loss
         self._plan = None
 
+        # (before anything in which this rank may differ from the others)
+        total = self._sharded_norm()
         work = []
+        empty_shards = False
         param_idx = 0
         for gi, group in enumerate(self.param_groups):
             for p in group["params"]:
@@ -993,6 +1004,7 @@ class LUMA(Optimizer):
                 param = self._unwrap_tensor(p)
                 grad = self._unwrap_tensor(p.grad)
                 if param.numel() == 0:
+                    empty_shards |= param is not p
                     continue
                 if grad.is_sparse:
                     raise RuntimeError("LUMA does not support sparse gradients")
@@ -1008,6 +1020,8 @@ class LUMA(Optimizer):
                     raise ValueError("LUMA requires dense (contiguous) parameters")
                 work.append((gi, p, param, grad, param_idx - 1))
         if not work:
+            if total is not None:
+                self._clip(None, self._scaling(total.device), total)
             self._noise = None
             return loss
 
@@ -1076,11 +1090,13 @@ class LUMA(Optimizer):
                          state["param_id"], code, gi, shard_offset(p), summ))
         tt = engine.table(rows)
         engine.launch(tt, self._group_table(), self._base_seed, noise_mode, self._flags,
-                      self._clip(tt, self._scaling(engine.device), work))
+                      self._clip(tt, self._scaling(engine.device), total))
         # host count of step() calls; the kernels use the slot's device count
         for state in states:
             state["step"] += 1
-        if noise_mode == L.NOISE_PHILOX and engine.host is not None and _Plan.usable(work, rows):
+        # (a planned step clips by the norm of its own table)
+        if (noise_mode == L.NOISE_PHILOX and engine.host is not None and not empty_shards
+                and _Plan.usable(work, rows)):
             self._plan = _Plan(self.param_groups, work, rows, states, tt, engine.host)
             self._plan.chunk_setting = engine.chunk_elems
         self._noise = None
