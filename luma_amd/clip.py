@@ -54,7 +54,8 @@ def check_max_norm(max_norm) -> float:
 
 # Up to this many rows travel as launch arguments, a launch for each 160; more
 # take a device table (a copy of 24 bytes per row, which a launch or two less
-# does not pay for).
+# does not pay for).  Under capture there is no table: the library takes up to
+# 40,960 rows without one and refuses more.
 NO_TABLE = 2 * L.GRADS_INLINE
 
 
@@ -122,7 +123,9 @@ def _quick(tensors, of_grad: bool, apart: bool) -> Optional[_Batch]:
     if module is None:
         return None
     host, n = None, len(tensors)
-    if n > NO_TABLE and torch.cuda.is_available():
+    # (under capture the rows go as launch arguments, and nothing may be pinned)
+    if (n > NO_TABLE and torch.cuda.is_available()
+            and not torch.cuda.is_current_stream_capturing()):
         host = torch.empty(n * L.GRAD_DTYPE.itemsize, dtype=torch.uint8, pin_memory=True)
         rows = host.numpy().view(L.GRAD_DTYPE)
     else:

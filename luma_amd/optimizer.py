@@ -356,7 +356,7 @@ class _Engine:
         else:
             rows = grad_rows(tt["grad"], tt["numel"], tt["grad_dtype"])
             table = None
-        # (as launch arguments a list of any length is captured)
+        # (a captured list goes as launch arguments, up to the library's 40,960 rows)
         if table is None and len(rows) > NO_TABLE and not capturing:
             table = self._upload(rows)
         self._norm = (tt, rows, table)
