@@ -306,6 +306,8 @@ def get_total_norm(tensors: _Tensors, norm_type: float = 2.0, error_if_nonfinite
 
 @torch.no_grad()
 def _total_norm(tensors, code: int) -> torch.Tensor:
+    if not tensors:
+        return torch.tensor(0.0)
     batch = _quick(tensors, False, False)
     if batch is None:
         return _Slow(tensors, False).norm(code)
