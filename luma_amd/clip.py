@@ -69,6 +69,10 @@ class _Batch:
         self.host = host
         self.hold = hold      # keeps tensors alive that only the rows point to
 
+    def zero(self) -> torch.Tensor:
+        """The norm where there is no row."""
+        return torch.zeros((), dtype=torch.float32, device=self.device)
+
     def args(self, norm: int, max_norm: float, total: Optional[torch.Tensor],
              power: Optional[torch.Tensor] = None) -> L.NormArgs:
         """The call's arguments, with a workspace (and, for a long list, a
@@ -133,7 +137,9 @@ def _quick(tensors, of_grad: bool, apart: bool) -> Optional[_Batch]:
     got = module.grad_rows(tensors, of_grad, apart, rows.ctypes.data)
     if got is None:
         return None
-    return _Batch(rows[:got[0]], torch.device("cuda", max(got[1], 0)), host)
+    # (no tensor at all has no device, and as in torch a norm on the host)
+    device = torch.device("cpu") if got[1] < 0 else torch.device("cuda", got[1])
+    return _Batch(rows[:got[0]], device, host)
 
 
 def grad_rows(data, numel, dtype) -> np.ndarray:
@@ -312,7 +318,7 @@ def _total_norm(tensors, code: int) -> torch.Tensor:
     if batch is None:
         return _Slow(tensors, False).norm(code)
     if not len(batch.rows):
-        return torch.tensor(0.0)
+        return batch.zero()
     total = torch.empty((), dtype=torch.float32, device=batch.device)
     batch.call("luma_grad_norm", batch.args(code, 0.0, total))
     return total
@@ -344,7 +350,7 @@ def _clip(parameters, max_norm: float, norm_type, code: int,
     batch = None if error_if_nonfinite else _quick(parameters, True, True)
     if batch is not None:
         if not len(batch.rows):
-            return torch.tensor(0.0)
+            return batch.zero()
         total = torch.empty((), dtype=torch.float32, device=batch.device)
         batch.call("luma_grad_clip", batch.args(code, max_norm, total))
         return total
