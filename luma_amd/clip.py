@@ -167,7 +167,8 @@ def _shard_dims(t) -> tuple:
         if place.is_partial():
             raise ValueError("luma_amd: the norm of a DTensor with a Partial placement needs its "
                              "sum: redistribute it first")
-        if place.is_shard():
+        # (what a tensor-parallel weight's shards are cut into does not call itself a shard)
+        if not place.is_replicate():
             dims.append(d)
     return tuple(dims)
 
