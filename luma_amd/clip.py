@@ -263,7 +263,11 @@ def _join_shards(power: torch.Tensor, code: int, mesh, dims) -> None:
     of the mesh's dimensions."""
     import torch.distributed as dist
 
-    op = dist.ReduceOp.MAX if code == L.NORM_INF else dist.ReduceOp.SUM
+    op = dist.ReduceOp.SUM
+    if code == L.NORM_INF:
+        # (by its bits, as the kernels keep it, NaN above infinity: a maximum of
+        # floats may lose a NaN, and not on every rank)
+        op, power = dist.ReduceOp.MAX, power.view(torch.int64)
     for d in dims:
         dist.all_reduce(power, op=op, group=mesh.get_group(d))
 
