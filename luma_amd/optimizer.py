@@ -787,8 +787,12 @@ class LUMA(Optimizer):
         one in the same reductions, in the order of the parameters."""
         if self._max_grad_norm is None:
             return None
-        return sharded_norm([p.grad for group in self.param_groups for p in group["params"]
-                             if p.grad is not None])
+        grads = [p.grad for group in self.param_groups for p in group["params"]
+                 if p.grad is not None]
+        if not any(hasattr(g, "_local_tensor") for g in grads):
+            return None
+        # (of other types as the float32 that the step takes them as)
+        return sharded_norm([g if g.dtype in _GRAD_CODES else g.float() for g in grads])
 
     def _clip(self, tt: Optional[np.ndarray], scaling: Tuple[int, int],
               total: Optional[torch.Tensor] = None) -> Tuple[int, int]:

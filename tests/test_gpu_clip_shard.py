@@ -89,3 +89,20 @@ def test_only_an_empty_shard(mesh, joined):
     opt.max_grad_norm = None
     opt.step()
     assert len(joined) == 3
+
+
+def test_gradients_that_the_step_promotes(mesh, joined):
+    """float64 gradients count as the float32 ones that the step takes them as."""
+    from torch.distributed.tensor import Shard, distribute_tensor
+
+    q = _plain(0)
+    p = torch.nn.Parameter(distribute_tensor(q.detach().clone(), mesh, [Shard(0)]))
+    p.grad_dtype = q.grad_dtype = None
+    g = q.grad.double()
+    p.grad, q.grad = distribute_tensor(g, mesh, [Shard(0)]), g
+    a, b = _opt([p], max_grad_norm=1.0), _opt([q], max_grad_norm=1.0)
+    for t in range(1, 3):
+        a.step()
+        b.step()
+        assert joined == [(0,)] * t and torch.equal(a.grad_norm, b.grad_norm)
+    assert torch.equal(p.detach().to_local(), q.detach())
