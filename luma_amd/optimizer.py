@@ -805,7 +805,8 @@ class LUMA(Optimizer):
         else:
             scale = (self._scaling_keep[0] if scaling[0] else torch.ones_like(total)).reshape(())
             total = total / scale
-            factor = (self._max_grad_norm / (total + 1e-6)).clamp(max=1.0)
+            # (a division of tensors, as the kernels': of a number torch takes the reciprocal)
+            factor = (torch.full_like(total, self._max_grad_norm) / (total + 1e-6)).clamp(max=1.0)
             out = torch.stack([total, scale / factor])
             self._scaling_keep.append(out)
         self.grad_norm = out[0]

@@ -106,3 +106,23 @@ def test_gradients_that_the_step_promotes(mesh, joined):
         b.step()
         assert joined == [(0,)] * t and torch.equal(a.grad_norm, b.grad_norm)
     assert torch.equal(p.detach().to_local(), q.detach())
+
+
+def test_sharded_factor_is_the_plain_one(mesh, joined):
+    """The factor of a joined norm is the same division as the kernel's, so that a
+    sharded parameter's step is the plain one's, bit for bit."""
+    from torch.distributed.tensor import Shard, distribute_tensor
+
+    q = _plain(0)
+    p = torch.nn.Parameter(distribute_tensor(q.detach().clone(), mesh, [Shard(0)]))
+    a, b = _opt([p]), _opt([q])
+    g = q.grad
+    for t in range(24):
+        q.grad = g * (1.0 + 0.37 * t)
+        p.grad = distribute_tensor(q.grad, mesh, [Shard(0)])
+        for opt in (a, b):
+            opt.max_grad_norm = 0.3 + 0.11 * t
+            opt.grad_scale = torch.tensor(3.0 + t, device="cuda")
+            opt.step()
+        assert torch.equal(a.grad_norm, b.grad_norm)
+        assert torch.equal(p.detach().to_local(), q.detach()), t
