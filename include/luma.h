@@ -375,8 +375,10 @@ int luma_hyper_rows(const LumaGroup *group, int64_t t0, int32_t n, float *out, v
  * clips with torch.nn.utils.clip_grad_norm_ between backward() and step()
  * (benchmarks/bench_nanogpt.py).  Sums are formed in float64 (a float32
  * gradient's square is exact there and cannot overflow or vanish) in an order
- * that only the rows' sizes determine, so that a result is reproduced bit for
- * bit.  A NaN anywhere makes the norm NaN.
+ * that the rows' sizes and the way they are passed (LumaNormArgs.table or not)
+ * determine: the same call gives the same bits every time, and the same rows
+ * passed the other way the same sum but for float64's rounding.  A NaN anywhere
+ * makes the norm NaN.
  */
 #define LUMA_NORM_L2 0
 #define LUMA_NORM_L1 1

@@ -475,8 +475,8 @@ bool grad_range(PyObject *const *objs, int64_t n, bool of_grad, GradRow *rows,
 
 // Records that the kernels will write to these tensors, as torch's in-place
 // operations do (what autograd has saved of them is then stale).  By the calling
-// thread: the counters are written, and eight threads that take the lines from
-// each other need 390 us for those of 20,000 tensors, one 200.
+// thread, an increment for each tensor: 20,000 views of one buffer, which share one
+// counter, take 200 us, by eight threads that take its line from each other 390.
 void bump_versions(const c10::TensorImpl *const *impls, int64_t n) {
   auto at = [&](int64_t i) { return const_cast<c10::TensorImpl *>(impls[i]); };
   uint32_t seen = 0;
