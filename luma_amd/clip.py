@@ -103,10 +103,10 @@ class _Batch:
 def _check_not_recorded() -> None:
     """The calls below are no operators: a tracer would record the allocation of
     their outputs and not the kernels that fill them."""
-    recorded = torch._C._get_tracing_state() is not None or (
-        torch._C._len_torch_dispatch_stack() > 0
-        and torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None)
-    if recorded:
+    proxy = torch._C._TorchDispatchModeKey.PROXY
+    if (torch._C._get_tracing_state() is not None
+            or torch._C._get_dispatch_mode(proxy) is not None
+            or torch._ops._get_dispatch_mode_pre_dispatch(proxy) is not None):
         raise RuntimeError("luma_amd: the gradients' norm and clipping cannot be recorded by make_fx "
                            "or torch.jit.trace (a HIP graph can capture them)")
 

@@ -18,6 +18,7 @@
 #include <ATen/ATen.h>
 #include <ATen/core/dispatch/Dispatcher.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <pybind11/numpy.h>
 #include <pybind11/pybind11.h>
@@ -719,7 +720,8 @@ struct Xent : torch::autograd::Function<Xent> {
       const int64_t reduction = ctx->saved_data["reduction"].toInt();
       {
         at::AutoDispatchBelowADInplaceOrView below;
-        if (c10::impl::dispatch_mode_enabled()) {
+        if (c10::impl::dispatch_mode_enabled() ||
+            c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch)) {
           // (a tracer or another mode, begun since the forward, watches the operators
           // called: it is given one, which holds the kernels)
           std::tie(d_hidden, d_weight) =

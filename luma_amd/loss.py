@@ -170,6 +170,7 @@ def _plain(*tensors) -> bool:
     the module's outputs, and not the kernels that fill them), and no tensor is
     of a subclass with a dispatch of its own, or one of torch.func's."""
     return (torch._C._len_torch_dispatch_stack() == 0
+            and torch._ops._len_torch_dispatch_stack_pre_dispatch() == 0
             and torch._C._get_tracing_state() is None
             and not torch._C._are_functorch_transforms_active()
             and all(type(t) is torch.Tensor or type(t) is torch.nn.Parameter for t in tensors))

@@ -39,6 +39,24 @@ def test_make_fx(reduction):
         assert all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("reduction", ["mean", "none"])
+def test_make_fx_before_dispatch(reduction):
+    """The graph is one of operators that autograd has yet to see.  (Gradients taken
+    inside such a graph use what the recorded forward saved, of any operator.)"""
+    def f(x, w, t):
+        return linear_cross_entropy(x, w, t, -100, reduction)
+
+    graph = make_fx(f, pre_dispatch=True)(*_inputs(0))
+    assert FORWARD in [node.target for node in graph.graph.nodes]
+    for seed in (1, 2):
+        inputs = _inputs(seed)
+        got, want = graph(*inputs), f(*inputs)
+        assert torch.equal(got, want)
+        for p, q in zip(torch.autograd.grad(got.sum(), inputs[:2]),
+                        torch.autograd.grad(want.sum(), inputs[:2])):
+            assert torch.equal(p, q)
+
+
 @pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
 @pytest.mark.parametrize("reduction", ["mean", "none"])
 def test_jit_trace(reduction):
@@ -74,8 +92,9 @@ def test_dispatch_modes_see_both_directions():
     assert torch.equal(loss, want_loss) and all(torch.equal(p, q) for p, q in zip(got, want))
 
 
+@pytest.mark.parametrize("pre_dispatch", [False, True])
 @pytest.mark.parametrize("only", ["both", "hidden", "weight"])
-def test_make_fx_of_the_backward_alone(only):
+def test_make_fx_of_the_backward_alone(only, pre_dispatch):
     """The forward ran before the tracer began."""
     x, w, t = _inputs(4)
     loss = linear_cross_entropy(x, w, t, -100, "none")
@@ -84,7 +103,7 @@ def test_make_fx_of_the_backward_alone(only):
     def f(g):
         return torch.autograd.grad(loss, wanted, g, retain_graph=True)
 
-    graph = make_fx(f)(torch.ones_like(loss))
+    graph = make_fx(f, pre_dispatch=pre_dispatch)(torch.ones_like(loss))
     assert BACKWARD in [node.target for node in graph.graph.nodes]
     for seed in (5, 6):
         gen = torch.Generator(device="cuda").manual_seed(seed)

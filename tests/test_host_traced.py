@@ -25,6 +25,7 @@ def _in_mode(f, x):
 
 
 WAYS = {"make_fx": lambda f, x: make_fx(f)(x),
+        "make_fx before dispatch": lambda f, x: make_fx(f, pre_dispatch=True)(x),
         "jit.trace": lambda f, x: torch.jit.trace(f, x, check_trace=False),
         "dispatch mode": _in_mode}
 
@@ -66,7 +67,7 @@ def _scale(x):
     return x
 
 
-@pytest.mark.parametrize("how", ["make_fx", "jit.trace"])
+@pytest.mark.parametrize("how", ["make_fx", "make_fx before dispatch", "jit.trace"])
 @pytest.mark.parametrize("f", [lambda x: luma_amd.get_total_norm([x]), _clip, _scale],
                          ids=["get_total_norm", "clip_grad_norm_", "clip_grads_with_norm_"])
 def test_norm_and_clipping_refuse_a_tracer(f, how):
