@@ -65,7 +65,7 @@
 extern "C" {
 #endif
 
-#define LUMA_ABI_VERSION 11
+#define LUMA_ABI_VERSION 12
 
 /*
  * Elements per chunk-table entry (one workgroup's share of a tensor): the
@@ -482,6 +482,135 @@ typedef struct LumaXentArgs {
 int64_t luma_xent_workspace_bytes(const LumaXentArgs *args, int32_t backward);
 int luma_xent_forward(const LumaXentArgs *args, void *stream);
 int luma_xent_backward(const LumaXentArgs *args, void *stream);
+
+/*
+ * Dropout whose mask is drawn from a counter-based generator and never stored.
+ *
+ * Element e of an operand (its index, rows one after the other) has 32 bits
+ * u(e): the high 16 are half e % 8 (of the words x, y, z, w from the low end) of
+ * the Philox4x32-10 block with counter (lo32(e / 8), hi32(e / 8), 0, call) and
+ * the seed as key, the low 16 that half of the block with counter word 1 in
+ * place of 0.  It is dropped (0, whatever it holds) where u(e) <
+ * floor(p 2^32 + 1/2) and scaled by 1 / (1 - p) where not.  The backward draws
+ * the same bits again.
+ */
+typedef struct LumaDropout {
+  const int64_t *seed_at; /* device: the seed, read by the kernels; or NULL        */
+  uint64_t seed;          /* the seed where seed_at is NULL                        */
+  double p;               /* in [0, 1]; 0: nothing is drawn                        */
+  uint32_t call;          /* tells the calls that share a seed from each other     */
+  uint32_t reserved;      /* 0                                                     */
+} LumaDropout;
+
+/* y = residual + dropout(x), or dropout(x) without a residual; dense. */
+typedef struct LumaDropoutArgs {
+  const void *x;          /* device [numel], type `in`                             */
+  const void *residual;   /* device [numel], type `out`, or NULL                   */
+  void *y;                /* device [numel], type `out`                            */
+  int64_t numel;          /* >= 1                                                  */
+  int32_t in, out;        /* LUMA_GRAD_*: the same, or one of them float32         */
+  LumaDropout drop;
+} LumaDropoutArgs;
+
+/* (the backward is the same call on y's gradient, without a residual) */
+int luma_dropout(const LumaDropoutArgs *args, void *stream);
+
+/*
+ * Layer normalisation over rows of h elements, alone or of the sum that a
+ * block's border forms:
+ *   s = x, or s = total = round(residual + dropout(x)) where residual is given;
+ *   m = mean(s), r = 1 / sqrt(mean((s - m)^2) + eps), z = (s - m) r,
+ *   y = z weight + bias
+ * and for y's and total's gradients d_y, d_total, with g = d_y weight:
+ *   d_s = r (g - mean(g) - z mean(g z)) + d_total,
+ *   d_x = d_s, or d_residual = d_s and d_x = dropout's gradient of d_s,
+ *   d_weight = sum over the rows of d_y z, d_bias = that of d_y.
+ * Everything is formed in float32 and rounded once.  The sum's rounding to the
+ * stream's type comes before its norm, so that y is the norm of the sum that a
+ * program goes on with, and the backward, which reads that, has the same z.
+ */
+typedef struct LumaLayerNormArgs {
+  const void *x;          /* device [n][h], rows ld_x elements apart; of the stream's
+                             type, with a residual of the branch's                 */
+  const void *residual;   /* device [n][h], rows ld_residual apart, or NULL        */
+  const void *weight;     /* device [h] or NULL (1)                                */
+  const void *bias;       /* device [h] or NULL (0)                                */
+  int64_t n, h;           /* each >= 1                                             */
+  int64_t ld_x, ld_residual;
+  int32_t stream;         /* LUMA_GRAD_*: of the residual and total                */
+  int32_t branch;         /* LUMA_GRAD_*: of y; the stream's, or the stream is float32 */
+  int32_t param;          /* LUMA_GRAD_*: of weight and bias: float32 or the branch's */
+  int32_t reserved;       /* 0                                                     */
+  double eps;
+  LumaDropout drop;       /* of x, with a residual                                 */
+  void *y;                /* forward: device [n][h] dense                          */
+  void *total;            /* device [n][h] dense, with a residual: the forward writes
+                             it, the backward reads it (and not x or residual)     */
+  float *stats;           /* device [2 n]: each row's m, then each one's r; the
+                             forward writes it (or NULL), the backward reads it    */
+  const void *d_y;        /* backward: device [n][h] dense, the branch's type      */
+  const void *d_total;    /* backward: device [n][h] dense, the stream's, or NULL  */
+  void *d_x;              /* backward: device [n][h] dense, x's type, or NULL      */
+  void *d_residual;       /* backward: device [n][h] dense, the stream's, or NULL  */
+  void *d_weight;         /* backward: device [h], or NULL                         */
+  void *d_bias;           /* backward: device [h], or NULL                         */
+  void *workspace;        /* backward: device, 16-byte aligned                     */
+  int64_t workspace_bytes;
+} LumaLayerNormArgs;
+
+/* Bytes of workspace that the backward needs (from n and h); < 0: refused. */
+int64_t luma_layer_norm_workspace_bytes(const LumaLayerNormArgs *args);
+int luma_layer_norm_forward(const LumaLayerNormArgs *args, void *stream);
+int luma_layer_norm_backward(const LumaLayerNormArgs *args, void *stream);
+
+/*
+ * The clipped policy loss of sampled tokens, with a KL term.
+ *
+ * For a token's log-probability l under the policy that learns, l_old under the
+ * one that drew it, l_ref under a reference, and its advantage A:
+ *   r = exp(l - l_old),  value = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
+ *   q = l_ref - l,       value += kl_weight (exp(q) - 1 - q)
+ * and d value / d l = -r A where r A is the smaller (or both are the same),
+ * else 0, plus kl_weight (1 - exp(q)).  Which side of a limit r lies on is
+ * decided on l - l_old in float64; values are float32, sums float64.  A token
+ * whose mask is 0 has value and gradient 0, and counts nowhere; nothing is
+ * formed of what its operands hold.
+ */
+#define LUMA_POLICY_SEQUENCE 3 /* the mean over the sequences that have tokens of each
+                                  one's mean; LUMA_XENT_NONE, _SUM and _MEAN (over
+                                  the tokens) are the others                       */
+/* Floats at `stats`. */
+#define LUMA_POLICY_STATS 4
+
+typedef struct LumaPolicyArgs {
+  const void *logp;       /* device [rows][length], rows ld_logp elements apart    */
+  const void *old_logp;
+  const void *ref_logp;   /* or NULL: no KL term                                   */
+  const float *advantage; /* device [rows], or [rows][length] (advantage_each)     */
+  const uint8_t *mask;    /* device [rows][length], 0 or 1, or NULL: every token   */
+  int64_t rows, length;   /* each >= 1; rows of more than 1,024: up to 2^22 of them */
+  int64_t ld_logp, ld_old, ld_ref, ld_advantage, ld_mask;
+  int32_t advantage_each; /* 1: an advantage for each token                        */
+  int32_t dtype;          /* LUMA_GRAD_*: the log-probabilities and d_logp         */
+  int32_t reduction;
+  int32_t reserved;       /* 0                                                     */
+  double clip_low, clip_high, kl_weight;
+  float *loss;            /* forward: device [rows][length] dense, or [1]          */
+  float *stats;           /* forward: device [LUMA_POLICY_STATS]: the share of the
+                             tokens whose ratio was clipped, the means of exp(q) - 1
+                             - q and of r - 1 - log r, the number of tokens        */
+  float *share;           /* device [rows + 1]: each row's and the whole's factor of a
+                             mean; the forward writes it, the backward reads it    */
+  const float *grad_loss; /* backward: device [rows][length] dense, or [1]         */
+  void *d_logp;           /* backward: device [rows][length] dense                 */
+  void *workspace;        /* forward: device, 16-byte aligned                      */
+  int64_t workspace_bytes;
+} LumaPolicyArgs;
+
+/* Bytes of workspace that the forward needs (from the sizes); < 0: refused. */
+int64_t luma_policy_workspace_bytes(const LumaPolicyArgs *args);
+int luma_policy_forward(const LumaPolicyArgs *args, void *stream);
+int luma_policy_backward(const LumaPolicyArgs *args, void *stream);
 
 /* Host: one Philox4x32-10 block. */
 void luma_philox4x32(const uint32_t ctr[4], const uint32_t key[2], uint32_t out[4]);

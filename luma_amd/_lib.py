@@ -25,7 +25,7 @@ STEP_TENSOR_CHUNK_MIN = 16384  # LUMA_STEP_TENSOR_CHUNK_MIN
 SLOT_BYTES = 512             # LUMA_SLOT_BYTES
 NOALLOC_MAX_CHUNKS = 262144  # LUMA_NOALLOC_MAX_CHUNKS
 SUMMARY_WORDS = 256          # LUMA_SUMMARY_WORDS (per chunk)
-ABI_VERSION = 11             # LUMA_ABI_VERSION
+ABI_VERSION = 12             # LUMA_ABI_VERSION
 GRAD_TILE = 2048             # LUMA_GRAD_TILE
 GRADS_INLINE = 160           # LUMA_GRADS_INLINE
 NORM_PARTIALS = 1024         # LUMA_NORM_PARTIALS
@@ -33,6 +33,8 @@ NORM_PARTIALS = 1024         # LUMA_NORM_PARTIALS
 GRAD_F32, GRAD_BF16, GRAD_F16 = 0, 1, 2
 NORM_L2, NORM_L1, NORM_INF = 0, 1, 2
 XENT_NONE, XENT_SUM, XENT_MEAN = 0, 1, 2
+POLICY_SEQUENCE = 3          # LUMA_POLICY_SEQUENCE
+POLICY_STATS = 4             # LUMA_POLICY_STATS
 NOISE_PHILOX, NOISE_INJECTED = 0, 1
 FLAG_EXACT_ONLY = 1
 FLAG_SPLIT = 2               # LUMA_FLAG_SPLIT
@@ -124,6 +126,93 @@ class XentArgs(ctypes.Structure):
     ]
 
 
+class Dropout(ctypes.Structure):
+    """LumaDropout."""
+    _fields_ = [
+        ("seed_at", ctypes.c_void_p),
+        ("seed", ctypes.c_uint64),
+        ("p", ctypes.c_double),
+        ("call", ctypes.c_uint32),
+        ("reserved", ctypes.c_uint32),
+    ]
+
+
+class DropoutArgs(ctypes.Structure):
+    """LumaDropoutArgs."""
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("y", ctypes.c_void_p),
+        ("numel", ctypes.c_int64),
+        ("in_type", ctypes.c_int32),
+        ("out_type", ctypes.c_int32),
+        ("drop", Dropout),
+    ]
+
+
+class LayerNormArgs(ctypes.Structure):
+    """LumaLayerNormArgs."""
+    _fields_ = [
+        ("x", ctypes.c_void_p),
+        ("residual", ctypes.c_void_p),
+        ("weight", ctypes.c_void_p),
+        ("bias", ctypes.c_void_p),
+        ("n", ctypes.c_int64),
+        ("h", ctypes.c_int64),
+        ("ld_x", ctypes.c_int64),
+        ("ld_residual", ctypes.c_int64),
+        ("stream", ctypes.c_int32),
+        ("branch", ctypes.c_int32),
+        ("param", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("eps", ctypes.c_double),
+        ("drop", Dropout),
+        ("y", ctypes.c_void_p),
+        ("total", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("d_y", ctypes.c_void_p),
+        ("d_total", ctypes.c_void_p),
+        ("d_x", ctypes.c_void_p),
+        ("d_residual", ctypes.c_void_p),
+        ("d_weight", ctypes.c_void_p),
+        ("d_bias", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
+class PolicyArgs(ctypes.Structure):
+    """LumaPolicyArgs."""
+    _fields_ = [
+        ("logp", ctypes.c_void_p),
+        ("old_logp", ctypes.c_void_p),
+        ("ref_logp", ctypes.c_void_p),
+        ("advantage", ctypes.c_void_p),
+        ("mask", ctypes.c_void_p),
+        ("rows", ctypes.c_int64),
+        ("length", ctypes.c_int64),
+        ("ld_logp", ctypes.c_int64),
+        ("ld_old", ctypes.c_int64),
+        ("ld_ref", ctypes.c_int64),
+        ("ld_advantage", ctypes.c_int64),
+        ("ld_mask", ctypes.c_int64),
+        ("advantage_each", ctypes.c_int32),
+        ("dtype", ctypes.c_int32),
+        ("reduction", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+        ("clip_low", ctypes.c_double),
+        ("clip_high", ctypes.c_double),
+        ("kl_weight", ctypes.c_double),
+        ("loss", ctypes.c_void_p),
+        ("stats", ctypes.c_void_p),
+        ("share", ctypes.c_void_p),
+        ("grad_loss", ctypes.c_void_p),
+        ("d_logp", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_int64),
+    ]
+
+
 class LumaLibraryError(RuntimeError):
     pass
 
@@ -159,6 +248,13 @@ _SIGNATURES = {
     "luma_xent_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(XentArgs), ctypes.c_int32]),
     "luma_xent_forward": (ctypes.c_int, [ctypes.POINTER(XentArgs), _VP]),
     "luma_xent_backward": (ctypes.c_int, [ctypes.POINTER(XentArgs), _VP]),
+    "luma_dropout": (ctypes.c_int, [ctypes.POINTER(DropoutArgs), _VP]),
+    "luma_layer_norm_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(LayerNormArgs)]),
+    "luma_layer_norm_forward": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), _VP]),
+    "luma_layer_norm_backward": (ctypes.c_int, [ctypes.POINTER(LayerNormArgs), _VP]),
+    "luma_policy_workspace_bytes": (ctypes.c_int64, [ctypes.POINTER(PolicyArgs)]),
+    "luma_policy_forward": (ctypes.c_int, [ctypes.POINTER(PolicyArgs), _VP]),
+    "luma_policy_backward": (ctypes.c_int, [ctypes.POINTER(PolicyArgs), _VP]),
     "luma_philox4x32": (None, [ctypes.POINTER(ctypes.c_uint32), ctypes.POINTER(ctypes.c_uint32),
                                ctypes.POINTER(ctypes.c_uint32)]),
 }
@@ -216,16 +312,23 @@ def load_host():
 @functools.lru_cache(maxsize=1)
 def host_calls():
     """The host module with the library's entry points bound (the eager paths
-    of the norm, clipping and linear_cross_entropy); None without it."""
+    of the operators beside the step); None without it."""
     import torch
 
     host = load_host()
     if host is not None:
         lib = load()
-        host.bind(*(ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in (
-            "luma_xent_workspace_bytes", "luma_xent_forward", "luma_xent_backward",
-            "luma_grad_norm", "luma_grad_clip", "luma_last_error")),
-            torch._C._cuda_getCurrentRawStream)
+
+        def at(*names):
+            return [ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in names]
+
+        host.bind(*at("luma_xent_workspace_bytes", "luma_xent_forward", "luma_xent_backward",
+                      "luma_grad_norm", "luma_grad_clip", "luma_last_error"),
+                  torch._C._cuda_getCurrentRawStream)
+        host.bind_more(at("luma_dropout", "luma_layer_norm_workspace_bytes",
+                          "luma_layer_norm_forward", "luma_layer_norm_backward",
+                          "luma_policy_workspace_bytes", "luma_policy_forward",
+                          "luma_policy_backward"))
     return host
 
 

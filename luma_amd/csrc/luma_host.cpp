@@ -35,6 +35,8 @@
 #include <cstring>
 #include <functional>
 #include <mutex>
+#include <optional>
+#include <string>
 #include <thread>
 #include <vector>
 
@@ -773,9 +775,513 @@ py::object xent(const at::Tensor &hidden, const at::Tensor &weight, const at::Te
   return py::cast(reduction == LUMA_XENT_NONE ? loss.view(target.sizes()) : loss);
 }
 
+// -- the residual stream's operators and the policy loss ---------------------------
+
+// The gradients' entry points and the operators that hold them for a tracer.
+struct More {
+  int (*dropout)(const LumaDropoutArgs *, void *) = nullptr;
+  int64_t (*norm_workspace)(const LumaLayerNormArgs *) = nullptr;
+  int (*norm_forward)(const LumaLayerNormArgs *, void *) = nullptr;
+  int (*norm_backward)(const LumaLayerNormArgs *, void *) = nullptr;
+  int64_t (*policy_workspace)(const LumaPolicyArgs *) = nullptr;
+  int (*policy_forward)(const LumaPolicyArgs *, void *) = nullptr;
+  int (*policy_backward)(const LumaPolicyArgs *, void *) = nullptr;
+} g_more;
+
+void bind_more(const std::vector<uintptr_t> &at) {
+  TORCH_CHECK(at.size() == 7, "bind_more: seven entry points");
+  g_more = {reinterpret_cast<int (*)(const LumaDropoutArgs *, void *)>(at[0]),
+            reinterpret_cast<int64_t (*)(const LumaLayerNormArgs *)>(at[1]),
+            reinterpret_cast<int (*)(const LumaLayerNormArgs *, void *)>(at[2]),
+            reinterpret_cast<int (*)(const LumaLayerNormArgs *, void *)>(at[3]),
+            reinterpret_cast<int64_t (*)(const LumaPolicyArgs *)>(at[4]),
+            reinterpret_cast<int (*)(const LumaPolicyArgs *, void *)>(at[5]),
+            reinterpret_cast<int (*)(const LumaPolicyArgs *, void *)>(at[6])};
+}
+
+typedef std::optional<at::Tensor> MaybeTensor;
+typedef torch::autograd::AutogradContext Context;
+typedef torch::autograd::variable_list Variables;
+
+const at::ScalarType kTypes[] = {at::kFloat, at::kBFloat16, at::kHalf};   // by LUMA_GRAD_*
+
+bool given(const MaybeTensor &t) { return t.has_value() && t->defined(); }
+
+at::Tensor value(const MaybeTensor &t) { return given(t) ? *t : at::Tensor(); }
+
+MaybeTensor maybe(const at::Tensor &t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
+
+// Whether a tracer or another mode watches the operators that are called.
+bool watched() {
+  return c10::impl::dispatch_mode_enabled() ||
+         c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::PreDispatch);
+}
+
+// t with memory that holds its values.
+at::Tensor resolved(const at::Tensor &t) {
+  if (t._is_zerotensor()) return at::zeros(t.sizes(), t.options());
+  return t.is_neg() ? t.resolve_neg() : t;
+}
+
+at::Tensor dense(const at::Tensor &t) { return resolved(t).contiguous(); }
+
+// t (or a copy) as rows of its last dimension, elements of a row next to each other.
+at::Tensor as_rows(const at::Tensor &t) {
+  const int64_t h = t.size(t.dim() - 1);
+  at::Tensor r = resolved(t);
+  if (r.dim() != 2) r = r.reshape({-1, h});
+  return h > 1 && r.stride(1) != 1 ? r.contiguous() : r;
+}
+
+int64_t ld_of(const at::Tensor &rows) {
+  return rows.size(0) > 1 ? rows.stride(0) : rows.size(1);
+}
+
+void run(int rc) { TORCH_CHECK(rc == 0, g_lib.error()); }
+
+// A gradient under create_graph=True: depends on what it was formed of, and says so
+// when it is differentiated.
+struct Once : torch::autograd::Function<Once> {
+  static at::Tensor forward(Context *ctx, const at::Tensor &grad, std::string name,
+                            const MaybeTensor &, const MaybeTensor &, const MaybeTensor &,
+                            const MaybeTensor &) {
+    ctx->saved_data["name"] = name;
+    return grad.detach();
+  }
+  static Variables backward(Context *ctx, Variables) {
+    TORCH_CHECK(false, ctx->saved_data["name"].toStringRef(),
+                ": its gradients cannot be differentiated again");
+  }
+};
+
+void once(std::initializer_list<at::Tensor *> grads, const char *name, const at::Tensor &a,
+          const at::Tensor &b = {}, const at::Tensor &c = {}, const at::Tensor &d = {}) {
+  if (!at::GradMode::is_enabled()) return;
+  for (at::Tensor *g : grads)
+    if (g->defined())
+      *g = Once::apply(*g, std::string(name), maybe(a), maybe(b), maybe(c), maybe(d));
+}
+
+// What a call of dropout is drawn from.
+struct Draws {
+  at::Tensor seed_at;
+  double p;
+  int64_t seed, call;
+
+  LumaDropout args() const {
+    LumaDropout d{};
+    d.seed_at = seed_at.defined() ? seed_at.const_data_ptr<int64_t>() : nullptr;
+    d.seed = (uint64_t)seed;
+    d.p = p;
+    d.call = (uint32_t)call;
+    return d;
+  }
+};
+
+void dropout_call(const at::Tensor &x, const at::Tensor &residual, const at::Tensor &y,
+                  const Draws &d) {
+  LumaDropoutArgs a{};
+  a.x = x.const_data_ptr();
+  a.residual = residual.defined() ? residual.const_data_ptr() : nullptr;
+  a.y = y.mutable_data_ptr();
+  a.numel = x.numel();
+  a.in = grad_code(x.scalar_type());
+  a.out = grad_code(y.scalar_type());
+  a.drop = d.args();
+  const c10::DeviceGuard guard(x.device());
+  run(g_more.dropout(&a, current_stream(x.device().index())));
+}
+
+// An operator of the package, by its name.
+template <typename F>
+auto op_of(const char *name) {
+  return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
+}
+
+struct Dropout : torch::autograd::Function<Dropout> {
+  static at::Tensor forward(Context *ctx, const at::Tensor &x, const MaybeTensor &residual,
+                            const MaybeTensor &seed_at, double p, int64_t seed, int64_t call) {
+    const Draws d{value(seed_at), p, seed, call};
+    const at::Tensor like = given(residual) ? *residual : x;
+    at::Tensor y = at::empty(x.sizes(), like.options());
+    dropout_call(dense(x), given(residual) ? dense(*residual) : at::Tensor(), y, d);
+    ctx->save_for_backward({d.seed_at});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["call"] = call;
+    ctx->saved_data["code"] = (int64_t)grad_code(x.scalar_type());
+    ctx->saved_data["residual"] = given(residual);
+    ctx->set_materialize_grads(false);
+    return y;
+  }
+
+  static Variables backward(Context *ctx, Variables grads) {
+    const bool residual = ctx->saved_data["residual"].toBool();
+    at::Tensor d_x, d_residual;
+    if (grads[0].defined()) {
+      if (residual && ctx->needs_input_grad(1)) d_residual = grads[0];
+      if (ctx->needs_input_grad(0)) {
+        at::AutoDispatchBelowADInplaceOrView below;
+        const Draws d{ctx->get_saved_variables()[0], ctx->saved_data["p"].toDouble(),
+                      ctx->saved_data["seed"].toInt(), ctx->saved_data["call"].toInt()};
+        const int64_t code = ctx->saved_data["code"].toInt();
+        if (watched()) {
+          static const auto op =
+              op_of<at::Tensor(const at::Tensor &, const MaybeTensor &, double, int64_t, int64_t,
+                               int64_t)>("luma_amd::dropout_backward");
+          d_x = op.call(grads[0], maybe(d.seed_at), d.p, d.seed, d.call, code);
+        } else {
+          d_x = at::empty(grads[0].sizes(), grads[0].options().dtype(kTypes[code]));
+          dropout_call(dense(grads[0]), at::Tensor(), d_x, d);
+        }
+      }
+      once({&d_x}, "dropout", grads[0]);
+    }
+    return {d_x, d_residual, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+bool same_place(const at::Tensor &t, const at::Tensor &like) {
+  return t.layout() == at::kStrided && t.device() == like.device();
+}
+
+bool fit_draws(const at::Tensor &x, const MaybeTensor &seed_at, double p, int64_t call) {
+  return p >= 0.0 && p <= 1.0 && call >= 0 && call <= (int64_t)UINT32_MAX &&
+         (!given(seed_at) || (same_place(*seed_at, x) && seed_at->scalar_type() == at::kLong &&
+                              seed_at->numel() == 1));
+}
+
+// dropout of plain tensors; None where its arguments do not fit (the caller then
+// says which) and for no elements.
+py::object dropout(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &seed_at,
+                   double p, int64_t seed, int64_t call) {
+  if (!g_more.dropout || !x.is_cuda() || x.layout() != at::kStrided || x.numel() == 0 ||
+      grad_code(x.scalar_type()) < 0 || !fit_draws(x, seed_at, p, call))
+    return py::none();
+  if (given(residual) && (!same_place(*residual, x) || residual->sizes() != x.sizes() ||
+                          (residual->scalar_type() != x.scalar_type() &&
+                           residual->scalar_type() != at::kFloat)))
+    return py::none();
+  return py::cast(Dropout::apply(x, residual, seed_at, p, seed, call));
+}
+
+// The sizes, types and draws of a call of layer_norm or add_layer_norm.
+LumaLayerNormArgs norm_args(int64_t n, int64_t h, int64_t stream, int64_t branch, int64_t param,
+                            double eps, const Draws &d) {
+  LumaLayerNormArgs a{};
+  a.n = n;
+  a.h = h;
+  a.stream = (int32_t)stream;
+  a.branch = (int32_t)branch;
+  a.param = (int32_t)param;
+  a.eps = eps;
+  a.drop = d.args();
+  return a;
+}
+
+struct LayerNorm : torch::autograd::Function<LayerNorm> {
+  // y, or y and the sum.
+  static Variables forward(Context *ctx, const at::Tensor &x, const MaybeTensor &residual,
+                           const MaybeTensor &weight, const MaybeTensor &bias,
+                           const MaybeTensor &seed_at, double eps, double p, int64_t seed,
+                           int64_t call, int64_t branch, bool keep) {
+    const bool adds = given(residual);
+    const Draws d{value(seed_at), p, seed, call};
+    const at::Tensor &like = adds ? *residual : x;
+    const int64_t h = x.size(x.dim() - 1), n = x.numel() / h;
+    const int64_t stream = grad_code(like.scalar_type());
+    const int64_t param = given(weight) ? grad_code(weight->scalar_type())
+                          : given(bias) ? grad_code(bias->scalar_type())
+                                        : LUMA_GRAD_F32;
+    LumaLayerNormArgs a = norm_args(n, h, stream, branch, param, eps, d);
+    const at::Tensor xs = as_rows(x), rs = adds ? as_rows(*residual) : at::Tensor();
+    const at::Tensor w = given(weight) ? dense(*weight) : at::Tensor();
+    const at::Tensor b = given(bias) ? dense(*bias) : at::Tensor();
+    at::Tensor y = at::empty(x.sizes(), x.options().dtype(kTypes[branch]));
+    at::Tensor total, stats;
+    a.x = xs.const_data_ptr();
+    a.ld_x = ld_of(xs);
+    if (adds) {
+      total = at::empty(x.sizes(), like.options());
+      a.residual = rs.const_data_ptr();
+      a.ld_residual = ld_of(rs);
+      a.total = total.mutable_data_ptr();
+    }
+    a.weight = w.defined() ? w.const_data_ptr() : nullptr;
+    a.bias = b.defined() ? b.const_data_ptr() : nullptr;
+    a.y = y.mutable_data_ptr();
+    if (keep) {
+      stats = at::empty({2 * n}, x.options().dtype(at::kFloat));
+      a.stats = stats.mutable_data_ptr<float>();
+    }
+    {
+      const c10::DeviceGuard guard(x.device());
+      run(g_more.norm_forward(&a, current_stream(x.device().index())));
+    }
+    if (keep) {
+      ctx->save_for_backward({adds ? total : x, value(weight), stats, d.seed_at});
+      ctx->saved_data["p"] = p;
+      ctx->saved_data["seed"] = seed;
+      ctx->saved_data["call"] = call;
+      ctx->saved_data["branch"] = branch;
+      ctx->saved_data["param"] = param;
+      // (which inputs there are: a gradient's number counts those alone)
+      ctx->saved_data["inputs"] = (int64_t)(1 | adds << 1 | given(weight) << 2 | given(bias) << 3);
+    }
+    ctx->set_materialize_grads(false);
+    return adds ? Variables{y, total} : Variables{y};
+  }
+
+  static Variables backward(Context *ctx, Variables grads) {
+    const auto saved = ctx->get_saved_variables();
+    const at::Tensor &s = saved[0], &weight = saved[1], &stats = saved[2];
+    const Draws d{saved[3], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
+                  ctx->saved_data["call"].toInt()};
+    const int64_t branch = ctx->saved_data["branch"].toInt();
+    const int64_t param = ctx->saved_data["param"].toInt();
+    const int64_t inputs = ctx->saved_data["inputs"].toInt();
+    const bool adds = inputs >> 1 & 1;
+    bool want[4];
+    for (int i = 0, edge = 0; i < 4; ++i)
+      want[i] = (inputs >> i & 1) && ctx->needs_input_grad(edge++);
+    at::Tensor out[4];      // of x, residual, weight, bias
+    at::Tensor d_y = grads[0], d_total = adds ? grads[1] : at::Tensor();
+    if (d_y.defined() || d_total.defined()) {
+      at::AutoDispatchBelowADInplaceOrView below;
+      const int64_t stream = grad_code(s.scalar_type());
+      if (!d_y.defined()) d_y = at::zeros(s.sizes(), s.options().dtype(kTypes[branch]));
+      // (without draws the sum's gradient is that of both)
+      const bool one = adds && d.p == 0.0 && stream == branch;
+      const bool want_x = want[0] && !one, want_r = want[1] || (one && want[0]);
+      if (watched()) {
+        static const auto op =
+            op_of<std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor>(
+                const at::Tensor &, const MaybeTensor &, const at::Tensor &, const MaybeTensor &,
+                const at::Tensor &, const MaybeTensor &, double, int64_t, int64_t, int64_t, int64_t,
+                bool, bool, bool, bool, bool)>("luma_amd::layer_norm_backward");
+        std::tie(out[0], out[1], out[2], out[3]) =
+            op.call(d_y, maybe(d_total), s, maybe(weight), stats, maybe(d.seed_at), d.p, d.seed,
+                    d.call, branch, param, adds, want_x, want_r, want[2], want[3]);
+        const bool keep[4] = {want_x, want_r, want[2], want[3]};
+        for (int i = 0; i < 4; ++i)
+          if (!keep[i]) out[i].reset();
+      } else {
+        const int64_t h = s.size(s.dim() - 1), n = s.numel() / h;
+        LumaLayerNormArgs a = norm_args(n, h, stream, branch, param, 0.0, d);
+        const at::Tensor ss = as_rows(s), dy = dense(d_y.to(kTypes[branch]));
+        const at::Tensor w = weight.defined() ? dense(weight) : at::Tensor();
+        const at::Tensor dt = d_total.defined() ? dense(d_total.to(s.scalar_type())) : at::Tensor();
+        auto new_like = [&](at::IntArrayRef sizes, int64_t code) {
+          return at::empty(sizes, s.options().dtype(kTypes[code]));
+        };
+        if (want_x) out[0] = new_like(s.sizes(), adds ? branch : stream);
+        if (want_r) out[1] = new_like(s.sizes(), stream);
+        if (want[2]) out[2] = new_like({h}, param);
+        if (want[3]) out[3] = new_like({h}, param);
+        a.x = ss.const_data_ptr();
+        a.ld_x = ld_of(ss);
+        if (adds) a.total = const_cast<void *>(ss.const_data_ptr());
+        a.weight = w.defined() ? w.const_data_ptr() : nullptr;
+        a.stats = const_cast<float *>(stats.const_data_ptr<float>());
+        a.d_y = dy.const_data_ptr();
+        a.d_total = dt.defined() ? dt.const_data_ptr() : nullptr;
+        void **to[4] = {&a.d_x, &a.d_residual, &a.d_weight, &a.d_bias};
+        for (int i = 0; i < 4; ++i) *to[i] = out[i].defined() ? out[i].mutable_data_ptr() : nullptr;
+        at::Tensor workspace;
+        const c10::DeviceGuard guard(s.device());
+        if (want[2] || want[3]) {
+          const int64_t bytes = g_more.norm_workspace(&a);
+          TORCH_CHECK(bytes >= 0, g_lib.error());
+          workspace = at::empty({bytes}, s.options().dtype(at::kByte));
+          a.workspace = workspace.mutable_data_ptr();
+          a.workspace_bytes = bytes;
+        }
+        run(g_more.norm_backward(&a, current_stream(s.device().index())));
+      }
+      if (one && want[0]) out[0] = out[1];
+      if (one && !want[1]) out[1].reset();
+    }
+    once({&out[0], &out[1], &out[2], &out[3]}, adds ? "add_layer_norm" : "layer_norm", s, weight,
+         grads[0], adds ? grads[1] : at::Tensor());
+    return {out[0], out[1], out[2], out[3], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// layer_norm and (with a residual) add_layer_norm of plain tensors: y, or y and the
+// sum; None where the arguments do not fit (the caller then says which) and for no
+// elements.  branch: y's LUMA_GRAD_*.
+py::object layer_norm(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight,
+                      const MaybeTensor &bias, const MaybeTensor &seed_at, double eps, double p,
+                      int64_t seed, int64_t call, int64_t branch) {
+  if (!g_more.norm_forward || !x.is_cuda() || x.layout() != at::kStrided || x.dim() < 1 ||
+      x.numel() == 0 || grad_code(x.scalar_type()) < 0 || branch < 0 || branch > 2 ||
+      !(eps >= 0.0) || !fit_draws(x, seed_at, p, call))
+    return py::none();
+  const bool adds = given(residual);
+  const at::Tensor &like = adds ? *residual : x;
+  if (adds && (!same_place(like, x) || like.sizes() != x.sizes())) return py::none();
+  const int64_t stream = grad_code(like.scalar_type());
+  if (stream < 0 || (stream != branch && stream != LUMA_GRAD_F32)) return py::none();
+  if (adds && grad_code(x.scalar_type()) != branch) return py::none();
+  const MaybeTensor *const params[2] = {&weight, &bias};
+  for (const MaybeTensor *t : params)
+    if (given(*t)) {
+      const int64_t code = grad_code((*t)->scalar_type());
+      if (!same_place(**t, x) || (*t)->dim() != 1 || (*t)->size(0) != x.size(x.dim() - 1) ||
+          (code != LUMA_GRAD_F32 && code != branch) ||
+          (given(weight) && given(bias) && weight->scalar_type() != bias->scalar_type()))
+        return py::none();
+    }
+  const bool keep = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || like.requires_grad() ||
+                     (given(weight) && weight->requires_grad()) ||
+                     (given(bias) && bias->requires_grad()));
+  const Variables out = LayerNorm::apply(x, residual, weight, bias, seed_at, eps, p, seed, call,
+                                         branch, keep);
+  return adds ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
+}
+
+// The operands of a policy loss as rows.
+struct PolicyRows {
+  at::Tensor logp, old, ref, advantage, mask;
+};
+
+LumaPolicyArgs policy_args(const at::Tensor &logp, const at::Tensor &old,
+                           const at::Tensor &advantage, const at::Tensor &mask,
+                           const at::Tensor &ref, const at::Tensor &share, double low, double high,
+                           double kl, int64_t reduction, PolicyRows &r) {
+  const bool each = advantage.dim() == logp.dim();
+  r.logp = as_rows(logp);
+  r.old = as_rows(old);
+  if (ref.defined()) r.ref = as_rows(ref);
+  if (mask.defined()) r.mask = as_rows(mask);
+  r.advantage = each ? as_rows(advantage) : dense(advantage);
+  LumaPolicyArgs a{};
+  a.logp = r.logp.const_data_ptr();
+  a.old_logp = r.old.const_data_ptr();
+  a.ref_logp = ref.defined() ? r.ref.const_data_ptr() : nullptr;
+  a.advantage = r.advantage.const_data_ptr<float>();
+  a.mask = mask.defined() ? static_cast<const uint8_t *>(r.mask.const_data_ptr()) : nullptr;
+  a.rows = r.logp.size(0);
+  a.length = r.logp.size(1);
+  a.ld_logp = ld_of(r.logp);
+  a.ld_old = ld_of(r.old);
+  a.ld_ref = ref.defined() ? ld_of(r.ref) : 0;
+  a.ld_mask = mask.defined() ? ld_of(r.mask) : 0;
+  a.ld_advantage = each ? ld_of(r.advantage) : 1;
+  a.advantage_each = each;
+  a.dtype = grad_code(logp.scalar_type());
+  a.reduction = (int32_t)reduction;
+  a.clip_low = low;
+  a.clip_high = high;
+  a.kl_weight = kl;
+  a.share = share.mutable_data_ptr<float>();
+  return a;
+}
+
+struct Policy : torch::autograd::Function<Policy> {
+  static Variables forward(Context *ctx, const at::Tensor &logp, const at::Tensor &old,
+                           const at::Tensor &advantage, const MaybeTensor &mask,
+                           const MaybeTensor &ref, double low, double high, double kl,
+                           int64_t reduction) {
+    const auto f32 = logp.options().dtype(at::kFloat);
+    const int64_t rows = logp.numel() / logp.size(logp.dim() - 1);
+    at::Tensor loss = reduction == LUMA_XENT_NONE ? at::empty(logp.sizes(), f32)
+                                                  : at::empty({}, f32);
+    at::Tensor stats = at::empty({LUMA_POLICY_STATS}, f32);
+    const at::Tensor share = at::empty({rows + 1}, f32);
+    PolicyRows r;
+    LumaPolicyArgs a = policy_args(logp, old, advantage, value(mask), value(ref), share, low, high,
+                                   kl, reduction, r);
+    a.loss = loss.mutable_data_ptr<float>();
+    a.stats = stats.mutable_data_ptr<float>();
+    const c10::DeviceGuard guard(logp.device());
+    const int64_t bytes = g_more.policy_workspace(&a);
+    TORCH_CHECK(bytes >= 0, g_lib.error());
+    at::Tensor workspace;
+    if (bytes) {
+      workspace = at::empty({bytes}, logp.options().dtype(at::kByte));
+      a.workspace = workspace.mutable_data_ptr();
+      a.workspace_bytes = bytes;
+    }
+    run(g_more.policy_forward(&a, current_stream(logp.device().index())));
+    ctx->save_for_backward({logp, old, advantage, value(mask), value(ref), share});
+    ctx->saved_data["low"] = low;
+    ctx->saved_data["high"] = high;
+    ctx->saved_data["kl"] = kl;
+    ctx->saved_data["reduction"] = reduction;
+    ctx->mark_non_differentiable({stats});
+    ctx->set_materialize_grads(false);
+    return {loss, stats};
+  }
+
+  static Variables backward(Context *ctx, Variables grads) {
+    at::Tensor d_logp;
+    if (grads[0].defined() && ctx->needs_input_grad(0)) {
+      const auto saved = ctx->get_saved_variables();
+      const at::Tensor &logp = saved[0];
+      const double low = ctx->saved_data["low"].toDouble();
+      const double high = ctx->saved_data["high"].toDouble();
+      const double kl = ctx->saved_data["kl"].toDouble();
+      const int64_t reduction = ctx->saved_data["reduction"].toInt();
+      {
+        at::AutoDispatchBelowADInplaceOrView below;
+        if (watched()) {
+          static const auto op =
+              op_of<at::Tensor(const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                               const at::Tensor &, const MaybeTensor &, const MaybeTensor &,
+                               const at::Tensor &, double, double, double, int64_t)>(
+                  "luma_amd::policy_loss_backward");
+          d_logp = op.call(grads[0], logp, saved[1], saved[2], maybe(saved[3]), maybe(saved[4]),
+                           saved[5], low, high, kl, reduction);
+        } else {
+          const at::Tensor g = dense(grads[0].to(at::kFloat));
+          d_logp = at::empty(logp.sizes(), logp.options());
+          PolicyRows r;
+          LumaPolicyArgs a = policy_args(logp, saved[1], saved[2], saved[3], saved[4], saved[5],
+                                         low, high, kl, reduction, r);
+          a.grad_loss = g.const_data_ptr<float>();
+          a.d_logp = d_logp.mutable_data_ptr();
+          const c10::DeviceGuard guard(logp.device());
+          run(g_more.policy_backward(&a, current_stream(logp.device().index())));
+        }
+      }
+      once({&d_logp}, "policy_loss", logp, grads[0]);
+    }
+    return {d_logp, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
+            at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+
+// policy_loss of plain tensors: the loss and its figures; None where its arguments do
+// not fit (the caller then says which) and for no tokens.
+py::object policy_loss(const at::Tensor &logp, const at::Tensor &old, const at::Tensor &advantage,
+                       const MaybeTensor &mask, const MaybeTensor &ref, double low, double high,
+                       double kl, int64_t reduction) {
+  const int64_t d = logp.dim();
+  if (!g_more.policy_forward || !logp.is_cuda() || logp.layout() != at::kStrided || d < 1 ||
+      logp.numel() == 0 || grad_code(logp.scalar_type()) < 0 || !same_place(old, logp) ||
+      old.scalar_type() != logp.scalar_type() || old.sizes() != logp.sizes() ||
+      !same_place(advantage, logp) || advantage.scalar_type() != at::kFloat ||
+      (advantage.sizes() != logp.sizes() && advantage.sizes() != logp.sizes().slice(0, d - 1)) ||
+      !(low >= 0.0 && low <= 1.0) || !(high >= 0.0) || kl != kl)
+    return py::none();
+  if (given(mask) && (!same_place(*mask, logp) || mask->scalar_type() != at::kBool ||
+                      mask->sizes() != logp.sizes()))
+    return py::none();
+  if (given(ref) && (!same_place(*ref, logp) || ref->scalar_type() != logp.scalar_type() ||
+                     ref->sizes() != logp.sizes()))
+    return py::none();
+  const Variables out = Policy::apply(logp, old.detach(), advantage.detach(), mask,
+                                      given(ref) ? MaybeTensor(ref->detach()) : ref, low, high, kl,
+                                      reduction);
+  return py::make_tuple(out[0], out[1]);
+}
+
 PYBIND11_MODULE(_luma_host, m) {
   m.doc() = "Host-side bookkeeping of LUMA.step (pointer refresh of a planned step) and of the "
-            "gradient norm (its table); linear_cross_entropy's eager calls.";
+            "gradient norm (its table); the eager calls of the operators beside the step.";
   py::object torch = py::module_::import("torch");
   g_tensor_type = reinterpret_cast<PyTypeObject *>(torch.attr("Tensor").ptr());
   g_param_type = reinterpret_cast<PyTypeObject *>(torch.attr("nn").attr("Parameter").ptr());
@@ -792,6 +1298,10 @@ PYBIND11_MODULE(_luma_host, m) {
   m.def("xent", &xent);
   m.def("grad_norm", &grad_norm);
   m.def("bind", &bind);
+  m.def("bind_more", &bind_more);
+  m.def("dropout", &dropout);
+  m.def("layer_norm", &layer_norm);
+  m.def("policy_loss", &policy_loss);
   // the torch whose headers this module was compiled against: it reads
   // TensorImpl fields in that version's inline layout
   m.attr("torch_version") = LUMA_TORCH_VERSION;

@@ -1,0 +1,452 @@
+// The clipped policy loss of sampled tokens with a KL term (include/luma.h,
+// luma_policy_forward / luma_policy_backward).
+//
+//   r = exp(l - l_old),  value = -min(r A, clip(r) A) + kl (exp(q) - 1 - q),  q = l_ref - l
+//   d value / d l = -r A (or 0 where the clipped product is the smaller) + kl (1 - exp(q))
+//
+// A few numbers are read for each token and one is written: bound by HBM for
+// large batches and by launches for small ones.  A workgroup takes a piece of
+// one long row, or whole short rows, a wavefront each, and leaves one record of
+// its sums; a join makes the loss of them in a fixed order (no atomics).  Up to
+// kAlone short rows are one workgroup's, which joins them itself: one launch.
+// The backward forms the token's terms again, which is cheaper than keeping
+// them: the operands of small batches are still in the caches.
+#include "luma_error.h"
+#include "luma_rows.h"
+
+namespace luma {
+namespace policy {
+
+using namespace rows;
+
+constexpr int kThreads = 256, kWaves = kThreads / 64;
+constexpr int kTokens = 4;                        // of a lane at a time
+constexpr int64_t kShort = 1024;                  // tokens of a row that a wavefront takes
+constexpr int64_t kMostLong = (int64_t)1 << 22;   // longer rows
+constexpr int64_t kAlone = 32;                    // short rows that one workgroup takes
+constexpr int kJoinThreads = 1024;
+constexpr int64_t kBlocks = 2048;                 // workgroups, about
+
+// A workgroup's sums.
+struct Part {
+  double value;        // of the values; of whole rows' means for the mean of sequences
+  double kl, moved;    // of exp(q) - 1 - q, of r - 1 - log r
+  int64_t count, clipped, sequences;
+};
+
+// How a call is shared out.
+struct Plan {
+  bool shorts;         // whole rows, a wavefront each; else pieces of rows
+  int64_t piece;       // tokens of a piece
+  int64_t pieces;      // of a row
+  int64_t each;        // rows of a wavefront, one after the other
+  int64_t blocks;
+};
+
+inline Plan plan(const LumaPolicyArgs *a) {
+  Plan p;
+  p.shorts = a->length <= kShort;
+  if (p.shorts) {
+    p.piece = a->length;
+    p.pieces = 1;
+    p.each = (a->rows + kBlocks * kWaves - 1) / (kBlocks * kWaves);
+    const int64_t rows = p.each * kWaves;
+    p.blocks = (a->rows + rows - 1) / rows;
+  } else {
+    // (pieces of at least 1,024 tokens, longer where that makes too many)
+    const int64_t steps = (a->length + kShort - 1) / kShort, total = steps * a->rows;
+    const int64_t run = (total + kBlocks - 1) / kBlocks;
+    p.piece = (run < steps ? run : steps) * kShort;
+    p.pieces = (a->length + p.piece - 1) / p.piece;
+    p.each = 1;
+    p.blocks = p.pieces * a->rows;
+  }
+  return p;
+}
+
+// exp(x) and exp(x) - 1 - x, the latter by its series where it is a difference
+// of near numbers (the terms left out are below 2^-24 of it).
+__device__ __forceinline__ void exp_excess(float x, float &e, float &excess) {
+  e = expf(x);
+  float s = 1.0f / 40320.0f;
+  s = __builtin_fmaf(s, x, 1.0f / 5040.0f);
+  s = __builtin_fmaf(s, x, 1.0f / 720.0f);
+  s = __builtin_fmaf(s, x, 1.0f / 120.0f);
+  s = __builtin_fmaf(s, x, 1.0f / 24.0f);
+  s = __builtin_fmaf(s, x, 1.0f / 6.0f);
+  s = __builtin_fmaf(s, x, 0.5f);
+  excess = __builtin_fabsf(x) < 0.5f ? s * x * x : e - 1.0f - x;
+}
+
+struct Limits {
+  double up, low;               // of l - l_old
+  float high_ratio, low_ratio;  // 1 + clip_high, 1 - clip_low
+  float kl;
+};
+
+struct Token {
+  float value, grad, kl, moved;
+  bool clipped;
+};
+
+__device__ __forceinline__ Token token(float l, float old, float ref, bool has_ref, float adv,
+                                       const Limits &lim) {
+  Token t;
+  // (exact: float32 numbers' difference in float64)
+  const double d = (double)l - (double)old;
+  float r;
+  exp_excess((float)d, r, t.moved);
+  const bool up = d > lim.up, low = d < lim.low;
+  t.clipped = adv > 0.0f ? up : low && adv < 0.0f;
+  const float held = up ? lim.high_ratio : lim.low_ratio;
+  t.value = -(t.clipped ? held : r) * adv;
+  t.grad = t.clipped ? 0.0f : -r * adv;
+  t.kl = 0.0f;
+  if (has_ref) {
+    const float q = ref - l;
+    float e;
+    exp_excess(q, e, t.kl);
+    // (exp(q) - 1 with the excess's digits)
+    const float minus = __builtin_fabsf(q) < 0.5f ? t.kl + q : e - 1.0f;
+    t.value = __builtin_fmaf(lim.kl, t.kl, t.value);
+    t.grad = __builtin_fmaf(-lim.kl, minus, t.grad);
+  }
+  return t;
+}
+
+// A row's operands at a lane's tokens.
+template <typename T>
+struct Row {
+  const T *logp, *old, *ref;
+  const float *advantage;
+  const uint8_t *mask;
+  float one;           // the row's advantage
+  bool each;
+
+  __device__ __forceinline__ Row(const LumaPolicyArgs &a, int64_t row) {
+    logp = (const T *)a.logp + row * a.ld_logp;
+    old = (const T *)a.old_logp + row * a.ld_old;
+    ref = a.ref_logp ? (const T *)a.ref_logp + row * a.ld_ref : nullptr;
+    mask = a.mask ? a.mask + row * a.ld_mask : nullptr;
+    advantage = a.advantage + row * a.ld_advantage;
+    each = a.advantage_each != 0;
+    one = each ? 0.0f : *advantage;
+  }
+};
+
+template <typename T>
+struct Tokens {
+  Vec<T, kTokens> l, old, ref;
+  Vec<float, kTokens> adv;
+  uint32_t keep;       // bit j: token j counts
+
+  __device__ __forceinline__ void load(const Row<T> &r, int64_t t, int64_t end) {
+    if (r.mask) {
+      const Vec<uint8_t, kTokens> m = rows::load<kTokens>(r.mask, t, end);
+      keep = 0u;
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) keep |= m[j] && t + j < end ? 1u << j : 0u;
+    } else {
+      const int64_t left = end - t;
+      keep = left >= kTokens ? (1u << kTokens) - 1u : left > 0 ? (1u << left) - 1u : 0u;
+    }
+    l = rows::load<kTokens>(r.logp, t, end);
+    old = rows::load<kTokens>(r.old, t, end);
+    if (r.ref) ref = rows::load<kTokens>(r.ref, t, end);
+    if (r.each) adv = rows::load<kTokens>(r.advantage, t, end);
+  }
+
+  __device__ __forceinline__ Token at(const Row<T> &r, int j, const Limits &lim) const {
+    return token((float)l[j], (float)old[j], r.ref ? (float)ref[j] : 0.0f, r.ref != nullptr,
+                 r.each ? adv[j] : r.one, lim);
+  }
+};
+
+__device__ __forceinline__ double wave_sum(double v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
+  return v;
+}
+
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor((long long)v, m);
+  return v;
+}
+
+// Tokens first, first + step, ... of a row before end, into p (a lane's own sums).
+template <typename T>
+__device__ __forceinline__ void row_sums(const LumaPolicyArgs &a, const Limits &lim, int64_t row,
+                                         int64_t first, int64_t step, int64_t end, Part &p) {
+  const Row<T> r(a, row);
+  float *out = a.reduction == LUMA_XENT_NONE ? a.loss + row * a.length : nullptr;
+  for (int64_t t = first; t < end; t += step) {
+    Tokens<T> in;
+    in.load(r, t, end);
+    float v[kTokens];
+#pragma unroll
+    for (int j = 0; j < kTokens; ++j) {
+      const Token k = in.at(r, j, lim);
+      const bool keep = in.keep >> j & 1u;
+      v[j] = keep ? k.value : 0.0f;
+      p.value += (double)v[j];
+      p.kl += keep ? (double)k.kl : 0.0;
+      p.moved += keep ? (double)k.moved : 0.0;
+      p.count += keep;
+      p.clipped += keep && k.clipped;
+    }
+    if (out) store<kTokens>(out, t, end, v);
+  }
+}
+
+// The sums of all the wavefronts' lanes, in every thread of the first.
+template <int W>
+__device__ __forceinline__ Part block_sum(Part p, Part *lds) {
+  p.value = wave_sum(p.value);
+  p.kl = wave_sum(p.kl);
+  p.moved = wave_sum(p.moved);
+  p.count = wave_sum(p.count);
+  p.clipped = wave_sum(p.clipped);
+  p.sequences = wave_sum(p.sequences);
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = p;
+  __syncthreads();
+  Part sum = lds[0];
+  if (threadIdx.x < 64)
+    for (int i = 1; i < W; ++i) {
+      sum.value += lds[i].value;
+      sum.kl += lds[i].kl;
+      sum.moved += lds[i].moved;
+      sum.count += lds[i].count;
+      sum.clipped += lds[i].clipped;
+      sum.sequences += lds[i].sequences;
+    }
+  return sum;
+}
+
+// The loss and what goes with it, by one thread.
+__device__ __forceinline__ void finish(const LumaPolicyArgs &a, const Part &p) {
+  const double n = (double)p.count, s = (double)p.sequences;
+  if (a.reduction == LUMA_XENT_SUM) *a.loss = (float)p.value;
+  if (a.reduction == LUMA_XENT_MEAN) *a.loss = (float)(p.value / n);
+  if (a.reduction == LUMA_POLICY_SEQUENCE) *a.loss = (float)(p.value / s);
+  if (a.share)
+    a.share[a.rows] = a.reduction == LUMA_XENT_MEAN          ? (float)(1.0 / n)
+                      : a.reduction == LUMA_POLICY_SEQUENCE ? (float)(1.0 / s)
+                                                             : 1.0f;
+  a.stats[0] = (float)((double)p.clipped / n);
+  a.stats[1] = (float)(p.kl / n);
+  a.stats[2] = (float)(p.moved / n);
+  a.stats[3] = (float)p.count;
+}
+
+// A wavefront's whole rows; a sequence's mean is taken here.
+template <typename T>
+__device__ __forceinline__ void whole_rows(const LumaPolicyArgs &a, const Limits &lim,
+                                           int64_t first, int64_t end, Part &p) {
+  const int lane = threadIdx.x % 64;
+  for (int64_t row = first; row < end; ++row) {
+    Part one = {};
+    row_sums<T>(a, lim, row, lane * kTokens, 64 * kTokens, a.length, one);
+    if (a.reduction == LUMA_POLICY_SEQUENCE) {
+      const int64_t count = wave_sum(one.count);
+      one.value = count ? one.value / (double)count : 0.0;
+      one.sequences = lane == 0 && count;
+      if (lane == 0 && a.share) a.share[row] = count ? (float)(1.0 / (double)count) : 0.0f;
+    }
+    p.value += one.value;
+    p.kl += one.kl;
+    p.moved += one.moved;
+    p.count += one.count;
+    p.clipped += one.clipped;
+    p.sequences += one.sequences;
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void sums_kernel(LumaPolicyArgs a, Limits lim, Plan plan) {
+  __shared__ Part lds[kWaves];
+  Part p = {};
+  if (plan.shorts) {
+    const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / 64) * plan.each;
+    const int64_t end = first + plan.each < a.rows ? first + plan.each : a.rows;
+    whole_rows<T>(a, lim, first, end, p);
+  } else {
+    const int64_t row = blockIdx.x / plan.pieces, first = blockIdx.x % plan.pieces * plan.piece;
+    const int64_t end = first + plan.piece < a.length ? first + plan.piece : a.length;
+    row_sums<T>(a, lim, row, first + threadIdx.x * kTokens, kThreads * kTokens, end, p);
+  }
+  p = block_sum<kWaves>(p, lds);
+  if (threadIdx.x == 0) ((Part *)a.workspace)[blockIdx.x] = p;
+}
+
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(LumaPolicyArgs a, Plan plan) {
+  __shared__ Part lds[kJoinThreads / 64];
+  const Part *part = (const Part *)a.workspace;
+  Part p = {};
+  auto take = [&](const Part &o) {
+    p.kl += o.kl;
+    p.moved += o.moved;
+    p.count += o.count;
+    p.clipped += o.clipped;
+    p.sequences += o.sequences;
+  };
+  if (!plan.shorts && a.reduction == LUMA_POLICY_SEQUENCE) {
+    for (int64_t row = threadIdx.x; row < a.rows; row += kJoinThreads) {
+      double value = 0.0;
+      int64_t count = 0;
+      for (int64_t i = 0; i < plan.pieces; ++i) {
+        const Part o = part[row * plan.pieces + i];
+        take(o);
+        value += o.value;
+        count += o.count;
+      }
+      p.value += count ? value / (double)count : 0.0;
+      p.sequences += count != 0;
+      if (a.share) a.share[row] = count ? (float)(1.0 / (double)count) : 0.0f;
+    }
+  } else {
+    for (int64_t i = threadIdx.x; i < plan.blocks; i += kJoinThreads) {
+      const Part o = part[i];
+      take(o);
+      p.value += o.value;
+    }
+  }
+  p = block_sum<kJoinThreads / 64>(p, lds);
+  if (threadIdx.x == 0) finish(a, p);
+}
+
+// A few short rows in one launch.
+template <typename T>
+__global__ __launch_bounds__(kJoinThreads) void alone_kernel(LumaPolicyArgs a, Limits lim) {
+  constexpr int W = kJoinThreads / 64;
+  __shared__ Part lds[W];
+  Part p = {};
+  for (int64_t row = threadIdx.x / 64; row < a.rows; row += W)
+    whole_rows<T>(a, lim, row, row + 1, p);
+  p = block_sum<W>(p, lds);
+  if (threadIdx.x == 0) finish(a, p);
+}
+
+template <typename T>
+__device__ __forceinline__ void row_grads(const LumaPolicyArgs &a, const Limits &lim, int64_t row,
+                                          int64_t first, int64_t step, int64_t end) {
+  const Row<T> r(a, row);
+  const bool none = a.reduction == LUMA_XENT_NONE;
+  const float *each = none ? a.grad_loss + row * a.length : nullptr;
+  float g = 1.0f;
+  if (!none) g = *a.grad_loss * a.share[a.rows];
+  if (a.reduction == LUMA_POLICY_SEQUENCE) g *= a.share[row];
+  for (int64_t t = first; t < end; t += step) {
+    Tokens<T> in;
+    in.load(r, t, end);
+    float o[kTokens], f[kTokens];
+    if (none) {
+      widen<kTokens, float>(load<kTokens>(each, t, end), f);
+    } else {
+#pragma unroll
+      for (int j = 0; j < kTokens; ++j) f[j] = g;
+    }
+#pragma unroll
+    for (int j = 0; j < kTokens; ++j)
+      o[j] = in.keep >> j & 1u ? in.at(r, j, lim).grad * f[j] : 0.0f;
+    store<kTokens>((T *)a.d_logp + row * a.length, t, end, o);
+  }
+}
+
+template <typename T>
+__global__ __launch_bounds__(kThreads) void grad_kernel(LumaPolicyArgs a, Limits lim, Plan plan) {
+  if (plan.shorts) {
+    const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / 64) * plan.each;
+    const int64_t end = first + plan.each < a.rows ? first + plan.each : a.rows;
+    for (int64_t row = first; row < end; ++row)
+      row_grads<T>(a, lim, row, threadIdx.x % 64 * kTokens, 64 * kTokens, a.length);
+  } else {
+    const int64_t row = blockIdx.x / plan.pieces, first = blockIdx.x % plan.pieces * plan.piece;
+    const int64_t end = first + plan.piece < a.length ? first + plan.piece : a.length;
+    row_grads<T>(a, lim, row, first + threadIdx.x * kTokens, kThreads * kTokens, end);
+  }
+}
+
+Limits limits_of(const LumaPolicyArgs *a) {
+  Limits l;
+  l.up = log1p(a->clip_high);
+  l.low = a->clip_low >= 1.0 ? -INFINITY : log1p(-a->clip_low);
+  l.high_ratio = (float)(1.0 + a->clip_high);
+  l.low_ratio = (float)(1.0 - a->clip_low);
+  l.kl = (float)a->kl_weight;
+  return l;
+}
+
+bool alone(const LumaPolicyArgs *a) { return a->length <= kShort && a->rows <= kAlone; }
+
+bool check_args(const LumaPolicyArgs *a, bool backward) {
+  if (!a) return fail("luma_policy: null arguments"), false;
+  if (a->rows < 1 || a->length < 1) return fail("luma_policy: empty operands"), false;
+  if (a->rows > INT32_MAX || a->length > INT32_MAX || a->rows > ((int64_t)1 << 40) / a->length)
+    return fail("luma_policy: operands too large"), false;
+  // (a workgroup each, if they are long)
+  if (a->length > kShort && a->rows > kMostLong)
+    return fail("luma_policy: operands too large"), false;
+  if (!known_type(a->dtype)) return fail("luma_policy: unknown type"), false;
+  if (a->reduction < LUMA_XENT_NONE || a->reduction > LUMA_POLICY_SEQUENCE)
+    return fail("luma_policy: unknown reduction"), false;
+  if (!(a->clip_low >= 0.0 && a->clip_low <= 1.0))
+    return fail("luma_policy: clip_low is not in [0, 1]"), false;
+  if (!(a->clip_high >= 0.0)) return fail("luma_policy: clip_high is negative"), false;
+  if (a->kl_weight != a->kl_weight) return fail("luma_policy: kl_weight is NaN"), false;
+  if (a->reserved) return fail("luma_policy: reserved fields must be 0"), false;
+  if (!a->logp || !a->old_logp || !a->advantage) return fail("luma_policy: null operand"), false;
+  if (backward ? !a->grad_loss || !a->d_logp || (a->reduction != LUMA_XENT_NONE && !a->share)
+               : !a->loss || !a->stats)
+    return fail("luma_policy: null operand"), false;
+  if (a->rows > 1 && (a->ld_logp < 0 || a->ld_old < 0 || (a->ref_logp && a->ld_ref < 0) ||
+                      a->ld_advantage < 0 || (a->mask && a->ld_mask < 0)))
+    return fail("luma_policy: rows lie backwards"), false;
+  return true;
+}
+
+}  // namespace policy
+}  // namespace luma
+
+using namespace luma;
+using namespace luma::policy;
+
+extern "C" {
+
+int64_t luma_policy_workspace_bytes(const LumaPolicyArgs *a) {
+  if (!check_args(a, false)) return -1;
+  return alone(a) ? 0 : plan(a).blocks * (int64_t)sizeof(Part);
+}
+
+int luma_policy_forward(const LumaPolicyArgs *a, void *stream) {
+  if (!check_args(a, false)) return -1;
+  const hipStream_t s = (hipStream_t)stream;
+  const Limits lim = limits_of(a);
+  if (alone(a)) {
+    with_type(a->dtype, [&](auto t) {
+      alone_kernel<decltype(t)><<<1, kJoinThreads, 0, s>>>(*a, lim);
+    });
+    return check_launch("luma_policy_forward");
+  }
+  const Plan p = plan(a);
+  if (!a->workspace || (uintptr_t)a->workspace % 16 ||
+      a->workspace_bytes < p.blocks * (int64_t)sizeof(Part))
+    return fail("luma_policy_forward: workspace too small or not aligned");
+  with_type(a->dtype, [&](auto t) {
+    sums_kernel<decltype(t)><<<(uint32_t)p.blocks, kThreads, 0, s>>>(*a, lim, p);
+  });
+  join_kernel<<<1, kJoinThreads, 0, s>>>(*a, p);
+  return check_launch("luma_policy_forward");
+}
+
+int luma_policy_backward(const LumaPolicyArgs *a, void *stream) {
+  if (!check_args(a, true)) return -1;
+  const Plan p = plan(a);
+  with_type(a->dtype, [&](auto t) {
+    grad_kernel<decltype(t)>
+        <<<(uint32_t)p.blocks, kThreads, 0, (hipStream_t)stream>>>(*a, limits_of(a), p);
+  });
+  return check_launch("luma_policy_backward");
+}
+
+}  // extern "C"
