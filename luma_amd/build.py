@@ -26,7 +26,7 @@ ROOT = os.path.dirname(HERE)
 SOURCES = [(os.path.join(HERE, "csrc", "luma_step.hip"), (3, 2, 1, 0)),
            (os.path.join(HERE, "csrc", "luma_norm.hip"), (0,)),
            (os.path.join(HERE, "csrc", "luma_xent.hip"), (0,)),
-           (os.path.join(HERE, "csrc", "luma_residual.hip"), (1, 0)),
+           (os.path.join(HERE, "csrc", "luma_residual.hip"), (6, 5, 4, 3, 2, 1, 0)),
            (os.path.join(HERE, "csrc", "luma_policy.hip"), (0,))]
 
 OUT = os.path.join(HERE, "libluma_hip.so")

@@ -341,7 +341,7 @@ __device__ __forceinline__ void row_grads(const LumaPolicyArgs &a, const Limits 
     in.load(r, t, end);
     float o[kTokens], f[kTokens];
     if (none) {
-      widen<kTokens, float>(load<kTokens>(each, t, end), f);
+      widen<kTokens>(load<kTokens>(each, t, end), f);
     } else {
 #pragma unroll
       for (int j = 0; j < kTokens; ++j) f[j] = g;

@@ -15,11 +15,14 @@
 #include "luma_error.h"
 #include "luma_rows.h"
 
-// Unit 0: the entry points, dropout and the forward; unit 1: the backward (side
-// by side: a minute each).
+// Units, compiled side by side (a minute each): 0 holds the entry points and
+// dropout, 1 to 3 the forward of a branch of float32, bfloat16 and float16, 4 to 6
+// the backward.
 #ifndef LUMA_UNIT
 #define LUMA_UNIT 0
 #endif
+#define LUMA_FORWARD (LUMA_UNIT >= 1 && LUMA_UNIT <= 3)
+#define LUMA_BACKWARD (LUMA_UNIT >= 4)
 
 namespace luma {
 namespace residual {
@@ -32,44 +35,94 @@ constexpr int kLongThreads = 1024;     // of a workgroup that holds no row
 constexpr int kJoinCols = 32, kJoinRows = 32;
 constexpr int64_t kMostThreads = (int64_t)1 << 31;   // of one launch
 
-// Which team holds a row of h: the narrowest that does with one eight a lane.
-template <int L_, int K_>
+// Elements that a lane has next to each other: 16 bytes of the stream's type, so
+// that each load or store of a wavefront is one run of memory.  (Eight float32 a
+// lane, in two loads of every other 16 bytes: 8,192 x 4,096 of a float32 stream
+// and a bfloat16 branch 77 us with non-temporal accesses, 74 without.)
+template <typename S>
+constexpr int kVec = 16 / sizeof(S);
+
+// A team of L lanes holds a row, K runs of V elements a lane (WHOLE: rows of whole
+// runs).
+template <int L_, int K_, int V_, bool WHOLE_>
 struct Team {
-  static constexpr int L = L_, K = K_;
+  static constexpr int L = L_, K = K_, V = V_;
+  static constexpr bool WHOLE = WHOLE_;
+  static constexpr int kRow = L * K * V;
   static constexpr int kThreads = L < 256 ? 256 : L;
   static constexpr int kTeams = kThreads / L;
+
+  // The column of this thread's run k.
+  static __device__ __forceinline__ int64_t column(int k) {
+    return (k * L + (int)(threadIdx.x % L)) * V;
+  }
 };
 
-inline int lanes_of(int64_t h) {
-  int lanes = 8;
-  while (lanes < 1024 && lanes * 8 < h) lanes *= 2;
-  return lanes;
-}
-
-template <typename F>
+// f(team) of the narrowest team that holds a row of h.  Lanes without elements cost
+// their instructions (8,192 x 768 in teams for 2,048 took 1.4 times as long), a
+// wavefront needs no barrier for its sums (8,192 x 768 bfloat16 backward 15.7 us
+// in teams of 64 lanes, 21.7 in 128), and of wide rows one run a lane is best
+// (16,384 x 4,096 bfloat16: 512 lanes 90 and 86 us, 256 lanes 95 and 88) as long as
+// the backward, which holds five numbers an element, has the registers.
+template <int V, bool WHOLE, typename F>
 void with_team(int64_t h, F f) {
-  switch (lanes_of(h)) {
-    case 8: return f(Team<8, 1>{});
-    case 16: return f(Team<16, 1>{});
-    case 32: return f(Team<32, 1>{});
-    case 64: return f(Team<64, 1>{});
-    case 128: return f(Team<128, 1>{});
-    case 256: return f(Team<256, 1>{});
-    case 512: return f(Team<512, 1>{});
-    default: return h <= 8192 ? f(Team<1024, 1>{}) : f(Team<1024, 2>{});
-  }
+  const int64_t runs = (h + V - 1) / V;
+  if (runs <= 8) return f(Team<8, 1, V, WHOLE>{});
+  if (runs <= 16) return f(Team<16, 1, V, WHOLE>{});
+  if (runs <= 32) return f(Team<32, 1, V, WHOLE>{});
+  if (runs <= 64) return f(Team<64, 1, V, WHOLE>{});
+  if (runs <= 128) return f(Team<64, 2, V, WHOLE>{});
+  if (runs <= 192) return f(Team<64, 3, V, WHOLE>{});
+  if (runs <= 256) return f(Team<256, 1, V, WHOLE>{});
+  if (runs <= 512) return f(Team<512, 1, V, WHOLE>{});
+  if (runs <= 768) return f(Team<256, 3, V, WHOLE>{});
+  if (runs <= 1024) return f(Team<512, 2, V, WHOLE>{});
+  if (runs <= 1536) return f(Team<512, 3, V, WHOLE>{});
+  if (V == 8 || runs <= 2048) return f(Team<512, 4, V, WHOLE>{});
+  if constexpr (V == 4) f(Team<512, 8, V, WHOLE>{});
 }
 
-// Workgroups that the backward keeps on the chip, each with its own sums of the
-// weight's and bias's gradients.
-inline int64_t grad_blocks(int64_t n, int64_t h) {
+template <int V, typename F>
+void with_team(int64_t h, F f) {
+  if (h % V == 0)
+    with_team<V, true>(h, f);
+  else
+    with_team<V, false>(h, f);
+}
+
+// Whether a call's operands (so many of the stream's type and of the branch's) are
+// more than the last-level cache holds: they then go past it.
+inline bool apart(const LumaLayerNormArgs *a, int streams, int branches) {
+  const int64_t size = streams * (a->stream == LUMA_GRAD_F32 ? 4 : 2) +
+                       branches * (a->branch == LUMA_GRAD_F32 ? 4 : 2);
+  return a->n * a->h * size > (int64_t)256 << 20;
+}
+
+// Workgroups of T that a call of n rows is given: `threads` threads of each of the
+// 256 CUs, or fewer.
+template <typename T>
+int64_t blocks_of(int64_t n, int threads) {
+  const int64_t most = 256 * (threads < T::kThreads ? 1 : threads / T::kThreads);
+  const int64_t need = (n + T::kTeams - 1) / T::kTeams;
+  return need < most ? need : most;
+}
+
+constexpr int kForwardThreads = 1024, kGradThreads = 512;
+
+// Workgroups of the backward, each with its own sums of the weight's and bias's
+// gradients.
+inline int64_t grad_blocks(int64_t n, int64_t h, int stream) {
   if (h > kWidest) {      // (norm_long_sums_kernel's shares of the rows)
     const int64_t most = 1024 / ((h + 2047) / 2048);
     return most < 1 ? 1 : n < most ? n : most;
   }
-  const int64_t lanes = lanes_of(h), threads = lanes < 256 ? 256 : lanes;
-  const int64_t most = 256 * (1024 / threads), need = (n + threads / lanes - 1) / (threads / lanes);
-  return need < most ? need : most;
+  int64_t blocks = 0;
+  auto count = [&](auto team) { blocks = blocks_of<decltype(team)>(n, kGradThreads); };
+  if (stream == LUMA_GRAD_F32)
+    with_team<4>(h, count);
+  else
+    with_team<8>(h, count);
+  return blocks;
 }
 
 // launch(first, blocks) for runs of the workgroups that one launch can hold.
@@ -81,7 +134,7 @@ void in_runs(int64_t blocks, int threads, F launch) {
 }
 
 // Sum of v over a team's lanes, in all of them; `at`: a float for each of the
-// workgroup's wavefronts, used for this sum alone until the next barrier but one.
+// workgroup's wavefronts, that no wavefront writes again before the next barrier.
 template <int L>
 __device__ __forceinline__ float team_sum(float v, float *at) {
   v = lanes_sum<(L < 64 ? L : 64)>(v);
@@ -97,28 +150,48 @@ __device__ __forceinline__ float team_sum(float v, float *at) {
   return v;
 }
 
-// Eight of the weight or bias, of float32 or the branch's type.
-template <typename B>
+// Two at once.
+template <int L>
+__device__ __forceinline__ void team_sum2(float &u, float &v, float *at_u, float *at_v) {
+  u = lanes_sum<(L < 64 ? L : 64)>(u);
+  v = lanes_sum<(L < 64 ? L : 64)>(v);
+  if constexpr (L > 64) {
+    const int wave = threadIdx.x / 64;
+    if (threadIdx.x % 64 == 0) {
+      at_u[wave] = u;
+      at_v[wave] = v;
+    }
+    __syncthreads();
+    const int first = wave / (L / 64) * (L / 64);
+    u = v = 0.0f;
+#pragma unroll
+    for (int i = 0; i < L / 64; ++i) {
+      u += at_u[first + i];
+      v += at_v[first + i];
+    }
+  }
+}
+
+// N of the weight or bias, of float32 or the branch's type.
+template <int N, bool WHOLE, typename B>
 __device__ __forceinline__ void load_param(const void *p, bool wide, int64_t c, int64_t h,
                                            float fill, float *f) {
   if (!p) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = fill;
+    for (int j = 0; j < N; ++j) f[j] = fill;
   } else if (wide) {
-    widen<8, float>(load<8>((const float *)p, c, h), f);
+#pragma unroll
+    for (int i = 0; i < N; i += 4) widen<4>(load<4, WHOLE>((const float *)p, c + i, h), f + i);
   } else {
-    widen<8, B>(load<8>((const B *)p, c, h), f);
+    widen<N>(load<N, WHOLE>((const B *)p, c, h), f);
   }
 }
 
-// f, kept and scaled or dropped.
-__device__ __forceinline__ void drop8(float *f, uint64_t e, const Draw &d) {
-  const uint32_t kept = kept_from(e, d);
-#pragma unroll
-  for (int j = 0; j < 8; ++j) f[j] = kept >> j & 1u ? f[j] * d.scale : 0.0f;
-}
-
-void backward(const LumaLayerNormArgs *a, hipStream_t s);
+// The forward and the backward of a branch of type B (units 1 to 6).
+template <typename B>
+void forward_of(const LumaLayerNormArgs *a, hipStream_t s);
+template <typename B>
+void backward_of(const LumaLayerNormArgs *a, hipStream_t s);
 
 #if LUMA_UNIT == 0
 
@@ -126,209 +199,278 @@ void backward(const LumaLayerNormArgs *a, hipStream_t s);
 
 constexpr int kDropThreads = 256;
 
-// U eights a thread, a workgroup's next to each other.
-template <typename I, typename O, int U>
+// U runs a thread, a workgroup's next to each other.  A run is 16 bytes of the wider
+// type (its lanes' 8 bytes of the other are one run of memory, too).
+template <typename I, typename O, int U, bool NT>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(LumaDropoutArgs a) {
+  constexpr int V = kVec<I> < kVec<O> ? kVec<I> : kVec<O>;
   const I *x = (const I *)a.x;
   const O *residual = (const O *)a.residual;
   O *y = (O *)a.y;
   const bool draws = a.drop.p > 0.0;
   const Draw d = draw_of(a.drop);
-  const int64_t first = ((int64_t)blockIdx.x * U * kDropThreads + threadIdx.x) * 8;
-  Vec<I, 8> in[U];
-  Vec<O, 8> add[U];
+  const int64_t first = ((int64_t)blockIdx.x * U * kDropThreads + threadIdx.x) * V;
+  Vec<I, V> in[U];
+  Vec<O, V> add[U];
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t e = first + u * (kDropThreads * 8);
-    in[u] = load<8>(x, e, a.numel);
-    if (residual) add[u] = load<8>(residual, e, a.numel);
+    const int64_t e = first + u * (kDropThreads * V);
+    in[u] = load<V, false, NT>(x, e, a.numel);
+    if (residual) add[u] = load<V, false, NT>(residual, e, a.numel);
   }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t e = first + u * (kDropThreads * 8);
+    const int64_t e = first + u * (kDropThreads * V);
     if (e >= a.numel) break;
-    float f[8], r[8];
-    widen<8, I>(in[u], f);
-    if (draws) drop8(f, (uint64_t)e, d);
+    float f[V];
+    widen<V>(in[u], f);
+    if (draws) drop<V>(f, (uint64_t)e, d);
     if (residual) {
-      widen<8, O>(add[u], r);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) f[j] = r[j] + f[j];
+      for (int j = 0; j < V; ++j) f[j] = (float)add[u][j] + f[j];
     }
-    store<8>(y, e, a.numel, f);
+    store<V, false, NT>(y, e, a.numel, f);
   }
 }
 
 template <typename I, typename O>
 void dropout(const LumaDropoutArgs *a, hipStream_t s) {
-  const int64_t eights = (a->numel + 7) / 8;
-  if (eights >= 256 * 1024) {
-    const int64_t each = 4 * kDropThreads;
-    dropout_kernel<I, O, 4><<<(uint32_t)((eights + each - 1) / each), kDropThreads, 0, s>>>(*a);
-  } else {
-    dropout_kernel<I, O, 1>
-        <<<(uint32_t)((eights + kDropThreads - 1) / kDropThreads), kDropThreads, 0, s>>>(*a);
-  }
+  constexpr int V = kVec<I> < kVec<O> ? kVec<I> : kVec<O>;
+  const int64_t runs = (a->numel + V - 1) / V;
+  const int64_t bytes = a->numel * (int64_t)(sizeof(I) + sizeof(O) * (a->residual ? 2 : 1));
+  auto go = [&](auto kernel, int64_t each) {
+    kernel<<<(uint32_t)((runs + each - 1) / each), kDropThreads, 0, s>>>(*a);
+  };
+  if (bytes > (int64_t)256 << 20)
+    go(dropout_kernel<I, O, 4, true>, 4 * kDropThreads);
+  else if (runs >= 256 * 1024)
+    go(dropout_kernel<I, O, 4, false>, 4 * kDropThreads);
+  else
+    go(dropout_kernel<I, O, 1, false>, kDropThreads);
 }
+
+#endif  // LUMA_UNIT == 0
+
+#if LUMA_FORWARD
 
 // -- the forward ------------------------------------------------------------------
 
-// The row's elements before its norm: x, or the sum (also stored).
-template <typename S, typename B, bool RES>
-__device__ __forceinline__ void row_elements(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
-                                             int64_t c, float *f) {
-  if constexpr (!RES) {
-    widen<8, S>(load<8>((const S *)a.x + row * a.ld_x, c, a.h), f);
-  } else {
-    float r[8];
-    widen<8, S>(load<8>((const S *)a.residual + row * a.ld_residual, c, a.h), r);
-    widen<8, B>(load<8>((const B *)a.x + row * a.ld_x, c, a.h), f);
-    if (a.drop.p > 0.0 && c < a.h) drop8(f, (uint64_t)(row * a.h + c), d);
-#pragma unroll
-    for (int j = 0; j < 8; ++j) f[j] = (float)(S)(r[j] + f[j]);
-    store<8>((S *)a.total + row * a.h, c, a.h, f);
+// How the elements before a norm come about.
+// x, residual + x, residual + dropout(x) (or residual + x all the same)
+constexpr int kAlone = 0, kAdds = 1, kDrops = 2;
+
+// A run of a row's columns as they are read: x, and the residual.
+template <typename S, typename B, int HOW, int V, bool WHOLE, bool NT>
+struct Columns {
+  typedef typename std::conditional<HOW == kAlone, S, B>::type X;
+  Vec<X, V> x;
+  typename std::conditional<HOW == kAlone, char, Vec<S, V>>::type residual;
+
+  __device__ __forceinline__ void load(const LumaLayerNormArgs &a, int64_t row, int64_t c) {
+    x = rows::load<V, WHOLE, NT>((const X *)a.x + row * a.ld_x, c, a.h);
+    if constexpr (HOW != kAlone)
+      residual = rows::load<V, WHOLE, NT>((const S *)a.residual + row * a.ld_residual, c, a.h);
   }
+
+  // The elements before the norm: x, or the sum (also stored).
+  __device__ __forceinline__ void elements(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
+                                           int64_t c, float *f) const {
+    widen<V>(x, f);
+    if constexpr (HOW != kAlone) {
+      if constexpr (HOW == kDrops) {
+        if (a.drop.p > 0.0 && c < a.h) drop<V>(f, (uint64_t)(row * a.h + c), d);
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] = (float)(S)((float)residual[j] + f[j]);
+      store<V, WHOLE, NT>((S *)a.total + row * a.h, c, a.h, f);
+    }
+  }
+};
+
+// 1 / sqrt(v): the instruction, within a unit in the last place, which takes
+// numbers below 2^-126 for 0.
+__device__ __forceinline__ float rsqrt_of(float v) {
+  if (v < 1e-30f) return __builtin_amdgcn_rsqf(v * 1.8446744e19f) * 4.2949673e9f;
+  return __builtin_amdgcn_rsqf(v);
 }
 
-// The mean of h elements about `about` with the squares about it: m and r.  The
-// mean of the differences is not quite 0 where the elements stand far from 0;
-// it is put into both.
-__device__ __forceinline__ void moments(float about, float first, float second, float h, float eps,
-                                        float &off, float &m, float &r) {
-  off = first / h;
-  float v = second / h - off * off;
+// The mean and the deviation from the sums of the differences from `about` and of
+// their squares: m = about + off and r.  The mean of the differences is not quite
+// 0 where the elements stand far from 0; it is put into both.
+__device__ __forceinline__ void moments(float about, float first, float second, float one_h,
+                                        float eps, float &off, float &m, float &r) {
+  off = first * one_h;
+  float v = second * one_h - off * off;
   v = v < 0.0f ? 0.0f : v;
   m = about + off;
-  r = 1.0f / sqrtf(v + eps);
+  r = rsqrt_of(v + eps);
 }
 
-template <typename S, typename B, bool RES, typename T>
-__global__ __launch_bounds__(T::kThreads) void norm_kernel(LumaLayerNormArgs a,
-                                                             int64_t block) {
-  constexpr int L = T::L, K = T::K;
-  __shared__ float at[3][T::kThreads / 64];
-  const int lane = threadIdx.x % L;
-  const int64_t row = (block + blockIdx.x) * T::kTeams + threadIdx.x / L;
-  const bool live = row < a.n;
+// A team goes from row to row, the next one's loads under way while it forms the
+// sums of one.
+template <typename S, typename B, int HOW, bool NT, typename T>
+__global__ __launch_bounds__(T::kThreads) void norm_kernel(LumaLayerNormArgs a) {
+  constexpr int L = T::L, K = T::K, V = T::V;
+  __shared__ float at[2][3][T::kThreads / 64];
+  const int64_t step = (int64_t)gridDim.x * T::kTeams;
+  int64_t row = (int64_t)blockIdx.x * T::kTeams + threadIdx.x / L;
   Draw d;
-  if constexpr (RES) d = draw_of(a.drop);
-  float f[K][8], sum = 0.0f;
+  if constexpr (HOW == kDrops) d = draw_of(a.drop);
+  Columns<S, B, HOW, V, T::WHOLE, NT> next[K];
+  if (row < a.n) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t c = (int64_t)(k * L + lane) * 8;
-    if (live) {
-      row_elements<S, B, RES>(a, d, row, c, f[k]);
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) f[k][j] = 0.0f;
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j) sum += f[k][j];      // (0 past the row)
+    for (int k = 0; k < K; ++k) next[k].load(a, row, T::column(k));
   }
-  float w[K][8], b[K][8];
+  float w[K][V], b[K][V];
   const bool wide = a.param == LUMA_GRAD_F32;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    const int64_t c = (int64_t)(k * L + lane) * 8;
-    load_param<B>(a.weight, wide, c, a.h, 1.0f, w[k]);
-    load_param<B>(a.bias, wide, c, a.h, 0.0f, b[k]);
+    load_param<V, T::WHOLE, B>(a.weight, wide, T::column(k), a.h, 1.0f, w[k]);
+    load_param<V, T::WHOLE, B>(a.bias, wide, T::column(k), a.h, 0.0f, b[k]);
   }
-  const float h = (float)a.h;
-  const float about = team_sum<L>(sum, at[0]) / h;
-  float first = 0.0f, second = 0.0f;
+  const float one_h = 1.0f / (float)a.h;
+  // (the workgroup's teams make as many turns as its first, which has the most rows)
+  int turn = 0;
+  for (int64_t base = (int64_t)blockIdx.x * T::kTeams; base < a.n;
+       base += step, row += step, turn ^= 1) {
+    const bool live = row < a.n;
+    float f[K][V], sum = 0.0f;
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t c = (int64_t)(k * L + lane) * 8;
+    for (int k = 0; k < K; ++k) {
+      if (live) {
+        next[k].elements(a, d, row, T::column(k), f[k]);
+      } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      f[k][j] = c + j < a.h ? f[k][j] - about : 0.0f;
-      first += f[k][j];
-      second = __builtin_fmaf(f[k][j], f[k][j], second);
+        for (int j = 0; j < V; ++j) f[k][j] = 0.0f;
+      }
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum += f[k][j];      // (0 past the row)
     }
-  }
-  first = team_sum<L>(first, at[1]);
-  second = team_sum<L>(second, at[2]);
-  float off, m, r;
-  moments(about, first, second, h, (float)a.eps, off, m, r);
-  if (!live) return;
-  if (a.stats && lane == 0) {
-    a.stats[row] = m;
-    a.stats[a.n + row] = r;
-  }
+    if (row + step < a.n) {
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    const int64_t c = (int64_t)(k * L + lane) * 8;
+      for (int k = 0; k < K; ++k) next[k].load(a, row + step, T::column(k));
+    }
+    const float about = team_sum<L>(sum, at[turn][0]) * one_h;
+    float first = 0.0f, second = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      f[k][j] = __builtin_fmaf((f[k][j] - off) * r, w[k][j], b[k][j]);
-    store<8>((B *)a.y + row * a.h, c, a.h, f[k]);
+    for (int k = 0; k < K; ++k) {
+      differences<V, T::WHOLE>(f[k], about, T::column(k), a.h);
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        first += f[k][j];
+        second = __builtin_fmaf(f[k][j], f[k][j], second);
+      }
+    }
+    team_sum2<L>(first, second, at[turn][1], at[turn][2]);
+    float off, m, r;
+    moments(about, first, second, one_h, (float)a.eps, off, m, r);
+    if (!live) continue;
+    if (a.stats && threadIdx.x % L == 0) {
+      a.stats[row] = m;
+      a.stats[a.n + row] = r;
+    }
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+      for (int j = 0; j < V; ++j)
+        f[k][j] = __builtin_fmaf((f[k][j] - off) * r, w[k][j], b[k][j]);
+      store<V, T::WHOLE, NT>((B *)a.y + row * a.h, T::column(k), a.h, f[k]);
+    }
   }
 }
 
 // A row that no team holds, one workgroup each: three passes over it.
-template <typename S, typename B, bool RES>
+template <typename S, typename B, int HOW>
 __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(LumaLayerNormArgs a, int64_t block) {
-  constexpr int L = kLongThreads, kStep = L * 8;
+  constexpr int L = kLongThreads, V = kVec<S>, kStep = L * V;
   __shared__ float at[3][L / 64];
   const int64_t row = block + blockIdx.x;
   Draw d;
-  if constexpr (RES) d = draw_of(a.drop);
-  const S *s = RES ? (const S *)a.total + row * a.h : (const S *)a.x + row * a.ld_x;
-  float f[8], sum = 0.0f;
-  for (int64_t c = threadIdx.x * 8; c < a.h; c += kStep) {
-    row_elements<S, B, RES>(a, d, row, c, f);
+  if constexpr (HOW == kDrops) d = draw_of(a.drop);
+  const S *s = HOW == kAlone ? (const S *)a.x + row * a.ld_x : (const S *)a.total + row * a.h;
+  float f[V], sum = 0.0f;
+  for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
+    Columns<S, B, HOW, V, false, false> in;
+    in.load(a, row, c);
+    in.elements(a, d, row, c, f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) sum += f[j];
+    for (int j = 0; j < V; ++j) sum += f[j];
   }
-  const float h = (float)a.h;
-  const float about = team_sum<L>(sum, at[0]) / h;
+  const float one_h = 1.0f / (float)a.h;
+  const float about = team_sum<L>(sum, at[0]) * one_h;
   float first = 0.0f, second = 0.0f;
   // (a thread reads the elements of the sum that it wrote itself)
-  for (int64_t c = threadIdx.x * 8; c < a.h; c += kStep) {
-    widen<8, S>(load<8>(s, c, a.h), f);
+  for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
+    widen<V>(load<V>(s, c, a.h), f);
+    differences<V>(f, about, c, a.h);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float g = c + j < a.h ? f[j] - about : 0.0f;
-      first += g;
-      second = __builtin_fmaf(g, g, second);
+    for (int j = 0; j < V; ++j) {
+      first += f[j];
+      second = __builtin_fmaf(f[j], f[j], second);
     }
   }
-  first = team_sum<L>(first, at[1]);
-  second = team_sum<L>(second, at[2]);
+  team_sum2<L>(first, second, at[1], at[2]);
   float off, m, r;
-  moments(about, first, second, h, (float)a.eps, off, m, r);
+  moments(about, first, second, one_h, (float)a.eps, off, m, r);
   if (a.stats && threadIdx.x == 0) {
     a.stats[row] = m;
     a.stats[a.n + row] = r;
   }
   const bool wide = a.param == LUMA_GRAD_F32;
-  for (int64_t c = threadIdx.x * 8; c < a.h; c += kStep) {
-    float w[8], b[8];
-    load_param<B>(a.weight, wide, c, a.h, 1.0f, w);
-    load_param<B>(a.bias, wide, c, a.h, 0.0f, b);
-    widen<8, S>(load<8>(s, c, a.h), f);
+  for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
+    float w[V], b[V];
+    load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
+    load_param<V, false, B>(a.bias, wide, c, a.h, 0.0f, b);
+    widen<V>(load<V>(s, c, a.h), f);
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-      f[j] = __builtin_fmaf((f[j] - about - off) * r, w[j], b[j]);
-    store<8>((B *)a.y + row * a.h, c, a.h, f);
+    for (int j = 0; j < V; ++j) f[j] = __builtin_fmaf((f[j] - about - off) * r, w[j], b[j]);
+    store<V>((B *)a.y + row * a.h, c, a.h, f);
   }
 }
 
-template <typename S, typename B, bool RES>
+template <typename S, typename B, int HOW>
 void forward(const LumaLayerNormArgs *a, hipStream_t s) {
   if (a->h > kWidest) {
     in_runs(a->n, kLongThreads, [&](int64_t first, uint32_t blocks) {
-      norm_long_kernel<S, B, RES><<<blocks, kLongThreads, 0, s>>>(*a, first);
+      norm_long_kernel<S, B, HOW><<<blocks, kLongThreads, 0, s>>>(*a, first);
     });
     return;
   }
-  with_team(a->h, [&](auto team) {
+  with_team<kVec<S>>(a->h, [&](auto team) {
     typedef decltype(team) T;
-    in_runs((a->n + T::kTeams - 1) / T::kTeams, T::kThreads, [&](int64_t first, uint32_t blocks) {
-      norm_kernel<S, B, RES, T><<<blocks, T::kThreads, 0, s>>>(*a, first);
-    });
+    if constexpr (T::WHOLE || HOW != kAdds) {
+      auto kernel = norm_kernel<S, B, HOW, false, T>;
+      if constexpr (T::WHOLE && T::L >= 64)
+        if (apart(a, HOW == kAlone ? 1 : 2, HOW == kAlone ? 1 : 2))
+          kernel = norm_kernel<S, B, HOW, true, T>;
+      kernel<<<(uint32_t)blocks_of<T>(a->n, kForwardThreads), T::kThreads, 0, s>>>(*a);
+    }
   });
 }
+
+template <typename S, typename B>
+void forward(const LumaLayerNormArgs *a, hipStream_t s) {
+  if (!a->residual)
+    forward<S, B, kAlone>(a, s);
+  else if (a->drop.p == 0.0 && a->h % kVec<S> == 0)
+    forward<S, B, kAdds>(a, s);
+  else
+    forward<S, B, kDrops>(a, s);
+}
+
+template <typename B>
+void forward_of(const LumaLayerNormArgs *a, hipStream_t s) {
+  if (std::is_same<B, float>::value || a->stream != LUMA_GRAD_F32)
+    forward<B, B>(a, s);
+  else
+    forward<float, B>(a, s);
+}
+
+template void forward_of<Elem<LUMA_UNIT - 1>::type>(const LumaLayerNormArgs *, hipStream_t);
+
+#endif  // LUMA_FORWARD
+
+#if LUMA_UNIT == 0
 
 // -- checks -----------------------------------------------------------------------
 
@@ -375,152 +517,165 @@ bool check_args(const LumaLayerNormArgs *a, bool backward) {
 
 #endif  // LUMA_UNIT == 0
 
-#if LUMA_UNIT == 1
+#if LUMA_BACKWARD
 
 // -- the backward -----------------------------------------------------------------
 
-// One row's share of the gradients in a lane's eight columns: from s and d_y,
-// z and g, and into the sums over the rows.
-struct Eight {
-  float z[8], g[8];
+// A run of a row's columns as the backward reads them.
+template <typename S, typename B, int V, bool WHOLE>
+struct GradColumns {
+  Vec<S, V> s, d_total;
+  Vec<B, V> d_y;
+
+  template <bool NT>
+  __device__ __forceinline__ void load(const LumaLayerNormArgs &a, int64_t row, int64_t c) {
+    if (a.total)
+      s = rows::load<V, WHOLE, NT>((const S *)a.total + row * a.h, c, a.h);
+    else
+      s = rows::load<V, WHOLE, NT>((const S *)a.x + row * a.ld_x, c, a.h);
+    d_y = rows::load<V, WHOLE, NT>((const B *)a.d_y + row * a.h, c, a.h);
+    if (a.d_total) d_total = rows::load<V, WHOLE, NT>((const S *)a.d_total + row * a.h, c, a.h);
+  }
+
+  // Into the row's sums of g and g z, and the columns' of d_y z and d_y.
+  __device__ __forceinline__ void sums(const float *w, float m, float r, float *dw, float *db,
+                                       float &s1, float &s2) const {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float d = (float)d_y[j], z = ((float)s[j] - m) * r, g = d * w[j];
+      s1 += g;
+      s2 = __builtin_fmaf(g, z, s2);
+      dw[j] = __builtin_fmaf(d, z, dw[j]);
+      db[j] += d;
+    }
+  }
+
+  // z and g are formed again of what was read: kept from the sums on they would
+  // take two registers an element.
+  __device__ __forceinline__ void forget() {
+    typedef uint32_t Bits __attribute__((ext_vector_type(4)));
+    static_assert(sizeof(Vec<S, V>) == 16, "16 bytes of the stream");
+    Bits b = __builtin_bit_cast(Bits, s);
+    asm("" : "+v"(b));
+    s = __builtin_bit_cast(decltype(s), b);
+  }
+
+  // d_s, and what is stored of it.
+  template <bool DROPS, bool NT>
+  __device__ __forceinline__ void store(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
+                                        int64_t c, const float *w, float m, float r, float mean_g,
+                                        float mean_gz) const {
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      const float z = ((float)s[j] - m) * r, g = (float)d_y[j] * w[j];
+      f[j] = r * (g - mean_g - z * mean_gz);
+    }
+    if (a.d_total) {
+#pragma unroll
+      for (int j = 0; j < V; ++j) f[j] += (float)d_total[j];
+    }
+    if (!a.total) {
+      rows::store<V, WHOLE, NT>((S *)a.d_x + row * a.h, c, a.h, f);
+      return;
+    }
+    if (a.d_residual) rows::store<V, WHOLE, NT>((S *)a.d_residual + row * a.h, c, a.h, f);
+    if (a.d_x) {
+      if constexpr (DROPS) {
+        if (a.drop.p > 0.0 && c < a.h) drop<V>(f, (uint64_t)(row * a.h + c), d);
+      }
+      rows::store<V, WHOLE, NT>((B *)a.d_x + row * a.h, c, a.h, f);
+    }
+  }
 };
-
-template <typename S, typename B>
-__device__ __forceinline__ void eight(const Vec<S, 8> &s, const Vec<B, 8> &dy, const float *w,
-                                      float m, float r, Eight &o, float *dw, float *db, float &s1,
-                                      float &s2) {
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float d = (float)dy[j];
-    o.z[j] = ((float)s[j] - m) * r;
-    o.g[j] = d * w[j];
-    s1 += o.g[j];
-    s2 = __builtin_fmaf(o.g[j], o.z[j], s2);
-    dw[j] = __builtin_fmaf(d, o.z[j], dw[j]);
-    db[j] += d;
-  }
-}
-
-// d_s of eight columns, and what is stored of it.
-template <typename S, typename B>
-__device__ __forceinline__ void finish(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
-                                       int64_t c, const Eight &e, const Vec<S, 8> &dt, float r,
-                                       float mean_g, float mean_gz) {
-  float f[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    f[j] = r * (e.g[j] - mean_g - e.z[j] * mean_gz);
-    if (a.d_total) f[j] += (float)dt[j];
-  }
-  if (!a.total) {
-    store<8>((S *)a.d_x + row * a.h, c, a.h, f);
-    return;
-  }
-  if (a.d_residual) store<8>((S *)a.d_residual + row * a.h, c, a.h, f);
-  if (a.d_x) {
-    if (a.drop.p > 0.0 && c < a.h) drop8(f, (uint64_t)(row * a.h + c), d);
-    store<8>((B *)a.d_x + row * a.h, c, a.h, f);
-  }
-}
 
 // A team's sums over its rows go into LDS, those of the workgroup's teams
 // together to the workspace: [block][d_weight, d_bias][h].
 template <typename T>
-__device__ __forceinline__ void put_sums(const float (&v)[T::K][8], float *lds, float *out,
+__device__ __forceinline__ void put_sums(const float (&v)[T::K][T::V], float *lds, float *out,
                                          int64_t h) {
-  constexpr int L = T::L, K = T::K, kRow = L * K * 8;
   if constexpr (T::kTeams == 1) {
 #pragma unroll
-    for (int k = 0; k < K; ++k)
-      store<8>(out, (int64_t)(k * L + threadIdx.x) * 8, h, v[k]);
+    for (int k = 0; k < T::K; ++k)
+#pragma unroll
+      for (int i = 0; i < T::V; i += 4) store<4, T::WHOLE>(out, T::column(k) + i, h, v[k] + i);
   } else {
-    const int lane = threadIdx.x % L, team = threadIdx.x / L;
+    const int team = threadIdx.x / T::L;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < K; ++k)
+    for (int k = 0; k < T::K; ++k)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) lds[team * kRow + (k * L + lane) * 8 + j] = v[k][j];
+      for (int j = 0; j < T::V; ++j) lds[team * T::kRow + T::column(k) + j] = v[k][j];
     __syncthreads();
     for (int64_t c = threadIdx.x; c < h; c += T::kThreads) {
       float sum = 0.0f;
 #pragma unroll 8
-      for (int t = 0; t < T::kTeams; ++t) sum += lds[t * kRow + c];
+      for (int t = 0; t < T::kTeams; ++t) sum += lds[t * T::kRow + c];
       out[c] = sum;
     }
   }
 }
 
-template <typename S, typename B, typename T>
+// A team goes from row to row; the next one's loads are under way while it forms
+// the sums of one (with 32 elements a lane there are no registers for
+// it, nor of cut rows, whose loads take many).
+template <typename S, typename B, bool DROPS, bool NT, typename T>
 __global__ __launch_bounds__(T::kThreads) void norm_grad_kernel(LumaLayerNormArgs a) {
-  constexpr int L = T::L, K = T::K;
+  constexpr int L = T::L, K = T::K, V = T::V;
+  constexpr bool kAhead = T::WHOLE && K * V <= 24;
   __shared__ float at[2][2][T::kThreads / 64];
-  __shared__ float lds[T::kTeams == 1 ? 1 : T::kThreads * K * 8];
-  const int lane = threadIdx.x % L, team = threadIdx.x / L;
-  const S *s = a.total ? (const S *)a.total : (const S *)a.x;
-  const int64_t ld = a.total ? a.h : a.ld_x;
-  const B *dy = (const B *)a.d_y;
+  __shared__ float lds[T::kTeams == 1 ? 1 : T::kTeams * T::kRow];
+  const int64_t step = (int64_t)gridDim.x * T::kTeams;
+  int64_t row = (int64_t)blockIdx.x * T::kTeams + threadIdx.x / L;
   const bool stores = a.d_x || a.d_residual;
   Draw d;
-  if (a.drop.p > 0.0) d = draw_of(a.drop);
+  if constexpr (DROPS) d = draw_of(a.drop);
+  GradColumns<S, B, V, T::WHOLE> now[K], next[kAhead ? K : 1];
+  float m = 0.0f, r = 0.0f, next_m = 0.0f, next_r = 0.0f;
+  auto load = [&](auto &to, int64_t of, float &to_m, float &to_r) {
+    to_m = a.stats[of];
+    to_r = a.stats[a.n + of];
+#pragma unroll
+    for (int k = 0; k < K; ++k) to[k].template load<NT>(a, of, T::column(k));
+  };
+  if constexpr (kAhead) {
+    if (row < a.n) load(next, row, next_m, next_r);
+  }
   const bool wide = a.param == LUMA_GRAD_F32;
-  float w[K][8], dw[K][8], db[K][8];
+  float w[K][V], dw[K][V], db[K][V];
 #pragma unroll
   for (int k = 0; k < K; ++k) {
-    load_param<B>(a.weight, wide, (int64_t)(k * L + lane) * 8, a.h, 1.0f, w[k]);
+    load_param<V, T::WHOLE, B>(a.weight, wide, T::column(k), a.h, 1.0f, w[k]);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) dw[k][j] = db[k][j] = 0.0f;
+    for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.0f;
   }
-  const float h = (float)a.h;
+  const float one_h = 1.0f / (float)a.h;
   int turn = 0;
   for (int64_t base = (int64_t)blockIdx.x * T::kTeams; base < a.n;
-       base += (int64_t)gridDim.x * T::kTeams) {
-    const int64_t row = base + team;
+       base += step, row += step, turn ^= 1) {
     const bool live = row < a.n;
-    Vec<S, 8> vs[K], vt[K];
-    Vec<B, 8> vd[K];
-    float m = 0.0f, r = 0.0f;
-    if (live) {
-      m = a.stats[row];
-      r = a.stats[a.n + row];
+    if constexpr (kAhead) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) now[k] = next[k];
+      m = next_m;
+      r = next_r;
+      if (row + step < a.n) load(next, row + step, next_m, next_r);
+    } else {
+      if (live) load(now, row, m, r);
     }
+    float s1 = 0.0f, s2 = 0.0f;
+    if (live) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) now[k].sums(w[k], m, r, dw[k], db[k], s1, s2);
+    }
+    if (!stores) continue;
+    // (one barrier a row: the next row's sums go to the other half)
+    team_sum2<L>(s1, s2, at[turn][0], at[turn][1]);
+    if (!live) continue;
 #pragma unroll
     for (int k = 0; k < K; ++k) {
-      const int64_t c = (int64_t)(k * L + lane) * 8;
-      const int64_t end = live ? a.h : 0;      // (a row past the last: zeros)
-      vs[k] = load<8>(s + row * ld, c, end);
-      vd[k] = load<8>(dy + row * a.h, c, end);
-      if (a.d_total) vt[k] = load<8>((const S *)a.d_total + row * a.h, c, end);
-    }
-    Eight e[K];
-    float s1 = 0.0f, s2 = 0.0f;
-#pragma unroll
-    for (int k = 0; k < K; ++k)
-      eight<S, B>(vs[k], vd[k], w[k], m, r, e[k], dw[k], db[k], s1, s2);
-    if (stores) {
-      s1 = lanes_sum<(L < 64 ? L : 64)>(s1);
-      s2 = lanes_sum<(L < 64 ? L : 64)>(s2);
-      if constexpr (L > 64) {
-        // (one barrier a row: the next row's sums go to the other half)
-        const int wave = threadIdx.x / 64;
-        if (threadIdx.x % 64 == 0) {
-          at[turn][0][wave] = s1;
-          at[turn][1][wave] = s2;
-        }
-        __syncthreads();
-        const int first = wave / (L / 64) * (L / 64);
-        s1 = s2 = 0.0f;
-#pragma unroll
-        for (int i = 0; i < L / 64; ++i) {
-          s1 += at[turn][0][first + i];
-          s2 += at[turn][1][first + i];
-        }
-        turn ^= 1;
-      }
-      if (live) {
-#pragma unroll
-        for (int k = 0; k < K; ++k)
-          finish<S, B>(a, d, row, (int64_t)(k * L + lane) * 8, e[k], vt[k], r, s1 / h, s2 / h);
-      }
+      now[k].forget();
+      now[k].template store<DROPS, NT>(a, d, row, T::column(k), w[k], m, r, s1 * one_h, s2 * one_h);
     }
   }
   float *out = (float *)a.workspace + (int64_t)blockIdx.x * 2 * a.h;
@@ -532,51 +687,49 @@ __global__ __launch_bounds__(T::kThreads) void norm_grad_kernel(LumaLayerNormArg
 template <typename S, typename B>
 __global__ __launch_bounds__(kLongThreads) void norm_long_grad_kernel(LumaLayerNormArgs a,
                                                                   int64_t block) {
-  constexpr int L = kLongThreads, kStep = L * 8;
+  constexpr int L = kLongThreads, V = kVec<S>, kStep = L * V;
   __shared__ float at[2][L / 64];
   const int64_t row = block + blockIdx.x;
-  const S *s = a.total ? (const S *)a.total + row * a.h : (const S *)a.x + row * a.ld_x;
-  const B *dy = (const B *)a.d_y + row * a.h;
   const bool wide = a.param == LUMA_GRAD_F32;
-  Draw d;
-  if (a.drop.p > 0.0) d = draw_of(a.drop);
-  const float m = a.stats[row], r = a.stats[a.n + row], h = (float)a.h;
-  float s1 = 0.0f, s2 = 0.0f, dw[8] = {}, db[8] = {};
-  auto at_column = [&](int64_t c, Eight &e) {
-    float w[8];
-    load_param<B>(a.weight, wide, c, a.h, 1.0f, w);
-    eight<S, B>(load<8>(s, c, a.h), load<8>(dy, c, a.h), w, m, r, e, dw, db, s1, s2);
-  };
-  Eight e;
-  for (int64_t c = threadIdx.x * 8; c < a.h; c += kStep) at_column(c, e);
-  s1 = team_sum<L>(s1, at[0]);
-  s2 = team_sum<L>(s2, at[1]);
-  const float mean_g = s1 / h, mean_gz = s2 / h;
-  for (int64_t c = threadIdx.x * 8; c < a.h; c += kStep) {
-    at_column(c, e);
-    Vec<S, 8> dt;
-    if (a.d_total) dt = load<8>((const S *)a.d_total + row * a.h, c, a.h);
-    finish<S, B>(a, d, row, c, e, dt, r, mean_g, mean_gz);
+  const Draw d = draw_of(a.drop);
+  const float m = a.stats[row], r = a.stats[a.n + row], one_h = 1.0f / (float)a.h;
+  float s1 = 0.0f, s2 = 0.0f, w[V], dw[V] = {}, db[V] = {};
+  GradColumns<S, B, V, false> in;
+  for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
+    load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
+    in.template load<false>(a, row, c);
+    in.sums(w, m, r, dw, db, s1, s2);
+  }
+  team_sum2<L>(s1, s2, at[0], at[1]);
+  for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
+    load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
+    in.template load<false>(a, row, c);
+    in.template store<true, false>(a, d, row, c, w, m, r, s1 * one_h, s2 * one_h);
   }
 }
 
-// Its share of d_weight and d_bias: 2,048 columns a workgroup, the rows shared
+// Its share of d_weight and d_bias: 256 lanes' columns a workgroup, the rows shared
 // out over gridDim.y.
 template <typename S, typename B>
 __global__ __launch_bounds__(256) void norm_long_sums_kernel(LumaLayerNormArgs a) {
-  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+  constexpr int V = kVec<S>;
+  const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * V;
   if (c >= a.h) return;
-  const int64_t ld = a.total ? a.h : a.ld_x;
-  const S *s = a.total ? (const S *)a.total : (const S *)a.x;
-  const float one[8] = {1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f, 1.0f};
-  float s1 = 0.0f, s2 = 0.0f, dw[8] = {}, db[8] = {};
-  Eight e;
-  for (int64_t row = blockIdx.y; row < a.n; row += gridDim.y)
-    eight<S, B>(load<8>(s + row * ld, c, a.h), load<8>((const B *)a.d_y + row * a.h, c, a.h), one,
-                a.stats[row], a.stats[a.n + row], e, dw, db, s1, s2);
+  float s1 = 0.0f, s2 = 0.0f, one[V], dw[V] = {}, db[V] = {};
+#pragma unroll
+  for (int j = 0; j < V; ++j) one[j] = 1.0f;
+  a.d_total = nullptr;
+  GradColumns<S, B, V, false> in;
+  for (int64_t row = blockIdx.y; row < a.n; row += gridDim.y) {
+    in.template load<false>(a, row, c);
+    in.sums(one, a.stats[row], a.stats[a.n + row], dw, db, s1, s2);
+  }
   float *out = (float *)a.workspace + (int64_t)blockIdx.y * 2 * a.h;
-  store<8>(out, c, a.h, dw);
-  store<8>(out + a.h, c, a.h, db);
+#pragma unroll
+  for (int i = 0; i < V; i += 4) {
+    store<4>(out, c + i, a.h, dw + i);
+    store<4>(out + a.h, c + i, a.h, db + i);
+  }
 }
 
 // d_weight and d_bias from the workgroups' sums: 32 columns a workgroup, whose 32
@@ -606,28 +759,38 @@ __global__ __launch_bounds__(kJoinCols *kJoinRows) void join_kernel(const float 
   }
 }
 
+template <typename S, typename B>
 void backward(const LumaLayerNormArgs *a, hipStream_t stream) {
-  const int64_t blocks = grad_blocks(a->n, a->h);
+  const int64_t blocks = grad_blocks(a->n, a->h, a->stream);
   const bool sums = a->d_weight || a->d_bias, stores = a->d_x || a->d_residual;
   if (!sums && !stores) return;
-  with_types(a->stream, a->branch, [&](auto s, auto b) {
-    typedef decltype(s) S;
-    typedef decltype(b) B;
-    if (a->h > kWidest) {
-      if (stores)
-        in_runs(a->n, kLongThreads, [&](int64_t first, uint32_t count) {
-          norm_long_grad_kernel<S, B><<<count, kLongThreads, 0, stream>>>(*a, first);
-        });
-      if (sums)
-        norm_long_sums_kernel<S, B><<<dim3((uint32_t)((a->h + 2047) / 2048), (uint32_t)blocks), 256,
-                                      0, stream>>>(*a);
-      return;
-    }
-    with_team(a->h, [&](auto team) {
+  if (a->h > kWidest) {
+    if (stores)
+      in_runs(a->n, kLongThreads, [&](int64_t first, uint32_t count) {
+        norm_long_grad_kernel<S, B><<<count, kLongThreads, 0, stream>>>(*a, first);
+      });
+    const int64_t each = 256 * kVec<S>;
+    if (sums)
+      norm_long_sums_kernel<S, B><<<dim3((uint32_t)((a->h + each - 1) / each), (uint32_t)blocks), 256,
+                                    0, stream>>>(*a);
+  } else {
+    // (what is read and stored of the stream's type and of the branch's)
+    const int streams = 1 + (a->d_total != nullptr) + ((a->total ? a->d_residual : a->d_x) != nullptr);
+    const bool nt = apart(a, streams, 1 + (a->total && a->d_x));
+    const bool drops = a->drop.p > 0.0 && a->d_x;
+    with_team<kVec<S>>(a->h, [&](auto team) {
       typedef decltype(team) T;
-      norm_grad_kernel<S, B, T><<<(uint32_t)blocks, T::kThreads, 0, stream>>>(*a);
+      auto kernel = norm_grad_kernel<S, B, true, false, T>;
+      if constexpr (T::WHOLE) {
+        if (!drops) kernel = norm_grad_kernel<S, B, false, false, T>;
+        if constexpr (T::L >= 64)
+          if (nt)
+            kernel = drops ? norm_grad_kernel<S, B, true, true, T>
+                           : norm_grad_kernel<S, B, false, true, T>;
+      }
+      kernel<<<(uint32_t)blocks, T::kThreads, 0, stream>>>(*a);
     });
-  });
+  }
   if (!sums) return;
   with_type(a->param, [&](auto p) {
     typedef decltype(p) P;
@@ -637,7 +800,17 @@ void backward(const LumaLayerNormArgs *a, hipStream_t stream) {
   });
 }
 
-#endif  // LUMA_UNIT == 1
+template <typename B>
+void backward_of(const LumaLayerNormArgs *a, hipStream_t s) {
+  if (std::is_same<B, float>::value || a->stream != LUMA_GRAD_F32)
+    backward<B, B>(a, s);
+  else
+    backward<float, B>(a, s);
+}
+
+template void backward_of<Elem<LUMA_UNIT - 4>::type>(const LumaLayerNormArgs *, hipStream_t);
+
+#endif  // LUMA_BACKWARD
 
 }  // namespace residual
 }  // namespace luma
@@ -675,19 +848,13 @@ int64_t luma_layer_norm_workspace_bytes(const LumaLayerNormArgs *a) {
   if (a->n < 1 || a->h < 1) return fail("luma_layer_norm: empty operands"), -1;
   if (a->n > INT32_MAX || a->h > kLargest)
     return fail("luma_layer_norm: operands too large"), -1;
-  return grad_blocks(a->n, a->h) * 2 * a->h * (int64_t)sizeof(float);
+  if (!known_type(a->stream)) return fail("luma_layer_norm: unknown type"), -1;
+  return grad_blocks(a->n, a->h, a->stream) * 2 * a->h * (int64_t)sizeof(float);
 }
 
 int luma_layer_norm_forward(const LumaLayerNormArgs *a, void *stream) {
   if (!check_args(a, false)) return -1;
-  with_types(a->stream, a->branch, [&](auto s, auto b) {
-    typedef decltype(s) S;
-    typedef decltype(b) B;
-    if (a->residual)
-      forward<S, B, true>(a, (hipStream_t)stream);
-    else
-      forward<S, B, false>(a, (hipStream_t)stream);
-  });
+  with_type(a->branch, [&](auto b) { forward_of<decltype(b)>(a, (hipStream_t)stream); });
   return check_launch("luma_layer_norm_forward");
 }
 
@@ -697,7 +864,7 @@ int luma_layer_norm_backward(const LumaLayerNormArgs *a, void *stream) {
       (!a->workspace || (uintptr_t)a->workspace % 16 ||
        a->workspace_bytes < luma_layer_norm_workspace_bytes(a)))
     return fail("luma_layer_norm_backward: workspace too small or not aligned");
-  backward(a, (hipStream_t)stream);
+  with_type(a->branch, [&](auto b) { backward_of<decltype(b)>(a, (hipStream_t)stream); });
   return check_launch("luma_layer_norm_backward");
 }
 

@@ -28,37 +28,115 @@ struct Elem<LUMA_GRAD_F16> {
   typedef _Float16 type;
 };
 
-// (element alignment only: a row may begin anywhere)
+// N elements with the alignment of one: a row may begin anywhere.  (Typedefs of
+// their own: in an alias template the attribute is lost, and the compiler then
+// takes 16-byte alignment for given.)
 template <typename T, int N>
-using Vec = T __attribute__((ext_vector_type(N), aligned(sizeof(T)), may_alias));
+struct VecOf;
+template <>
+struct VecOf<float, 4> {
+  typedef float type __attribute__((ext_vector_type(4), aligned(4), may_alias));
+};
+template <>
+struct VecOf<__bf16, 4> {
+  typedef __bf16 type __attribute__((ext_vector_type(4), aligned(2), may_alias));
+};
+template <>
+struct VecOf<__bf16, 8> {
+  typedef __bf16 type __attribute__((ext_vector_type(8), aligned(2), may_alias));
+};
+template <>
+struct VecOf<_Float16, 4> {
+  typedef _Float16 type __attribute__((ext_vector_type(4), aligned(2), may_alias));
+};
+template <>
+struct VecOf<_Float16, 8> {
+  typedef _Float16 type __attribute__((ext_vector_type(8), aligned(2), may_alias));
+};
+template <>
+struct VecOf<uint8_t, 4> {
+  typedef uint8_t type __attribute__((ext_vector_type(4), aligned(1), may_alias));
+};
+template <typename T, int N>
+using Vec = typename VecOf<T, N>::type;
 
-// N elements of a row of h from column c on; 0 past the row's end.
-template <int N, typename T>
+// N elements of a row of h from column c on; 0 past the row's end.  WHOLE: h is a
+// multiple of N, and a run lies in the row or outside.  Else the run that the end
+// cuts is read as the row's N last elements, moved down: one load, as the other
+// lanes' (a row shorter than N goes element by element).
+template <int N, bool WHOLE = false, bool NT = false, typename T>
 __device__ __forceinline__ Vec<T, N> load(const T *row, int64_t c, int64_t h) {
-  if (c + N <= h) return *(const Vec<T, N> *)(row + c);
+  static_assert(alignof(Vec<T, N>) == sizeof(T), "an element's alignment");
   Vec<T, N> v;
+  if (WHOLE ? c < h : c + N <= h) {
+    if constexpr (NT)
+      v = __builtin_nontemporal_load((const Vec<T, N> *)(row + c));
+    else
+      v = *(const Vec<T, N> *)(row + c);
+    return v;
+  }
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = c + j < h ? row[c + j] : (T)0.0f;
+  for (int j = 0; j < N; ++j) v[j] = (T)0.0f;
+  if constexpr (!WHOLE) {
+    if (c < h) {
+      if (h >= N) {
+        v = *(const Vec<T, N> *)(row + h - N);
+        for (int64_t cut = c + N - h; cut > 0; --cut) {
+#pragma unroll
+          for (int j = 0; j + 1 < N; ++j) v[j] = v[j + 1];
+          v[N - 1] = (T)0.0f;
+        }
+      } else {
+        for (int64_t at = h - 1; at >= c; --at) {
+#pragma unroll
+          for (int j = N - 1; j > 0; --j) v[j] = v[j - 1];
+          v[0] = row[at];
+        }
+      }
+    }
+  }
   return v;
 }
 
 // Rounds f to nearest and stores those of the elements that lie in the row.
-template <int N, typename T>
+template <int N, bool WHOLE = false, bool NT = false, typename T>
 __device__ __forceinline__ void store(T *row, int64_t c, int64_t h, const float *f) {
-  if (c + N <= h) {
-    Vec<T, N> v;
+  if (c >= h) return;
+  Vec<T, N> v;
 #pragma unroll
-    for (int j = 0; j < N; ++j) v[j] = (T)f[j];
-    *(Vec<T, N> *)(row + c) = v;
-    return;
+  for (int j = 0; j < N; ++j) v[j] = (T)f[j];
+  if (WHOLE || c + N <= h) {
+    if constexpr (NT)
+      __builtin_nontemporal_store(v, (Vec<T, N> *)(row + c));
+    else
+      *(Vec<T, N> *)(row + c) = v;
+  } else {
+    for (int64_t at = c; at < h; ++at) {
+      row[at] = v[0];
+#pragma unroll
+      for (int j = 0; j + 1 < N; ++j) v[j] = v[j + 1];
+    }
   }
-#pragma unroll
-  for (int j = 0; j < N; ++j)
-    if (c + j < h) row[c + j] = (T)f[j];
 }
 
-template <int N, typename T>
-__device__ __forceinline__ void widen(const Vec<T, N> &v, float *f) {
+// f - about for those of the N elements from column c on that lie in the row, 0
+// for the others.
+template <int N, bool WHOLE = false>
+__device__ __forceinline__ void differences(float *f, float about, int64_t c, int64_t h) {
+  if constexpr (WHOLE) about = c < h ? about : 0.0f;      // (past the row f is 0)
+#pragma unroll
+  for (int j = 0; j < N; ++j) f[j] -= about;
+  if constexpr (!WHOLE) {
+    if (c + N > h) {
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (c + j >= h) f[j] = 0.0f;
+    }
+  }
+}
+
+template <int N, typename V>
+__device__ __forceinline__ void widen(V v, float *f) {
 #pragma unroll
   for (int j = 0; j < N; ++j) f[j] = (float)v[j];
 }
@@ -89,33 +167,39 @@ __device__ __forceinline__ Draw draw_of(const LumaDropout &d) {
   return o;
 }
 
-// Bit j: whether element 8 block + j is kept.
+// Bit j: whether element 8 block + j is kept.  The verdicts are the signs of
+// differences of 17-bit numbers, gathered bit by bit (a select through a condition
+// takes several times a whole-number operation's time).
 __device__ __forceinline__ uint32_t kept_of_block(uint64_t block, const Draw &d) {
   const U4 top = philox4x32_10_v((uint32_t)block, (uint32_t)(block >> 32), 0u, d.call, d.k0, d.k1,
                                  kPhiloxM0, kPhiloxM1);
-  uint32_t kept = 0u, even = 0u;
+  uint32_t kept = 0u, most = 0u;
 #pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const uint32_t u = u4_half(top, j);
-    kept |= u >= d.high ? 1u << j : 0u;
-    even |= u == d.high ? 1u << j : 0u;
+  for (int j = 7; j >= 0; --j) {
+    const uint32_t off = d.high - 1u - u4_half(top, j);     // negative: kept
+    kept = __builtin_amdgcn_alignbit(kept, off, 31);        // kept << 1 | off >> 31
+    most = most > off ? most : off;                         // -1: some half is the limit's
   }
-  if (even && d.low) {
+  if (most == 0xFFFFFFFFu && d.low) {
     const U4 below = philox4x32_10_v((uint32_t)block, (uint32_t)(block >> 32), 1u, d.call, d.k0,
                                      d.k1, kPhiloxM0, kPhiloxM1);
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if ((even >> j & 1u) && u4_half(below, j) < d.low) kept &= ~(1u << j);
+      if (u4_half(top, j) == d.high && u4_half(below, j) < d.low) kept &= ~(1u << j);
   }
   return kept;
 }
 
-// Bit j: whether element e + j is kept, j < 8.
-__device__ __forceinline__ uint32_t kept_from(uint64_t e, const Draw &d) {
+// N elements from e on, kept and scaled, or 0.
+template <int N>
+__device__ __forceinline__ void drop(float *f, uint64_t e, const Draw &d) {
   const uint32_t at = (uint32_t)e & 7u;
-  uint32_t kept = kept_of_block(e >> 3, d);
-  if (at) kept = (kept | kept_of_block((e >> 3) + 1, d) << 8) >> at;
-  return kept;
+  uint32_t kept = kept_of_block(e >> 3, d) >> at;
+  if (at + N > 8) kept |= kept_of_block((e >> 3) + 1, d) << (8 - at);
+#pragma unroll
+  for (int j = 0; j < N; ++j)
+    f[j] = __uint_as_float(__float_as_uint(f[j] * d.scale) &
+                           (uint32_t)__builtin_amdgcn_sbfe((int)kept, j, 1));
 }
 
 // f(type) of an element type's code.
@@ -128,23 +212,35 @@ void with_type(int dtype, F f) {
   }
 }
 
-// f(stream's type, branch's type): the same, or a float32 stream.
-template <typename F>
-void with_types(int stream, int branch, F f) {
-  with_type(branch, [&](auto b) {
-    typedef decltype(b) B;
-    if (stream == branch) return f(B{}, B{});
-    f(float{}, B{});
-  });
-}
-
 inline bool known_type(int dtype) { return dtype >= LUMA_GRAD_F32 && dtype <= LUMA_GRAD_F16; }
 
-// Sum of v over the L lanes (a power of two, at most 64) that hold one row.
+// v of the lane that a DPP control word names (row-local exchanges in the vector
+// unit; a shuffle through LDS takes some 100 cycles, and a sum six of them).
+template <int CTRL>
+__device__ __forceinline__ float dpp(float v) {
+  return __uint_as_float(
+      __builtin_amdgcn_update_dpp(0, __float_as_uint(v), CTRL, 0xF, 0xF, true));
+}
+
+// Sum of v over the L lanes (a power of two, at most 64) that hold one row, in
+// each of them: pairs and quads, halves of a row of 16 mirrored, the row
+// mirrored, then rows and halves of the wavefront exchanged.
 template <int L>
 __device__ __forceinline__ float lanes_sum(float v) {
-#pragma unroll
-  for (int m = 1; m < L; m <<= 1) v += __shfl_xor(v, m);
+  if constexpr (L >= 2) v += dpp<0xB1>(v);
+  if constexpr (L >= 4) v += dpp<0x4E>(v);
+  if constexpr (L >= 8) v += dpp<0x141>(v);
+  if constexpr (L >= 16) v += dpp<0x140>(v);
+  if constexpr (L >= 32) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  if constexpr (L >= 64) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
+                                                    false);
+    v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
   return v;
 }
 
