@@ -598,9 +598,10 @@ typedef struct LumaPolicyArgs {
   float *loss;            /* forward: device [rows][length] dense, or [1]          */
   float *stats;           /* forward: device [LUMA_POLICY_STATS]: the share of the
                              tokens whose ratio was clipped, the means of exp(q) - 1
-                             - q and of r - 1 - log r, the number of tokens        */
+                             - q and of r - 1 - log r, the number of tokens; or NULL */
   float *share;           /* device [rows + 1]: each row's and the whole's factor of a
-                             mean; the forward writes it, the backward reads it    */
+                             mean; the forward writes it (or NULL: there will be no
+                             backward), the backward reads it                      */
   const float *grad_loss; /* backward: device [rows][length] dense, or [1]         */
   void *d_logp;           /* backward: device [rows][length] dense                 */
   void *workspace;        /* forward: device, 16-byte aligned                      */

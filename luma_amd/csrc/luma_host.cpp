@@ -1176,7 +1176,7 @@ LumaPolicyArgs policy_args(const at::Tensor &logp, const at::Tensor &old,
   a.clip_low = low;
   a.clip_high = high;
   a.kl_weight = kl;
-  a.share = share.mutable_data_ptr<float>();
+  a.share = share.defined() ? share.mutable_data_ptr<float>() : nullptr;
   return a;
 }
 
@@ -1184,18 +1184,19 @@ struct Policy : torch::autograd::Function<Policy> {
   static Variables forward(Context *ctx, const at::Tensor &logp, const at::Tensor &old,
                            const at::Tensor &advantage, const MaybeTensor &mask,
                            const MaybeTensor &ref, double low, double high, double kl,
-                           int64_t reduction) {
+                           int64_t reduction, bool keep, bool figures) {
     const auto f32 = logp.options().dtype(at::kFloat);
     const int64_t rows = logp.numel() / logp.size(logp.dim() - 1);
     at::Tensor loss = reduction == LUMA_XENT_NONE ? at::empty(logp.sizes(), f32)
                                                   : at::empty({}, f32);
-    at::Tensor stats = at::empty({LUMA_POLICY_STATS}, f32);
-    const at::Tensor share = at::empty({rows + 1}, f32);
+    at::Tensor stats, share;
+    if (figures) stats = at::empty({LUMA_POLICY_STATS}, f32);
+    if (keep) share = at::empty({rows + 1}, f32);
     PolicyRows r;
     LumaPolicyArgs a = policy_args(logp, old, advantage, value(mask), value(ref), share, low, high,
                                    kl, reduction, r);
     a.loss = loss.mutable_data_ptr<float>();
-    a.stats = stats.mutable_data_ptr<float>();
+    a.stats = figures ? stats.mutable_data_ptr<float>() : nullptr;
     const c10::DeviceGuard guard(logp.device());
     const int64_t bytes = g_more.policy_workspace(&a);
     TORCH_CHECK(bytes >= 0, g_lib.error());
@@ -1206,13 +1207,16 @@ struct Policy : torch::autograd::Function<Policy> {
       a.workspace_bytes = bytes;
     }
     run(g_more.policy_forward(&a, current_stream(logp.device().index())));
-    ctx->save_for_backward({logp, old, advantage, value(mask), value(ref), share});
-    ctx->saved_data["low"] = low;
-    ctx->saved_data["high"] = high;
-    ctx->saved_data["kl"] = kl;
-    ctx->saved_data["reduction"] = reduction;
-    ctx->mark_non_differentiable({stats});
+    if (keep) {
+      ctx->save_for_backward({logp, old, advantage, value(mask), value(ref), share});
+      ctx->saved_data["low"] = low;
+      ctx->saved_data["high"] = high;
+      ctx->saved_data["kl"] = kl;
+      ctx->saved_data["reduction"] = reduction;
+    }
     ctx->set_materialize_grads(false);
+    if (!figures) return {loss};
+    ctx->mark_non_differentiable({stats});
     return {loss, stats};
   }
 
@@ -1250,15 +1254,15 @@ struct Policy : torch::autograd::Function<Policy> {
       once({&d_logp}, "policy_loss", logp, grads[0]);
     }
     return {d_logp, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor(), at::Tensor(), at::Tensor()};
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
-// policy_loss of plain tensors: the loss and its figures; None where its arguments do
+// policy_loss of plain tensors: the loss, or with its figures; None where its arguments do
 // not fit (the caller then says which) and for no tokens.
 py::object policy_loss(const at::Tensor &logp, const at::Tensor &old, const at::Tensor &advantage,
                        const MaybeTensor &mask, const MaybeTensor &ref, double low, double high,
-                       double kl, int64_t reduction) {
+                       double kl, int64_t reduction, bool figures) {
   const int64_t d = logp.dim();
   if (!g_more.policy_forward || !logp.is_cuda() || logp.layout() != at::kStrided || d < 1 ||
       logp.numel() == 0 || grad_code(logp.scalar_type()) < 0 || !same_place(old, logp) ||
@@ -1273,10 +1277,13 @@ py::object policy_loss(const at::Tensor &logp, const at::Tensor &old, const at::
   if (given(ref) && (!same_place(*ref, logp) || ref->scalar_type() != logp.scalar_type() ||
                      ref->sizes() != logp.sizes()))
     return py::none();
-  const Variables out = Policy::apply(logp, old.detach(), advantage.detach(), mask,
-                                      given(ref) ? MaybeTensor(ref->detach()) : ref, low, high, kl,
-                                      reduction);
-  return py::make_tuple(out[0], out[1]);
+  // (what requires a gradient and gets none stays out of the graph)
+  auto constant = [](const at::Tensor &t) { return t.requires_grad() ? t.detach() : t; };
+  const bool keep = at::GradMode::is_enabled() && logp.requires_grad();
+  const Variables out = Policy::apply(logp, constant(old), constant(advantage), mask,
+                                      given(ref) ? MaybeTensor(constant(*ref)) : ref, low, high, kl,
+                                      reduction, keep, figures);
+  return figures ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
 }
 
 PYBIND11_MODULE(_luma_host, m) {

@@ -31,7 +31,13 @@ constexpr int64_t kBlocks = 2048;                 // workgroups, about
 struct Part {
   double value;        // of the values; of whole rows' means for the mean of sequences
   double kl, moved;    // of exp(q) - 1 - q, of r - 1 - log r
-  int64_t count, clipped, sequences;
+  double count, clipped, sequences;      // (whole numbers)
+};
+
+// A wavefront's: the first three differ from lane to lane, the counts do not.
+struct Sums {
+  double value = 0.0, kl = 0.0, moved = 0.0;
+  int64_t count = 0, clipped = 0, sequences = 0;
 };
 
 // How a call is shared out.
@@ -162,70 +168,66 @@ struct Tokens {
   }
 };
 
-__device__ __forceinline__ double wave_sum(double v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor(v, m);
-  return v;
-}
-
-__device__ __forceinline__ int64_t wave_sum(int64_t v) {
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) v += __shfl_xor((long long)v, m);
-  return v;
-}
-
-// Tokens first, first + step, ... of a row before end, into p (a lane's own sums).
-template <typename T>
+// Tokens base + 4 lane of a row, base from `first` in steps of `step` (those of a
+// wavefront) to before `end`, into s.  FIGURES: with what only a log wants.
+template <typename T, bool FIGURES>
 __device__ __forceinline__ void row_sums(const LumaPolicyArgs &a, const Limits &lim, int64_t row,
-                                         int64_t first, int64_t step, int64_t end, Part &p) {
+                                         int64_t first, int64_t step, int64_t end, Sums &s) {
   const Row<T> r(a, row);
+  const int64_t lane = threadIdx.x % 64 * kTokens;
   float *out = a.reduction == LUMA_XENT_NONE ? a.loss + row * a.length : nullptr;
-  for (int64_t t = first; t < end; t += step) {
-    Tokens<T> in;
-    in.load(r, t, end);
+  Tokens<T> next;
+  if (first < end) next.load(r, first + lane, end);
+  for (int64_t base = first; base < end; base += step) {
+    const Tokens<T> in = next;
+    if (base + step < end) next.load(r, base + step + lane, end);
     float v[kTokens];
 #pragma unroll
     for (int j = 0; j < kTokens; ++j) {
       const Token k = in.at(r, j, lim);
       const bool keep = in.keep >> j & 1u;
       v[j] = keep ? k.value : 0.0f;
-      p.value += (double)v[j];
-      p.kl += keep ? (double)k.kl : 0.0;
-      p.moved += keep ? (double)k.moved : 0.0;
-      p.count += keep;
-      p.clipped += keep && k.clipped;
+      s.value += (double)v[j];
+      s.count += __builtin_popcountll(__ballot(keep));
+      if constexpr (FIGURES) {
+        s.kl += (double)(keep ? k.kl : 0.0f);
+        s.moved += (double)(keep ? k.moved : 0.0f);
+        s.clipped += __builtin_popcountll(__ballot(keep && k.clipped));
+      }
     }
-    if (out) store<kTokens>(out, t, end, v);
+    if (out) store<kTokens>(out, base + lane, end, v);
   }
 }
 
-// The sums of all the wavefronts' lanes, in every thread of the first.
-template <int W>
-__device__ __forceinline__ Part block_sum(Part p, Part *lds) {
-  p.value = wave_sum(p.value);
-  p.kl = wave_sum(p.kl);
-  p.moved = wave_sum(p.moved);
-  p.count = wave_sum(p.count);
-  p.clipped = wave_sum(p.clipped);
-  p.sequences = wave_sum(p.sequences);
-  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = p;
+// The sums of W wavefronts, in the lanes of the first (W a power of two from 4 to 16).
+template <int W, bool FIGURES>
+__device__ __forceinline__ Part block_sum(Sums s, Part *lds) {
+  s.value = lanes_sum<64>(s.value);
+  if constexpr (FIGURES) {
+    s.kl = lanes_sum<64>(s.kl);
+    s.moved = lanes_sum<64>(s.moved);
+  }
+  if (threadIdx.x % 64 == 0)
+    lds[threadIdx.x / 64] = Part{s.value,         s.kl,
+                                 s.moved,         (double)s.count,
+                                 (double)s.clipped, (double)s.sequences};
   __syncthreads();
-  Part sum = lds[0];
-  if (threadIdx.x < 64)
-    for (int i = 1; i < W; ++i) {
-      sum.value += lds[i].value;
-      sum.kl += lds[i].kl;
-      sum.moved += lds[i].moved;
-      sum.count += lds[i].count;
-      sum.clipped += lds[i].clipped;
-      sum.sequences += lds[i].sequences;
-    }
-  return sum;
+  Part p = lds[threadIdx.x % W];
+  p.value = lanes_sum<W>(p.value);
+  p.count = lanes_sum<W>(p.count);
+  p.sequences = lanes_sum<W>(p.sequences);
+  if constexpr (FIGURES) {
+    p.kl = lanes_sum<W>(p.kl);
+    p.moved = lanes_sum<W>(p.moved);
+    p.clipped = lanes_sum<W>(p.clipped);
+  }
+  return p;
 }
 
 // The loss and what goes with it, by one thread.
+template <bool FIGURES>
 __device__ __forceinline__ void finish(const LumaPolicyArgs &a, const Part &p) {
-  const double n = (double)p.count, s = (double)p.sequences;
+  const double n = p.count, s = p.sequences;
   if (a.reduction == LUMA_XENT_SUM) *a.loss = (float)p.value;
   if (a.reduction == LUMA_XENT_MEAN) *a.loss = (float)(p.value / n);
   if (a.reduction == LUMA_POLICY_SEQUENCE) *a.loss = (float)(p.value / s);
@@ -233,52 +235,56 @@ __device__ __forceinline__ void finish(const LumaPolicyArgs &a, const Part &p) {
     a.share[a.rows] = a.reduction == LUMA_XENT_MEAN          ? (float)(1.0 / n)
                       : a.reduction == LUMA_POLICY_SEQUENCE ? (float)(1.0 / s)
                                                              : 1.0f;
-  a.stats[0] = (float)((double)p.clipped / n);
-  a.stats[1] = (float)(p.kl / n);
-  a.stats[2] = (float)(p.moved / n);
-  a.stats[3] = (float)p.count;
+  if constexpr (FIGURES) {
+    a.stats[0] = (float)(p.clipped / n);
+    a.stats[1] = (float)(p.kl / n);
+    a.stats[2] = (float)(p.moved / n);
+    a.stats[3] = (float)p.count;
+  }
 }
 
 // A wavefront's whole rows; a sequence's mean is taken here.
-template <typename T>
+template <typename T, bool FIGURES>
 __device__ __forceinline__ void whole_rows(const LumaPolicyArgs &a, const Limits &lim,
-                                           int64_t first, int64_t end, Part &p) {
-  const int lane = threadIdx.x % 64;
+                                           int64_t first, int64_t end, Sums &s) {
+  const bool lead = threadIdx.x % 64 == 0;
   for (int64_t row = first; row < end; ++row) {
-    Part one = {};
-    row_sums<T>(a, lim, row, lane * kTokens, 64 * kTokens, a.length, one);
-    if (a.reduction == LUMA_POLICY_SEQUENCE) {
-      const int64_t count = wave_sum(one.count);
-      one.value = count ? one.value / (double)count : 0.0;
-      one.sequences = lane == 0 && count;
-      if (lane == 0 && a.share) a.share[row] = count ? (float)(1.0 / (double)count) : 0.0f;
+    if (a.reduction != LUMA_POLICY_SEQUENCE) {
+      row_sums<T, FIGURES>(a, lim, row, 0, 64 * kTokens, a.length, s);
+      continue;
     }
-    p.value += one.value;
-    p.kl += one.kl;
-    p.moved += one.moved;
-    p.count += one.count;
-    p.clipped += one.clipped;
-    p.sequences += one.sequences;
+    const double value = s.value;
+    const int64_t count = s.count;
+    s.value = 0.0;
+    row_sums<T, FIGURES>(a, lim, row, 0, 64 * kTokens, a.length, s);
+    const double own = (double)(s.count - count);
+    s.value = value + (own ? s.value / own : 0.0);
+    s.sequences += own != 0.0;
+    if (lead && a.share) a.share[row] = own ? (float)(1.0 / own) : 0.0f;
   }
 }
 
-template <typename T>
+template <typename T, bool FIGURES>
 __global__ __launch_bounds__(kThreads) void sums_kernel(LumaPolicyArgs a, Limits lim, Plan plan) {
   __shared__ Part lds[kWaves];
-  Part p = {};
+  Sums s;
   if (plan.shorts) {
     const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / 64) * plan.each;
     const int64_t end = first + plan.each < a.rows ? first + plan.each : a.rows;
-    whole_rows<T>(a, lim, first, end, p);
+    whole_rows<T, FIGURES>(a, lim, first, end, s);
   } else {
     const int64_t row = blockIdx.x / plan.pieces, first = blockIdx.x % plan.pieces * plan.piece;
     const int64_t end = first + plan.piece < a.length ? first + plan.piece : a.length;
-    row_sums<T>(a, lim, row, first + threadIdx.x * kTokens, kThreads * kTokens, end, p);
+    row_sums<T, FIGURES>(a, lim, row, first + threadIdx.x / 64 * (64 * kTokens),
+                         kThreads * kTokens, end, s);
   }
-  p = block_sum<kWaves>(p, lds);
+  // (each token's loss alone: nothing is summed)
+  if (!FIGURES && a.reduction == LUMA_XENT_NONE) return;
+  const Part p = block_sum<kWaves, FIGURES>(s, lds);
   if (threadIdx.x == 0) ((Part *)a.workspace)[blockIdx.x] = p;
 }
 
+template <bool FIGURES>
 __global__ __launch_bounds__(kJoinThreads) void join_kernel(LumaPolicyArgs a, Plan plan) {
   __shared__ Part lds[kJoinThreads / 64];
   const Part *part = (const Part *)a.workspace;
@@ -292,17 +298,16 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(LumaPolicyArgs a, Pl
   };
   if (!plan.shorts && a.reduction == LUMA_POLICY_SEQUENCE) {
     for (int64_t row = threadIdx.x; row < a.rows; row += kJoinThreads) {
-      double value = 0.0;
-      int64_t count = 0;
+      double value = 0.0, count = 0.0;
       for (int64_t i = 0; i < plan.pieces; ++i) {
         const Part o = part[row * plan.pieces + i];
         take(o);
         value += o.value;
         count += o.count;
       }
-      p.value += count ? value / (double)count : 0.0;
-      p.sequences += count != 0;
-      if (a.share) a.share[row] = count ? (float)(1.0 / (double)count) : 0.0f;
+      p.value += count ? value / count : 0.0;
+      p.sequences += count != 0.0;
+      if (a.share) a.share[row] = count ? (float)(1.0 / count) : 0.0f;
     }
   } else {
     for (int64_t i = threadIdx.x; i < plan.blocks; i += kJoinThreads) {
@@ -311,20 +316,30 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(LumaPolicyArgs a, Pl
       p.value += o.value;
     }
   }
-  p = block_sum<kJoinThreads / 64>(p, lds);
-  if (threadIdx.x == 0) finish(a, p);
+  // (here the counts differ from lane to lane, too)
+  double *const sums[] = {&p.value, &p.count, &p.sequences, &p.kl, &p.moved, &p.clipped};
+#pragma unroll
+  for (int i = 0; i < (FIGURES ? 6 : 3); ++i) *sums[i] = lanes_sum<64>(*sums[i]);
+  if (threadIdx.x % 64 == 0) lds[threadIdx.x / 64] = p;
+  __syncthreads();
+  if (threadIdx.x >= 64) return;
+  p = lds[threadIdx.x % (kJoinThreads / 64)];
+#pragma unroll
+  for (int i = 0; i < (FIGURES ? 6 : 3); ++i) *sums[i] = lanes_sum<kJoinThreads / 64>(*sums[i]);
+  if (threadIdx.x == 0) finish<FIGURES>(a, p);
 }
 
 // A few short rows in one launch.
-template <typename T>
+template <typename T, bool FIGURES>
 __global__ __launch_bounds__(kJoinThreads) void alone_kernel(LumaPolicyArgs a, Limits lim) {
   constexpr int W = kJoinThreads / 64;
   __shared__ Part lds[W];
-  Part p = {};
+  Sums s;
   for (int64_t row = threadIdx.x / 64; row < a.rows; row += W)
-    whole_rows<T>(a, lim, row, row + 1, p);
-  p = block_sum<W>(p, lds);
-  if (threadIdx.x == 0) finish(a, p);
+    whole_rows<T, FIGURES>(a, lim, row, row + 1, s);
+  if (!FIGURES && a.reduction == LUMA_XENT_NONE) return;
+  const Part p = block_sum<W, FIGURES>(s, lds);
+  if (threadIdx.x == 0) finish<FIGURES>(a, p);
 }
 
 template <typename T>
@@ -336,9 +351,11 @@ __device__ __forceinline__ void row_grads(const LumaPolicyArgs &a, const Limits 
   float g = 1.0f;
   if (!none) g = *a.grad_loss * a.share[a.rows];
   if (a.reduction == LUMA_POLICY_SEQUENCE) g *= a.share[row];
+  Tokens<T> next;
+  if (first < end) next.load(r, first, end);
   for (int64_t t = first; t < end; t += step) {
-    Tokens<T> in;
-    in.load(r, t, end);
+    const Tokens<T> in = next;
+    if (t + step < end) next.load(r, t + step, end);
     float o[kTokens], f[kTokens];
     if (none) {
       widen<kTokens>(load<kTokens>(each, t, end), f);
@@ -379,6 +396,11 @@ Limits limits_of(const LumaPolicyArgs *a) {
 
 bool alone(const LumaPolicyArgs *a) { return a->length <= kShort && a->rows <= kAlone; }
 
+// Whether workgroups' records are left to be joined.
+bool joins(const LumaPolicyArgs *a) {
+  return !alone(a) && (a->stats || a->reduction != LUMA_XENT_NONE);
+}
+
 bool check_args(const LumaPolicyArgs *a, bool backward) {
   if (!a) return fail("luma_policy: null arguments"), false;
   if (a->rows < 1 || a->length < 1) return fail("luma_policy: empty operands"), false;
@@ -397,7 +419,7 @@ bool check_args(const LumaPolicyArgs *a, bool backward) {
   if (a->reserved) return fail("luma_policy: reserved fields must be 0"), false;
   if (!a->logp || !a->old_logp || !a->advantage) return fail("luma_policy: null operand"), false;
   if (backward ? !a->grad_loss || !a->d_logp || (a->reduction != LUMA_XENT_NONE && !a->share)
-               : !a->loss || !a->stats)
+               : !a->loss)
     return fail("luma_policy: null operand"), false;
   if (a->rows > 1 && (a->ld_logp < 0 || a->ld_old < 0 || (a->ref_logp && a->ld_ref < 0) ||
                       a->ld_advantage < 0 || (a->mask && a->ld_mask < 0)))
@@ -415,27 +437,31 @@ extern "C" {
 
 int64_t luma_policy_workspace_bytes(const LumaPolicyArgs *a) {
   if (!check_args(a, false)) return -1;
-  return alone(a) ? 0 : plan(a).blocks * (int64_t)sizeof(Part);
+  return joins(a) ? plan(a).blocks * (int64_t)sizeof(Part) : 0;
 }
 
 int luma_policy_forward(const LumaPolicyArgs *a, void *stream) {
   if (!check_args(a, false)) return -1;
   const hipStream_t s = (hipStream_t)stream;
   const Limits lim = limits_of(a);
-  if (alone(a)) {
-    with_type(a->dtype, [&](auto t) {
-      alone_kernel<decltype(t)><<<1, kJoinThreads, 0, s>>>(*a, lim);
-    });
-    return check_launch("luma_policy_forward");
-  }
   const Plan p = plan(a);
-  if (!a->workspace || (uintptr_t)a->workspace % 16 ||
-      a->workspace_bytes < p.blocks * (int64_t)sizeof(Part))
+  if (joins(a) && (!a->workspace || (uintptr_t)a->workspace % 16 ||
+                   a->workspace_bytes < p.blocks * (int64_t)sizeof(Part)))
     return fail("luma_policy_forward: workspace too small or not aligned");
   with_type(a->dtype, [&](auto t) {
-    sums_kernel<decltype(t)><<<(uint32_t)p.blocks, kThreads, 0, s>>>(*a, lim, p);
+    typedef decltype(t) T;
+    if (alone(a)) {
+      const auto kernel = a->stats ? alone_kernel<T, true> : alone_kernel<T, false>;
+      kernel<<<1, kJoinThreads, 0, s>>>(*a, lim);
+    } else {
+      const auto kernel = a->stats ? sums_kernel<T, true> : sums_kernel<T, false>;
+      kernel<<<(uint32_t)p.blocks, kThreads, 0, s>>>(*a, lim, p);
+    }
   });
-  join_kernel<<<1, kJoinThreads, 0, s>>>(*a, p);
+  if (joins(a)) {
+    const auto kernel = a->stats ? join_kernel<true> : join_kernel<false>;
+    kernel<<<1, kJoinThreads, 0, s>>>(*a, p);
+  }
   return check_launch("luma_policy_forward");
 }
 

@@ -61,9 +61,10 @@ struct Team {
 // f(team) of the narrowest team that holds a row of h.  Lanes without elements cost
 // their instructions (8,192 x 768 in teams for 2,048 took 1.4 times as long), a
 // wavefront needs no barrier for its sums (8,192 x 768 bfloat16 backward 15.7 us
-// in teams of 64 lanes, 21.7 in 128), and of wide rows one run a lane is best
-// (16,384 x 4,096 bfloat16: 512 lanes 90 and 86 us, 256 lanes 95 and 88) as long as
-// the backward, which holds five numbers an element, has the registers.
+// in teams of 64 lanes, 21.7 in 128), and a lane of a wide row has eight elements at
+// least, for what a row costs besides (and, of float32, two runs: drop()), and as few
+// as that, for the backward's five numbers an element (16,384 x 4,096 bfloat16: 512
+// lanes 90 and 86 us, 256 lanes 95 and 88).
 template <int V, bool WHOLE, typename F>
 void with_team(int64_t h, F f) {
   const int64_t runs = (h + V - 1) / V;
@@ -73,8 +74,14 @@ void with_team(int64_t h, F f) {
   if (runs <= 64) return f(Team<64, 1, V, WHOLE>{});
   if (runs <= 128) return f(Team<64, 2, V, WHOLE>{});
   if (runs <= 192) return f(Team<64, 3, V, WHOLE>{});
-  if (runs <= 256) return f(Team<256, 1, V, WHOLE>{});
-  if (runs <= 512) return f(Team<512, 1, V, WHOLE>{});
+  if constexpr (V == 4) {
+    if (runs <= 256) return f(Team<128, 2, V, WHOLE>{});
+    if (runs <= 384) return f(Team<128, 3, V, WHOLE>{});
+    if (runs <= 512) return f(Team<256, 2, V, WHOLE>{});
+  } else {
+    if (runs <= 256) return f(Team<256, 1, V, WHOLE>{});
+    if (runs <= 512) return f(Team<512, 1, V, WHOLE>{});
+  }
   if (runs <= 768) return f(Team<256, 3, V, WHOLE>{});
   if (runs <= 1024) return f(Team<512, 2, V, WHOLE>{});
   if (runs <= 1536) return f(Team<512, 3, V, WHOLE>{});
@@ -218,18 +225,20 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(LumaDropoutArgs a
     in[u] = load<V, false, NT>(x, e, a.numel);
     if (residual) add[u] = load<V, false, NT>(residual, e, a.numel);
   }
+  float f[U][V];
+#pragma unroll
+  for (int u = 0; u < U; ++u) widen<V>(in[u], f[u]);
+  constexpr int kStep = kDropThreads * V;
+  if (draws) drop(f, first, kStep, true, d, [&](int u) { return first + u * kStep < a.numel; });
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    const int64_t e = first + u * (kDropThreads * V);
+    const int64_t e = first + u * kStep;
     if (e >= a.numel) break;
-    float f[V];
-    widen<V>(in[u], f);
-    if (draws) drop<V>(f, (uint64_t)e, d);
     if (residual) {
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = (float)add[u][j] + f[j];
+      for (int j = 0; j < V; ++j) f[u][j] = (float)add[u][j] + f[u][j];
     }
-    store<V, false, NT>(y, e, a.numel, f);
+    store<V, false, NT>(y, e, a.numel, f[u]);
   }
 }
 
@@ -256,7 +265,7 @@ void dropout(const LumaDropoutArgs *a, hipStream_t s) {
 // -- the forward ------------------------------------------------------------------
 
 // How the elements before a norm come about.
-// x, residual + x, residual + dropout(x) (or residual + x all the same)
+// x, residual + x, residual + dropout(x) (of rows with a cut run: either sum)
 constexpr int kAlone = 0, kAdds = 1, kDrops = 2;
 
 // A run of a row's columns as they are read: x, and the residual.
@@ -267,21 +276,22 @@ struct Columns {
   typename std::conditional<HOW == kAlone, char, Vec<S, V>>::type residual;
 
   __device__ __forceinline__ void load(const LumaLayerNormArgs &a, int64_t row, int64_t c) {
-    x = rows::load<V, WHOLE, NT>((const X *)a.x + row * a.ld_x, c, a.h);
+    x = load_raw<V, WHOLE, NT>((const X *)a.x + row * a.ld_x, c, a.h);
     if constexpr (HOW != kAlone)
-      residual = rows::load<V, WHOLE, NT>((const S *)a.residual + row * a.ld_residual, c, a.h);
+      residual = load_raw<V, WHOLE, NT>((const S *)a.residual + row * a.ld_residual, c, a.h);
   }
 
-  // The elements before the norm: x, or the sum (also stored).
-  __device__ __forceinline__ void elements(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
-                                           int64_t c, float *f) const {
-    widen<V>(x, f);
+  __device__ __forceinline__ void branch(const LumaLayerNormArgs &a, int64_t c, float *f) const {
+    widen<V>(settle<V, WHOLE>(x, c, a.h), f);
+  }
+
+  // f, x or what dropout has left of it, becomes the sum, which is stored.
+  __device__ __forceinline__ void sum(const LumaLayerNormArgs &a, int64_t row, int64_t c,
+                                      float *f) const {
     if constexpr (HOW != kAlone) {
-      if constexpr (HOW == kDrops) {
-        if (a.drop.p > 0.0 && c < a.h) drop<V>(f, (uint64_t)(row * a.h + c), d);
-      }
+      const Vec<S, V> r = settle<V, WHOLE>(residual, c, a.h);
 #pragma unroll
-      for (int j = 0; j < V; ++j) f[j] = (float)(S)((float)residual[j] + f[j]);
+      for (int j = 0; j < V; ++j) f[j] = (float)(S)((float)r[j] + f[j]);
       store<V, WHOLE, NT>((S *)a.total + row * a.h, c, a.h, f);
     }
   }
@@ -329,23 +339,50 @@ __global__ __launch_bounds__(T::kThreads) void norm_kernel(LumaLayerNormArgs a) 
     load_param<V, T::WHOLE, B>(a.bias, wide, T::column(k), a.h, 0.0f, b[k]);
   }
   const float one_h = 1.0f / (float)a.h;
+  // A row's results are stored while the next one is formed: whoever waits for that
+  // one's elements waits for all accesses before, and would wait for these stores
+  // (16,384 x 4,096 bfloat16 93 us, otherwise 97).  A wavefront alone has others
+  // beside it that need not wait (8,192 x 768 float32: 14.1 us, so 15.2).
+  constexpr bool kLate = L > 64;
+  Vec<B, V> y[K];
+  float m = 0.0f, r = 0.0f;
+  auto put = [&](int64_t of) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+      store<V, T::WHOLE, NT>((B *)a.y + of * a.h, T::column(k), a.h, y[k]);
+    if (a.stats && threadIdx.x % L == 0) {
+      a.stats[of] = m;
+      a.stats[a.n + of] = r;
+    }
+  };
   // (the workgroup's teams make as many turns as its first, which has the most rows)
   int turn = 0;
   for (int64_t base = (int64_t)blockIdx.x * T::kTeams; base < a.n;
        base += step, row += step, turn ^= 1) {
     const bool live = row < a.n;
     float f[K][V], sum = 0.0f;
+    if (live) {
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      if (live) {
-        next[k].elements(a, d, row, T::column(k), f[k]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < V; ++j) f[k][j] = 0.0f;
+      for (int k = 0; k < K; ++k) next[k].branch(a, T::column(k), f[k]);
+      if constexpr (HOW == kDrops) {
+        // (WHOLE teams: of a sum without draws there are others)
+        if (T::WHOLE || a.drop.p > 0.0)
+          drop(f, (uint64_t)(row * a.h + T::column(0)), L * V, a.h % 8 == 0, d,
+               [&](int k) { return T::column(k) < a.h; });
       }
 #pragma unroll
-      for (int j = 0; j < V; ++j) sum += f[k][j];      // (0 past the row)
+      for (int k = 0; k < K; ++k) {
+        next[k].sum(a, row, T::column(k), f[k]);
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum += f[k][j];      // (0 past the row)
+      }
+    } else {
+#pragma unroll
+      for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int j = 0; j < V; ++j) f[k][j] = 0.0f;
     }
+    if (kLate && row >= step) put(row - step);
     if (row + step < a.n) {
 #pragma unroll
       for (int k = 0; k < K; ++k) next[k].load(a, row + step, T::column(k));
@@ -362,21 +399,19 @@ __global__ __launch_bounds__(T::kThreads) void norm_kernel(LumaLayerNormArgs a) 
       }
     }
     team_sum2<L>(first, second, at[turn][1], at[turn][2]);
-    float off, m, r;
+    float off;
     moments(about, first, second, one_h, (float)a.eps, off, m, r);
-    if (!live) continue;
-    if (a.stats && threadIdx.x % L == 0) {
-      a.stats[row] = m;
-      a.stats[a.n + row] = r;
-    }
 #pragma unroll
     for (int k = 0; k < K; ++k) {
 #pragma unroll
       for (int j = 0; j < V; ++j)
         f[k][j] = __builtin_fmaf((f[k][j] - off) * r, w[k][j], b[k][j]);
-      store<V, T::WHOLE, NT>((B *)a.y + row * a.h, T::column(k), a.h, f[k]);
+      y[k] = rounded<B, V>(f[k]);
     }
+    if (!kLate && live) put(row);
   }
+  // (row is the one after the last turn's, whether that was there or not)
+  if (kLate && row - step < a.n) put(row - step);
 }
 
 // A row that no team holds, one workgroup each: three passes over it.
@@ -388,11 +423,14 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(LumaLayerNormAr
   Draw d;
   if constexpr (HOW == kDrops) d = draw_of(a.drop);
   const S *s = HOW == kAlone ? (const S *)a.x + row * a.ld_x : (const S *)a.total + row * a.h;
-  float f[V], sum = 0.0f;
+  float g[1][V], (&f)[V] = g[0], sum = 0.0f;
   for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
     Columns<S, B, HOW, V, false, false> in;
     in.load(a, row, c);
-    in.elements(a, d, row, c, f);
+    in.branch(a, c, f);
+    if constexpr (HOW == kDrops)
+      drop(g, (uint64_t)(row * a.h + c), 0, a.h % 8 == 0, d, [](int) { return true; });
+    in.sum(a, row, c, f);
 #pragma unroll
     for (int j = 0; j < V; ++j) sum += f[j];
   }
@@ -452,7 +490,7 @@ template <typename S, typename B>
 void forward(const LumaLayerNormArgs *a, hipStream_t s) {
   if (!a->residual)
     forward<S, B, kAlone>(a, s);
-  else if (a->drop.p == 0.0 && a->h % kVec<S> == 0)
+  else if (a->drop.p == 0.0 && (a->h % kVec<S> == 0 || a->h > kWidest))
     forward<S, B, kAdds>(a, s);
   else
     forward<S, B, kDrops>(a, s);
@@ -530,11 +568,17 @@ struct GradColumns {
   template <bool NT>
   __device__ __forceinline__ void load(const LumaLayerNormArgs &a, int64_t row, int64_t c) {
     if (a.total)
-      s = rows::load<V, WHOLE, NT>((const S *)a.total + row * a.h, c, a.h);
+      s = load_raw<V, WHOLE, NT>((const S *)a.total + row * a.h, c, a.h);
     else
-      s = rows::load<V, WHOLE, NT>((const S *)a.x + row * a.ld_x, c, a.h);
-    d_y = rows::load<V, WHOLE, NT>((const B *)a.d_y + row * a.h, c, a.h);
-    if (a.d_total) d_total = rows::load<V, WHOLE, NT>((const S *)a.d_total + row * a.h, c, a.h);
+      s = load_raw<V, WHOLE, NT>((const S *)a.x + row * a.ld_x, c, a.h);
+    d_y = load_raw<V, WHOLE, NT>((const B *)a.d_y + row * a.h, c, a.h);
+    if (a.d_total) d_total = load_raw<V, WHOLE, NT>((const S *)a.d_total + row * a.h, c, a.h);
+  }
+
+  __device__ __forceinline__ void settle(const LumaLayerNormArgs &a, int64_t c) {
+    s = rows::settle<V, WHOLE>(s, c, a.h);
+    d_y = rows::settle<V, WHOLE>(d_y, c, a.h);
+    if (a.d_total) d_total = rows::settle<V, WHOLE>(d_total, c, a.h);
   }
 
   // Into the row's sums of g and g z, and the columns' of d_y z and d_y.
@@ -553,19 +597,16 @@ struct GradColumns {
   // z and g are formed again of what was read: kept from the sums on they would
   // take two registers an element.
   __device__ __forceinline__ void forget() {
-    typedef uint32_t Bits __attribute__((ext_vector_type(4)));
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
     static_assert(sizeof(Vec<S, V>) == 16, "16 bytes of the stream");
-    Bits b = __builtin_bit_cast(Bits, s);
+    Words b = __builtin_bit_cast(Words, s);
     asm("" : "+v"(b));
     s = __builtin_bit_cast(decltype(s), b);
   }
 
-  // d_s, and what is stored of it.
-  template <bool DROPS, bool NT>
-  __device__ __forceinline__ void store(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
-                                        int64_t c, const float *w, float m, float r, float mean_g,
-                                        float mean_gz) const {
-    float f[V];
+  // d_s.
+  __device__ __forceinline__ void stream(const LumaLayerNormArgs &a, const float *w, float m,
+                                         float r, float mean_g, float mean_gz, float *f) const {
 #pragma unroll
     for (int j = 0; j < V; ++j) {
       const float z = ((float)s[j] - m) * r, g = (float)d_y[j] * w[j];
@@ -575,19 +616,37 @@ struct GradColumns {
 #pragma unroll
       for (int j = 0; j < V; ++j) f[j] += (float)d_total[j];
     }
-    if (!a.total) {
-      rows::store<V, WHOLE, NT>((S *)a.d_x + row * a.h, c, a.h, f);
-      return;
-    }
-    if (a.d_residual) rows::store<V, WHOLE, NT>((S *)a.d_residual + row * a.h, c, a.h, f);
-    if (a.d_x) {
-      if constexpr (DROPS) {
-        if (a.drop.p > 0.0 && c < a.h) drop<V>(f, (uint64_t)(row * a.h + c), d);
-      }
-      rows::store<V, WHOLE, NT>((B *)a.d_x + row * a.h, c, a.h, f);
-    }
   }
 };
+
+// f(first, how many) for pairs of K runs.
+template <int K, int K0 = 0, typename F>
+__device__ __forceinline__ void in_pairs(F f) {
+  if constexpr (K0 < K) {
+    f(std::integral_constant<int, K0>{}, std::integral_constant<int, (K0 + 1 < K ? 2 : 1)>{});
+    in_pairs<K, K0 + 2>(f);
+  }
+}
+
+// Stores K runs of d_s, and what dropout leaves of it.
+template <typename S, typename B, bool DROPS, bool WHOLE, bool NT, int K, int V, typename F>
+__device__ __forceinline__ void store_grads(const LumaLayerNormArgs &a, const Draw &d, int64_t row,
+                                            float (&f)[K][V], int64_t step, F column) {
+  if (S *to = (S *)(a.total ? a.d_residual : a.d_x)) {
+#pragma unroll
+    for (int k = 0; k < K; ++k) store<V, WHOLE, NT>(to + row * a.h, column(k), a.h, f[k]);
+  }
+  if (!a.total || !a.d_x) return;
+  if constexpr (DROPS) {
+    // (WHOLE teams: where nothing is drawn there are others)
+    if (WHOLE || a.drop.p > 0.0)
+      drop(f, (uint64_t)(row * a.h + column(0)), step, a.h % 8 == 0, d,
+           [&](int k) { return column(k) < a.h; });
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+    store<V, WHOLE, NT>((B *)a.d_x + row * a.h, column(k), a.h, f[k]);
+}
 
 // A team's sums over its rows go into LDS, those of the workgroup's teams
 // together to the workspace: [block][d_weight, d_bias][h].
@@ -618,11 +677,11 @@ __device__ __forceinline__ void put_sums(const float (&v)[T::K][T::V], float *ld
 
 // A team goes from row to row; the next one's loads are under way while it forms
 // the sums of one (with 32 elements a lane there are no registers for
-// it, nor of cut rows, whose loads take many).
+// it).
 template <typename S, typename B, bool DROPS, bool NT, typename T>
 __global__ __launch_bounds__(T::kThreads) void norm_grad_kernel(LumaLayerNormArgs a) {
   constexpr int L = T::L, K = T::K, V = T::V;
-  constexpr bool kAhead = T::WHOLE && K * V <= 24;
+  constexpr bool kAhead = K * V <= 24;
   __shared__ float at[2][2][T::kThreads / 64];
   __shared__ float lds[T::kTeams == 1 ? 1 : T::kTeams * T::kRow];
   const int64_t step = (int64_t)gridDim.x * T::kTeams;
@@ -666,17 +725,27 @@ __global__ __launch_bounds__(T::kThreads) void norm_grad_kernel(LumaLayerNormArg
     float s1 = 0.0f, s2 = 0.0f;
     if (live) {
 #pragma unroll
-      for (int k = 0; k < K; ++k) now[k].sums(w[k], m, r, dw[k], db[k], s1, s2);
+      for (int k = 0; k < K; ++k) {
+        now[k].settle(a, T::column(k));
+        now[k].sums(w[k], m, r, dw[k], db[k], s1, s2);
+      }
     }
     if (!stores) continue;
     // (one barrier a row: the next row's sums go to the other half)
     team_sum2<L>(s1, s2, at[turn][0], at[turn][1]);
     if (!live) continue;
+    // (two runs at a time: drop()'s draws are for as many, and f takes few registers)
+    in_pairs<K>([&](auto first, auto count) {
+      constexpr int K0 = decltype(first)::value, N = decltype(count)::value;
+      float f[N][V];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      now[k].forget();
-      now[k].template store<DROPS, NT>(a, d, row, T::column(k), w[k], m, r, s1 * one_h, s2 * one_h);
-    }
+      for (int k = 0; k < N; ++k) {
+        now[K0 + k].forget();
+        now[K0 + k].stream(a, w[K0 + k], m, r, s1 * one_h, s2 * one_h, f[k]);
+      }
+      store_grads<S, B, DROPS, T::WHOLE, NT>(a, d, row, f, L * V,
+                                             [](int k) { return T::column(K0 + k); });
+    });
   }
   float *out = (float *)a.workspace + (int64_t)blockIdx.x * 2 * a.h;
   if (a.d_weight) put_sums<T>(dw, lds, out, a.h);
@@ -698,13 +767,17 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_grad_kernel(LumaLayerN
   for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
     load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
     in.template load<false>(a, row, c);
+    in.settle(a, c);
     in.sums(w, m, r, dw, db, s1, s2);
   }
   team_sum2<L>(s1, s2, at[0], at[1]);
   for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
     load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
     in.template load<false>(a, row, c);
-    in.template store<true, false>(a, d, row, c, w, m, r, s1 * one_h, s2 * one_h);
+    in.settle(a, c);
+    float f[1][V];
+    in.stream(a, w, m, r, s1 * one_h, s2 * one_h, f[0]);
+    store_grads<S, B, true, false, false>(a, d, row, f, 0, [&](int) { return c; });
   }
 }
 
@@ -722,6 +795,7 @@ __global__ __launch_bounds__(256) void norm_long_sums_kernel(LumaLayerNormArgs a
   GradColumns<S, B, V, false> in;
   for (int64_t row = blockIdx.y; row < a.n; row += gridDim.y) {
     in.template load<false>(a, row, c);
+    in.settle(a, c);
     in.sums(one, a.stats[row], a.stats[a.n + row], dw, db, s1, s2);
   }
   float *out = (float *)a.workspace + (int64_t)blockIdx.y * 2 * a.h;

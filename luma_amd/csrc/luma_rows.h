@@ -60,51 +60,66 @@ struct VecOf<uint8_t, 4> {
 template <typename T, int N>
 using Vec = typename VecOf<T, N>::type;
 
-// N elements of a row of h from column c on; 0 past the row's end.  WHOLE: h is a
-// multiple of N, and a run lies in the row or outside.  Else the run that the end
-// cuts is read as the row's N last elements, moved down: one load, as the other
-// lanes' (a row shorter than N goes element by element).
+// N elements of a row of h from column c on, as one load: of a run that the row's
+// end cuts the row's N last elements, which settle() moves down when they are used
+// (so that a load can be under way meanwhile); 0 outside.  A row shorter than N is
+// read element by element, settled.  WHOLE: h is a multiple of N, and no run is cut.
 template <int N, bool WHOLE = false, bool NT = false, typename T>
-__device__ __forceinline__ Vec<T, N> load(const T *row, int64_t c, int64_t h) {
+__device__ __forceinline__ Vec<T, N> load_raw(const T *row, int64_t c, int64_t h) {
   static_assert(alignof(Vec<T, N>) == sizeof(T), "an element's alignment");
   Vec<T, N> v;
-  if (WHOLE ? c < h : c + N <= h) {
+  if (c >= h) {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = (T)0.0f;
+  } else if (WHOLE || h >= N) {
+    const T *at = row + (WHOLE || c + N <= h ? c : h - N);
     if constexpr (NT)
-      v = __builtin_nontemporal_load((const Vec<T, N> *)(row + c));
+      v = __builtin_nontemporal_load((const Vec<T, N> *)at);
     else
-      v = *(const Vec<T, N> *)(row + c);
-    return v;
-  }
+      v = *(const Vec<T, N> *)at;
+  } else {
 #pragma unroll
-  for (int j = 0; j < N; ++j) v[j] = (T)0.0f;
-  if constexpr (!WHOLE) {
-    if (c < h) {
-      if (h >= N) {
-        v = *(const Vec<T, N> *)(row + h - N);
-        for (int64_t cut = c + N - h; cut > 0; --cut) {
+    for (int j = 0; j < N; ++j) v[j] = (T)0.0f;
+    for (int64_t at = h - 1; at >= c; --at) {
 #pragma unroll
-          for (int j = 0; j + 1 < N; ++j) v[j] = v[j + 1];
-          v[N - 1] = (T)0.0f;
-        }
-      } else {
-        for (int64_t at = h - 1; at >= c; --at) {
-#pragma unroll
-          for (int j = N - 1; j > 0; --j) v[j] = v[j - 1];
-          v[0] = row[at];
-        }
-      }
+      for (int j = N - 1; j > 0; --j) v[j] = v[j - 1];
+      v[0] = row[at];
     }
   }
   return v;
 }
 
-// Rounds f to nearest and stores those of the elements that lie in the row.
+// What load_raw gave, with 0 past the row's end.
+template <int N, bool WHOLE = false, typename V>
+__device__ __forceinline__ V settle(V v, int64_t c, int64_t h) {
+  if (!WHOLE && c < h && c + N > h && h >= N) {
+    for (int64_t cut = c + N - h; cut > 0; --cut) {
+#pragma unroll
+      for (int j = 0; j + 1 < N; ++j) v[j] = v[j + 1];
+      v[N - 1] = (decltype(v[0] + v[0]))0.0f;
+    }
+  }
+  return v;
+}
+
 template <int N, bool WHOLE = false, bool NT = false, typename T>
-__device__ __forceinline__ void store(T *row, int64_t c, int64_t h, const float *f) {
-  if (c >= h) return;
+__device__ __forceinline__ Vec<T, N> load(const T *row, int64_t c, int64_t h) {
+  const Vec<T, N> v = load_raw<N, WHOLE, NT>(row, c, h);
+  return settle<N, WHOLE>(v, c, h);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ Vec<T, N> rounded(const float *f) {      // to nearest
   Vec<T, N> v;
 #pragma unroll
   for (int j = 0; j < N; ++j) v[j] = (T)f[j];
+  return v;
+}
+
+// Stores those of the elements that lie in the row.
+template <int N, bool WHOLE = false, bool NT = false, typename T>
+__device__ __forceinline__ void store(T *row, int64_t c, int64_t h, Vec<T, N> v) {
+  if (c >= h) return;
   if (WHOLE || c + N <= h) {
     if constexpr (NT)
       __builtin_nontemporal_store(v, (Vec<T, N> *)(row + c));
@@ -119,19 +134,22 @@ __device__ __forceinline__ void store(T *row, int64_t c, int64_t h, const float 
   }
 }
 
+template <int N, bool WHOLE = false, bool NT = false, typename T>
+__device__ __forceinline__ void store(T *row, int64_t c, int64_t h, const float *f) {
+  store<N, WHOLE, NT>(row, c, h, rounded<T, N>(f));
+}
+
 // f - about for those of the N elements from column c on that lie in the row, 0
 // for the others.
 template <int N, bool WHOLE = false>
 __device__ __forceinline__ void differences(float *f, float about, int64_t c, int64_t h) {
-  if constexpr (WHOLE) about = c < h ? about : 0.0f;      // (past the row f is 0)
+  if constexpr (WHOLE) about = c < h ? about : 0.0f;      // (f is 0 outside)
 #pragma unroll
   for (int j = 0; j < N; ++j) f[j] -= about;
-  if constexpr (!WHOLE) {
-    if (c + N > h) {
+  if (!WHOLE && c + N > h) {
 #pragma unroll
-      for (int j = 0; j < N; ++j)
-        if (c + j >= h) f[j] = 0.0f;
-    }
+    for (int j = 0; j < N; ++j)
+      if (c + j >= h) f[j] = 0.0f;
   }
 }
 
@@ -190,16 +208,46 @@ __device__ __forceinline__ uint32_t kept_of_block(uint64_t block, const Draw &d)
   return kept;
 }
 
-// N elements from e on, kept and scaled, or 0.
+// N elements, kept (bit j of `kept`) and scaled, or 0.
 template <int N>
-__device__ __forceinline__ void drop(float *f, uint64_t e, const Draw &d) {
-  const uint32_t at = (uint32_t)e & 7u;
-  uint32_t kept = kept_of_block(e >> 3, d) >> at;
-  if (at + N > 8) kept |= kept_of_block((e >> 3) + 1, d) << (8 - at);
+__device__ __forceinline__ void keep(float *f, uint32_t kept, float scale) {
 #pragma unroll
   for (int j = 0; j < N; ++j)
-    f[j] = __uint_as_float(__float_as_uint(f[j] * d.scale) &
+    f[j] = __uint_as_float(__float_as_uint(f[j] * scale) &
                            (uint32_t)__builtin_amdgcn_sbfe((int)kept, j, 1));
+}
+
+// Dropout of K runs of N elements a lane, run k from element e + k step on, those
+// for which inside(k).  aligned: e is a multiple of N, step of 8, and so a pair of
+// lanes with runs of four has one block: it draws two runs' blocks at a time.
+template <int K, int N, typename F>
+__device__ __forceinline__ void drop(float (&f)[K][N], uint64_t e, uint64_t step, bool aligned,
+                                     const Draw &d, F inside) {
+  if (aligned && N == 4) {
+    const bool odd = threadIdx.x & 1;
+#pragma unroll
+    for (int k = 0; k < K; k += 2) {
+      const uint64_t at = e + k * step;
+      const uint32_t own = kept_of_block((k + 1 < K && odd ? at + step : at) >> 3, d);
+      const uint32_t other = __builtin_amdgcn_update_dpp(0, own, 0xB1, 0xF, 0xF, true);
+      const uint32_t here = k + 1 < K && odd ? other : own;
+      keep<N>(f[k], odd ? here >> 4 : here, d.scale);
+      if (k + 1 < K) {
+        const uint32_t next = odd ? own >> 4 : other;
+        keep<N>(f[k + 1 < K ? k + 1 : k], next, d.scale);
+      }
+    }
+    return;
+  }
+#pragma unroll
+  for (int k = 0; k < K; ++k) {
+    if (!inside(k)) continue;
+    const uint64_t from = e + k * step;
+    const uint32_t at = (uint32_t)from & 7u;
+    uint32_t kept = kept_of_block(from >> 3, d) >> at;
+    if (!aligned && at + N > 8) kept |= kept_of_block((from >> 3) + 1, d) << (8 - at);
+    keep<N>(f[k], kept, d.scale);
+  }
 }
 
 // f(type) of an element type's code.
@@ -240,6 +288,40 @@ __device__ __forceinline__ float lanes_sum(float v) {
     const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false,
                                                     false);
     v = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+  }
+  return v;
+}
+
+// The same for the 64 lanes' float64 numbers (16 or fewer: the lanes of a row).
+template <int CTRL>
+__device__ __forceinline__ double dpp(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const uint32_t low = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, 0xF, 0xF, true);
+  const uint32_t high = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, 0xF, 0xF, true);
+  return __builtin_bit_cast(double, (uint64_t)high << 32 | low);
+}
+
+template <int L>
+__device__ __forceinline__ double lanes_sum(double v) {
+  v += dpp<0xB1>(v);
+  v += dpp<0x4E>(v);
+  if constexpr (L >= 8) v += dpp<0x141>(v);
+  if constexpr (L >= 16) v += dpp<0x140>(v);
+  auto both = [&](auto low, auto high) {
+    v = __builtin_bit_cast(double, (uint64_t)high[0] << 32 | low[0]) +
+        __builtin_bit_cast(double, (uint64_t)high[1] << 32 | low[1]);
+  };
+  if constexpr (L >= 32) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t l = (uint32_t)u, h = (uint32_t)(u >> 32);
+    both(__builtin_amdgcn_permlane16_swap(l, l, false, false),
+         __builtin_amdgcn_permlane16_swap(h, h, false, false));
+  }
+  if constexpr (L >= 64) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t l = (uint32_t)u, h = (uint32_t)(u >> 32);
+    both(__builtin_amdgcn_permlane32_swap(l, l, false, false),
+         __builtin_amdgcn_permlane32_swap(h, h, false, false));
   }
   return v;
 }

@@ -69,9 +69,9 @@ def _args(logp, old_logp, advantage, mask, ref_logp, share, clip_low, clip_high,
 @torch.library.custom_op("luma_amd::policy_loss", mutates_args=(), device_types="cuda")
 def _forward_op(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Tensor,
                 mask: Optional[torch.Tensor], ref_logp: Optional[torch.Tensor], clip_low: float,
-                clip_high: float, kl_weight: float,
-                reduction: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
-    """(the loss, its figures, the rows' shares of a mean)."""
+                clip_high: float, kl_weight: float, reduction: int,
+                figures: bool) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(the loss, its figures or nothing, the rows' shares of a mean)."""
     _check_device("policy_loss", logp=logp, old_logp=old_logp, advantage=advantage, mask=mask,
                   ref_logp=ref_logp)
     device = logp.device
@@ -83,16 +83,17 @@ def _forward_op(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
     def new(shape):
         return torch.empty(shape, dtype=torch.float32, device=device)
 
-    loss, stats, share = new(logp.shape if none else ()), new(L.POLICY_STATS), new(rows + 1)
+    loss, share = new(logp.shape if none else ()), new(rows + 1)
+    stats = new(L.POLICY_STATS if figures else 0)
     if logp.numel() == 0:
         # (a mean of nothing, as linear_cross_entropy's)
         loss.fill_(0.0 if reduction in (L.XENT_NONE, L.XENT_SUM) else float("nan"))
         stats.fill_(float("nan"))
-        stats[3] = 0.0
+        stats[3:] = 0.0
         return loss, stats, share.zero_()
     args, live = _args(logp, old_logp, advantage, mask, ref_logp, share, clip_low, clip_high,
                        kl_weight, reduction)
-    args.loss, args.stats = loss.data_ptr(), stats.data_ptr()
+    args.loss, args.stats = loss.data_ptr(), stats.data_ptr() if figures else None
     size = L.load().luma_policy_workspace_bytes(ctypes.byref(args))
     if size < 0:
         L.check(-1, "luma_policy_forward")
@@ -104,7 +105,7 @@ def _forward_op(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
 
 
 @_forward_op.register_fake
-def _(logp, old_logp, advantage, mask, ref_logp, clip_low, clip_high, kl_weight, reduction):
+def _(logp, old_logp, advantage, mask, ref_logp, clip_low, clip_high, kl_weight, reduction, figures):
     rows = 1
     for d in logp.shape[:-1]:
         rows = rows * d
@@ -112,8 +113,8 @@ def _(logp, old_logp, advantage, mask, ref_logp, clip_low, clip_high, kl_weight,
     def new(shape):
         return logp.new_empty(shape, dtype=torch.float32)
 
-    return (new(logp.shape if reduction == L.XENT_NONE else ()), new((L.POLICY_STATS,)),
-            new((rows + 1,)))
+    return (new(logp.shape if reduction == L.XENT_NONE else ()),
+            new((L.POLICY_STATS if figures else 0,)), new((rows + 1,)))
 
 
 @torch.library.custom_op("luma_amd::policy_loss_backward", mutates_args=(), device_types="cuda")
@@ -141,7 +142,7 @@ def _(grad, logp, old_logp, advantage, mask, ref_logp, share, clip_low, clip_hig
 
 def _setup(ctx, inputs, output):
     (logp, old_logp, advantage, mask, ref_logp, ctx.clip_low, ctx.clip_high, ctx.kl_weight,
-     ctx.reduction) = inputs
+     ctx.reduction, _) = inputs
     ctx.save_for_backward(logp, old_logp, advantage, mask, ref_logp, output[2])
     ctx.set_materialize_grads(False)
 
@@ -153,7 +154,7 @@ def _backward(ctx, grad, *_):
         d_logp = torch.ops.luma_amd.policy_loss_backward(
             grad, logp, old_logp, advantage, mask, ref_logp, share, ctx.clip_low, ctx.clip_high,
             ctx.kl_weight, ctx.reduction)
-    return (d_logp,) + (None,) * 8
+    return (d_logp,) + (None,) * 9
 
 
 _forward_op.register_autograd(_backward, setup_context=_setup)
@@ -201,9 +202,10 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
                                   if t is not None)):
         host = L.host_calls()
         out = None if host is None else host.policy_loss(logp, old_logp, advantage, mask, ref_logp,
-                                                         clip_low, clip_high, kl_weight, code)
+                                                         clip_low, clip_high, kl_weight, code,
+                                                         return_stats)
         if out is not None:
-            return out if return_stats else out[0]
+            return out
     _check_args(logp, old_logp, advantage, mask, ref_logp)
     if not compiling:
         _check_device("policy_loss", logp=logp, old_logp=old_logp, advantage=advantage, mask=mask,
@@ -211,5 +213,6 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
     old_logp, advantage = old_logp.detach(), advantage.detach()
     ref_logp = None if ref_logp is None else ref_logp.detach()
     loss, stats, _ = torch.ops.luma_amd.policy_loss(logp, old_logp, advantage, mask, ref_logp,
-                                                    clip_low, clip_high, kl_weight, code)
+                                                    clip_low, clip_high, kl_weight, code,
+                                                    return_stats)
     return (loss, stats.detach()) if return_stats else loss

@@ -193,4 +193,5 @@ def test_opcheck():
     torch.library.opcheck(OPS.dropout.default, (x, r, seed, 0.2, 0, 1), test_utils=check)
     for reduction in range(4):
         torch.library.opcheck(OPS.policy_loss.default,
-                              (x, r, r, r > 0, None, 0.2, 0.2, 0.1, reduction), test_utils=check)
+                              (x, r, r, r > 0, None, 0.2, 0.2, 0.1, reduction,
+                               reduction > 1), test_utils=check)

@@ -44,7 +44,6 @@ def test_library_refuses(change, text):
 def test_library_refuses_one_way():
     lib = L.load()
     for name, change, text in (("forward", dict(loss=None), "null"),
-                               ("forward", dict(stats=None), "null"),
                                ("forward", dict(), "workspace"),
                                ("forward", dict(workspace=256, workspace_bytes=16), "workspace"),
                                ("forward", dict(workspace=264, workspace_bytes=1 << 30), "workspace"),
