@@ -20,7 +20,7 @@ namespace policy {
 using namespace rows;
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kTokens = 4;                        // of a lane at a time
+constexpr int kTokens = 4;                        // of a lane at a time (rows of fewer: 1)
 constexpr int64_t kShort = 1024;                  // tokens of a row that a wavefront takes
 constexpr int64_t kMostLong = (int64_t)1 << 22;   // longer rows
 constexpr int64_t kAlone = 32;                    // short rows that one workgroup takes
@@ -140,26 +140,36 @@ struct Row {
   }
 };
 
-template <typename T>
+template <typename T, int N>
 struct Tokens {
-  Vec<T, kTokens> l, old, ref;
-  Vec<float, kTokens> adv;
+  Vec<T, N> l, old, ref;
+  Vec<float, N> adv;
+  Vec<uint8_t, N> mask;
   uint32_t keep;       // bit j: token j counts
 
-  __device__ __forceinline__ void load(const Row<T> &r, int64_t t, int64_t end) {
+  // The loads of tokens t .. t + N - 1 of a row of `length`,
+  __device__ __forceinline__ void load(const Row<T> &r, int64_t t, int64_t length) {
+    l = load_raw<N>(r.logp, t, length);
+    old = load_raw<N>(r.old, t, length);
+    if (r.ref) ref = load_raw<N>(r.ref, t, length);
+    if (r.each) adv = load_raw<N>(r.advantage, t, length);
+    if (r.mask) mask = load_raw<N>(r.mask, t, length);
+  }
+
+  // and what is before `end`.
+  __device__ __forceinline__ void settle(const Row<T> &r, int64_t t, int64_t length, int64_t end) {
+    l = rows::settle<N>(l, t, length);
+    old = rows::settle<N>(old, t, length);
+    if (r.ref) ref = rows::settle<N>(ref, t, length);
+    if (r.each) adv = rows::settle<N>(adv, t, length);
+    const int64_t left = end - t;
+    keep = left >= N ? (1u << N) - 1u : left > 0 ? (1u << left) - 1u : 0u;
     if (r.mask) {
-      const Vec<uint8_t, kTokens> m = rows::load<kTokens>(r.mask, t, end);
-      keep = 0u;
+      mask = rows::settle<N>(mask, t, length);
 #pragma unroll
-      for (int j = 0; j < kTokens; ++j) keep |= m[j] && t + j < end ? 1u << j : 0u;
-    } else {
-      const int64_t left = end - t;
-      keep = left >= kTokens ? (1u << kTokens) - 1u : left > 0 ? (1u << left) - 1u : 0u;
+      for (int j = 0; j < N; ++j)
+        if (!mask[j]) keep &= ~(1u << j);
     }
-    l = rows::load<kTokens>(r.logp, t, end);
-    old = rows::load<kTokens>(r.old, t, end);
-    if (r.ref) ref = rows::load<kTokens>(r.ref, t, end);
-    if (r.each) adv = rows::load<kTokens>(r.advantage, t, end);
   }
 
   __device__ __forceinline__ Token at(const Row<T> &r, int j, const Limits &lim) const {
@@ -168,22 +178,23 @@ struct Tokens {
   }
 };
 
-// Tokens base + 4 lane of a row, base from `first` in steps of `step` (those of a
+// Tokens base + N lane of a row, base from `first` in steps of `step` (those of a
 // wavefront) to before `end`, into s.  FIGURES: with what only a log wants.
-template <typename T, bool FIGURES>
+template <typename T, int N, bool FIGURES>
 __device__ __forceinline__ void row_sums(const LumaPolicyArgs &a, const Limits &lim, int64_t row,
                                          int64_t first, int64_t step, int64_t end, Sums &s) {
   const Row<T> r(a, row);
-  const int64_t lane = threadIdx.x % 64 * kTokens;
+  const int64_t lane = threadIdx.x % 64 * N;
   float *out = a.reduction == LUMA_XENT_NONE ? a.loss + row * a.length : nullptr;
-  Tokens<T> next;
-  if (first < end) next.load(r, first + lane, end);
+  Tokens<T, N> next;
+  if (first < end) next.load(r, first + lane, a.length);
   for (int64_t base = first; base < end; base += step) {
-    const Tokens<T> in = next;
-    if (base + step < end) next.load(r, base + step + lane, end);
-    float v[kTokens];
+    Tokens<T, N> in = next;
+    if (base + step < end) next.load(r, base + step + lane, a.length);
+    in.settle(r, base + lane, a.length, end);
+    float v[N];
 #pragma unroll
-    for (int j = 0; j < kTokens; ++j) {
+    for (int j = 0; j < N; ++j) {
       const Token k = in.at(r, j, lim);
       const bool keep = in.keep >> j & 1u;
       v[j] = keep ? k.value : 0.0f;
@@ -195,7 +206,7 @@ __device__ __forceinline__ void row_sums(const LumaPolicyArgs &a, const Limits &
         s.clipped += __builtin_popcountll(__ballot(keep && k.clipped));
       }
     }
-    if (out) store<kTokens>(out, base + lane, end, v);
+    if (out) store<N>(out, base + lane, end, v);
   }
 }
 
@@ -244,19 +255,19 @@ __device__ __forceinline__ void finish(const LumaPolicyArgs &a, const Part &p) {
 }
 
 // A wavefront's whole rows; a sequence's mean is taken here.
-template <typename T, bool FIGURES>
+template <typename T, int N, bool FIGURES>
 __device__ __forceinline__ void whole_rows(const LumaPolicyArgs &a, const Limits &lim,
                                            int64_t first, int64_t end, Sums &s) {
   const bool lead = threadIdx.x % 64 == 0;
   for (int64_t row = first; row < end; ++row) {
     if (a.reduction != LUMA_POLICY_SEQUENCE) {
-      row_sums<T, FIGURES>(a, lim, row, 0, 64 * kTokens, a.length, s);
+      row_sums<T, N, FIGURES>(a, lim, row, 0, 64 * N, a.length, s);
       continue;
     }
     const double value = s.value;
     const int64_t count = s.count;
     s.value = 0.0;
-    row_sums<T, FIGURES>(a, lim, row, 0, 64 * kTokens, a.length, s);
+    row_sums<T, N, FIGURES>(a, lim, row, 0, 64 * N, a.length, s);
     const double own = (double)(s.count - count);
     s.value = value + (own ? s.value / own : 0.0);
     s.sequences += own != 0.0;
@@ -264,19 +275,18 @@ __device__ __forceinline__ void whole_rows(const LumaPolicyArgs &a, const Limits
   }
 }
 
-template <typename T, bool FIGURES>
+template <typename T, int N, bool FIGURES>
 __global__ __launch_bounds__(kThreads) void sums_kernel(LumaPolicyArgs a, Limits lim, Plan plan) {
   __shared__ Part lds[kWaves];
   Sums s;
   if (plan.shorts) {
     const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / 64) * plan.each;
     const int64_t end = first + plan.each < a.rows ? first + plan.each : a.rows;
-    whole_rows<T, FIGURES>(a, lim, first, end, s);
+    whole_rows<T, N, FIGURES>(a, lim, first, end, s);
   } else {
     const int64_t row = blockIdx.x / plan.pieces, first = blockIdx.x % plan.pieces * plan.piece;
     const int64_t end = first + plan.piece < a.length ? first + plan.piece : a.length;
-    row_sums<T, FIGURES>(a, lim, row, first + threadIdx.x / 64 * (64 * kTokens),
-                         kThreads * kTokens, end, s);
+    row_sums<T, N, FIGURES>(a, lim, row, first + threadIdx.x / 64 * (64 * N), kThreads * N, end, s);
   }
   // (each token's loss alone: nothing is summed)
   if (!FIGURES && a.reduction == LUMA_XENT_NONE) return;
@@ -330,19 +340,19 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(LumaPolicyArgs a, Pl
 }
 
 // A few short rows in one launch.
-template <typename T, bool FIGURES>
+template <typename T, int N, bool FIGURES>
 __global__ __launch_bounds__(kJoinThreads) void alone_kernel(LumaPolicyArgs a, Limits lim) {
   constexpr int W = kJoinThreads / 64;
   __shared__ Part lds[W];
   Sums s;
   for (int64_t row = threadIdx.x / 64; row < a.rows; row += W)
-    whole_rows<T, FIGURES>(a, lim, row, row + 1, s);
+    whole_rows<T, N, FIGURES>(a, lim, row, row + 1, s);
   if (!FIGURES && a.reduction == LUMA_XENT_NONE) return;
   const Part p = block_sum<W, FIGURES>(s, lds);
   if (threadIdx.x == 0) finish<FIGURES>(a, p);
 }
 
-template <typename T>
+template <typename T, int N>
 __device__ __forceinline__ void row_grads(const LumaPolicyArgs &a, const Limits &lim, int64_t row,
                                           int64_t first, int64_t step, int64_t end) {
   const Row<T> r(a, row);
@@ -351,37 +361,48 @@ __device__ __forceinline__ void row_grads(const LumaPolicyArgs &a, const Limits 
   float g = 1.0f;
   if (!none) g = *a.grad_loss * a.share[a.rows];
   if (a.reduction == LUMA_POLICY_SEQUENCE) g *= a.share[row];
-  Tokens<T> next;
-  if (first < end) next.load(r, first, end);
+  Tokens<T, N> next;
+  if (first < end) next.load(r, first, a.length);
   for (int64_t t = first; t < end; t += step) {
-    const Tokens<T> in = next;
-    if (t + step < end) next.load(r, t + step, end);
-    float o[kTokens], f[kTokens];
+    Tokens<T, N> in = next;
+    if (t + step < end) next.load(r, t + step, a.length);
+    float o[N], f[N];
     if (none) {
-      widen<kTokens>(load<kTokens>(each, t, end), f);
+      widen<N>(load<N>(each, t, a.length), f);
     } else {
 #pragma unroll
-      for (int j = 0; j < kTokens; ++j) f[j] = g;
+      for (int j = 0; j < N; ++j) f[j] = g;
     }
+    in.settle(r, t, a.length, end);
 #pragma unroll
-    for (int j = 0; j < kTokens; ++j)
-      o[j] = in.keep >> j & 1u ? in.at(r, j, lim).grad * f[j] : 0.0f;
-    store<kTokens>((T *)a.d_logp + row * a.length, t, end, o);
+    for (int j = 0; j < N; ++j) o[j] = in.keep >> j & 1u ? in.at(r, j, lim).grad * f[j] : 0.0f;
+    store<N>((T *)a.d_logp + row * a.length, t, end, o);
   }
 }
 
-template <typename T>
+template <typename T, int N>
 __global__ __launch_bounds__(kThreads) void grad_kernel(LumaPolicyArgs a, Limits lim, Plan plan) {
   if (plan.shorts) {
     const int64_t first = ((int64_t)blockIdx.x * kWaves + threadIdx.x / 64) * plan.each;
     const int64_t end = first + plan.each < a.rows ? first + plan.each : a.rows;
     for (int64_t row = first; row < end; ++row)
-      row_grads<T>(a, lim, row, threadIdx.x % 64 * kTokens, 64 * kTokens, a.length);
+      row_grads<T, N>(a, lim, row, threadIdx.x % 64 * N, 64 * N, a.length);
   } else {
     const int64_t row = blockIdx.x / plan.pieces, first = blockIdx.x % plan.pieces * plan.piece;
     const int64_t end = first + plan.piece < a.length ? first + plan.piece : a.length;
-    row_grads<T>(a, lim, row, first + threadIdx.x * kTokens, kThreads * kTokens, end);
+    row_grads<T, N>(a, lim, row, first + threadIdx.x * N, kThreads * N, end);
   }
+}
+
+// f(type, how many tokens a lane takes at a time).
+template <typename F>
+void with_tokens(const LumaPolicyArgs *a, F f) {
+  with_type(a->dtype, [&](auto t) {
+    if (a->length < kTokens)
+      f(t, std::integral_constant<int, 1>{});
+    else
+      f(t, std::integral_constant<int, kTokens>{});
+  });
 }
 
 Limits limits_of(const LumaPolicyArgs *a) {
@@ -448,13 +469,14 @@ int luma_policy_forward(const LumaPolicyArgs *a, void *stream) {
   if (joins(a) && (!a->workspace || (uintptr_t)a->workspace % 16 ||
                    a->workspace_bytes < p.blocks * (int64_t)sizeof(Part)))
     return fail("luma_policy_forward: workspace too small or not aligned");
-  with_type(a->dtype, [&](auto t) {
+  with_tokens(a, [&](auto t, auto tokens) {
     typedef decltype(t) T;
+    constexpr int N = decltype(tokens)::value;
     if (alone(a)) {
-      const auto kernel = a->stats ? alone_kernel<T, true> : alone_kernel<T, false>;
+      const auto kernel = a->stats ? alone_kernel<T, N, true> : alone_kernel<T, N, false>;
       kernel<<<1, kJoinThreads, 0, s>>>(*a, lim);
     } else {
-      const auto kernel = a->stats ? sums_kernel<T, true> : sums_kernel<T, false>;
+      const auto kernel = a->stats ? sums_kernel<T, N, true> : sums_kernel<T, N, false>;
       kernel<<<(uint32_t)p.blocks, kThreads, 0, s>>>(*a, lim, p);
     }
   });
@@ -468,8 +490,8 @@ int luma_policy_forward(const LumaPolicyArgs *a, void *stream) {
 int luma_policy_backward(const LumaPolicyArgs *a, void *stream) {
   if (!check_args(a, true)) return -1;
   const Plan p = plan(a);
-  with_type(a->dtype, [&](auto t) {
-    grad_kernel<decltype(t)>
+  with_tokens(a, [&](auto t, auto tokens) {
+    grad_kernel<decltype(t), decltype(tokens)::value>
         <<<(uint32_t)p.blocks, kThreads, 0, (hipStream_t)stream>>>(*a, limits_of(a), p);
   });
   return check_launch("luma_policy_backward");

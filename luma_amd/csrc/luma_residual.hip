@@ -91,7 +91,9 @@ void with_team(int64_t h, F f) {
 
 template <int V, typename F>
 void with_team(int64_t h, F f) {
-  if (h % V == 0)
+  if (h < V)      // (no run of V: an element a lane)
+    f(Team<8, 1, 1, true>{});
+  else if (h % V == 0)
     with_team<V, true>(h, f);
   else
     with_team<V, false>(h, f);
@@ -179,18 +181,55 @@ __device__ __forceinline__ void team_sum2(float &u, float &v, float *at_u, float
   }
 }
 
-// N of the weight or bias, of float32 or the branch's type.
-template <int N, bool WHOLE, typename B>
-__device__ __forceinline__ void load_param(const void *p, bool wide, int64_t c, int64_t h,
-                                           float fill, float *f) {
-  if (!p) {
+// The elements of the weight (1 without one) and the bias (0) at the columns of K
+// runs, of P; all loads go out before the first is looked at.
+template <int K, int V, bool WHOLE, typename P, typename F>
+__device__ __forceinline__ void params_of(const P *weight, const P *bias, int64_t h, F column,
+                                          float (&w)[K][V], float (&b)[K][V]) {
+  constexpr int N = V * sizeof(P) > 16 ? 4 : V, R = V / N;
+  // (without one the other is read in its place: no condition, see load_raw)
+  const P *pw = weight ? weight : bias, *pb = bias ? bias : weight;
+  Vec<P, N> raw_w[K][R], raw_b[K][R];
 #pragma unroll
-    for (int j = 0; j < N; ++j) f[j] = fill;
-  } else if (wide) {
+  for (int k = 0; k < K; ++k)
 #pragma unroll
-    for (int i = 0; i < N; i += 4) widen<4>(load<4, WHOLE>((const float *)p, c + i, h), f + i);
+    for (int i = 0; i < R; ++i) {
+      raw_w[k][i] = load_raw<N, WHOLE>(pw, column(k) + i * N, h);
+      raw_b[k][i] = load_raw<N, WHOLE>(pb, column(k) + i * N, h);
+    }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      widen<N>(settle<N, WHOLE>(raw_w[k][i], column(k) + i * N, h), w[k] + i * N);
+      widen<N>(settle<N, WHOLE>(raw_b[k][i], column(k) + i * N, h), b[k] + i * N);
+    }
+#pragma unroll
+  for (int k = 0; k < K; ++k)
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      if (!weight) w[k][j] = 1.0f;
+      if (!bias) b[k][j] = 0.0f;
+    }
+}
+
+// Of float32 or of the branch's type B.
+template <int K, int V, bool WHOLE, typename B, typename F>
+__device__ __forceinline__ void load_params(const void *weight, const void *bias, bool wide,
+                                            int64_t h, F column, float (&w)[K][V],
+                                            float (&b)[K][V]) {
+  if (!weight && !bias) {
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        w[k][j] = 1.0f;
+        b[k][j] = 0.0f;
+      }
+  } else if (std::is_same<B, float>::value || wide) {
+    params_of<K, V, WHOLE>((const float *)weight, (const float *)bias, h, column, w, b);
   } else {
-    widen<N>(load<N, WHOLE>((const B *)p, c, h), f);
+    params_of<K, V, WHOLE>((const B *)weight, (const B *)bias, h, column, w, b);
   }
 }
 
@@ -208,9 +247,8 @@ constexpr int kDropThreads = 256;
 
 // U runs a thread, a workgroup's next to each other.  A run is 16 bytes of the wider
 // type (its lanes' 8 bytes of the other are one run of memory, too).
-template <typename I, typename O, int U, bool NT>
+template <typename I, typename O, int V, int U, bool NT>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(LumaDropoutArgs a) {
-  constexpr int V = kVec<I> < kVec<O> ? kVec<I> : kVec<O>;
   const I *x = (const I *)a.x;
   const O *residual = (const O *)a.residual;
   O *y = (O *)a.y;
@@ -250,12 +288,14 @@ void dropout(const LumaDropoutArgs *a, hipStream_t s) {
   auto go = [&](auto kernel, int64_t each) {
     kernel<<<(uint32_t)((runs + each - 1) / each), kDropThreads, 0, s>>>(*a);
   };
-  if (bytes > (int64_t)256 << 20)
-    go(dropout_kernel<I, O, 4, true>, 4 * kDropThreads);
+  if (a->numel < V)      // (one workgroup, an element a lane)
+    go(dropout_kernel<I, O, 1, 1, false>, kDropThreads);
+  else if (bytes > (int64_t)256 << 20)
+    go(dropout_kernel<I, O, V, 4, true>, 4 * kDropThreads);
   else if (runs >= 256 * 1024)
-    go(dropout_kernel<I, O, 4, false>, 4 * kDropThreads);
+    go(dropout_kernel<I, O, V, 4, false>, 4 * kDropThreads);
   else
-    go(dropout_kernel<I, O, 1, false>, kDropThreads);
+    go(dropout_kernel<I, O, V, 1, false>, kDropThreads);
 }
 
 #endif  // LUMA_UNIT == 0
@@ -327,17 +367,17 @@ __global__ __launch_bounds__(T::kThreads) void norm_kernel(LumaLayerNormArgs a) 
   Draw d;
   if constexpr (HOW == kDrops) d = draw_of(a.drop);
   Columns<S, B, HOW, V, T::WHOLE, NT> next[K];
-  if (row < a.n) {
+  auto load = [&](int64_t of) {
+    // (of cut rows without a condition, see load_raw: past the last row that again)
+    if (T::WHOLE && of >= a.n) return;
+    of = of < a.n ? of : a.n - 1;
 #pragma unroll
-    for (int k = 0; k < K; ++k) next[k].load(a, row, T::column(k));
-  }
+    for (int k = 0; k < K; ++k) next[k].load(a, of, T::column(k));
+  };
+  load(row);
   float w[K][V], b[K][V];
-  const bool wide = a.param == LUMA_GRAD_F32;
-#pragma unroll
-  for (int k = 0; k < K; ++k) {
-    load_param<V, T::WHOLE, B>(a.weight, wide, T::column(k), a.h, 1.0f, w[k]);
-    load_param<V, T::WHOLE, B>(a.bias, wide, T::column(k), a.h, 0.0f, b[k]);
-  }
+  load_params<K, V, T::WHOLE, B>(a.weight, a.bias, a.param == LUMA_GRAD_F32, a.h,
+                                 [](int k) { return T::column(k); }, w, b);
   const float one_h = 1.0f / (float)a.h;
   // A row's results are stored while the next one is formed: whoever waits for that
   // one's elements waits for all accesses before, and would wait for these stores
@@ -383,10 +423,7 @@ __global__ __launch_bounds__(T::kThreads) void norm_kernel(LumaLayerNormArgs a) 
         for (int j = 0; j < V; ++j) f[k][j] = 0.0f;
     }
     if (kLate && row >= step) put(row - step);
-    if (row + step < a.n) {
-#pragma unroll
-      for (int k = 0; k < K; ++k) next[k].load(a, row + step, T::column(k));
-    }
+    load(row + step);
     const float about = team_sum<L>(sum, at[turn][0]) * one_h;
     float first = 0.0f, second = 0.0f;
 #pragma unroll
@@ -454,14 +491,13 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_kernel(LumaLayerNormAr
     a.stats[row] = m;
     a.stats[a.n + row] = r;
   }
-  const bool wide = a.param == LUMA_GRAD_F32;
   for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
-    float w[V], b[V];
-    load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
-    load_param<V, false, B>(a.bias, wide, c, a.h, 0.0f, b);
+    float w[1][V], b[1][V];
+    load_params<1, V, false, B>(a.weight, a.bias, a.param == LUMA_GRAD_F32, a.h,
+                                [&](int) { return c; }, w, b);
     widen<V>(load<V>(s, c, a.h), f);
 #pragma unroll
-    for (int j = 0; j < V; ++j) f[j] = __builtin_fmaf((f[j] - about - off) * r, w[j], b[j]);
+    for (int j = 0; j < V; ++j) f[j] = __builtin_fmaf((f[j] - about - off) * r, w[0][j], b[0][j]);
     store<V>((B *)a.y + row * a.h, c, a.h, f);
   }
 }
@@ -567,10 +603,8 @@ struct GradColumns {
 
   template <bool NT>
   __device__ __forceinline__ void load(const LumaLayerNormArgs &a, int64_t row, int64_t c) {
-    if (a.total)
-      s = load_raw<V, WHOLE, NT>((const S *)a.total + row * a.h, c, a.h);
-    else
-      s = load_raw<V, WHOLE, NT>((const S *)a.x + row * a.ld_x, c, a.h);
+    const S *from = (const S *)(a.total ? a.total : a.x) + row * (a.total ? a.h : a.ld_x);
+    s = load_raw<V, WHOLE, NT>(from, c, a.h);
     d_y = load_raw<V, WHOLE, NT>((const B *)a.d_y + row * a.h, c, a.h);
     if (a.d_total) d_total = load_raw<V, WHOLE, NT>((const S *)a.d_total + row * a.h, c, a.h);
   }
@@ -598,10 +632,11 @@ struct GradColumns {
   // take two registers an element.
   __device__ __forceinline__ void forget() {
     typedef uint32_t Words __attribute__((ext_vector_type(4)));
-    static_assert(sizeof(Vec<S, V>) == 16, "16 bytes of the stream");
-    Words b = __builtin_bit_cast(Words, s);
-    asm("" : "+v"(b));
-    s = __builtin_bit_cast(decltype(s), b);
+    if constexpr (sizeof(Words) == sizeof(s)) {
+      Words b = __builtin_bit_cast(Words, s);
+      asm("" : "+v"(b));
+      s = __builtin_bit_cast(decltype(s), b);
+    }
   }
 
   // d_s.
@@ -654,10 +689,11 @@ template <typename T>
 __device__ __forceinline__ void put_sums(const float (&v)[T::K][T::V], float *lds, float *out,
                                          int64_t h) {
   if constexpr (T::kTeams == 1) {
+    constexpr int N = T::V < 4 ? T::V : 4;
 #pragma unroll
     for (int k = 0; k < T::K; ++k)
 #pragma unroll
-      for (int i = 0; i < T::V; i += 4) store<4, T::WHOLE>(out, T::column(k) + i, h, v[k] + i);
+      for (int i = 0; i < T::V; i += N) store<N, T::WHOLE>(out, T::column(k) + i, h, v[k] + i);
   } else {
     const int team = threadIdx.x / T::L;
     __syncthreads();
@@ -692,22 +728,22 @@ __global__ __launch_bounds__(T::kThreads) void norm_grad_kernel(LumaLayerNormArg
   GradColumns<S, B, V, T::WHOLE> now[K], next[kAhead ? K : 1];
   float m = 0.0f, r = 0.0f, next_m = 0.0f, next_r = 0.0f;
   auto load = [&](auto &to, int64_t of, float &to_m, float &to_r) {
+    // (of cut rows without a condition, see load_raw: past the last row that again)
+    if (T::WHOLE && of >= a.n) return;
+    of = of < a.n ? of : a.n - 1;
     to_m = a.stats[of];
     to_r = a.stats[a.n + of];
 #pragma unroll
     for (int k = 0; k < K; ++k) to[k].template load<NT>(a, of, T::column(k));
   };
-  if constexpr (kAhead) {
-    if (row < a.n) load(next, row, next_m, next_r);
-  }
-  const bool wide = a.param == LUMA_GRAD_F32;
+  if constexpr (kAhead) load(next, row, next_m, next_r);
   float w[K][V], dw[K][V], db[K][V];
+  load_params<K, V, T::WHOLE, B>(a.weight, nullptr, a.param == LUMA_GRAD_F32, a.h,
+                                 [](int k) { return T::column(k); }, w, dw);
 #pragma unroll
-  for (int k = 0; k < K; ++k) {
-    load_param<V, T::WHOLE, B>(a.weight, wide, T::column(k), a.h, 1.0f, w[k]);
+  for (int k = 0; k < K; ++k)
 #pragma unroll
     for (int j = 0; j < V; ++j) dw[k][j] = db[k][j] = 0.0f;
-  }
   const float one_h = 1.0f / (float)a.h;
   int turn = 0;
   for (int64_t base = (int64_t)blockIdx.x * T::kTeams; base < a.n;
@@ -718,9 +754,9 @@ __global__ __launch_bounds__(T::kThreads) void norm_grad_kernel(LumaLayerNormArg
       for (int k = 0; k < K; ++k) now[k] = next[k];
       m = next_m;
       r = next_r;
-      if (row + step < a.n) load(next, row + step, next_m, next_r);
+      load(next, row + step, next_m, next_r);
     } else {
-      if (live) load(now, row, m, r);
+      load(now, row, m, r);
     }
     float s1 = 0.0f, s2 = 0.0f;
     if (live) {
@@ -759,24 +795,27 @@ __global__ __launch_bounds__(kLongThreads) void norm_long_grad_kernel(LumaLayerN
   constexpr int L = kLongThreads, V = kVec<S>, kStep = L * V;
   __shared__ float at[2][L / 64];
   const int64_t row = block + blockIdx.x;
-  const bool wide = a.param == LUMA_GRAD_F32;
   const Draw d = draw_of(a.drop);
   const float m = a.stats[row], r = a.stats[a.n + row], one_h = 1.0f / (float)a.h;
-  float s1 = 0.0f, s2 = 0.0f, w[V], dw[V] = {}, db[V] = {};
+  float s1 = 0.0f, s2 = 0.0f, w[1][V], none[1][V], dw[V] = {}, db[V] = {};
   GradColumns<S, B, V, false> in;
+  auto weights = [&](int64_t c) {
+    load_params<1, V, false, B>(a.weight, nullptr, a.param == LUMA_GRAD_F32, a.h,
+                                [&](int) { return c; }, w, none);
+  };
   for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
-    load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
+    weights(c);
     in.template load<false>(a, row, c);
     in.settle(a, c);
-    in.sums(w, m, r, dw, db, s1, s2);
+    in.sums(w[0], m, r, dw, db, s1, s2);
   }
   team_sum2<L>(s1, s2, at[0], at[1]);
   for (int64_t c = threadIdx.x * V; c < a.h; c += kStep) {
-    load_param<V, false, B>(a.weight, wide, c, a.h, 1.0f, w);
+    weights(c);
     in.template load<false>(a, row, c);
     in.settle(a, c);
     float f[1][V];
-    in.stream(a, w, m, r, s1 * one_h, s2 * one_h, f[0]);
+    in.stream(a, w[0], m, r, s1 * one_h, s2 * one_h, f[0]);
     store_grads<S, B, true, false, false>(a, d, row, f, 0, [&](int) { return c; });
   }
 }
