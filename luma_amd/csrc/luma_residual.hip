@@ -583,6 +583,8 @@ bool check_args(const LumaLayerNormArgs *a, bool backward) {
   } else {
     if (!(adds ? a->total : a->x) || !a->d_y || !a->stats)
       return fail("luma_layer_norm: null operand"), false;
+    if (!adds && a->n > 1 && a->ld_x < 0)
+      return fail("luma_layer_norm: rows lie backwards"), false;
     if (!adds && (a->d_total || a->d_residual))
       return fail("luma_layer_norm: gradients of a sum without one"), false;
   }

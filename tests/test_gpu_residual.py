@@ -130,7 +130,7 @@ def test_widths(h, dtype):
 
 
 @pytest.mark.parametrize("n", [1, 2, 3, 31, 33, 255, 256, 257, 4097, 100001])
-@pytest.mark.parametrize("h", [24, 300])
+@pytest.mark.parametrize("h", [3, 24, 300])
 def test_rows(n, h):
     _check_norm(_randn((n, h), 1), _randn((h,), 2) + 1, _randn((h,), 4), torch.float32)
 
@@ -283,6 +283,25 @@ def test_one_call_is_the_two(dtype, h):
         assert torch.equal(p, q) or dtype != torch.float32
         assert bool(((p.double() - q.double()).abs() <= 2 * UNIT[dtype] * q.double().abs()
                      + TINY[dtype]).all())
+
+
+@pytest.mark.parametrize("p", [0.0, 0.5])
+def test_a_branch_that_is_its_residual(p):
+    """Both gradients go to one leaf (without draws they are one tensor)."""
+    x = _randn((12, 40), 1).requires_grad_()
+    a, b = (x.detach().clone().requires_grad_() for _ in range(2))
+    g, t = _randn((12, 40), 2), _randn((12, 40), 3)
+    d, = torch.autograd.grad(add_layer_norm(x, x, p=p, seed=1), x, (g, t))
+    d_a, d_b = torch.autograd.grad(add_layer_norm(a, b, p=p, seed=1), (a, b), (g, t))
+    assert torch.equal(d, d_a + d_b)
+    (add_layer_norm(x, x, p=p, seed=1)[0] * g).sum().backward()
+    add_layer_norm(a, b, p=p, seed=1)[0].backward(g)
+    assert torch.equal(x.grad, a.grad + b.grad)
+    if p == 0.0:
+        assert a.grad.data_ptr() != b.grad.data_ptr()
+    d, = torch.autograd.grad(dropout(x, p, 1, residual=x), x, g)
+    d_a, d_b = torch.autograd.grad(dropout(a, p, 1, residual=b), (a, b), g)
+    assert torch.equal(d, d_a + d_b)
 
 
 def test_unused_results():
@@ -447,6 +466,20 @@ def test_mutated_operands():
         x.add_(1.0)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         y.sum().backward()
+
+
+def test_mutated_results():
+    """The sum is what the backward reads: a program that writes to it is told so."""
+    x, res = _randn((8, 32), 1).requires_grad_(), _randn((8, 32), 2)
+    y, total = add_layer_norm(x, res, p=0.5, seed=1)
+    total.add_(1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    z = dropout(x, 0.5, 1)
+    z.mul_(2.0)                                   # (nothing of it is kept)
+    keep = residual_util.kept((8, 32), 0.5, 1, 0).cuda()
+    d, = torch.autograd.grad(z.sum(), x)
+    assert torch.equal(d, keep * 4.0)
 
 
 def test_another_stream():

@@ -174,6 +174,19 @@ def test_compile(dynamic):
             assert p is None or float((p - q).norm()) <= 1e-5 * float(q.norm())
 
 
+def test_compile_with_seeds():
+    """A seed as a number that changes from call to call, and one on the device."""
+    @torch.compile(fullgraph=True)
+    def f(x, r, seed):
+        return add_layer_norm(dropout(x, 0.3, seed, 1), r, p=0.4, seed=seed, call=2)[0]
+
+    x, r, _, _ = (t.detach() for t in _inputs(9))
+    for seed in (3, 4, -5, (1 << 63) - 1):
+        want = add_layer_norm(dropout(x, 0.3, seed, 1), r, p=0.4, seed=seed, call=2)[0]
+        assert torch.equal(f(x, r, seed), want)
+        assert torch.equal(f(x, r, torch.tensor(seed, device="cuda")), want)
+
+
 @pytest.mark.parametrize("name", CALLS)
 def test_functional_transforms_are_refused(name):
     """torch.func does not see through the operators' gradients: it says so."""

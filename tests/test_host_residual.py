@@ -45,6 +45,7 @@ def test_norm_refuses(change, text):
     ("forward", dict(residual=256), "null"), ("forward", dict(ld_x=-64), "backwards"),
     ("forward", dict(residual=256, total=256, ld_residual=-1), "backwards"),
     ("backward", dict(x=None), "null"), ("backward", dict(d_y=None), "null"),
+    ("backward", dict(ld_x=-64), "backwards"),
     ("backward", dict(stats=None), "null"), ("backward", dict(d_total=256), "without"),
     ("backward", dict(d_residual=256), "without"), ("backward", dict(), "workspace"),
     ("backward", dict(workspace=256, workspace_bytes=16), "workspace"),
