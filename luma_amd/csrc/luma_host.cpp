@@ -898,13 +898,18 @@ auto op_of(const char *name) {
   return c10::Dispatcher::singleton().findSchemaOrThrow(name, "").typed<F>();
 }
 
+at::Tensor dropped(const at::Tensor &x, const MaybeTensor &residual, const Draws &d) {
+  const at::Tensor &like = given(residual) ? *residual : x;
+  at::Tensor y = at::empty(x.sizes(), like.options());
+  dropout_call(dense(x), given(residual) ? dense(*residual) : at::Tensor(), y, d);
+  return y;
+}
+
 struct Dropout : torch::autograd::Function<Dropout> {
   static at::Tensor forward(Context *ctx, const at::Tensor &x, const MaybeTensor &residual,
                             const MaybeTensor &seed_at, double p, int64_t seed, int64_t call) {
     const Draws d{value(seed_at), p, seed, call};
-    const at::Tensor like = given(residual) ? *residual : x;
-    at::Tensor y = at::empty(x.sizes(), like.options());
-    dropout_call(dense(x), given(residual) ? dense(*residual) : at::Tensor(), y, d);
+    const at::Tensor y = dropped(x, residual, d);
     ctx->save_for_backward({d.seed_at});
     ctx->saved_data["p"] = p;
     ctx->saved_data["seed"] = seed;
@@ -941,6 +946,17 @@ struct Dropout : torch::autograd::Function<Dropout> {
   }
 };
 
+// Whether a call of these (some may be null) is one that autograd records, or, of
+// tensors with a tangent, refuses.
+bool differentiable(std::initializer_list<const at::Tensor *> tensors) {
+  const bool grad = at::GradMode::is_enabled();
+  for (const at::Tensor *t : tensors)
+    if (t && ((grad && t->requires_grad()) || t->_fw_grad(0).defined())) return true;
+  return false;
+}
+
+const at::Tensor *pointer(const MaybeTensor &t) { return given(t) ? &*t : nullptr; }
+
 bool same_place(const at::Tensor &t, const at::Tensor &like) {
   return t.layout() == at::kStrided && t.device() == like.device();
 }
@@ -962,6 +978,8 @@ py::object dropout(const at::Tensor &x, const MaybeTensor &residual, const Maybe
                           (residual->scalar_type() != x.scalar_type() &&
                            residual->scalar_type() != at::kFloat)))
     return py::none();
+  if (!differentiable({&x, pointer(residual)}))
+    return py::cast(dropped(x, residual, {value(seed_at), p, seed, call}));
   return py::cast(Dropout::apply(x, residual, seed_at, p, seed, call));
 }
 
@@ -979,57 +997,68 @@ LumaLayerNormArgs norm_args(int64_t n, int64_t h, int64_t stream, int64_t branch
   return a;
 }
 
+// y and, with a residual, the sum; (keep) each row's mean and 1 / deviation.
+struct Normed {
+  at::Tensor y, total, stats;
+};
+
+int64_t param_code(const MaybeTensor &weight, const MaybeTensor &bias) {
+  return given(weight) ? grad_code(weight->scalar_type())
+         : given(bias) ? grad_code(bias->scalar_type())
+                       : LUMA_GRAD_F32;
+}
+
+Normed normed(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight,
+              const MaybeTensor &bias, double eps, const Draws &d, int64_t branch, bool keep) {
+  const bool adds = given(residual);
+  const at::Tensor &like = adds ? *residual : x;
+  const int64_t h = x.size(x.dim() - 1), n = x.numel() / h;
+  LumaLayerNormArgs a = norm_args(n, h, grad_code(like.scalar_type()), branch,
+                                  param_code(weight, bias), eps, d);
+  const at::Tensor xs = as_rows(x), rs = adds ? as_rows(*residual) : at::Tensor();
+  const at::Tensor w = given(weight) ? dense(*weight) : at::Tensor();
+  const at::Tensor b = given(bias) ? dense(*bias) : at::Tensor();
+  Normed o;
+  o.y = at::empty(x.sizes(), x.options().dtype(kTypes[branch]));
+  a.x = xs.const_data_ptr();
+  a.ld_x = ld_of(xs);
+  if (adds) {
+    o.total = at::empty(x.sizes(), like.options());
+    a.residual = rs.const_data_ptr();
+    a.ld_residual = ld_of(rs);
+    a.total = o.total.mutable_data_ptr();
+  }
+  a.weight = w.defined() ? w.const_data_ptr() : nullptr;
+  a.bias = b.defined() ? b.const_data_ptr() : nullptr;
+  a.y = o.y.mutable_data_ptr();
+  if (keep) {
+    o.stats = at::empty({2 * n}, x.options().dtype(at::kFloat));
+    a.stats = o.stats.mutable_data_ptr<float>();
+  }
+  const c10::DeviceGuard guard(x.device());
+  run(g_more.norm_forward(&a, current_stream(x.device().index())));
+  return o;
+}
+
 struct LayerNorm : torch::autograd::Function<LayerNorm> {
   // y, or y and the sum.
   static Variables forward(Context *ctx, const at::Tensor &x, const MaybeTensor &residual,
                            const MaybeTensor &weight, const MaybeTensor &bias,
                            const MaybeTensor &seed_at, double eps, double p, int64_t seed,
-                           int64_t call, int64_t branch, bool keep) {
+                           int64_t call, int64_t branch) {
     const bool adds = given(residual);
     const Draws d{value(seed_at), p, seed, call};
-    const at::Tensor &like = adds ? *residual : x;
-    const int64_t h = x.size(x.dim() - 1), n = x.numel() / h;
-    const int64_t stream = grad_code(like.scalar_type());
-    const int64_t param = given(weight) ? grad_code(weight->scalar_type())
-                          : given(bias) ? grad_code(bias->scalar_type())
-                                        : LUMA_GRAD_F32;
-    LumaLayerNormArgs a = norm_args(n, h, stream, branch, param, eps, d);
-    const at::Tensor xs = as_rows(x), rs = adds ? as_rows(*residual) : at::Tensor();
-    const at::Tensor w = given(weight) ? dense(*weight) : at::Tensor();
-    const at::Tensor b = given(bias) ? dense(*bias) : at::Tensor();
-    at::Tensor y = at::empty(x.sizes(), x.options().dtype(kTypes[branch]));
-    at::Tensor total, stats;
-    a.x = xs.const_data_ptr();
-    a.ld_x = ld_of(xs);
-    if (adds) {
-      total = at::empty(x.sizes(), like.options());
-      a.residual = rs.const_data_ptr();
-      a.ld_residual = ld_of(rs);
-      a.total = total.mutable_data_ptr();
-    }
-    a.weight = w.defined() ? w.const_data_ptr() : nullptr;
-    a.bias = b.defined() ? b.const_data_ptr() : nullptr;
-    a.y = y.mutable_data_ptr();
-    if (keep) {
-      stats = at::empty({2 * n}, x.options().dtype(at::kFloat));
-      a.stats = stats.mutable_data_ptr<float>();
-    }
-    {
-      const c10::DeviceGuard guard(x.device());
-      run(g_more.norm_forward(&a, current_stream(x.device().index())));
-    }
-    if (keep) {
-      ctx->save_for_backward({adds ? total : x, value(weight), stats, d.seed_at});
-      ctx->saved_data["p"] = p;
-      ctx->saved_data["seed"] = seed;
-      ctx->saved_data["call"] = call;
-      ctx->saved_data["branch"] = branch;
-      ctx->saved_data["param"] = param;
-      // (which inputs there are: a gradient's number counts those alone)
-      ctx->saved_data["inputs"] = (int64_t)(1 | adds << 1 | given(weight) << 2 | given(bias) << 3);
-    }
+    const Normed o = normed(x, residual, weight, bias, eps, d, branch, true);
+    ctx->save_for_backward({adds ? o.total : x, value(weight), o.stats, d.seed_at});
+    ctx->saved_data["p"] = p;
+    ctx->saved_data["seed"] = seed;
+    ctx->saved_data["call"] = call;
+    ctx->saved_data["branch"] = branch;
+    ctx->saved_data["param"] = param_code(weight, bias);
+    // (which inputs there are: a gradient's number counts those alone)
+    ctx->saved_data["inputs"] = (int64_t)(1 | adds << 1 | given(weight) << 2 | given(bias) << 3);
     ctx->set_materialize_grads(false);
-    return adds ? Variables{y, total} : Variables{y};
+    return adds ? Variables{o.y, o.total} : Variables{o.y};
   }
 
   static Variables backward(Context *ctx, Variables grads) {
@@ -1104,7 +1133,7 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     once({&out[0], &out[1], &out[2], &out[3]}, adds ? "add_layer_norm" : "layer_norm", s, weight,
          grads[0], adds ? grads[1] : at::Tensor());
     return {out[0], out[1], out[2], out[3], at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor(), at::Tensor(), at::Tensor()};
+            at::Tensor(), at::Tensor()};
   }
 };
 
@@ -1133,12 +1162,13 @@ py::object layer_norm(const at::Tensor &x, const MaybeTensor &residual, const Ma
           (given(weight) && given(bias) && weight->scalar_type() != bias->scalar_type()))
         return py::none();
     }
-  const bool keep = at::GradMode::is_enabled() &&
-                    (x.requires_grad() || like.requires_grad() ||
-                     (given(weight) && weight->requires_grad()) ||
-                     (given(bias) && bias->requires_grad()));
+  if (!differentiable({&x, &like, pointer(weight), pointer(bias)})) {
+    const Normed o = normed(x, residual, weight, bias, eps, {value(seed_at), p, seed, call}, branch,
+                            false);
+    return adds ? py::object(py::make_tuple(o.y, o.total)) : py::cast(o.y);
+  }
   const Variables out = LayerNorm::apply(x, residual, weight, bias, seed_at, eps, p, seed, call,
-                                         branch, keep);
+                                         branch);
   return adds ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
 }
 
@@ -1180,44 +1210,54 @@ LumaPolicyArgs policy_args(const at::Tensor &logp, const at::Tensor &old,
   return a;
 }
 
+// The loss, (figures) its figures, (keep) the rows' shares of a mean.
+struct PolicyLoss {
+  at::Tensor loss, stats, share;
+};
+
+PolicyLoss policy_of(const at::Tensor &logp, const at::Tensor &old, const at::Tensor &advantage,
+                     const MaybeTensor &mask, const MaybeTensor &ref, double low, double high,
+                     double kl, int64_t reduction, bool keep, bool figures) {
+  const auto f32 = logp.options().dtype(at::kFloat);
+  const int64_t rows = logp.numel() / logp.size(logp.dim() - 1);
+  PolicyLoss o;
+  o.loss = reduction == LUMA_XENT_NONE ? at::empty(logp.sizes(), f32) : at::empty({}, f32);
+  if (figures) o.stats = at::empty({LUMA_POLICY_STATS}, f32);
+  if (keep) o.share = at::empty({rows + 1}, f32);
+  PolicyRows r;
+  LumaPolicyArgs a = policy_args(logp, old, advantage, value(mask), value(ref), o.share, low, high,
+                                 kl, reduction, r);
+  a.loss = o.loss.mutable_data_ptr<float>();
+  a.stats = figures ? o.stats.mutable_data_ptr<float>() : nullptr;
+  const c10::DeviceGuard guard(logp.device());
+  const int64_t bytes = g_more.policy_workspace(&a);
+  TORCH_CHECK(bytes >= 0, g_lib.error());
+  at::Tensor workspace;
+  if (bytes) {
+    workspace = at::empty({bytes}, logp.options().dtype(at::kByte));
+    a.workspace = workspace.mutable_data_ptr();
+    a.workspace_bytes = bytes;
+  }
+  run(g_more.policy_forward(&a, current_stream(logp.device().index())));
+  return o;
+}
+
 struct Policy : torch::autograd::Function<Policy> {
   static Variables forward(Context *ctx, const at::Tensor &logp, const at::Tensor &old,
                            const at::Tensor &advantage, const MaybeTensor &mask,
                            const MaybeTensor &ref, double low, double high, double kl,
-                           int64_t reduction, bool keep, bool figures) {
-    const auto f32 = logp.options().dtype(at::kFloat);
-    const int64_t rows = logp.numel() / logp.size(logp.dim() - 1);
-    at::Tensor loss = reduction == LUMA_XENT_NONE ? at::empty(logp.sizes(), f32)
-                                                  : at::empty({}, f32);
-    at::Tensor stats, share;
-    if (figures) stats = at::empty({LUMA_POLICY_STATS}, f32);
-    if (keep) share = at::empty({rows + 1}, f32);
-    PolicyRows r;
-    LumaPolicyArgs a = policy_args(logp, old, advantage, value(mask), value(ref), share, low, high,
-                                   kl, reduction, r);
-    a.loss = loss.mutable_data_ptr<float>();
-    a.stats = figures ? stats.mutable_data_ptr<float>() : nullptr;
-    const c10::DeviceGuard guard(logp.device());
-    const int64_t bytes = g_more.policy_workspace(&a);
-    TORCH_CHECK(bytes >= 0, g_lib.error());
-    at::Tensor workspace;
-    if (bytes) {
-      workspace = at::empty({bytes}, logp.options().dtype(at::kByte));
-      a.workspace = workspace.mutable_data_ptr();
-      a.workspace_bytes = bytes;
-    }
-    run(g_more.policy_forward(&a, current_stream(logp.device().index())));
-    if (keep) {
-      ctx->save_for_backward({logp, old, advantage, value(mask), value(ref), share});
-      ctx->saved_data["low"] = low;
-      ctx->saved_data["high"] = high;
-      ctx->saved_data["kl"] = kl;
-      ctx->saved_data["reduction"] = reduction;
-    }
+                           int64_t reduction, bool figures) {
+    const PolicyLoss o = policy_of(logp, old, advantage, mask, ref, low, high, kl, reduction, true,
+                                   figures);
+    ctx->save_for_backward({logp, old, advantage, value(mask), value(ref), o.share});
+    ctx->saved_data["low"] = low;
+    ctx->saved_data["high"] = high;
+    ctx->saved_data["kl"] = kl;
+    ctx->saved_data["reduction"] = reduction;
     ctx->set_materialize_grads(false);
-    if (!figures) return {loss};
-    ctx->mark_non_differentiable({stats});
-    return {loss, stats};
+    if (!figures) return {o.loss};
+    ctx->mark_non_differentiable({o.stats});
+    return {o.loss, o.stats};
   }
 
   static Variables backward(Context *ctx, Variables grads) {
@@ -1254,7 +1294,7 @@ struct Policy : torch::autograd::Function<Policy> {
       once({&d_logp}, "policy_loss", logp, grads[0]);
     }
     return {d_logp, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(),
-            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
 
@@ -1277,12 +1317,16 @@ py::object policy_loss(const at::Tensor &logp, const at::Tensor &old, const at::
   if (given(ref) && (!same_place(*ref, logp) || ref->scalar_type() != logp.scalar_type() ||
                      ref->sizes() != logp.sizes()))
     return py::none();
+  if (!differentiable({&logp, &old, &advantage, pointer(ref)})) {
+    const PolicyLoss o = policy_of(logp, old, advantage, mask, ref, low, high, kl, reduction, false,
+                                   figures);
+    return figures ? py::object(py::make_tuple(o.loss, o.stats)) : py::cast(o.loss);
+  }
   // (what requires a gradient and gets none stays out of the graph)
   auto constant = [](const at::Tensor &t) { return t.requires_grad() ? t.detach() : t; };
-  const bool keep = at::GradMode::is_enabled() && logp.requires_grad();
   const Variables out = Policy::apply(logp, constant(old), constant(advantage), mask,
                                       given(ref) ? MaybeTensor(constant(*ref)) : ref, low, high, kl,
-                                      reduction, keep, figures);
+                                      reduction, figures);
   return figures ? py::object(py::make_tuple(out[0], out[1])) : py::cast(out[0]);
 }
 

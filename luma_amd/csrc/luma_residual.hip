@@ -243,12 +243,18 @@ void backward_of(const LumaLayerNormArgs *a, hipStream_t s);
 
 // -- dropout ----------------------------------------------------------------------
 
-constexpr int kDropThreads = 256;
+constexpr int kDropThreads = 256, kDropRuns = 2;
+constexpr int64_t kL2Bytes = (int64_t)32 << 20;      // of all XCDs
 
-// U runs a thread, a workgroup's next to each other.  A run is 16 bytes of the wider
-// type (its lanes' 8 bytes of the other are one run of memory, too).
-template <typename I, typename O, int V, int U, bool NT>
+// Two runs a thread, a workgroup's next to each other: a pair of lanes has one
+// draw for each of float32's runs, and two are under way at a time (100M bfloat16,
+// 403 MB: one run 88 us, two 64, four 65, eight 70; 4.1M onto a residual 6.0, 6.0,
+// 6.8, 10).  A run is 16 bytes of the wider type (its lanes' 8 bytes of the other are
+// one run of memory, too).  What the L2 caches do not hold goes past them (100M
+// bfloat16 64 us, cached 74; 8 MB the same).
+template <typename I, typename O, int V, bool NT>
 __global__ __launch_bounds__(kDropThreads) void dropout_kernel(LumaDropoutArgs a) {
+  constexpr int U = kDropRuns;
   const I *x = (const I *)a.x;
   const O *residual = (const O *)a.residual;
   O *y = (O *)a.y;
@@ -283,19 +289,13 @@ __global__ __launch_bounds__(kDropThreads) void dropout_kernel(LumaDropoutArgs a
 template <typename I, typename O>
 void dropout(const LumaDropoutArgs *a, hipStream_t s) {
   constexpr int V = kVec<I> < kVec<O> ? kVec<I> : kVec<O>;
-  const int64_t runs = (a->numel + V - 1) / V;
   const int64_t bytes = a->numel * (int64_t)(sizeof(I) + sizeof(O) * (a->residual ? 2 : 1));
-  auto go = [&](auto kernel, int64_t each) {
-    kernel<<<(uint32_t)((runs + each - 1) / each), kDropThreads, 0, s>>>(*a);
-  };
-  if (a->numel < V)      // (one workgroup, an element a lane)
-    go(dropout_kernel<I, O, 1, 1, false>, kDropThreads);
-  else if (bytes > (int64_t)256 << 20)
-    go(dropout_kernel<I, O, V, 4, true>, 4 * kDropThreads);
-  else if (runs >= 256 * 1024)
-    go(dropout_kernel<I, O, V, 4, false>, 4 * kDropThreads);
-  else
-    go(dropout_kernel<I, O, V, 1, false>, kDropThreads);
+  const int64_t each = (int64_t)kDropThreads * kDropRuns * V;
+  // (fewer elements than a run has: one workgroup, an element a lane)
+  const auto kernel = a->numel < V       ? dropout_kernel<I, O, 1, false>
+                      : bytes > kL2Bytes ? dropout_kernel<I, O, V, true>
+                                         : dropout_kernel<I, O, V, false>;
+  kernel<<<(uint32_t)((a->numel + each - 1) / each), kDropThreads, 0, s>>>(*a);
 }
 
 #endif  // LUMA_UNIT == 0

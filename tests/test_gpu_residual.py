@@ -5,14 +5,14 @@ of a result's type: 2^-24, 2^-8 for bfloat16, 2^-11 for float16, whose smallest
 step adds 2^-25).
 
 * A lane adds the elements of a row that it holds one after the other, at most
-  q = 16 of them (8 ceil(h / 8192) past 16,384), the lanes' sums go up a tree of
+  q = 32 of them (8 ceil(h / 8192) past 16,384), the lanes' sums go up a tree of
   six, and at most 16 wavefronts' sums follow each other: a sum of positive terms
   is within (q + 22) e of itself, any sum within (q + 22) e of the terms' sizes.
 * So, relative to the deviation, the mean of the differences is within
   (q + 22) e, the deviation within (q + 22) e / 2 + 4 e, an element's difference
   within 2 e |z| + e: z is within ez = (q + 26) e (1 + |z|) (1 + k)^2, where
   k = (q + 22) e |m| r is how far the first mean, about which the differences are
-  taken, can be off (in deviations: 1 is reached where a row stands 4e5 of them
+  taken, can be off (in deviations: 1 is reached where a row stands 3e5 of them
   from 0).  The backward reads the mean rounded to float32, which adds e |m| r.
 * y = z w + b: |w| ez + 2 e (|z w| + |y|) + u |y|.
 * d_s = r (g - mean(g) - z mean(g z)) + d_total: r (4 e (|g| + |mean(g)| +
@@ -67,7 +67,7 @@ class Exact:
         s = s.detach().double()
         wd = torch.ones(h, dtype=torch.float64, device="cuda") if w is None else w.detach().double()
         bd = torch.zeros_like(wd) if b is None else b.detach().double()
-        q = 16 if h <= 16384 else 8 * -(-h // 8192)
+        q = 32 if h <= 16384 else 8 * -(-h // 8192)
         m = s.mean(1, keepdim=True)
         r = ((s - m).square().mean(1, keepdim=True) + eps).rsqrt()
         z = (s - m) * r

@@ -196,6 +196,18 @@ def test_functional_transforms_are_refused(name):
         torch.func.grad(lambda *a: call(*a).float().sum())(*plain)
 
 
+@pytest.mark.parametrize("grad", [True, False])
+@pytest.mark.parametrize("name", CALLS)
+def test_forward_mode_is_refused(name, grad):
+    """A tangent is not lost without a word."""
+    call, _ = CALLS[name]
+    plain = [t.detach() for t in _inputs(7)]
+    with torch.autograd.forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        dual = torch.autograd.forward_ad.make_dual(plain[0], torch.ones_like(plain[0]))
+        with pytest.raises(RuntimeError, match="jvp|forward AD|forward-mode"):
+            call(dual, *plain[1:])
+
+
 def test_opcheck():
     x, r, w, b = _inputs(8)
     seed = torch.tensor(3, device="cuda")
