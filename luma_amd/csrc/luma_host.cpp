@@ -811,6 +811,11 @@ at::Tensor value(const MaybeTensor &t) { return given(t) ? *t : at::Tensor(); }
 
 MaybeTensor maybe(const at::Tensor &t) { return t.defined() ? MaybeTensor(t) : std::nullopt; }
 
+// A tensor beside `like`, its memory not set.
+at::Tensor fresh(at::IntArrayRef sizes, at::ScalarType type, const at::Tensor &like) {
+  return at::empty(sizes, like.options().dtype(type));
+}
+
 // Whether a tracer or another mode watches the operators that are called.
 bool watched() {
   return c10::impl::dispatch_mode_enabled() ||
@@ -878,6 +883,7 @@ struct Draws {
   }
 };
 
+// (with x's device the current one)
 void dropout_call(const at::Tensor &x, const at::Tensor &residual, const at::Tensor &y,
                   const Draws &d) {
   LumaDropoutArgs a{};
@@ -888,7 +894,6 @@ void dropout_call(const at::Tensor &x, const at::Tensor &residual, const at::Ten
   a.in = grad_code(x.scalar_type());
   a.out = grad_code(y.scalar_type());
   a.drop = d.args();
-  const c10::DeviceGuard guard(x.device());
   run(g_more.dropout(&a, current_stream(x.device().index())));
 }
 
@@ -899,8 +904,9 @@ auto op_of(const char *name) {
 }
 
 at::Tensor dropped(const at::Tensor &x, const MaybeTensor &residual, const Draws &d) {
+  const c10::DeviceGuard guard(x.device());
   const at::Tensor &like = given(residual) ? *residual : x;
-  at::Tensor y = at::empty(x.sizes(), like.options());
+  at::Tensor y = fresh(x.sizes(), like.scalar_type(), x);
   dropout_call(dense(x), given(residual) ? dense(*residual) : at::Tensor(), y, d);
   return y;
 }
@@ -912,31 +918,31 @@ struct Dropout : torch::autograd::Function<Dropout> {
     const at::Tensor y = dropped(x, residual, d);
     ctx->save_for_backward({d.seed_at});
     ctx->saved_data["p"] = p;
-    ctx->saved_data["seed"] = seed;
-    ctx->saved_data["call"] = call;
-    ctx->saved_data["code"] = (int64_t)grad_code(x.scalar_type());
-    ctx->saved_data["residual"] = given(residual);
+    ctx->saved_data["numbers"] =
+        std::vector<int64_t>{seed, call, grad_code(x.scalar_type()), given(residual)};
     ctx->set_materialize_grads(false);
     return y;
   }
 
   static Variables backward(Context *ctx, Variables grads) {
-    const bool residual = ctx->saved_data["residual"].toBool();
+    const auto numbers = ctx->saved_data["numbers"].toIntVector();
+    const bool residual = numbers[3];
     at::Tensor d_x, d_residual;
     if (grads[0].defined()) {
       if (residual && ctx->needs_input_grad(1)) d_residual = grads[0];
       if (ctx->needs_input_grad(0)) {
         at::AutoDispatchBelowADInplaceOrView below;
-        const Draws d{ctx->get_saved_variables()[0], ctx->saved_data["p"].toDouble(),
-                      ctx->saved_data["seed"].toInt(), ctx->saved_data["call"].toInt()};
-        const int64_t code = ctx->saved_data["code"].toInt();
+        const Draws d{ctx->get_saved_variables()[0], ctx->saved_data["p"].toDouble(), numbers[0],
+                      numbers[1]};
+        const int64_t code = numbers[2];
         if (watched()) {
           static const auto op =
               op_of<at::Tensor(const at::Tensor &, const MaybeTensor &, double, int64_t, int64_t,
                                int64_t)>("luma_amd::dropout_backward");
           d_x = op.call(grads[0], maybe(d.seed_at), d.p, d.seed, d.call, code);
         } else {
-          d_x = at::empty(grads[0].sizes(), grads[0].options().dtype(kTypes[code]));
+          const c10::DeviceGuard guard(grads[0].device());
+          d_x = fresh(grads[0].sizes(), kTypes[code], grads[0]);
           dropout_call(dense(grads[0]), at::Tensor(), d_x, d);
         }
       }
@@ -1010,6 +1016,7 @@ int64_t param_code(const MaybeTensor &weight, const MaybeTensor &bias) {
 
 Normed normed(const at::Tensor &x, const MaybeTensor &residual, const MaybeTensor &weight,
               const MaybeTensor &bias, double eps, const Draws &d, int64_t branch, bool keep) {
+  const c10::DeviceGuard guard(x.device());
   const bool adds = given(residual);
   const at::Tensor &like = adds ? *residual : x;
   const int64_t h = x.size(x.dim() - 1), n = x.numel() / h;
@@ -1019,11 +1026,11 @@ Normed normed(const at::Tensor &x, const MaybeTensor &residual, const MaybeTenso
   const at::Tensor w = given(weight) ? dense(*weight) : at::Tensor();
   const at::Tensor b = given(bias) ? dense(*bias) : at::Tensor();
   Normed o;
-  o.y = at::empty(x.sizes(), x.options().dtype(kTypes[branch]));
+  o.y = fresh(x.sizes(), kTypes[branch], x);
   a.x = xs.const_data_ptr();
   a.ld_x = ld_of(xs);
   if (adds) {
-    o.total = at::empty(x.sizes(), like.options());
+    o.total = fresh(x.sizes(), like.scalar_type(), x);
     a.residual = rs.const_data_ptr();
     a.ld_residual = ld_of(rs);
     a.total = o.total.mutable_data_ptr();
@@ -1032,10 +1039,9 @@ Normed normed(const at::Tensor &x, const MaybeTensor &residual, const MaybeTenso
   a.bias = b.defined() ? b.const_data_ptr() : nullptr;
   a.y = o.y.mutable_data_ptr();
   if (keep) {
-    o.stats = at::empty({2 * n}, x.options().dtype(at::kFloat));
+    o.stats = fresh({2 * n}, at::kFloat, x);
     a.stats = o.stats.mutable_data_ptr<float>();
   }
-  const c10::DeviceGuard guard(x.device());
   run(g_more.norm_forward(&a, current_stream(x.device().index())));
   return o;
 }
@@ -1051,12 +1057,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
     const Normed o = normed(x, residual, weight, bias, eps, d, branch, true);
     ctx->save_for_backward({adds ? o.total : x, value(weight), o.stats, d.seed_at});
     ctx->saved_data["p"] = p;
-    ctx->saved_data["seed"] = seed;
-    ctx->saved_data["call"] = call;
-    ctx->saved_data["branch"] = branch;
-    ctx->saved_data["param"] = param_code(weight, bias);
-    // (which inputs there are: a gradient's number counts those alone)
-    ctx->saved_data["inputs"] = (int64_t)(1 | adds << 1 | given(weight) << 2 | given(bias) << 3);
+    // (last which inputs there are: a gradient's number counts those alone)
+    ctx->saved_data["numbers"] =
+        std::vector<int64_t>{seed, call, branch, param_code(weight, bias),
+                             1 | adds << 1 | given(weight) << 2 | given(bias) << 3};
     ctx->set_materialize_grads(false);
     return adds ? Variables{o.y, o.total} : Variables{o.y};
   }
@@ -1064,11 +1068,9 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
   static Variables backward(Context *ctx, Variables grads) {
     const auto saved = ctx->get_saved_variables();
     const at::Tensor &s = saved[0], &weight = saved[1], &stats = saved[2];
-    const Draws d{saved[3], ctx->saved_data["p"].toDouble(), ctx->saved_data["seed"].toInt(),
-                  ctx->saved_data["call"].toInt()};
-    const int64_t branch = ctx->saved_data["branch"].toInt();
-    const int64_t param = ctx->saved_data["param"].toInt();
-    const int64_t inputs = ctx->saved_data["inputs"].toInt();
+    const auto numbers = ctx->saved_data["numbers"].toIntVector();
+    const Draws d{saved[3], ctx->saved_data["p"].toDouble(), numbers[0], numbers[1]};
+    const int64_t branch = numbers[2], param = numbers[3], inputs = numbers[4];
     const bool adds = inputs >> 1 & 1;
     bool want[4];
     for (int i = 0, edge = 0; i < 4; ++i)
@@ -1100,13 +1102,11 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         const at::Tensor ss = as_rows(s), dy = dense(d_y.to(kTypes[branch]));
         const at::Tensor w = weight.defined() ? dense(weight) : at::Tensor();
         const at::Tensor dt = d_total.defined() ? dense(d_total.to(s.scalar_type())) : at::Tensor();
-        auto new_like = [&](at::IntArrayRef sizes, int64_t code) {
-          return at::empty(sizes, s.options().dtype(kTypes[code]));
-        };
-        if (want_x) out[0] = new_like(s.sizes(), adds ? branch : stream);
-        if (want_r) out[1] = new_like(s.sizes(), stream);
-        if (want[2]) out[2] = new_like({h}, param);
-        if (want[3]) out[3] = new_like({h}, param);
+        const c10::DeviceGuard guard(s.device());
+        if (want_x) out[0] = fresh(s.sizes(), kTypes[adds ? branch : stream], s);
+        if (want_r) out[1] = fresh(s.sizes(), kTypes[stream], s);
+        if (want[2]) out[2] = fresh({h}, kTypes[param], s);
+        if (want[3]) out[3] = fresh({h}, kTypes[param], s);
         a.x = ss.const_data_ptr();
         a.ld_x = ld_of(ss);
         if (adds) a.total = const_cast<void *>(ss.const_data_ptr());
@@ -1117,11 +1117,10 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
         void **to[4] = {&a.d_x, &a.d_residual, &a.d_weight, &a.d_bias};
         for (int i = 0; i < 4; ++i) *to[i] = out[i].defined() ? out[i].mutable_data_ptr() : nullptr;
         at::Tensor workspace;
-        const c10::DeviceGuard guard(s.device());
         if (want[2] || want[3]) {
           const int64_t bytes = g_more.norm_workspace(&a);
           TORCH_CHECK(bytes >= 0, g_lib.error());
-          workspace = at::empty({bytes}, s.options().dtype(at::kByte));
+          workspace = fresh({bytes}, at::kByte, s);
           a.workspace = workspace.mutable_data_ptr();
           a.workspace_bytes = bytes;
         }
@@ -1218,23 +1217,23 @@ struct PolicyLoss {
 PolicyLoss policy_of(const at::Tensor &logp, const at::Tensor &old, const at::Tensor &advantage,
                      const MaybeTensor &mask, const MaybeTensor &ref, double low, double high,
                      double kl, int64_t reduction, bool keep, bool figures) {
-  const auto f32 = logp.options().dtype(at::kFloat);
+  const c10::DeviceGuard guard(logp.device());
   const int64_t rows = logp.numel() / logp.size(logp.dim() - 1);
   PolicyLoss o;
-  o.loss = reduction == LUMA_XENT_NONE ? at::empty(logp.sizes(), f32) : at::empty({}, f32);
-  if (figures) o.stats = at::empty({LUMA_POLICY_STATS}, f32);
-  if (keep) o.share = at::empty({rows + 1}, f32);
+  o.loss = fresh(reduction == LUMA_XENT_NONE ? logp.sizes() : at::IntArrayRef(), at::kFloat,
+                 logp);
+  if (figures) o.stats = fresh({LUMA_POLICY_STATS}, at::kFloat, logp);
+  if (keep) o.share = fresh({rows + 1}, at::kFloat, logp);
   PolicyRows r;
   LumaPolicyArgs a = policy_args(logp, old, advantage, value(mask), value(ref), o.share, low, high,
                                  kl, reduction, r);
   a.loss = o.loss.mutable_data_ptr<float>();
   a.stats = figures ? o.stats.mutable_data_ptr<float>() : nullptr;
-  const c10::DeviceGuard guard(logp.device());
   const int64_t bytes = g_more.policy_workspace(&a);
   TORCH_CHECK(bytes >= 0, g_lib.error());
   at::Tensor workspace;
   if (bytes) {
-    workspace = at::empty({bytes}, logp.options().dtype(at::kByte));
+    workspace = fresh({bytes}, at::kByte, logp);
     a.workspace = workspace.mutable_data_ptr();
     a.workspace_bytes = bytes;
   }
@@ -1280,14 +1279,14 @@ struct Policy : torch::autograd::Function<Policy> {
           d_logp = op.call(grads[0], logp, saved[1], saved[2], maybe(saved[3]), maybe(saved[4]),
                            saved[5], low, high, kl, reduction);
         } else {
+          const c10::DeviceGuard guard(logp.device());
           const at::Tensor g = dense(grads[0].to(at::kFloat));
-          d_logp = at::empty(logp.sizes(), logp.options());
+          d_logp = fresh(logp.sizes(), logp.scalar_type(), logp);
           PolicyRows r;
           LumaPolicyArgs a = policy_args(logp, saved[1], saved[2], saved[3], saved[4], saved[5],
                                          low, high, kl, reduction, r);
           a.grad_loss = g.const_data_ptr<float>();
           a.d_logp = d_logp.mutable_data_ptr();
-          const c10::DeviceGuard guard(logp.device());
           run(g_more.policy_backward(&a, current_stream(logp.device().index())));
         }
       }
