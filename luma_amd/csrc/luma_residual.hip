@@ -7,11 +7,18 @@
 //   d_s = r (g - mean(g) - z mean(g z)) + d_total,  g = d_y weight
 //   d_weight = sum_rows d_y z,  d_bias = sum_rows d_y
 //
-// All of them are bound by HBM (a few operations an element, and 30 integer ones
-// for a draw): every operand is read once and every result written once.  A
-// row lies in the registers of a team of L lanes, K eights of elements a lane,
-// between its loads and its stores; rows that no team holds (h > kWidest) are
-// read again, from the caches.
+// All of them are bound by HBM (a few operations an element, and for a draw ten
+// rounds of the generator for eight): every operand is read once and every result written once.  A
+// row lies in the registers of a team of L lanes, K runs of 16 bytes a lane, between
+// its loads and its stores, the next row's loads under way; rows that no team holds
+// (h > kWidest) are read again, from the caches.  Measured: 16,384 x 4,096 bfloat16
+// (residual + x, no draws) 93 us forward, 5.8 TB/s, and 90 backward, 6.0 (kernels
+// that only move as much, two tensors in and two out or three and one, 91 and 86);
+// 8,192 x 4,096 of a float32 stream and a bfloat16 branch 68 us forward, 6.0; dropout
+// of 100M bfloat16 64 to 68 us, 6.3 to 5.9.  Small ones are launches: 2,048 x 128
+// float32 3.5 us, backward 3.9 and 3.0 (the join).  Not kept: sums by shuffles through
+// LDS (8,192 x 768, float32 and bfloat16, with draws: backward 33 us, by moves in the
+// vector unit 28); a wavefront a row of 4,096 (forward 191 us).
 #include "luma_error.h"
 #include "luma_rows.h"
 
@@ -100,7 +107,9 @@ void with_team(int64_t h, F f) {
 }
 
 // Whether a call's operands (so many of the stream's type and of the branch's) are
-// more than the last-level cache holds: they then go past it.
+// more than the last-level cache holds: they then go past it (16,384 x 4,096
+// bfloat16, 537 MB: backward 91 us, cached 101; of 75 MB the forward takes 14.5 us so
+// and 13.4 cached).
 inline bool apart(const LumaLayerNormArgs *a, int streams, int branches) {
   const int64_t size = streams * (a->stream == LUMA_GRAD_F32 ? 4 : 2) +
                        branches * (a->branch == LUMA_GRAD_F32 ? 4 : 2);
@@ -116,6 +125,8 @@ int64_t blocks_of(int64_t n, int threads) {
   return need < most ? need : most;
 }
 
+// (The backward: more workgroups are more sums to join; 16,384 x 4,096 bfloat16 in
+// teams of 256 lanes 91 us and 2.7 for the join, with twice as many 95 and 3.4.)
 constexpr int kForwardThreads = 1024, kGradThreads = 512;
 
 // Workgroups of the backward, each with its own sums of the weight's and bias's
