@@ -514,7 +514,7 @@ typedef struct LumaDropoutArgs {
   const void *x;          /* device [numel], type `in`                             */
   const void *residual;   /* device [numel], type `out`, or NULL                   */
   void *y;                /* device [numel], type `out`                            */
-  int64_t numel;          /* >= 1                                                  */
+  int64_t numel;          /* 1 to 2^34                                             */
   int32_t in, out;        /* LUMA_GRAD_*: the same, or one of them float32         */
   LumaDropout drop;
 } LumaDropoutArgs;

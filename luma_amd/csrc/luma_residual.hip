@@ -951,7 +951,8 @@ extern "C" {
 int luma_dropout(const LumaDropoutArgs *a, void *stream) {
   if (!a) return fail("luma_dropout: null arguments");
   if (a->numel < 1) return fail("luma_dropout: empty operands");
-  if (a->numel > (int64_t)1 << 36) return fail("luma_dropout: operands too large");
+  // (2,048 elements a workgroup at least: 2^31 threads)
+  if (a->numel > (int64_t)1 << 34) return fail("luma_dropout: operands too large");
   if (!check_drop(a->drop)) return -1;
   if (!known_type(a->in) || !known_type(a->out) ||
       (a->in != a->out && a->in != LUMA_GRAD_F32 && a->out != LUMA_GRAD_F32))

@@ -217,7 +217,7 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], call: int
 
     ``x`` is float32, bfloat16 or float16; ``residual`` has its shape and its
     type or float32, and the result the residual's type (x's without one); the
-    sum is formed in float32.  The gradients cannot be differentiated again
+    sum is formed in float32; at most 2^34 elements.  The gradients cannot be differentiated again
     (that raises).
     """
     p, seed_at, seed, call = _draws("dropout", p, seed, call)

@@ -65,6 +65,16 @@ def test_dropout_refuses(change, text):
     _refused("luma_dropout", L.DropoutArgs(**a), text)
 
 
+@pytest.mark.parametrize("numel", [(1 << 34) + 1, 1 << 35, 1 << 36])
+@pytest.mark.parametrize("in_type,out_type", [(L.GRAD_F32, L.GRAD_F32), (L.GRAD_BF16, L.GRAD_BF16),
+                                              (L.GRAD_F16, L.GRAD_F32)])
+def test_dropout_refuses_more_than_a_launch(numel, in_type, out_type):
+    """2,048 or 4,096 elements a workgroup of 256: more than 2^34 could be 2^32
+    threads, which no launch has."""
+    a = L.DropoutArgs(x=256, y=256, numel=numel, in_type=in_type, out_type=out_type)
+    _refused("luma_dropout", a, "large")
+
+
 @pytest.mark.parametrize("n,h", [(1, 1), (100, 64), (8192, 768), (16384, 4096), (10, 16384),
                                  (10, 16385), (3, 1 << 24), (1 << 30, 8)])
 def test_workspace(n, h):
