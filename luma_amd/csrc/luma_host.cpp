@@ -911,6 +911,19 @@ at::Tensor dropped(const at::Tensor &x, const MaybeTensor &residual, const Draws
   return y;
 }
 
+// Dropout's gradient for its result's, of type code.
+at::Tensor dropped_grad(const at::Tensor &grad, const Draws &d, int64_t code) {
+  if (watched()) {
+    static const auto op = op_of<at::Tensor(const at::Tensor &, const MaybeTensor &, double, int64_t,
+                                            int64_t, int64_t)>("luma_amd::dropout_backward");
+    return op.call(grad, maybe(d.seed_at), d.p, d.seed, d.call, code);
+  }
+  const c10::DeviceGuard guard(grad.device());
+  const at::Tensor d_x = fresh(grad.sizes(), kTypes[code], grad);
+  dropout_call(dense(grad), at::Tensor(), d_x, d);
+  return d_x;
+}
+
 struct Dropout : torch::autograd::Function<Dropout> {
   static at::Tensor forward(Context *ctx, const at::Tensor &x, const MaybeTensor &residual,
                             const MaybeTensor &seed_at, double p, int64_t seed, int64_t call) {
@@ -934,17 +947,7 @@ struct Dropout : torch::autograd::Function<Dropout> {
         at::AutoDispatchBelowADInplaceOrView below;
         const Draws d{ctx->get_saved_variables()[0], ctx->saved_data["p"].toDouble(), numbers[0],
                       numbers[1]};
-        const int64_t code = numbers[2];
-        if (watched()) {
-          static const auto op =
-              op_of<at::Tensor(const at::Tensor &, const MaybeTensor &, double, int64_t, int64_t,
-                               int64_t)>("luma_amd::dropout_backward");
-          d_x = op.call(grads[0], maybe(d.seed_at), d.p, d.seed, d.call, code);
-        } else {
-          const c10::DeviceGuard guard(grads[0].device());
-          d_x = fresh(grads[0].sizes(), kTypes[code], grads[0]);
-          dropout_call(dense(grads[0]), at::Tensor(), d_x, d);
-        }
+        d_x = dropped_grad(grads[0], d, numbers[2]);
       }
       once({&d_x}, "dropout", grads[0]);
     }
@@ -1077,12 +1080,20 @@ struct LayerNorm : torch::autograd::Function<LayerNorm> {
       want[i] = (inputs >> i & 1) && ctx->needs_input_grad(edge++);
     at::Tensor out[4];      // of x, residual, weight, bias
     at::Tensor d_y = grads[0], d_total = adds ? grads[1] : at::Tensor();
-    if (d_y.defined() || d_total.defined()) {
+    const int64_t stream = grad_code(s.scalar_type());
+    // (without draws the sum's gradient is that of both)
+    const bool one = adds && d.p == 0.0 && stream == branch;
+    if (!d_y.defined() && d_total.defined()) {
+      // The sum alone was used: its norm has no part in the gradients, whether those of
+      // its rows are numbers or not.
       at::AutoDispatchBelowADInplaceOrView below;
-      const int64_t stream = grad_code(s.scalar_type());
-      if (!d_y.defined()) d_y = at::zeros(s.sizes(), s.options().dtype(kTypes[branch]));
-      // (without draws the sum's gradient is that of both)
-      const bool one = adds && d.p == 0.0 && stream == branch;
+      d_total = d_total.to(s.scalar_type());
+      if (want[0]) out[0] = one ? d_total : dropped_grad(d_total, d, branch);
+      if (want[1]) out[1] = d_total;
+      for (int i = 2; i < 4; ++i)
+        if (want[i]) out[i] = at::zeros({s.size(s.dim() - 1)}, s.options().dtype(kTypes[param]));
+    } else if (d_y.defined()) {
+      at::AutoDispatchBelowADInplaceOrView below;
       const bool want_x = want[0] && !one, want_r = want[1] || (one && want[0]);
       if (watched()) {
         static const auto op =

@@ -356,10 +356,18 @@ def _norm_grad(ctx, d_y, d_total, _):
         d_total = None
     if (d_y is None and d_total is None) or not any(want):
         return (None,) * 10
-    if d_y is None:
-        d_y = torch.zeros(s.shape, dtype=_TYPES[ctx.branch], device=s.device)
     # (without draws the sum's gradient is that of both)
     one = ctx.adds and ctx.p == 0.0 and _CODES[s.dtype] == ctx.branch
+    if d_y is None:
+        # The sum alone was used: its norm has no part in the gradients, whether those of
+        # its rows are numbers or not.
+        d_total = d_x = d_total.to(s.dtype)
+        if want[0] and not one:
+            d_x = torch.ops.luma_amd.dropout_backward(d_total, seed_at, ctx.p, ctx.seed, ctx.call,
+                                                      ctx.branch)
+        zero = s.new_zeros(s.shape[-1:], dtype=_TYPES[ctx.param])
+        got = (d_x, d_total, zero, zero)
+        return tuple(g if w else None for g, w in zip(got, want)) + (None,) * 6
     want_x, want_residual = want[0] and not one, want[1] or (one and want[0])
     d_x, d_residual, d_weight, d_bias = torch.ops.luma_amd.layer_norm_backward(
         d_y, d_total, s, weight, stats, seed_at, ctx.p, ctx.seed, ctx.call, ctx.branch, ctx.param,
@@ -418,7 +426,9 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
     and eps ``layer_norm``'s.  ``total`` is rounded to the stream's type before
     its norm is taken: the results are those of ``dropout(x, p, seed, call,
     residual)`` and of ``layer_norm`` of that, but for float16's double
-    roundings.  The gradients cannot be differentiated again (that raises).
+    roundings.  A ``y`` that goes unused leaves the sum's gradients, and zeros
+    for weight and bias.  The gradients cannot be differentiated again (that
+    raises).
     """
     p, seed_at, seed, call = _draws("add_layer_norm", p, seed, call)
     code = _CODES.get(x.dtype, -1)
