@@ -578,7 +578,8 @@ int luma_layer_norm_backward(const LumaLayerNormArgs *args, void *stream);
  *   r = exp(l - l_old),  value = -min(r A, clip(r, 1 - clip_low, 1 + clip_high) A)
  *   q = l_ref - l,       value += kl_weight (exp(q) - 1 - q)
  * and d value / d l = -r A where r A is the smaller (or both are the same),
- * else 0, plus kl_weight (1 - exp(q)).  Which side of a limit r lies on is
+ * else 0, plus kl_weight (1 - exp(q)); a kl_weight of 0 leaves the term out,
+ * whatever it is.  Which side of a limit r lies on is
  * decided on l - l_old in float64; values are float32, sums float64.  A token
  * whose mask is 0 has value and gradient 0, and counts nowhere; nothing is
  * formed of what its operands hold.

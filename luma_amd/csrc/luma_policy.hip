@@ -117,8 +117,11 @@ __device__ __forceinline__ Token token(float l, float old, float ref, bool has_r
     exp_excess(q, e, t.kl);
     // (exp(q) - 1 with the excess's digits)
     const float minus = __builtin_fabsf(q) < 0.5f ? t.kl + q : e - 1.0f;
-    t.value = __builtin_fmaf(lim.kl, t.kl, t.value);
-    t.grad = __builtin_fmaf(-lim.kl, minus, t.grad);
+    // (a weight of 0 leaves the term out: an infinite one times 0 is no number)
+    if (lim.kl != 0.0f) {
+      t.value = __builtin_fmaf(lim.kl, t.kl, t.value);
+      t.grad = __builtin_fmaf(-lim.kl, minus, t.grad);
+    }
   }
   return t;
 }

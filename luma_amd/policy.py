@@ -170,7 +170,8 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
     With r = exp(logp - old_logp) a token's loss is -min(r A, clip(r, 1 -
     clip_low, 1 + clip_high) A), plus, where ``ref_logp`` is given, kl_weight
     (exp(q) - 1 - q) with q = ref_logp - logp (an estimate of the divergence
-    from the reference that is never negative).  ``advantage`` A is float32, one
+    from the reference that is never negative; a ``kl_weight`` of 0 leaves it to
+    the figures alone, whatever it is).  ``advantage`` A is float32, one
     for each token or one for each sequence (logp's shape without its last
     dimension); the log-probabilities are float32, bfloat16 or float16, all of
     one type.  The gradient is logp's alone: the others are constants, whatever

@@ -1,0 +1,66 @@
+"""policy_loss where a token's terms leave float32's range: probabilities of 0,
+ratios past exp(88.7), advantages of 0, a KL term that is only a figure."""
+
+import math
+
+import pytest
+import torch
+
+from luma_amd import _lib as L
+from luma_amd import policy_loss
+
+pytestmark = pytest.mark.gpu
+
+REDUCTIONS = ["mean", "sequence", "sum", "none"]
+LENGTHS = [1, 3, 50, 1500]      # one launch, tokens one by one, pieces of rows
+DTYPES = [torch.float32, torch.bfloat16, torch.float16]
+
+
+def _tokens(length, dtype, at, **places):
+    """Three rows of ordinary tokens; `places`: what stands at token `at` of row 1."""
+    g = torch.Generator(device="cuda").manual_seed(length)
+    shape = (3, length)
+    t = {"logp": torch.rand(shape, generator=g, device="cuda").add_(1e-3).log_()}
+    t["old"] = t["logp"] + torch.randn(shape, generator=g, device="cuda") * 0.1
+    t["ref"] = t["logp"] + torch.randn(shape, generator=g, device="cuda") * 0.1
+    t = {name: v.to(dtype) for name, v in t.items()}
+    t["advantage"] = torch.randn(shape, generator=g, device="cuda")
+    for name, value in places.items():
+        t[name][1, at] = value
+    t["logp"].requires_grad_()
+    return t
+
+
+def _loss(t, ref=True, **kw):
+    return policy_loss(t["logp"], t["old"], t["advantage"], None, t["ref"] if ref else None, **kw)
+
+
+def _with_grad(t, loss):
+    g = torch.Generator(device="cuda").manual_seed(1)
+    out = torch.rand(loss.shape, generator=g, device="cuda") + 0.5
+    return loss.detach(), torch.autograd.grad(loss, t["logp"], out)[0]
+
+
+@pytest.fixture(params=["the host module", "operators"])
+def path(request, monkeypatch):
+    if request.param == "operators":
+        monkeypatch.setattr(L, "host_calls", lambda: None)
+
+
+@pytest.mark.parametrize("reduction", REDUCTIONS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", LENGTHS)
+@pytest.mark.parametrize("figures", [False, True])
+@pytest.mark.parametrize("logp,ref", [(-math.inf, -1.0), (-200.0, -1.0), (-1.0, math.inf),
+                                      (-1.0, math.nan)])
+def test_a_weight_of_0_leaves_the_term_out(path, logp, ref, figures, length, dtype, reduction):
+    """Loss and gradient are those without a reference, bit for bit, whatever exp(q) is."""
+    t = _tokens(length, dtype, length // 2, logp=logp, ref=ref)
+    want = _with_grad(t, _loss(t, False, reduction=reduction))
+    loss = _loss(t, reduction=reduction, kl_weight=0.0, return_stats=figures)
+    if figures:
+        loss, stats = loss
+        assert not bool(stats[1].isfinite())        # (the figure is the divergence's all the same)
+    got = _with_grad(t, loss)
+    assert all(bool(v.isfinite().all()) for v in want)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
