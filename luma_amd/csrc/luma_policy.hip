@@ -108,8 +108,10 @@ __device__ __forceinline__ Token token(float l, float old, float ref, bool has_r
   const bool up = d > lim.up, low = d < lim.low;
   t.clipped = adv > 0.0f ? up : low && adv < 0.0f;
   const float held = up ? lim.high_ratio : lim.low_ratio;
-  t.value = -(t.clipped ? held : r) * adv;
-  t.grad = t.clipped ? 0.0f : -r * adv;
+  // (an advantage of 0 makes nothing of a ratio that passes float32, not 0 inf)
+  const float product = adv == 0.0f && r > 1.0f ? 0.0f : r * adv;
+  t.value = t.clipped ? -held * adv : -product;
+  t.grad = t.clipped ? 0.0f : -product;
   t.kl = 0.0f;
   if (has_ref) {
     const float q = ref - l;

@@ -64,3 +64,30 @@ def test_a_weight_of_0_leaves_the_term_out(path, logp, ref, figures, length, dty
     got = _with_grad(t, loss)
     assert all(bool(v.isfinite().all()) for v in want)
     assert all(torch.equal(p, q) for p, q in zip(got, want))
+
+
+@pytest.mark.parametrize("reduction", REDUCTIONS)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", LENGTHS)
+@pytest.mark.parametrize("high", [0.2, math.inf])
+@pytest.mark.parametrize("old", [-200.0, -math.inf])
+def test_an_advantage_of_0(path, old, high, length, dtype, reduction):
+    """min(r A, clip(r) A) is 0, and so is its gradient, past float32's largest ratio too;
+    the other tokens are as beside an ordinary ratio."""
+    at = length // 2
+    got, want = [], []
+    for values, token in ((got, old), (want, -1.0)):
+        t = _tokens(length, dtype, at, logp=-1.0, old=token, advantage=0.0)
+        values += _with_grad(t, _loss(t, False, clip_high=high, reduction=reduction))
+    assert bool(want[0].isfinite().all()) and bool(want[1].isfinite().all())
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    assert float(got[1][1, at]) == 0.0
+    if reduction == "none":
+        assert float(got[0][1, at]) == 0.0
+    # (an advantage for each row, and what is no number stays none)
+    t = _tokens(length, dtype, at, logp=-1.0, old=old)
+    zero = torch.tensor([1.0, 0.0, 1.0], device="cuda")
+    loss = policy_loss(t["logp"], t["old"], zero, clip_high=high, reduction=reduction)
+    assert bool(loss.isfinite().all())
+    t = _tokens(length, dtype, at, logp=math.nan, old=old, advantage=0.0)
+    assert bool(_loss(t, False, clip_high=high, reduction=reduction).sum().isnan())
