@@ -84,7 +84,9 @@ __device__ __forceinline__ void exp_excess(float x, float &e, float &excess) {
   s = __builtin_fmaf(s, x, 1.0f / 24.0f);
   s = __builtin_fmaf(s, x, 1.0f / 6.0f);
   s = __builtin_fmaf(s, x, 0.5f);
-  excess = __builtin_fabsf(x) < 0.5f ? s * x * x : e - 1.0f - x;
+  // (of an infinite x, too, exp(x) is the larger: what is taken from it stays finite)
+  const float less = __builtin_fminf(x, 3e38f);
+  excess = __builtin_fabsf(x) < 0.5f ? s * x * x : e - 1.0f - less;
 }
 
 struct Limits {

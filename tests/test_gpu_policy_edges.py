@@ -91,3 +91,24 @@ def test_an_advantage_of_0(path, old, high, length, dtype, reduction):
     assert bool(loss.isfinite().all())
     t = _tokens(length, dtype, at, logp=math.nan, old=old, advantage=0.0)
     assert bool(_loss(t, False, clip_high=high, reduction=reduction).sum().isnan())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("length", LENGTHS)
+def test_infinite_divergences(path, length, dtype):
+    """exp(x) - 1 - x grows without end: an infinite x has an infinite one."""
+    at = length // 2
+    t = _tokens(length, dtype, at, logp=-1.0, old=-math.inf, advantage=2.0)
+    loss, stats = _loss(t, False, clip_high=0.25, reduction="none", return_stats=True)
+    assert float(loss[1, at].detach()) == -2.5 and float(stats[2]) == math.inf
+    for low in (-math.inf, -200.0):
+        t = _tokens(length, dtype, at, logp=low, ref=-1.0)
+        loss, stats = _loss(t, kl_weight=0.5, reduction="none", return_stats=True)
+        assert float(loss[1, at].detach()) == math.inf and float(stats[1]) == math.inf
+        d, = torch.autograd.grad(loss.sum(), t["logp"])
+        assert float(d[1, at]) == -math.inf
+        loss = _loss(t, kl_weight=0.5)
+        assert float(loss.detach()) == math.inf
+    # (a probability of 0 that was one before: a ratio of 0, which has moved as far)
+    t = _tokens(length, dtype, at, logp=-math.inf, old=-1.0)
+    assert float(_loss(t, False, return_stats=True)[1][2]) == math.inf
