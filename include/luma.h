@@ -542,7 +542,7 @@ typedef struct LumaLayerNormArgs {
   const void *residual;   /* device [n][h], rows ld_residual apart, or NULL        */
   const void *weight;     /* device [h] or NULL (1)                                */
   const void *bias;       /* device [h] or NULL (0)                                */
-  int64_t n, h;           /* each >= 1                                             */
+  int64_t n, h;           /* each >= 1; n below 2^31, h at most 2^24               */
   int64_t ld_x, ld_residual;
   int32_t stream;         /* LUMA_GRAD_*: of the residual and total                */
   int32_t branch;         /* LUMA_GRAD_*: of y; the stream's, or the stream is float32 */
@@ -565,7 +565,7 @@ typedef struct LumaLayerNormArgs {
   int64_t workspace_bytes;
 } LumaLayerNormArgs;
 
-/* Bytes of workspace that the backward needs (from n and h); < 0: refused. */
+/* Bytes of workspace that the backward needs (from n, h and stream); < 0: refused. */
 int64_t luma_layer_norm_workspace_bytes(const LumaLayerNormArgs *args);
 int luma_layer_norm_forward(const LumaLayerNormArgs *args, void *stream);
 int luma_layer_norm_backward(const LumaLayerNormArgs *args, void *stream);
@@ -579,10 +579,10 @@ int luma_layer_norm_backward(const LumaLayerNormArgs *args, void *stream);
  *   q = l_ref - l,       value += kl_weight (exp(q) - 1 - q)
  * and d value / d l = -r A where r A is the smaller (or both are the same),
  * else 0, plus kl_weight (1 - exp(q)); a kl_weight of 0 leaves the term out,
- * whatever it is.  Which side of a limit r lies on is
- * decided on l - l_old in float64; values are float32, sums float64.  A token
- * whose mask is 0 has value and gradient 0, and counts nowhere; nothing is
- * formed of what its operands hold.
+ * whatever it is, and an A of 0 the ratio, if it is a number.  Which side of a
+ * limit r lies on is decided on l - l_old in float64; values are float32, sums
+ * float64.  A token whose mask is 0 has value and gradient 0, and counts
+ * nowhere; nothing is formed of what its operands hold.
  */
 #define LUMA_POLICY_SEQUENCE 3 /* the mean over the sequences that have tokens of each
                                   one's mean; LUMA_XENT_NONE, _SUM and _MEAN (over
@@ -596,7 +596,8 @@ typedef struct LumaPolicyArgs {
   const void *ref_logp;   /* or NULL: no KL term                                   */
   const float *advantage; /* device [rows], or [rows][length] (advantage_each)     */
   const uint8_t *mask;    /* device [rows][length], 0 or 1, or NULL: every token   */
-  int64_t rows, length;   /* each >= 1; rows of more than 1,024: up to 2^22 of them */
+  int64_t rows, length;   /* each >= 1 and below 2^31, 2^40 tokens at most; rows of
+                             more than 1,024: up to 2^22 of them                   */
   int64_t ld_logp, ld_old, ld_ref, ld_advantage, ld_mask;
   int32_t advantage_each; /* 1: an advantage for each token                        */
   int32_t dtype;          /* LUMA_GRAD_*: the log-probabilities and d_logp         */

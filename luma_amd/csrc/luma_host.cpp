@@ -777,7 +777,7 @@ py::object xent(const at::Tensor &hidden, const at::Tensor &weight, const at::Te
 
 // -- the residual stream's operators and the policy loss ---------------------------
 
-// The gradients' entry points and the operators that hold them for a tracer.
+// The entry points of dropout, the norm and the policy loss, both ways.
 struct More {
   int (*dropout)(const LumaDropoutArgs *, void *) = nullptr;
   int64_t (*norm_workspace)(const LumaLayerNormArgs *) = nullptr;

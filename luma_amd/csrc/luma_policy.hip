@@ -11,9 +11,11 @@
 // kAlone short rows are one workgroup's, which joins them itself: one launch.
 // The backward forms the token's terms again, which is cheaper than keeping
 // them: the operands of small batches are still in the caches.  Measured: 512 x
-// 8,192 float32 15 us (54 MB, 3.6 TB/s), 4.7 for the join, 16 backward (71 MB, 4.4
-// TB/s); 16 x 65 5.2 and 4.4 us; 61 x 4,097 without sums 4.5.  (With the sums by
+// 8,192 float32 15.7 us (54 MB, 3.4 TB/s), 4.5 for the join, 16.3 backward (71 MB, 4.4
+// TB/s); 16 x 65 5.4 and 4.5 us; 61 x 4,097 without sums 4.9.  (With the sums by
 // shuffles through LDS, and always formed, 16 x 65 took 7.8 us forward.)
+// The limits below carry a forward's (with its join) and a backward's times, calls in a
+// row, float32, with a reference and a mask.
 #include "luma_error.h"
 #include "luma_rows.h"
 
@@ -23,12 +25,28 @@ namespace policy {
 using namespace rows;
 
 constexpr int kThreads = 256, kWaves = kThreads / 64;
-constexpr int kTokens = 4;                        // of a lane at a time (rows of fewer: 1)
-constexpr int64_t kShort = 1024;                  // tokens of a row that a wavefront takes
-constexpr int64_t kMostLong = (int64_t)1 << 22;   // longer rows
-constexpr int64_t kAlone = 32;                    // short rows that one workgroup takes
+// Tokens of a lane at a time, 16 bytes of float32 (rows of fewer: 1).  32 x 1,024 20.4
+// and 7.0 us, one at a time 24.0 and 7.4; 512 x 8,192 18.5 and 15.5, so 18.5 and 13.6;
+// rows that fill no wavefront lose by four: 20,000 x 60 18.3 and 14.9, so 10.7 and 8.3.
+constexpr int kTokens = 4;
+// Tokens of a row that a wavefront takes whole; longer ones are cut in pieces.  2,000 x
+// 600 9.6 and 7.0 us, with a limit of 512 10.3 and 6.4; 2,000 x 1,500 14.4 and 11.1, with
+// one of 2,048 14.5 and 12.7.  Few rows would rather be cut: 64 x 600 8.5 and 6.0, by
+// pieces 5.7 and 3.2.
+constexpr int64_t kShort = 1024;
+constexpr int64_t kMostLong = (int64_t)1 << 22;   // longer rows (a workgroup each)
+// Short rows that one workgroup takes, and joins: one launch for two, on the host too.
+// 16 x 65 5.3 us forward, in two launches 6.3; 4 x 1,024 7.1 and 9.2.  More tokens are
+// sooner done by more workgroups: 32 x 10 7.5 and 6.3, 16 x 1,024 11.3 and 9.4, 32 x 1,024
+// 20.4 and 9.7, and 64 x 10 would take 12.9 in one, 6.5 in two.
+constexpr int64_t kAlone = 32;
+// Of the workgroup that joins or takes all.  16 x 65 5.3 us forward, with 512 6.4, with
+// 256 9.8; the join of 2,000 x 1,500's records (all 14.4, 14.6, 15.7).
 constexpr int kJoinThreads = 1024;
-constexpr int64_t kBlocks = 2048;                 // workgroups, about
+// Workgroups, about.  2,000 x 1,500 14.4 and 11.1 us, with twice as many 17.2 and 12.6;
+// 20,000 x 60 18.3 and 14.9, with half 18.1 and 15.4; 512 x 8,192 18.5 and 15.5, with half
+// 16.7 and 13.8, with twice 22.6 and 15.0.
+constexpr int64_t kBlocks = 2048;
 
 // A workgroup's sums.
 struct Part {
@@ -317,6 +335,8 @@ __global__ __launch_bounds__(kJoinThreads) void join_kernel(LumaPolicyArgs a, Pl
     p.sequences += o.sequences;
   };
   if (!plan.shorts && a.reduction == LUMA_POLICY_SEQUENCE) {
+    // (a thread a row: few long rows keep most threads idle, and the forward of 1 x
+    // 1,000,000 takes 148 us, for the mean over the tokens 7.7; 8 x 131,072 30 and 7.7)
     for (int64_t row = threadIdx.x; row < a.rows; row += kJoinThreads) {
       double value = 0.0, count = 0.0;
       for (int64_t i = 0; i < plan.pieces; ++i) {

@@ -12,7 +12,7 @@
 // row lies in the registers of a team of L lanes, K runs of 16 bytes a lane, between
 // its loads and its stores, the next row's loads under way; rows that no team holds
 // (h > kWidest) are read again, from the caches.  Measured: 16,384 x 4,096 bfloat16
-// (residual + x, no draws) 93 us forward, 5.8 TB/s, and 90 backward, 6.0 (kernels
+// (residual + x, no draws) 93 to 94 us forward, 5.8 TB/s, and 90 to 93 backward, 5.9 (kernels
 // that only move as much, two tensors in and two out or three and one, 91 and 86);
 // 8,192 x 4,096 of a float32 stream and a bfloat16 branch 68 us forward, 6.0; dropout
 // of 100M bfloat16 64 to 68 us, 6.3 to 5.9.  Small ones are launches: 2,048 x 128
@@ -36,9 +36,18 @@ namespace residual {
 
 using namespace rows;
 
-constexpr int64_t kWidest = 16384;     // elements of a row that a team holds
+// Elements of a row that a team holds.  2,048 x 16,384 float32 onto a residual 95 us
+// forward and 119 backward, by the kernels of longer rows 124 and 198.  A lane then has
+// 32 float32 of everything and spills: up to 96 bytes forward and 236 backward, of cut
+// rows 876 and 984 (16,381 columns 237 and 326 us, by the kernels of longer rows 129
+// and 203).
+constexpr int64_t kWidest = 16384;
 constexpr int64_t kLargest = (int64_t)1 << 24;
-constexpr int kLongThreads = 1024;     // of a workgroup that holds no row
+// Of a workgroup that holds no row.  64 x 65,536 float32 onto a residual 30 us forward
+// and 48 backward, with 512 threads 42 and 55; 1,024 x 32,768 134 and 206, 137 and 207.
+constexpr int kLongThreads = 1024;
+// Of a workgroup that joins sums.  2,048 x 128 float32, the backward with its join 5.6 us,
+// with 64 x 16 threads 5.5, with 16 x 64 6.4; 16,384 x 4,096 175, 175 and 177.
 constexpr int kJoinCols = 32, kJoinRows = 32;
 constexpr int64_t kMostThreads = (int64_t)1 << 31;   // of one launch
 
@@ -109,7 +118,10 @@ void with_team(int64_t h, F f) {
 // Whether a call's operands (so many of the stream's type and of the branch's) are
 // more than the last-level cache holds: they then go past it (16,384 x 4,096
 // bfloat16, 537 MB: backward 91 us, cached 101; of 75 MB the forward takes 14.5 us so
-// and 13.4 cached).
+// and 13.4 cached).  Rows of whole runs in teams of a wavefront and more have kernels for
+// that.  The others would gain less or are fewer, and have none (bfloat16 onto a residual,
+// forward and backward: 16,384 x 4,093 132 and 137 us, past the cache 126 and 134; 51,105
+// x 1,078 100 and 95, so 102 and 93; 1,048,576 x 64 100 and 98, so 95 and 86).
 inline bool apart(const LumaLayerNormArgs *a, int streams, int branches) {
   const int64_t size = streams * (a->stream == LUMA_GRAD_F32 ? 4 : 2) +
                        branches * (a->branch == LUMA_GRAD_F32 ? 4 : 2);

@@ -187,8 +187,9 @@ def policy_loss(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
     ``return_stats``: also four float32 numbers for a log, over the tokens that
     count: the share whose ratio was clipped, the mean of the KL term (without
     its weight; 0 without ``ref_logp``), that of r - 1 - log r (how far the
-    policy has moved), and how many tokens there are.  The gradient cannot be
-    differentiated again (that raises).
+    policy has moved), and how many tokens there are.  Rows of more than 1,024
+    tokens: 2^22 at most.  The gradient cannot be differentiated again (that
+    raises).
     """
     code = _POLICY_REDUCTIONS.get(reduction)
     if code is None:

@@ -217,8 +217,8 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], call: int
 
     ``x`` is float32, bfloat16 or float16; ``residual`` has its shape and its
     type or float32, and the result the residual's type (x's without one); the
-    sum is formed in float32; at most 2^34 elements.  The gradients cannot be differentiated again
-    (that raises).
+    sum is formed in float32; at most 2^34 elements.  The gradients cannot be
+    differentiated again (that raises).
     """
     p, seed_at, seed, call = _draws("dropout", p, seed, call)
     compiling = torch.compiler.is_compiling()
@@ -390,8 +390,8 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
     here.  ``weight`` and ``bias`` [h] (either may be left out) are float32 or of
     the result's type, both the same.  Mean, deviation and the sums of the
     gradients are float32, the result and each gradient are rounded once, and
-    the weight's gradient is the same on every call.  The gradients cannot be
-    differentiated again (that raises).
+    the weight's gradient is the same on every call.  At most 2^31 - 1 rows, of
+    2^24 elements.  The gradients cannot be differentiated again (that raises).
     """
     dtype = x.dtype if dtype is None else dtype
     code = _CODES.get(dtype, -1)

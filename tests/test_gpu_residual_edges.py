@@ -115,3 +115,25 @@ def test_differentiated_again(path):
     g, = torch.autograd.grad(total, leaves[0], d.requires_grad_(), create_graph=True)
     with pytest.raises(RuntimeError, match="cannot|does not|no autograd"):
         g.sum().backward()
+
+
+@pytest.mark.parametrize("where", ["in the step", "after it"])
+@pytest.mark.parametrize("compiled", [False, True])
+def test_a_seed_written_before_the_backward_is_told(compiled, where):
+    """The masks would be others: eager and compiled programs raise."""
+    x = torch.ones(4096, device="cuda", requires_grad=True)
+
+    def step(x, seed):
+        y = dropout(x, 0.5, seed, 1)
+        z = add_layer_norm(y.view(64, 64), y.view(64, 64), p=0.5, seed=seed, call=2)[1]
+        if where == "in the step":
+            seed.add_(1)
+        return z
+
+    seed = torch.tensor(7, device="cuda")
+    # (of a step that writes it itself the compiler says so, when it records the backward)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z = (torch.compile(step, fullgraph=True) if compiled else step)(x, seed)
+        if where == "after it":
+            seed += 1
+        z.sum().backward()
