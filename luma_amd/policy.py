@@ -29,6 +29,8 @@ _POLICY_REDUCTIONS = dict(_REDUCTIONS, sequence=L.POLICY_SEQUENCE)
 __all__ = ["policy_loss"]
 
 
+# (by the public function and by the operators, which a recorded graph calls with
+# operands that the function has not seen)
 def _check_args(logp, old_logp, advantage, mask, ref_logp) -> None:
     _check_dtype("policy_loss", "logp", logp.dtype)
     if logp.dim() < 1:
@@ -74,6 +76,7 @@ def _forward_op(logp: torch.Tensor, old_logp: torch.Tensor, advantage: torch.Ten
     """(the loss, its figures or nothing, the rows' shares of a mean)."""
     _check_device("policy_loss", logp=logp, old_logp=old_logp, advantage=advantage, mask=mask,
                   ref_logp=ref_logp)
+    _check_args(logp, old_logp, advantage, mask, ref_logp)
     device = logp.device
     rows = 1
     for d in logp.shape[:-1]:
@@ -122,6 +125,17 @@ def _backward_op(grad: torch.Tensor, logp: torch.Tensor, old_logp: torch.Tensor,
                  advantage: torch.Tensor, mask: Optional[torch.Tensor],
                  ref_logp: Optional[torch.Tensor], share: torch.Tensor, clip_low: float,
                  clip_high: float, kl_weight: float, reduction: int) -> torch.Tensor:
+    _check_device("policy_loss", logp=logp, old_logp=old_logp, advantage=advantage, mask=mask,
+                  ref_logp=ref_logp, grad=grad, share=share)
+    _check_args(logp, old_logp, advantage, mask, ref_logp)
+    rows = 1
+    for d in logp.shape[:-1]:
+        rows *= d
+    if grad.shape != (logp.shape if reduction == L.XENT_NONE else ()):
+        raise ValueError(f"policy_loss: the gradient {tuple(grad.shape)} is not that of a loss of "
+                         f"{tuple(logp.shape)}")
+    if share.dtype != torch.float32 or share.shape != (rows + 1,) or not share.is_contiguous():
+        raise ValueError(f"policy_loss: share {tuple(share.shape)} is not that of {rows} rows")
     d_logp = torch.empty(logp.shape, dtype=logp.dtype, device=logp.device)
     if logp.numel() == 0:
         return d_logp

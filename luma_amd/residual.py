@@ -76,6 +76,8 @@ def _run(name: str, args, device) -> None:
 
 
 # -- checks -----------------------------------------------------------------------
+# (by the public functions, and by the operators: a recorded graph calls those with
+# operands that the functions have not seen)
 
 
 def _check_device(what: str, **tensors) -> None:
@@ -105,6 +107,12 @@ def _check_stream(what: str, residual, x) -> None:
                          "x's type or float32)")
 
 
+def _check_seed(what: str, seed) -> None:
+    if seed is not None and (seed.dtype != torch.int64 or seed.numel() != 1):
+        raise ValueError(f"{what}: a seed on the device is one int64 number (got "
+                         f"{tuple(seed.shape)} {seed.dtype})")
+
+
 def _draws(what: str, p, seed, call) -> Tuple[float, Optional[torch.Tensor], int, int]:
     """(p, the seed's tensor or None, the seed as a signed 64-bit number, call)."""
     p = float(p)
@@ -114,9 +122,7 @@ def _draws(what: str, p, seed, call) -> Tuple[float, Optional[torch.Tensor], int
     if not 0 <= call < 1 << 32:
         raise ValueError(f"{what}: call must be in [0, 2^32) (got {call})")
     if isinstance(seed, torch.Tensor):
-        if seed.dtype != torch.int64 or seed.numel() != 1:
-            raise ValueError(f"{what}: a seed on the device is one int64 number (got "
-                             f"{tuple(seed.shape)} {seed.dtype})")
+        _check_seed(what, seed)
         return p, seed, 0, call
     seed = int(seed)
     if not -1 << 63 <= seed < 1 << 64:
@@ -124,7 +130,14 @@ def _draws(what: str, p, seed, call) -> Tuple[float, Optional[torch.Tensor], int
     return p, None, seed - (1 << 64) if seed >= 1 << 63 else seed, call
 
 
-def _check_norm(what: str, x, weight, bias, eps, branch) -> None:
+def _check_norm(what: str, x, residual, weight, bias, eps, branch) -> None:
+    _check_dtype(what, "x", x.dtype)
+    _check_dtype(what, "dtype", branch)
+    if residual is not None:
+        _check_stream(what, residual, x)
+    if branch != x.dtype and (residual is not None or x.dtype != torch.float32):
+        raise ValueError(f"{what}: dtype {branch} of a result from {x.dtype} (it is x's, or a "
+                         "16-bit one for a float32 x)")
     if x.dim() < 1 or x.shape[-1] == 0:
         raise ValueError(f"{what}: x {tuple(x.shape)} has no rows of elements")
     if not eps >= 0.0:
@@ -144,6 +157,12 @@ def _check_norm(what: str, x, weight, bias, eps, branch) -> None:
 # -- dropout ----------------------------------------------------------------------
 
 
+def _check_dropout(x, residual) -> None:
+    _check_dtype("dropout", "x", x.dtype)
+    if residual is not None:
+        _check_stream("dropout", residual, x)
+
+
 def _dropout_call(x, residual, y, seed_at, p, seed, call) -> None:
     if x.numel() == 0:
         return
@@ -158,6 +177,8 @@ def _dropout_call(x, residual, y, seed_at, p, seed, call) -> None:
 def _dropout_op(x: torch.Tensor, residual: Optional[torch.Tensor],
                 seed_at: Optional[torch.Tensor], p: float, seed: int, call: int) -> torch.Tensor:
     _check_device("dropout", x=x, residual=residual, seed=seed_at)
+    _check_seed("dropout", seed_at)
+    _check_dropout(x, residual)
     y = torch.empty(x.shape, dtype=(x if residual is None else residual).dtype, device=x.device)
     _dropout_call(x, residual, y, seed_at, p, seed, call)
     return y
@@ -171,6 +192,9 @@ def _(x, residual, seed_at, p, seed, call):
 @torch.library.custom_op("luma_amd::dropout_backward", mutates_args=(), device_types="cuda")
 def _dropout_backward_op(grad: torch.Tensor, seed_at: Optional[torch.Tensor], p: float, seed: int,
                          call: int, code: int) -> torch.Tensor:
+    _check_device("dropout", grad=grad, seed=seed_at)
+    _check_dtype("dropout", "the gradient", grad.dtype)
+    _check_seed("dropout", seed_at)
     d_x = torch.empty(grad.shape, dtype=_TYPES[code], device=grad.device)
     _dropout_call(grad, None, d_x, seed_at, p, seed, call)
     return d_x
@@ -227,9 +251,7 @@ def dropout(x: torch.Tensor, p: float, seed: Union[int, torch.Tensor], call: int
         y = None if host is None else host.dropout(x, residual, seed_at, p, seed, call)
         if y is not None:
             return y
-    _check_dtype("dropout", "x", x.dtype)
-    if residual is not None:
-        _check_stream("dropout", residual, x)
+    _check_dropout(x, residual)
     if not compiling:
         _check_device("dropout", x=x, residual=residual, seed=seed_at)
     return torch.ops.luma_amd.dropout(x, residual, seed_at, p, seed, call)
@@ -257,7 +279,10 @@ def _norm_op(x: torch.Tensor, residual: Optional[torch.Tensor], weight: Optional
              seed: int, call: int,
              branch: int) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, the sum or nothing, each row's mean and 1 / deviation)."""
-    _check_device("layer_norm", x=x, residual=residual, weight=weight, bias=bias, seed=seed_at)
+    what = "layer_norm" if residual is None else "add_layer_norm"
+    _check_device(what, x=x, residual=residual, weight=weight, bias=bias, seed=seed_at)
+    _check_seed(what, seed_at)
+    _check_norm(what, x, residual, weight, bias, eps, _TYPES.get(branch))
     like, device = x if residual is None else residual, x.device
     rows = x.numel() // x.shape[-1]
     y = torch.empty(x.shape, dtype=_TYPES[branch], device=device)
@@ -298,6 +323,21 @@ def _norm_backward_op(d_y: torch.Tensor, d_total: Optional[torch.Tensor], s: tor
     """The gradients of x, the residual, weight and bias (empty ones where not
     wanted); s is the sum, or x without a residual."""
     device, h = s.device, s.shape[-1]
+    what = "add_layer_norm" if adds else "layer_norm"
+    _check_device(what, sum=s, d_y=d_y, d_total=d_total, weight=weight, stats=stats, seed=seed_at)
+    _check_seed(what, seed_at)
+    _check_dtype(what, "the sum", s.dtype)
+    for name, t in (("d_y", d_y), ("d_total", d_total)):
+        if t is not None and t.shape != s.shape:
+            raise ValueError(f"{what}: {name} {tuple(t.shape)} and the sum {tuple(s.shape)} do not "
+                             "match")
+    if weight is not None and (weight.shape != s.shape[-1:] or weight.dtype != _TYPES.get(param)):
+        raise ValueError(f"{what}: weight {tuple(weight.shape)} {weight.dtype} does not match the sum "
+                         f"{tuple(s.shape)}")
+    if (stats.dtype != torch.float32 or stats.numel() * h != 2 * s.numel()
+            or not stats.is_contiguous()):
+        raise ValueError(f"{what}: stats {tuple(stats.shape)} are not those of rows "
+                         f"{tuple(s.shape)}")
 
     def new(wanted, shape, dtype):
         return torch.empty(shape if wanted else (0,), dtype=dtype, device=device)
@@ -402,12 +442,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None,
                                                       code)
         if y is not None:
             return y
-    _check_dtype("layer_norm", "x", x.dtype)
-    _check_dtype("layer_norm", "dtype", dtype)
-    if dtype != x.dtype and x.dtype != torch.float32:
-        raise ValueError(f"layer_norm: dtype {dtype} of a result from {x.dtype} (it is x's, or a "
-                         "16-bit one for a float32 x)")
-    _check_norm("layer_norm", x, weight, bias, eps, dtype)
+    _check_norm("layer_norm", x, None, weight, bias, eps, dtype)
     if not compiling:
         _check_device("layer_norm", x=x, weight=weight, bias=bias)
     return torch.ops.luma_amd.layer_norm(x, None, weight, bias, None, eps, 0.0, 0, 0, code)[0]
@@ -440,9 +475,7 @@ def add_layer_norm(x: torch.Tensor, residual: torch.Tensor, weight: Optional[tor
                                                         seed, call, code)
         if out is not None:
             return out
-    _check_dtype("add_layer_norm", "x", x.dtype)
-    _check_stream("add_layer_norm", residual, x)
-    _check_norm("add_layer_norm", x, weight, bias, eps, x.dtype)
+    _check_norm("add_layer_norm", x, residual, weight, bias, eps, x.dtype)
     if not compiling:
         _check_device("add_layer_norm", x=x, residual=residual, weight=weight, bias=bias,
                       seed=seed_at)
