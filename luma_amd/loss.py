@@ -60,6 +60,19 @@ def _check_types(hidden, weight, target) -> None:
                          "empty")
 
 
+def _check_operands(hidden, weight, target, **more) -> None:
+    """What an operator is called with (by a recorded graph, with operands that the
+    public function has not seen)."""
+    _check(hidden, weight, target)
+    for name, t in more.items():
+        if t.device != hidden.device:
+            raise ValueError(f"linear_cross_entropy: {name} is on {t.device}, hidden on "
+                             f"{hidden.device}")
+    if hidden.dim() != 2:
+        raise ValueError(f"linear_cross_entropy: hidden {tuple(hidden.shape)} are not rows")
+    _check_types(hidden, weight, target)
+
+
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """t, or a copy, with elements of a row next to each other and rows apart."""
     if t.is_neg() or t._is_zerotensor() or (t.shape[1] > 1 and t.stride(1) != 1) or (
@@ -93,7 +106,7 @@ def _call(name: str, args: L.XentArgs, device) -> None:
 @torch.library.custom_op("luma_amd::linear_cross_entropy", mutates_args=(), device_types="cuda")
 def _forward_op(hidden: torch.Tensor, weight: torch.Tensor, target: torch.Tensor,
                 ignore_index: int, reduction: int) -> Tuple[torch.Tensor, torch.Tensor]:
-    _check(hidden, weight, target)
+    _check_operands(hidden, weight, target)
     n, device = hidden.shape[0], hidden.device
     loss = torch.empty((n,) if reduction == L.XENT_NONE else (), dtype=torch.float32,
                        device=device)
@@ -120,7 +133,14 @@ def _(hidden, weight, target, ignore_index, reduction):
 def _backward_op(grad: torch.Tensor, hidden: torch.Tensor, weight: torch.Tensor,
                  target: torch.Tensor, stats: torch.Tensor, ignore_index: int, reduction: int,
                  want_hidden: bool, want_weight: bool) -> Tuple[torch.Tensor, torch.Tensor]:
+    _check_operands(hidden, weight, target, grad=grad, stats=stats)
     n, device = hidden.shape[0], hidden.device
+    if grad.shape != ((n,) if reduction == L.XENT_NONE else ()):
+        raise ValueError(f"linear_cross_entropy: the gradient {tuple(grad.shape)} is not that of a "
+                         f"loss of {n} tokens")
+    if stats.dtype != torch.float32 or stats.shape != (2 * n + 1,) or not stats.is_contiguous():
+        raise ValueError(f"linear_cross_entropy: stats {tuple(stats.shape)} are not those of {n} "
+                         "tokens")
     d_hidden = torch.empty(hidden.shape if want_hidden else (0,), dtype=hidden.dtype,
                            device=device)
     d_weight = torch.empty(weight.shape if want_weight else (0,), dtype=weight.dtype,

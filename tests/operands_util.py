@@ -1,5 +1,5 @@
-"""Operands of the residual stream's operators and of the policy loss, by name and in
-the operators' order, that fit each other, and changes of them that do not."""
+"""Operands of the operators beside the step, by name and in the operators' order, that
+fit each other, and changes of them that do not."""
 
 import torch
 
@@ -25,6 +25,10 @@ def _mask(*s):
     return tensor(*s) > 0
 
 
+def _words(*s):
+    return torch.zeros(s[0], dtype=torch.int64, device=DEVICE)
+
+
 # Operands (by name, in the operators' order) that fit.
 CALLS = {
     "dropout": dict(x=tensor, residual=tensor, seed=None, p=0.5, number=1, call=0),
@@ -40,6 +44,12 @@ CALLS = {
     "policy_loss_backward": dict(grad=lambda *s: tensor(), logp=tensor, old=tensor, advantage=_rows,
                                  mask=_mask, ref=tensor, share=lambda *s: tensor(s[0] + 1), low=0.2,
                                  high=0.2, kl=0.1, reduction=2),
+    "linear_cross_entropy": dict(hidden=tensor, weight=lambda *s: tensor(50, s[1]), target=_words,
+                                 ignore=-100, reduction=2),
+    "linear_cross_entropy_backward": dict(grad=lambda *s: tensor(), hidden=tensor,
+                                          weight=lambda *s: tensor(50, s[1]), target=_words,
+                                          stats=lambda *s: tensor(2 * s[0] + 1), ignore=-100,
+                                          reduction=2, want_hidden=True, want_weight=True),
 }
 SEEDS = [dict(seed=torch.zeros(1, dtype=torch.int32)), dict(seed=torch.zeros(2, dtype=torch.int64)),
          dict(seed=torch.zeros(0, dtype=torch.int64))]
@@ -63,6 +73,14 @@ BAD = {
                              dict(mask=(6, 23)), dict(mask=torch.uint8), dict(grad=(1,)),
                              dict(grad=(6, 24)), dict(reduction=0), dict(share=(6,)),
                              dict(share=F64), dict(reduction=4)],
+    "linear_cross_entropy": [dict(hidden=(6, 23)), dict(hidden=(2, 3, 24)), dict(hidden=F16),
+                             dict(hidden=F64, weight=F64), dict(weight=(50, 20)), dict(weight=(24,)),
+                             dict(weight=(0, 24)), dict(target=(5,)), dict(target=torch.int32),
+                             dict(reduction=3)],
+    "linear_cross_entropy_backward": [dict(hidden=(6, 23)), dict(hidden=F16), dict(weight=(50, 20)),
+                                      dict(target=(5,)), dict(target=torch.int32), dict(grad=(6,)),
+                                      dict(reduction=0), dict(reduction=3), dict(stats=(12,)),
+                                      dict(stats=F16)],
 }
 
 
