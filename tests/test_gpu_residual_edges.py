@@ -137,3 +137,19 @@ def test_a_seed_written_before_the_backward_is_told(compiled, where):
         if where == "after it":
             seed += 1
         z.sum().backward()
+
+
+@pytest.mark.parametrize("p", [0.0, 0.5])
+@pytest.mark.parametrize("stream,branch", [(torch.float32, torch.float32),
+                                           (torch.float32, torch.bfloat16)])
+def test_the_sum_alone_compiled(stream, branch, p):
+    leaves, d = _inputs(stream, branch)
+
+    def f(*leaves):
+        return add_layer_norm(*leaves, 0.0, p, 3, 4)[1]
+
+    want = torch.autograd.grad(f(*leaves), leaves, d)
+    got = torch.autograd.grad(torch.compile(f, fullgraph=True)(*leaves), leaves, d)
+    assert all(torch.equal(s, t) for s, t in zip(got, want))
+    got = torch.autograd.grad(torch.compile(lambda *a: f(*a) * 1.0, fullgraph=True)(*leaves), leaves, d)
+    assert all(torch.equal(s, t) for s, t in zip(got, want))
